@@ -264,7 +264,9 @@ def _plain(s):
         return {"y": y.to(s["x"].dtype)}
     if op == "quantize":
         x = s["x"].float() if s["axis"] == "rows" else s["x"].float().t()
-        scale = (x.abs().amax(1) / 127.0).clamp(min=2.0 ** -126)
+        # divided by a tensor: torch divides by a number as a product with its reciprocal
+        top = x.abs().amax(1)
+        scale = (top / torch.full_like(top, 127.0)).clamp(min=2.0 ** -126)
         return {"q": torch.round(x / scale[:, None]).to(torch.int8).contiguous(),
                 "scale": scale}
     total = s["a"].float() @ s["b"].float().t()
