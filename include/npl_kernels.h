@@ -46,6 +46,11 @@ extern "C" {
 #define NPLK_ACT_RELU 1
 #define NPLK_ACT_LEAKY_RELU 7
 
+/* Element types of the calls that take one (same values as npl_dtype_t). */
+#define NPLK_DTYPE_FP32 0
+#define NPLK_DTYPE_FP16 1
+#define NPLK_DTYPE_BF16 2
+
 /* GEMM flags. */
 #define NPLK_GEMM_TF32_FAST 1u /* one TF32 pass instead of three (reported separately) */
 /* Operand form of nplk_gemm. With a workspace of nplk_gemm_workspace_size()
@@ -298,6 +303,102 @@ NPL_API int nplk_global_avg_pool(void *stream, int64_t planes, int64_t hw, const
  * `inner` elements. */
 NPL_API int nplk_binary(void *stream, int op, int64_t n, const float *a, const float *b, float *c,
                 int b_mode, int64_t channels, int64_t inner);
+
+/* ---- group norm with an activation, channels last ---------------------------- */
+/* No counterpart in the reference, whose normalisations are NCHW batch norm and
+ * layer norm (npl_activation_norm.cpp:118-182). For each image and each of
+ * `groups` runs of c / groups channels, over the hw pixels of the image:
+ *   mean, var = the run's mean and biased variance,  rstd = 1/sqrt(var + eps),
+ *   y = act(gamma[ch] * (x - mean) * rstd + beta[ch]).
+ *
+ * Layout: x[(i * hw + pixel) * ldx + channel] for image i, ldx >= c (a channel
+ * slice of a wider tensor has ldx > c), and the same with ldy; x and y are of
+ * type `dtype` (NPLK_DTYPE_*), gamma and beta [c] and mean and rstd [n][groups]
+ * are fp32. gamma, beta (1 and 0), mean and rstd may be NULL. act is 0..10 with
+ * the formulas of nplk_activation; statistics and the normalised value are fp32,
+ * y is rounded once. y may be x itself (then ldy == ldx). A NaN or an infinity
+ * makes its group NaN and no other.
+ *
+ * Sizes: c a multiple of groups, c / groups <= 8192, hw < 2^31, n < 2^31; else
+ * NPL_ERR_INVALID_ARG (not a multiple, a size < 1) or NPL_ERR_UNSUPPORTED (too
+ * large). All alignments of an element's own size are taken; 16-byte aligned
+ * pointers with ldx, ldy and c multiples of 16 bytes are the fastest.
+ *
+ * workspace: nplk_group_norm_workspace_size bytes (the same for forward and
+ * backward and every type), 256-byte aligned; 0 where the arguments are
+ * refused. Calls that may overlap on the GPU need a workspace each. */
+NPL_API size_t nplk_group_norm_workspace_size(int64_t n, int64_t hw, int64_t c, int64_t groups);
+NPL_API int nplk_group_norm_act(void *stream, int64_t n, int64_t hw, int64_t c, int64_t groups,
+                                int dtype, const void *x, int64_t ldx, const float *gamma,
+                                const float *beta, float eps, int act, float act_alpha, void *y,
+                                int64_t ldy, float *mean, float *rstd, void *workspace,
+                                size_t workspace_bytes);
+
+/* Gradient of nplk_group_norm_act for its output gradient dy, from x and the
+ * mean and rstd that the forward call stored. With xh = (x - mean) * rstd,
+ * z = gamma * xh + beta and dz = dy * act'(z) (act' of ReLU and LeakyReLU at 0
+ * taken from the left, of ReLU6 0 at both bends):
+ *   dgamma[ch] = sum dz * xh,  dbeta[ch] = sum dz  over images and pixels,
+ *   dx = rstd * (gamma * dz - (sum gamma * dz + xh * sum gamma * dz * xh) / M),
+ * the sums of dx over the group's M = hw * c / groups values. dgamma and dbeta
+ * (fp32 [c], overwritten) may be NULL, each by itself; dx may be dy or x itself
+ * (with the same pitch). Sums are fp32 in a fixed order: the same call gives
+ * the same bits. Other arguments as the forward call. */
+NPL_API int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw, int64_t c,
+                                         int64_t groups, int dtype, const void *dy, int64_t lddy,
+                                         const void *x, int64_t ldx, const float *mean,
+                                         const float *rstd, const float *gamma, const float *beta,
+                                         int act, float act_alpha, void *dx, int64_t lddx,
+                                         float *dgamma, float *dbeta, void *workspace,
+                                         size_t workspace_bytes);
+
+/* ---- dropout ------------------------------------------------------------------ */
+/* y[i] = x[i] * 65536 / (65536 - t) where r(i) >= t, else 0, for n elements of
+ * type `dtype`: t = p * 65536 rounded to the nearest integer (p in [0, 1]; t ==
+ * 65536 gives all zeros) and r(i) 16 random bits that depend on seed and
+ * offset + i only. The mask is never stored: the gradient is the same call on
+ * dy. In place (y == x) allowed; a dropped NaN or infinity gives 0. r(i) is the
+ * 16-bit number j % 8 (the low half of word 0 first) of Philox4x32-10 with key
+ * (seed low, seed high) and counter (j / 8 low, j / 8 high, 0, 0), for
+ * j = offset + i (modulo 2^64). device_offset, if not NULL, is a device word
+ * added to offset when the kernel runs: a captured graph draws new masks on
+ * each replay if the caller advances the word by n in between. No counterpart
+ * in the reference. */
+NPL_API int nplk_dropout(void *stream, int64_t n, int dtype, const void *x, void *y, float p,
+                         uint64_t seed, uint64_t offset, const uint64_t *device_offset);
+
+/* ---- matrix product in 8-bit integers ------------------------------------------ */
+/* Operands of nplk_gemm_i8. The reference names 8-bit tensors (npl_dtype_t) and
+ * computes none.
+ *
+ * nplk_quantize_rows: for each row of x (rows x cols of type `dtype`, pitch
+ * ldx), scale[r] = max(max|x[r,:]| / 127, 2^-126) and
+ * q[r*ldq + j] = round(x[r,j] / scale[r]) to the nearest integer, ties to even:
+ * |q| <= 127 and q * scale is within scale / 2 of x. Columns cols..ldq of q are
+ * left as they are. A row that holds a NaN gets scale NaN, one that holds an
+ * infinity (and no NaN) scale +infinity, both with q = 0, so that products
+ * with the row are NaN.
+ * nplk_quantize_cols: the same for the columns of x (a weight matrix [K][N],
+ * as nplk_gemm takes it, laid out once): q[c*ldq + r] and scale[c] of column c.
+ * ldq a multiple of 16 and q 16-byte aligned give nplk_gemm_i8 its fastest form. */
+NPL_API int nplk_quantize_rows(void *stream, int64_t rows, int64_t cols, int dtype,
+                               const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale);
+NPL_API int nplk_quantize_cols(void *stream, int64_t rows, int64_t cols, int dtype,
+                               const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale);
+
+/* C[m,n] = act((sum_k A[m,k] * B[n,k]) * a_scale[m] * b_scale[n] + bias[n]): A is
+ * [M][K] (tokens), B is [N][K] (output channels), 8-bit signed with pitches lda
+ * and ldb; a_scale [M], b_scale [N] and bias [N] (may be NULL) fp32; C row-major
+ * of type c_dtype (NPLK_DTYPE_*), pitch ldc. The sums are exact 32-bit integers
+ * (K <= 131071, else NPL_ERR_UNSUPPORTED), converted once to fp32; act is 0..10
+ * as in nplk_activation; C is rounded once and must not overlap the inputs.
+ * Any pitch and alignment is taken; the tensor-core kernels need A and B
+ * 16-byte aligned with lda and ldb multiples of 16, other operands take a
+ * slower kernel. M, N <= 2^30. No workspace. */
+NPL_API int nplk_gemm_i8(void *stream, int64_t M, int64_t N, int64_t K, const int8_t *A,
+                         int64_t lda, const float *a_scale, const int8_t *B, int64_t ldb,
+                         const float *b_scale, const float *bias, int act, float act_alpha,
+                         int c_dtype, void *C, int64_t ldc, int *status);
 
 /* ---- multi-GPU helpers ------------------------------------------------------ */
 /* The reference has no multi-device path: these serve npl_matmul's product

@@ -1,0 +1,115 @@
+// Element types of the kernels that take fp32, fp16 and bf16 tensors: values
+// are read in packs of up to 16 bytes, computed in fp32 and rounded once
+// (to nearest even) on the way out.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "npl_kernels.h"
+
+namespace nplk {
+
+inline int dtype_bytes(int dtype) {
+  return dtype == NPLK_DTYPE_FP32 ? 4
+         : dtype == NPLK_DTYPE_FP16 || dtype == NPLK_DTYPE_BF16 ? 2
+                                                                : 0;
+}
+
+// V consecutive elements, moved by one load or store of sizeof(T) * V bytes.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T e[V];
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V> &p, float (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = to_float(p.e[j]);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> pack(const float (&v)[V]) {
+  Pack<T, V> p;
+#pragma unroll
+  for (int j = 0; j < V; ++j) p.e[j] = from_float<T>(v[j]);
+  return p;
+}
+
+// Loads with no reuse in L1 (each value is read once by one thread). Not the
+// non-coherent path: the destination may be the source.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
+  Pack<T, V> r;
+  if constexpr (sizeof(T) * V == 16) {
+    uint4 &u = reinterpret_cast<uint4 &>(r);
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                 : "l"(p));
+  } else if constexpr (sizeof(T) * V == 8) {
+    uint2 &u = reinterpret_cast<uint2 &>(r);
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
+                 : "=r"(u.x), "=r"(u.y)
+                 : "l"(p));
+  } else {
+    r = *reinterpret_cast<const Pack<T, V> *>(p);
+  }
+  return r;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &v) {
+  *reinterpret_cast<Pack<T, V> *>(p) = v;
+}
+
+// Copies one pack from global to shared memory without passing through
+// registers where the hardware can (4, 8 and 16 bytes), counted in the
+// thread's cp.async groups; a 2-byte pack is copied at once.
+template <typename T, int V>
+__device__ __forceinline__ void copy_pack_async(Pack<T, V> *dst, const T *src) {
+  constexpr int kBytes = sizeof(T) * V;
+  if constexpr (kBytes == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src)
+                 : "memory");
+  } else if constexpr (kBytes == 4 || kBytes == 8) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src), "n"(kBytes)
+                 : "memory");
+  } else {
+    *dst = *reinterpret_cast<const Pack<T, V> *>(src);
+  }
+}
+__device__ __forceinline__ void copy_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+}  // namespace nplk

@@ -33,6 +33,7 @@ NPL_DTYPE_FP32, NPL_DTYPE_FP16, NPL_DTYPE_BF16, NPL_DTYPE_INT8, NPL_DTYPE_INT32 
 NPL_PAD_VALID, NPL_PAD_SAME, NPL_PAD_EXPLICIT = 0, 1, 2
 NPL_POOL_MAX, NPL_POOL_AVG, NPL_POOL_GLOBAL_AVG, NPL_POOL_GLOBAL_MAX = 0, 1, 2, 3
 NPL_MAX_DIMS = 8
+NPLK_DTYPE_FP32, NPLK_DTYPE_FP16, NPLK_DTYPE_BF16 = 0, 1, 2
 NPLK_CONV_ALGO_AUTO, NPLK_CONV_ALGO_DIRECT, NPLK_CONV_ALGO_IM2COL = 0, 1, 2
 NPLK_CONV_ALGO_WINDOW, NPLK_CONV_ALGO_WINDOW_GATHER, NPLK_CONV_ALGO_WINDOW_PAIR = 3, 4, 5
 NPLK_GEMM_TF32_FAST = 1
@@ -200,6 +201,17 @@ NPLK_SIGNATURES = {
     "nplk_pool2d": (C.c_int, [_VP] + [_I64] * 12 + [C.c_int, C.c_int, _VP, _VP]),
     "nplk_global_avg_pool": (C.c_int, [_VP, _I64, _I64, _VP, _VP]),
     "nplk_binary": (C.c_int, [_VP, C.c_int, _I64, _VP, _VP, _VP, C.c_int, _I64, _I64]),
+    "nplk_group_norm_workspace_size": (C.c_size_t, [_I64] * 4),
+    "nplk_group_norm_act": (C.c_int, [_VP, _I64, _I64, _I64, _I64, C.c_int, _VP, _I64, _VP, _VP,
+                                      _F, C.c_int, _F, _VP, _I64, _VP, _VP, _VP, C.c_size_t]),
+    "nplk_group_norm_act_backward": (C.c_int, [_VP, _I64, _I64, _I64, _I64, C.c_int, _VP, _I64,
+                                               _VP, _I64, _VP, _VP, _VP, _VP, C.c_int, _F, _VP,
+                                               _I64, _VP, _VP, _VP, C.c_size_t]),
+    "nplk_dropout": (C.c_int, [_VP, _I64, C.c_int, _VP, _VP, _F, C.c_uint64, C.c_uint64, _VP]),
+    "nplk_quantize_rows": (C.c_int, [_VP, _I64, _I64, C.c_int, _VP, _I64, _VP, _I64, _VP]),
+    "nplk_quantize_cols": (C.c_int, [_VP, _I64, _I64, C.c_int, _VP, _I64, _VP, _I64, _VP]),
+    "nplk_gemm_i8": (C.c_int, [_VP, _I64, _I64, _I64, _VP, _I64, _VP, _VP, _I64, _VP, _VP,
+                               C.c_int, _F, C.c_int, _VP, _I64, _VP]),
     "nplk_colshard_relayout": (C.c_int, [_VP, _I64, _I64, _I64, _VP, _VP]),
     "nplk_ipc_handle_size": (C.c_size_t, []),
     "nplk_ipc_get_handle": (C.c_int, [_VP, _VP, _P(C.c_uint64)]),
