@@ -536,7 +536,7 @@ NPL_API int nplk_gemm_tune(void *stream, int64_t M, int64_t N, int64_t K, const 
 /* No reference counterpart: the reference's CPU loops cannot time out or run
  * out of device memory. Both hooks are off unless armed. */
 
-#define NPLK_DEBUG_GEMM 1        /* the tcgen05 GEMM kernels (split and raw forms) */
+#define NPLK_DEBUG_GEMM 1        /* the tcgen05 GEMM kernels (split and raw forms, nplk_gemm_i8's) */
 #define NPLK_DEBUG_CONV_WINDOW 2 /* the window conv kernels (gather and plane forms) */
 
 /* Arms the next launch of one kernel family, from any thread, to exercise its

@@ -1,34 +1,57 @@
 // Matrix product in 8-bit integers with a scale for each token and channel:
-//   C[m,n] = act(a_scale[m] * b_scale[n] * sum_k A[m,k] B[n,k] + bias[n]).
-// |A * B| <= 2^14, so 32-bit sums are exact up to K = 131071.
-#include "nplk_device.cuh"
+//   C[m,n] = act((sum_k A[m,k] B[n,k]) * a_scale[m] * b_scale[n] + bias[n]).
+// |A * B| <= 2^14, so 32-bit sums are exact up to K = 131071 in any order.
+//
+// Four kernels, by what bounds the product (choose_plan):
+//   rows    few tokens: the weights' bytes. Each warp streams 16 channels with
+//           plain 16-byte loads into mma.sync fragments, warps share K;
+//   split   middle sizes: tcgen05 tiles of 128 channels x MT tokens, K shared
+//           by a cluster of up to 8 CTAs that add their sums over distributed
+//           shared memory;
+//   pair    large sizes: persistent CTA pairs, 256 channels x 256 tokens;
+//   bytes   operands that TMA and 16-byte loads cannot read.
+// In all tcgen05 tiles the channels are the accumulator's 128 lanes and the
+// tokens its columns: a warp then holds 32 consecutive channels of one token,
+// which are consecutive in C, so its stores are whole 64- or 128-byte pieces
+// without a transpose, and b_scale and bias are one register each.
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <utility>
+
+#include "act_epilogue.cuh"
 #include "nplk_host.h"
+#include "ptx_sm100.cuh"
 #include "typed_io.cuh"
 
 namespace nplk {
 namespace {
 
 struct I8Args {
-  int64_t M, N, K, lda, ldb, ldc;
+  int64_t lda, ldb, ldc;
   const int8_t *A, *B;
   const float *a_scale, *b_scale, *bias;
+  int M, N, K;
   int act;
   float alpha;
+  uint32_t stall_us;  // fault injection: 0 except on an armed launch (injected_stall)
+  int *status;
 };
 
-// Any pitch and alignment: 64 x 64 tiles, 64 bytes of K at a time gathered by
-// bytes into shared memory, four products an instruction (dp4a). 256 threads,
-// 4 x 4 results each.
+// ---------------------------------------------------------------------------
+// bytes: 64 x 64 tiles, 64 bytes of K at a time gathered by bytes into shared
+// memory, four products an instruction (dp4a). 256 threads, 4 x 4 results each.
+// ---------------------------------------------------------------------------
 constexpr int kTile = 64, kPitch = 17;  // words a row: 16, and one against bank conflicts
 
 template <typename T>
 __global__ void __launch_bounds__(256) gemm_i8_bytes_kernel(I8Args p, T *C) {
   __shared__ int sa[kTile * kPitch], sb[kTile * kPitch];
-  const int64_t m_tiles = (p.M + kTile - 1) / kTile;
+  const int64_t m_tiles = (static_cast<int64_t>(p.M) + kTile - 1) / kTile;
   const int64_t m0 = blockIdx.x % m_tiles * kTile, n0 = blockIdx.x / m_tiles * kTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   int acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.K; k0 += 64) {
+  for (int k0 = 0; k0 < p.K; k0 += 64) {
     for (int i = threadIdx.x; i < kTile * 64; i += 256) {
       const int r = i >> 6, k = i & 63;
       const bool in_k = k0 + k < p.K;
@@ -55,14 +78,677 @@ __global__ void __launch_bounds__(256) gemm_i8_bytes_kernel(I8Args p, T *C) {
   }
   for (int i = 0; i < 4; ++i) {
     const int64_t m = m0 + ty + 16 * i;
+    float v[4];
+#pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t n = n0 + tx + 16 * j;
-      if (m < p.M && n < p.N) {
-        const float v = fmaf(static_cast<float>(acc[i][j]) * p.a_scale[m], p.b_scale[n],
-                             p.bias ? p.bias[n] : 0.0f);
-        C[m * p.ldc + n] = from_float<T>(apply_act(v, p.act, p.alpha));
+      v[j] = m < p.M && n < p.N ? fmaf(static_cast<float>(acc[i][j]) * p.a_scale[m], p.b_scale[n],
+                                       p.bias ? p.bias[n] : 0.0f)
+                                : 0.0f;
+    }
+    act_array<T>(v, p.act, p.alpha);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = n0 + tx + 16 * j;
+      if (m < p.M && n < p.N) C[m * p.ldc + n] = from_float<T>(v[j]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// rows: up to 8 * NT tokens. A CTA takes 16 channels; its 8 warps take every
+// eighth 64-byte piece of K. mma.sync m16n8k32 with the channels as its rows:
+// lane (g, t) loads the 16 bytes at 64 c + 16 t of channels g and g + 8 and of
+// token g, and uses words 0, 1 and then 2, 3 as its two fragments -- K in the
+// same other order on both sides, which a sum does not mind. The warps' sums
+// meet in shared memory.
+// ---------------------------------------------------------------------------
+constexpr int kRowsWarps = 8, kRowsUnroll = 4;
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                       uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 load16(const int8_t *p) {
+  return __ldg(reinterpret_cast<const uint4 *>(p));
+}
+
+// The first `count` (1..15) of 16 bytes, then zeros.
+__device__ __forceinline__ uint4 load_bytes(const int8_t *p, int count) {
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 15; ++i)
+    if (i < count) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p[i])) << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(kRowsWarps * 32) gemm_i8_rows_kernel(I8Args p, T *C) {
+  __shared__ int red[kRowsWarps][NT * 8][16];
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  // rows past the last are read as the last, their results dropped
+  const int8_t *b0 = p.B + (n0 + g < p.N ? n0 + g : p.N - 1) * p.ldb + 16 * t;
+  const int8_t *b1 = p.B + (n0 + g + 8 < p.N ? n0 + g + 8 : p.N - 1) * p.ldb + 16 * t;
+  const int8_t *a[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    a[j] = p.A + static_cast<int64_t>(8 * j + g < p.M ? 8 * j + g : p.M - 1) * p.lda + 16 * t;
+  int acc[NT][4] = {};
+  auto step = [&](const uint4 &x, const uint4 &y, const uint4 (&z)[NT]) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      mma_s8(acc[j], x.x, y.x, x.y, y.y, z[j].x, z[j].y);
+      mma_s8(acc[j], x.z, y.z, x.w, y.w, z[j].z, z[j].w);
+    }
+  };
+  const int full = p.K >> 6;
+  int c = warp;
+  for (; c + (kRowsUnroll - 1) * kRowsWarps < full; c += kRowsUnroll * kRowsWarps) {
+    uint4 x[kRowsUnroll], y[kRowsUnroll], z[kRowsUnroll][NT];
+#pragma unroll
+    for (int u = 0; u < kRowsUnroll; ++u) {
+      const int64_t o = static_cast<int64_t>(c + u * kRowsWarps) * 64;
+      x[u] = load16(b0 + o);
+      y[u] = load16(b1 + o);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) z[u][j] = load16(a[j] + o);
+    }
+#pragma unroll
+    for (int u = 0; u < kRowsUnroll; ++u) step(x[u], y[u], z[u]);
+  }
+  for (; c < full; c += kRowsWarps) {
+    const int64_t o = static_cast<int64_t>(c) * 64;
+    uint4 z[NT];
+    const uint4 x = load16(b0 + o), y = load16(b1 + o);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) z[j] = load16(a[j] + o);
+    step(x, y, z);
+  }
+  if ((p.K & 63) && warp == full % kRowsWarps) {  // the last, shorter piece
+    const int64_t o = static_cast<int64_t>(full) * 64;
+    const int left = (p.K & 63) - 16 * t;  // bytes of this lane's 16 inside K
+    uint4 x = make_uint4(0, 0, 0, 0), y = x, z[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) z[j] = x;
+    if (left >= 16) {
+      x = load16(b0 + o);
+      y = load16(b1 + o);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) z[j] = load16(a[j] + o);
+    } else if (left > 0) {
+      x = load_bytes(b0 + o, left);
+      y = load_bytes(b1 + o, left);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) z[j] = load_bytes(a[j] + o, left);
+    }
+    step(x, y, z);
+  }
+  // accumulator: channels g, g + 8 (rows), tokens 2t, 2t + 1 (columns)
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    red[warp][8 * j + 2 * t][g] = acc[j][0];
+    red[warp][8 * j + 2 * t + 1][g] = acc[j][1];
+    red[warp][8 * j + 2 * t][g + 8] = acc[j][2];
+    red[warp][8 * j + 2 * t + 1][g + 8] = acc[j][3];
+  }
+  __syncthreads();
+  if (threadIdx.x < NT * 128) {
+    const int ch = threadIdx.x & 15, m = threadIdx.x >> 4;
+    const int64_t n = n0 + ch;
+    if (m < p.M && n < p.N) {
+      int s = 0;
+#pragma unroll
+      for (int w = 0; w < kRowsWarps; ++w) s += red[w][m][ch];
+      float v[1] = {fmaf(static_cast<float>(s) * p.a_scale[m], p.b_scale[n],
+                         p.bias ? p.bias[n] : 0.0f)};
+      act_array<T>(v, p.act, p.alpha);
+      C[m * p.ldc + n] = from_float<T>(v[0]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The tcgen05 kernels' common parts. A stage holds 128 bytes of K of 128
+// channels and of the tile's tokens (or this CTA's half of them), as TMA's
+// 128-byte swizzle lays them out; one MMA takes 32 bytes of K.
+// ---------------------------------------------------------------------------
+constexpr int kI8BK = 128, kI8Channels = 128, kI8WeightBytes = kI8Channels * kI8BK;
+
+// 32 columns (tokens m0..) of this thread's channel n, from their integer sums
+// to C. `scales`: 32 floats of this warp's own in shared memory.
+template <typename T>
+__device__ __forceinline__ void i8_store_chunk(const I8Args &p, const uint32_t (&acc)[32], int m0,
+                                               int64_t n, float sb, float bias, float *scales,
+                                               T *C) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();  // the previous chunk's scales have been read
+  scales[lane] = m0 + lane < p.M ? p.a_scale[m0 + lane] : 0.0f;
+  __syncwarp();
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 s = *reinterpret_cast<const float4 *>(scales + j);
+    v[j] = fmaf(static_cast<float>(static_cast<int>(acc[j])) * s.x, sb, bias);
+    v[j + 1] = fmaf(static_cast<float>(static_cast<int>(acc[j + 1])) * s.y, sb, bias);
+    v[j + 2] = fmaf(static_cast<float>(static_cast<int>(acc[j + 2])) * s.z, sb, bias);
+    v[j + 3] = fmaf(static_cast<float>(static_cast<int>(acc[j + 3])) * s.w, sb, bias);
+  }
+  act_array<T>(v, p.act, p.alpha);
+  if (n >= p.N) return;
+  T *c = C + static_cast<int64_t>(m0) * p.ldc + n;
+  if (m0 + 32 <= p.M) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) c[j * p.ldc] = from_float<T>(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (m0 + j < p.M) c[j * p.ldc] = from_float<T>(v[j]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// split: one 128-channel x MT-token tile per cluster of S CTAs, CTA r taking
+// its share of the K blocks. 192 threads: TMA producer, MMA issuer, four
+// epilogue warps. With S > 1 each CTA lays its partial sums in its own shared
+// memory ([token][channel], over the stages, which are read out by then), and
+// CTA r adds tokens [r MT / S, (r + 1) MT / S) of all S CTAs.
+// ---------------------------------------------------------------------------
+template <int MT>
+struct SplitTraits {
+  static constexpr int kStageBytes = kI8WeightBytes + MT * kI8BK;
+  static constexpr int kStages = MT >= 256 ? 4 : MT >= 128 ? 6 : MT >= 64 ? 8 : 10;
+  static constexpr int kTmemCols = MT < 32 ? 32 : MT;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 256 + 4 * 32 * 4;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static_assert(MT * kI8Channels * 4 <= kStages * kStageBytes, "partial sums over the stages");
+};
+
+template <int MT, typename T>
+__global__ void __launch_bounds__(192, 1)
+    gemm_i8_split_kernel(const __grid_constant__ CUtensorMap map_w,
+                         const __grid_constant__ CUtensorMap map_x, const I8Args p, T *C,
+                         int slices, int n_tiles) {
+  using S = SplitTraits<MT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = align_smem_1024(smem_raw);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kStages * S::kStageBytes);
+  uint64_t *empty = full + S::kStages;
+  uint64_t *acc_full = empty + S::kStages;
+  uint64_t *never = acc_full + 1;  // never arrived on (injected_stall)
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(never + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  float *scales = reinterpret_cast<float *>(smem + S::kStages * S::kStageBytes + 256);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % slices;
+  const int tile = static_cast<int>(blockIdx.x) / slices;
+  const int n0 = tile % n_tiles * kI8Channels, m0 = tile / n_tiles * MT;
+  const int blocks = (p.K + kI8BK - 1) / kI8BK;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * blocks / slices);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * blocks / slices);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(never, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+
+  bool have = false;  // epilogue threads: the accumulator is complete
+  const int quad = warp & 3;
+  const int ch = quad * 32 + lane;
+  const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, pending = 0, pending_phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer))
+          break;
+        uint8_t *st = smem + stage * S::kStageBytes;
+        mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
+        tma_load_2d(&map_w, &full[stage], st, kb * kI8BK, n0);
+        tma_load_2d(&map_x, &full[stage], st + kI8WeightBytes, kb * kI8BK, m0);
+        pending |= 1u << stage;
+        pending_phase = (pending_phase & ~(1u << stage)) | (phase << stage);
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      // the last copy into each stage lands before the CTA can exit
+      for (int s = 0; s < S::kStages; ++s)
+        if ((pending >> s) & 1u) mbar_drain(&full[s], (pending_phase >> s) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_s8(kI8Channels, MT);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool go = injected_stall(never, p.stall_us, abort_flag, p.status);
+      for (int kb = kb0; go && kb < kb1; ++kb) {
+        go = mbar_wait(&full[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
+        if (!go) break;
+        tc_fence_after_sync();
+        const uint32_t st = smem_u32(smem + stage * S::kStageBytes);
+        const uint64_t w = umma_desc_sw128(st), x = umma_desc_sw128(st + kI8WeightBytes);
+#pragma unroll
+        for (int kk = 0; kk < kI8BK / 32; ++kk)
+          mma_i8_ss(tmem_base, w + 2 * kk, x + 2 * kk, idesc, kb > kb0 || kk > 0 ? 1u : 0u);
+        mma_commit(&empty[stage]);
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (go) mma_commit(acc_full);
+    }
+    __syncwarp();
+  } else {
+    have = mbar_wait(acc_full, 0u, abort_flag, p.status, kStatusTimeoutEpilogue);
+    __syncwarp();
+    tc_fence_after_sync();
+    if (have && slices == 1) {
+      const int64_t n = static_cast<int64_t>(n0) + ch;
+      const float sb = n < p.N ? p.b_scale[n] : 0.0f;
+      const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
+#pragma unroll 1
+      for (int c0 = 0; c0 < MT && m0 + c0 < p.M; c0 += 32) {
+        uint32_t acc[32];
+        tmem_ld32(t_row + c0, acc);
+        tmem_wait_ld(acc);
+        i8_store_chunk<T>(p, acc, m0 + c0, n, sb, bias, scales + (warp - 2) * 32, C);
+      }
+    } else if (have) {
+      int *part = reinterpret_cast<int *>(smem);
+#pragma unroll 1
+      for (int c0 = 0; c0 < MT; c0 += 32) {
+        uint32_t acc[32];
+        tmem_ld32(t_row + c0, acc);
+        tmem_wait_ld(acc);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c0 + j < MT) part[(c0 + j) * kI8Channels + ch] = static_cast<int>(acc[j]);
       }
     }
+    tc_fence_before_sync();
+  }
+  if (slices > 1) {
+    cluster_sync();  // every CTA's partial sums are in its shared memory
+    if (warp >= 2 && have) {
+      const int64_t n = static_cast<int64_t>(n0) + ch;
+      const float sb = n < p.N ? p.b_scale[n] : 0.0f;
+      const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
+      const int per = MT / slices;
+      for (int i = 0; i < per; ++i) {
+        const int tok = rank * per + i;
+        const int m = m0 + tok;
+        if (m >= p.M) break;
+        const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(tok * kI8Channels + ch) * 4u;
+        int s = 0;
+        for (int r = 0; r < slices; ++r)
+          s += static_cast<int>(ld_shared_cluster_u32(mapa_shared(at, static_cast<uint32_t>(r))));
+        float v[1] = {fmaf(static_cast<float>(s) * p.a_scale[m], sb, bias)};
+        act_array<T>(v, p.act, p.alpha);
+        if (n < p.N) C[m * p.ldc + n] = from_float<T>(v[0]);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while another reads its shared memory
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, S::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// pair: persistent clusters of two CTAs (tcgen05 cta_group::2), tiles of 256
+// channels x 256 tokens. Each CTA loads its 128 channels and 128 of the tokens
+// (32 KB a stage), so a K block's bytes serve twice the products of a one-SM
+// 128 x 256 tile's. Two accumulators of 256 columns: the epilogue of one tile
+// runs under the next tile's MMAs. 8 epilogue warps, two per lane quadrant.
+//   full (leader)       the leader's expect_tx for both CTAs' copies
+//   empty, acc_full     in each CTA, by the leader's commit to both
+//   acc_empty (leader)  16 arrivals: the 8 epilogue warps of each CTA
+// ---------------------------------------------------------------------------
+constexpr int kPairTokens = 256, kPairStages = 6, kPairEpiWarps = 8;
+constexpr int kPairStage = kI8WeightBytes + kPairTokens / 2 * kI8BK;
+constexpr int kPairThreads = 64 + kPairEpiWarps * 32;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kPairEpiWarps * 32 * 4;
+static_assert(kPairSmem <= 232448, "shared memory budget");
+
+// Groups of 8 channel tiles sweep all token tiles, so that the pairs at work
+// at one time share operand rows in L2.
+__device__ __forceinline__ void pair_tile(int tile, int n_tiles, int m_tiles, int &nt, int &mt) {
+  constexpr int kGroup = 8;
+  const int group = tile / (kGroup * m_tiles);
+  const int first = group * kGroup;
+  const int size = min(n_tiles - first, kGroup);
+  const int local = tile - group * kGroup * m_tiles;
+  nt = first + local % size;
+  mt = local / size;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w,
+                        const __grid_constant__ CUtensorMap map_x, const I8Args p, T *C,
+                        int n_tiles, int m_tiles) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = align_smem_1024(smem_raw);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kPairStages * kPairStage);
+  uint64_t *empty = full + kPairStages;
+  uint64_t *acc_full = empty + kPairStages;
+  uint64_t *acc_empty = acc_full + 2;
+  uint64_t *never = acc_empty + 2;  // never arrived on (injected_stall)
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(never + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  float *scales = reinterpret_cast<float *>(smem + kPairStages * kPairStage + 256);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t peer_abort = mapa_shared(smem_u32(const_cast<int *>(abort_flag)), rank ^ 1u);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 2 * kPairEpiWarps);
+    }
+    mbar_init(never, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before any remote arrival
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+
+  const int tiles = n_tiles * m_tiles;
+  const int pairs = static_cast<int>(gridDim.x >> 1), pair = static_cast<int>(blockIdx.x >> 1);
+  const int blocks = (p.K + kI8BK - 1) / kI8BK;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, issued_phase = 0;
+      bool aborted = false;
+      for (int tile = pair; tile < tiles && !aborted; tile += pairs) {
+        int nt, mt;
+        pair_tile(tile, n_tiles, m_tiles, nt, mt);
+        const int row_w = nt * 2 * kI8Channels + static_cast<int>(rank) * kI8Channels;
+        const int row_x = mt * kPairTokens + static_cast<int>(rank) * (kPairTokens / 2);
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait_pair(&empty[stage], phase ^ 1u, abort_flag, peer_abort, p.status,
+                              kStatusTimeoutProducer)) {
+            aborted = true;
+            break;
+          }
+          uint8_t *st = smem + stage * kPairStage;
+          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0u);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kPairStage);
+          tma_load_2d_pair(&map_w, bar, st, kb * kI8BK, row_w);
+          tma_load_2d_pair(&map_x, bar, st + kI8WeightBytes, kb * kI8BK, row_x);
+          issued |= 1u << stage;
+          issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+          if (++stage == kPairStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (rank == 0) {
+        // both CTAs' copies complete on the leader's barriers: every issued
+        // phase lands before the pair can exit
+        for (int s = 0; s < kPairStages; ++s)
+          if ((issued >> s) & 1u) mbar_drain(&full[s], (issued_phase >> s) & 1u);
+      } else if (aborted && issued) {
+        // this CTA cannot observe its own copies: give those in flight time to land
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader) ----------------
+    if (rank == 0 && lane == 0) {
+      const uint32_t idesc = umma_idesc_s8(2 * kI8Channels, kPairTokens);
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool go = injected_stall(never, p.stall_us, abort_flag, p.status);
+      if (!go) pair_raise_abort(peer_abort);
+      for (int tile = pair; go && tile < tiles; tile += pairs, ++local) {
+        const int acc = local & 1;
+        go = mbar_wait_pair(&acc_empty[acc], ((local >> 1) & 1) ^ 1u, abort_flag, peer_abort,
+                            p.status, kStatusTimeoutAccFree);
+        if (!go) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem_base + acc * kPairTokens;
+        for (int kb = 0; kb < blocks; ++kb) {
+          go = mbar_wait_pair(&full[stage], phase, abort_flag, peer_abort, p.status,
+                              kStatusTimeoutMma);
+          if (!go) break;
+          tc_fence_after_sync();
+          const uint32_t st = smem_u32(smem + stage * kPairStage);
+          const uint64_t w = umma_desc_sw128(st), x = umma_desc_sw128(st + kI8WeightBytes);
+#pragma unroll
+          for (int kk = 0; kk < kI8BK / 32; ++kk)
+            mma_i8_ss_pair(d, w + 2 * kk, x + 2 * kk, idesc, kb > 0 || kk > 0 ? 1u : 0u);
+          mma_commit_pair_both(&empty[stage]);
+          if (++stage == kPairStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (go) mma_commit_pair_both(&acc_full[acc]);
+      }
+    }
+  } else {
+    // ---------------- epilogue: 2 warps per lane quadrant, half the tokens each ----------------
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    float *mine = scales + (warp - 2) * 32;
+    int local = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++local) {
+      int nt, mt;
+      pair_tile(tile, n_tiles, m_tiles, nt, mt);
+      const int64_t n = static_cast<int64_t>(nt) * 2 * kI8Channels + rank * kI8Channels +
+                        quad * 32 + lane;
+      const float sb = n < p.N ? p.b_scale[n] : 0.0f;
+      const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
+      const int acc = local & 1;
+      if (!mbar_wait_pair(&acc_full[acc], (local >> 1) & 1, abort_flag, peer_abort, p.status,
+                          kStatusTimeoutEpilogue))
+        break;
+      tc_fence_after_sync();
+      const int m0 = mt * kPairTokens + half * 128;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
+                             static_cast<uint32_t>(acc * kPairTokens + half * 128);
+#pragma unroll 1
+      for (int c0 = 0; c0 < 128 && m0 + c0 < p.M; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld32(t_row + c0, v);
+        tmem_wait_ld(v);
+        i8_store_chunk<T>(p, v, m0 + c0, n, sb, bias, mine, C);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0u));
+    }
+  }
+  __syncthreads();
+  cluster_sync();  // no remote arrival, copy or MMA into either CTA is left
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Choice and launch
+// ---------------------------------------------------------------------------
+enum class I8Kernel { kBytes, kRows, kSplit, kPair };
+
+struct I8Plan {
+  I8Kernel kernel;
+  int mt, slices;
+};
+
+I8Plan choose_plan(int64_t M, int64_t N, int64_t K, bool aligned) {
+  if (!aligned) return {I8Kernel::kBytes, 0, 0};
+  if (M <= 16) return {I8Kernel::kRows, 0, 0};
+  const int64_t sms = sm_count(), blocks = ceil_div(K, kI8BK);
+  // Clocks, from the bytes each SM takes from L2 (about 40 a clock with all SMs
+  // at work) and a fixed cost per tile.
+  const double per_byte = 1.0 / 40;
+  I8Plan best{I8Kernel::kPair, 0, 0};
+  double least = static_cast<double>(ceil_div(ceil_div(N, 256) * ceil_div(M, kPairTokens), sms / 2)) *
+                     blocks * kPairStage * per_byte +
+                 5000;
+  for (int mt : {32, 64, 128, 256}) {
+    for (int s : {1, 2, 4, 8}) {
+      if (s > blocks || (mt == 256 && s > 1)) continue;
+      const int64_t ctas = ceil_div(N, kI8Channels) * ceil_div(M, mt) * s;
+      const double cost =
+          static_cast<double>(ceil_div(ctas, sms)) *
+          (3000 + (s > 1 ? 1000 : 0) +
+           static_cast<double>(ceil_div(blocks, s)) * (kI8Channels + mt) * kI8BK * per_byte);
+      if (cost < least) {
+        least = cost;
+        best = {I8Kernel::kSplit, mt, s};
+      }
+    }
+  }
+  return best;
+}
+
+int launch_cluster(cudaStream_t s, const void *fn, cudaLaunchConfig_t &cfg, unsigned cluster,
+                   cudaLaunchAttribute (&attr)[2]) {
+  (void)fn;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cfg.stream = s;
+  return kOk;
+}
+
+template <int MT, typename T>
+int launch_split(cudaStream_t s, const I8Args &p, T *C, int slices) {
+  using Tr = SplitTraits<MT>;
+  CUtensorMap mw, mx;
+  int rc = encode_tmap_2d_u8_sw128(&mw, p.B, p.K, p.N, p.ldb, kI8Channels);
+  if (rc) return rc;
+  rc = encode_tmap_2d_u8_sw128(&mx, p.A, p.K, p.M, p.lda, MT);
+  if (rc) return rc;
+  auto *fn = gemm_i8_split_kernel<MT, T>;
+  rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), Tr::kSmemBytes);
+  if (rc) return rc;
+  const int n_tiles = static_cast<int>(ceil_div(p.N, kI8Channels));
+  const int64_t ctas = static_cast<int64_t>(n_tiles) * ceil_div(p.M, MT) * slices;
+  if (ctas >= (int64_t(1) << 31)) return kErrUnsupported;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = Tr::kSmemBytes;
+  launch_cluster(s, nullptr, cfg, static_cast<unsigned>(slices), attr);
+  count_launch();
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, p, C, slices, n_tiles));
+}
+
+template <typename T>
+int launch_pair(cudaStream_t s, const I8Args &p, T *C) {
+  CUtensorMap mw, mx;
+  int rc = encode_tmap_2d_u8_sw128(&mw, p.B, p.K, p.N, p.ldb, kI8Channels);
+  if (rc) return rc;
+  rc = encode_tmap_2d_u8_sw128(&mx, p.A, p.K, p.M, p.lda, kPairTokens / 2);
+  if (rc) return rc;
+  auto *fn = gemm_i8_pair_kernel<T>;
+  rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), kPairSmem);
+  if (rc) return rc;
+  const int64_t n_tiles = ceil_div(p.N, 2 * kI8Channels), m_tiles = ceil_div(p.M, kPairTokens);
+  if (n_tiles * m_tiles >= (int64_t(1) << 30)) return kErrUnsupported;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  launch_cluster(s, nullptr, cfg, 2, attr);
+  // A grid beyond the pairs that fit at once would still be right (no pair
+  // waits for another); all of them at once is what the tile order counts on.
+  const int64_t fit = sm_count() / 2;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(n_tiles * m_tiles, fit)));
+  count_launch();
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, p, C, static_cast<int>(n_tiles),
+                                           static_cast<int>(m_tiles)));
+}
+
+template <typename T>
+int run(cudaStream_t s, I8Args p, T *C, const I8Plan &plan) {
+  if (plan.kernel == I8Kernel::kBytes) {
+    const int64_t tiles = ceil_div(p.M, kTile) * ceil_div(p.N, kTile);
+    if (tiles >= (int64_t(1) << 31)) return kErrUnsupported;
+    gemm_i8_bytes_kernel<T><<<static_cast<unsigned>(tiles), 256, 0, s>>>(p, C);
+    count_launch();
+    return launch_result();
+  }
+  if (plan.kernel == I8Kernel::kRows) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.N, 16))), block(kRowsWarps * 32);
+    return p.M <= 8 ? launch_programmatic(gemm_i8_rows_kernel<1, T>, grid, block, 0, s, p, C)
+                    : launch_programmatic(gemm_i8_rows_kernel<2, T>, grid, block, 0, s, p, C);
+  }
+  if (!p.status) p.status = device_status_word();
+  if (!p.status) return kErrInternal;
+  p.stall_us = take_armed_stall(NPLK_DEBUG_GEMM);
+  if (plan.kernel == I8Kernel::kPair) return launch_pair<T>(s, p, C);
+  switch (plan.mt) {
+    case 32:
+      return launch_split<32, T>(s, p, C, plan.slices);
+    case 64:
+      return launch_split<64, T>(s, p, C, plan.slices);
+    case 128:
+      return launch_split<128, T>(s, p, C, plan.slices);
+    default:
+      return launch_split<256, T>(s, p, C, plan.slices);
   }
 }
 
@@ -81,18 +767,14 @@ extern "C" int nplk_gemm_i8(void *stream, int64_t M, int64_t N, int64_t K, const
     return kErrInvalidArg;
   if (reinterpret_cast<uintptr_t>(C) % size) return kErrInvalidArg;
   if (M > (int64_t(1) << 30) || N > (int64_t(1) << 30) || K > 131071) return kErrUnsupported;
-  (void)status;
-  I8Args p{M, N, K, lda, ldb, ldc, A, B, a_scale, b_scale, bias, act, act_alpha};
+  const bool aligned = reinterpret_cast<uintptr_t>(A) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(B) % 16 == 0 && lda % 16 == 0 &&
+                       ldb % 16 == 0;
+  const I8Args p{lda, ldb, ldc, A, B, a_scale, b_scale, bias, static_cast<int>(M),
+                 static_cast<int>(N), static_cast<int>(K), act, act_alpha, 0u, status};
+  const I8Plan plan = choose_plan(M, N, K, aligned);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t tiles = ceil_div(M, kTile) * ceil_div(N, kTile);
-  if (tiles >= (int64_t(1) << 31)) return kErrUnsupported;
-  auto go = [&](auto zero) {
-    using T = decltype(zero);
-    gemm_i8_bytes_kernel<T><<<static_cast<unsigned>(tiles), 256, 0, s>>>(p, static_cast<T *>(C));
-  };
-  if (c_dtype == NPLK_DTYPE_FP32) go(float{});
-  else if (c_dtype == NPLK_DTYPE_FP16) go(__half{});
-  else go(__nv_bfloat16{});
-  count_launch();
-  return launch_result();
+  if (c_dtype == NPLK_DTYPE_FP32) return run(s, p, static_cast<float *>(C), plan);
+  if (c_dtype == NPLK_DTYPE_FP16) return run(s, p, static_cast<__half *>(C), plan);
+  return run(s, p, static_cast<__nv_bfloat16 *>(C), plan);
 }

@@ -164,6 +164,22 @@ int encode_2d_f32(CUtensorMap *map, const void *base, uint64_t inner, uint64_t o
 }
 }  // namespace
 
+int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                            uint64_t row_pitch_bytes, uint32_t box_outer) {
+  auto fn = encode_fn();
+  if (!fn) return kErrInternal;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (row_pitch_bytes & 15u) != 0)
+    return kErrInvalidArg;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {row_pitch_bytes};
+  cuuint32_t box[2] = {128, box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? kOk : kErrInternal;
+}
+
 int encode_tmap_im2col_nhwc_f32_sw128(CUtensorMap *map, const void *base, uint64_t c,
                                      uint64_t w, uint64_t h, uint64_t n, int lower_w,
                                      int lower_h, int upper_w, int upper_h, uint32_t stride_w,

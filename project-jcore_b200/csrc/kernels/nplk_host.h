@@ -62,6 +62,11 @@ int encode_tmap_2d_f32_sw128_atom32(CUtensorMap *map, const void *base, uint64_t
                                     uint64_t outer, uint64_t row_pitch_bytes,
                                     uint32_t box_inner, uint32_t box_outer);
 
+// 2-D map of bytes: dims {inner, outer} bytes, row pitch in bytes, box {128,
+// box_outer}, 128-byte swizzle, zero fill out of bounds.
+int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                            uint64_t row_pitch_bytes, uint32_t box_outer);
+
 // 4-D NHWC fp32 im2col tensor map (dims {c, w, h, n}, densely packed): each
 // load gathers `pixels` output pixels x `channels` channels, walking the
 // bounding box [lower, dim-1+upper] of every image with the given traversal

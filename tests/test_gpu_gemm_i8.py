@@ -304,3 +304,21 @@ def test_quantised_projection_is_near_the_fp32_one(m):
              + k * sa.double()[:, None] * sb.double()[None] / 4)
     err = (c.double() - x.double() @ w.double()).abs()
     assert (err <= bound * (1 + 1e-3)).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 256, 1024), (2048, 2048, 1024)])
+def test_expired_wait_is_reported_and_leaves_nothing_behind(m, n, k):
+    # the MMA issuer of one armed launch waits 20 ms on a barrier that nothing
+    # arrives on: status 102, and the next call is right
+    lib = S.gpu_lib()
+    ops = operands(m, n, k)
+    c = torch.empty(m, n, device="cuda")
+    status = torch.zeros(1, device="cuda", dtype=torch.int32)
+    assert lib.nplk_debug_arm_wait_timeout(nb.NPLK_DEBUG_GEMM, 20_000) == 0
+    rc = lib.nplk_gemm_i8(S.cuda_stream(), m, n, k, ops[0].data_ptr(), ops[0].stride(0),
+                          ops[2].data_ptr(), ops[1].data_ptr(), ops[1].stride(0),
+                          ops[3].data_ptr(), None, 0, 0.0, 0, c.data_ptr(), n,
+                          status.data_ptr())
+    assert rc == 0 and status.item() == nb.NPLK_STATUS_TIMEOUT_MMA
+    assert lib.nplk_debug_arm_wait_timeout(nb.NPLK_DEBUG_GEMM, 0) == 0
+    check_product(product(lib, *ops), *ops, "fp32")
