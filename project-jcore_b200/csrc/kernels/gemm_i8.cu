@@ -96,14 +96,14 @@ __global__ void __launch_bounds__(256) gemm_i8_bytes_kernel(I8Args p, T *C) {
 }
 
 // ---------------------------------------------------------------------------
-// rows: up to 8 * NT tokens. A CTA takes 16 channels; its 8 warps take every
-// eighth 64-byte piece of K. mma.sync m16n8k32 with the channels as its rows:
+// rows: up to 8 * NT tokens. A CTA takes 16 channels; its 16 warps take every
+// 16th 64-byte piece of K. mma.sync m16n8k32 with the channels as its rows:
 // lane (g, t) loads the 16 bytes at 64 c + 16 t of channels g and g + 8 and of
 // token g, and uses words 0, 1 and then 2, 3 as its two fragments -- K in the
 // same other order on both sides, which a sum does not mind. The warps' sums
 // meet in shared memory.
 // ---------------------------------------------------------------------------
-constexpr int kRowsWarps = 8, kRowsUnroll = 4;
+constexpr int kRowsWarps = 16, kRowsUnroll = 4;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                        uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -116,6 +116,15 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 
 __device__ __forceinline__ uint4 load16(const int8_t *p) {
   return __ldg(reinterpret_cast<const uint4 *>(p));
+}
+
+// Weights: each byte is read once, and the bytes after it soon by other warps.
+__device__ __forceinline__ uint4 load16_stream(const int8_t *p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
 }
 
 // The first `count` (1..15) of 16 bytes, then zeros.
@@ -131,6 +140,7 @@ template <int NT, typename T>
 __global__ void __launch_bounds__(kRowsWarps * 32) gemm_i8_rows_kernel(I8Args p, T *C) {
   __shared__ int red[kRowsWarps][NT * 8][16];
   griddep_wait();
+  griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
@@ -156,8 +166,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32) gemm_i8_rows_kernel(I8Args p,
 #pragma unroll
     for (int u = 0; u < kRowsUnroll; ++u) {
       const int64_t o = static_cast<int64_t>(c + u * kRowsWarps) * 64;
-      x[u] = load16(b0 + o);
-      y[u] = load16(b1 + o);
+      x[u] = load16_stream(b0 + o);
+      y[u] = load16_stream(b1 + o);
 #pragma unroll
       for (int j = 0; j < NT; ++j) z[u][j] = load16(a[j] + o);
     }
@@ -222,70 +232,213 @@ __global__ void __launch_bounds__(kRowsWarps * 32) gemm_i8_rows_kernel(I8Args p,
 // ---------------------------------------------------------------------------
 constexpr int kI8BK = 128, kI8Channels = 128, kI8WeightBytes = kI8Channels * kI8BK;
 
+// a_scale of `count` tokens from m0 on (0 past the last token) into this
+// warp's own `scales` in shared memory.
+__device__ __forceinline__ void i8_stage_scales(const I8Args &p, int m0, int count,
+                                                float *scales) {
+  __syncwarp();  // the previous tile's have been read
+  for (int i = threadIdx.x & 31; i < count; i += 32)
+    scales[i] = m0 + i < p.M ? p.a_scale[m0 + i] : 0.0f;
+  __syncwarp();
+}
+
+// Whether C takes 16-bit results by pairs of channels.
+template <typename T>
+__device__ __forceinline__ bool i8_by_pairs(const I8Args &p, const T *C) {
+  return sizeof(T) == 2 && p.ldc % 2 == 0 && (reinterpret_cast<uintptr_t>(C) & 3u) == 0;
+}
+
+// (a0, a1) * (b0, b1) and (a0, a1) * (b0, b1) + (c0, c1), two fp32 products an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+  return reinterpret_cast<const float2 &>(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)),
+        "l"(reinterpret_cast<const uint64_t &>(c)));
+  return reinterpret_cast<const float2 &>(r);
+}
+
 // 32 columns (tokens m0..) of this thread's channel n, from their integer sums
-// to C. `scales`: 32 floats of this warp's own in shared memory.
+// to C. `scales`: their a_scale in shared memory.
+//
+// 16-bit results: neighbouring lanes (channels n, n + 1) swap halves so that
+// the even lane holds both channels of the even tokens and the odd lane those
+// of the odd ones; a store instruction then writes 64 bytes of two tokens
+// instead of one, and half as many are issued.
 template <typename T>
 __device__ __forceinline__ void i8_store_chunk(const I8Args &p, const uint32_t (&acc)[32], int m0,
-                                               int64_t n, float sb, float bias, float *scales,
-                                               T *C) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();  // the previous chunk's scales have been read
-  scales[lane] = m0 + lane < p.M ? p.a_scale[m0 + lane] : 0.0f;
-  __syncwarp();
+                                               int64_t n, float sb, float bias,
+                                               const float *scales, bool by_pairs, T *C) {
   float v[32];
+  const float2 sb2 = make_float2(sb, sb), bias2 = make_float2(bias, bias);
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 s = *reinterpret_cast<const float4 *>(scales + j);
-    v[j] = fmaf(static_cast<float>(static_cast<int>(acc[j])) * s.x, sb, bias);
-    v[j + 1] = fmaf(static_cast<float>(static_cast<int>(acc[j + 1])) * s.y, sb, bias);
-    v[j + 2] = fmaf(static_cast<float>(static_cast<int>(acc[j + 2])) * s.z, sb, bias);
-    v[j + 3] = fmaf(static_cast<float>(static_cast<int>(acc[j + 3])) * s.w, sb, bias);
+    const float2 x = make_float2(static_cast<float>(static_cast<int>(acc[j])),
+                                 static_cast<float>(static_cast<int>(acc[j + 1])));
+    const float2 y = make_float2(static_cast<float>(static_cast<int>(acc[j + 2])),
+                                 static_cast<float>(static_cast<int>(acc[j + 3])));
+    const float2 u = fma2(mul2(x, make_float2(s.x, s.y)), sb2, bias2);
+    const float2 w = fma2(mul2(y, make_float2(s.z, s.w)), sb2, bias2);
+    v[j] = u.x;
+    v[j + 1] = u.y;
+    v[j + 2] = w.x;
+    v[j + 3] = w.y;
   }
   act_array<T>(v, p.act, p.alpha);
+  const int rows = p.M - m0;
+  if constexpr (sizeof(T) == 2) {
+    if (by_pairs) {
+      const uint32_t odd = threadIdx.x & 1u;
+      // byte selectors: the halves sent (the other lane's tokens); then even
+      // lanes take {own low, got low}, {own low, got high}, odd lanes
+      // {got low, own high}, {got high, own high}
+      const uint32_t send = odd ? 0x5410u : 0x7632u;
+      const uint32_t first = odd ? 0x3254u : 0x5410u, second = odd ? 0x3276u : 0x7610u;
+      uint32_t o[16];
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const uint32_t w0 = pack2<T>(v[j], v[j + 1]), w1 = pack2<T>(v[j + 2], v[j + 3]);
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(w0, w1, send), 1);
+        o[j / 2] = __byte_perm(w0, got, first);
+        o[j / 2 + 1] = __byte_perm(w1, got, second);
+      }
+      const int64_t ne = n - odd;
+      const int64_t pitch = 2 * p.ldc;
+      T *c = C + (static_cast<int64_t>(m0) + odd) * p.ldc + ne;
+      if (rows >= 32 && ne + 1 < p.N) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          *reinterpret_cast<uint32_t *>(c + j * pitch) = o[j];
+      } else if (ne < p.N) {
+        const bool both = ne + 1 < p.N;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (2 * j + static_cast<int>(odd) < rows) {
+            if (both) *reinterpret_cast<uint32_t *>(c + j * pitch) = o[j];
+            else *reinterpret_cast<uint16_t *>(c + j * pitch) = static_cast<uint16_t>(o[j]);
+          }
+        }
+      }
+      return;
+    }
+  }
   if (n >= p.N) return;
   T *c = C + static_cast<int64_t>(m0) * p.ldc + n;
-  if (m0 + 32 <= p.M) {
+  if (rows >= 32) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) c[j * p.ldc] = from_float<T>(v[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (m0 + j < p.M) c[j * p.ldc] = from_float<T>(v[j]);
+      if (j < rows) c[j * p.ldc] = from_float<T>(v[j]);
   }
 }
 
 // ---------------------------------------------------------------------------
 // split: one 128-channel x MT-token tile per cluster of S CTAs, CTA r taking
-// its share of the K blocks. 192 threads: TMA producer, MMA issuer, four
-// epilogue warps. With S > 1 each CTA lays its partial sums in its own shared
+// its share of the K blocks. TMA producer, MMA issuer, 8 epilogue warps (two
+// per lane quadrant, every second 32 tokens each: one warp per scheduler alone
+// would wait out every latency of the epilogue). With S > 1 each CTA lays its partial sums in its own shared
 // memory ([token][channel], over the stages, which are read out by then), and
 // CTA r adds tokens [r MT / S, (r + 1) MT / S) of all S CTAs.
 // ---------------------------------------------------------------------------
+constexpr int kSplitThreads = 64 + 8 * 32;
+
 template <int MT>
 struct SplitTraits {
   static constexpr int kStageBytes = kI8WeightBytes + MT * kI8BK;
-  static constexpr int kStages = MT >= 256 ? 4 : MT >= 128 ? 6 : MT >= 64 ? 8 : 10;
-  static constexpr int kTmemCols = MT < 32 ? 32 : MT;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 256 + 4 * 32 * 4;
-  static_assert(kSmemBytes <= 232448, "shared memory budget");
-  static_assert(MT * kI8Channels * 4 <= kStages * kStageBytes, "partial sums over the stages");
+  static constexpr int kMostStages = MT >= 256 ? 4 : MT >= 128 ? 6 : MT >= 64 ? 8 : 10;
+  static constexpr int kTmemCols = MT;
+  static constexpr int kPartialBytes = MT * kI8Channels * 4;  // over the stages
+  // Shared memory after the stages: barriers, then the epilogue warps' scales.
+  static constexpr int kTailBytes = 256 + MT * 4;
+  static constexpr int smem_bytes(int stages, bool partials) {
+    const int area = stages * kStageBytes;
+    return 1024 + (partials && area < kPartialBytes ? kPartialBytes : area) + kTailBytes;
+  }
+  static_assert(1024 + kMostStages * kStageBytes + kTailBytes <= 232448, "shared memory budget");
 };
 
+// This CTA's share of the cluster's tokens: the sums of all S CTAs' partial
+// sums, a token per warp at a time, four channels per lane.
+template <int MT, int S, typename T>
+__device__ __forceinline__ void i8_add_slices(const I8Args &p, const uint8_t *part, int rank,
+                                              int n0, int m0, T *C) {
+  constexpr int kPer = MT / S, kBatch = kPer / 8 < 1 ? 1 : kPer / 8 < 4 ? kPer / 8 : 4;
+  const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 2;
+  const int64_t n = static_cast<int64_t>(n0) + 4 * lane;
+  float sb[4], bias[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    sb[j] = n + j < p.N ? p.b_scale[n + j] : 0.0f;
+    bias[j] = p.bias && n + j < p.N ? p.bias[n + j] : 0.0f;
+  }
+  const bool whole = n + 4 <= p.N && p.ldc % 4 == 0 &&
+                     reinterpret_cast<uintptr_t>(C) % (4 * sizeof(T)) == 0;
+#pragma unroll 1
+  for (int i = w * kBatch; i < kPer; i += 8 * kBatch) {
+    const int tok = rank * kPer + i;
+    if (m0 + tok >= p.M) break;
+    uint4 v[kBatch][S];  // all loads first: a round trip to another SM each
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+      for (int r = 0; r < S; ++r)
+        v[b][r] = ld_shared_cluster_v4(mapa_shared(
+            smem_u32(part) + static_cast<uint32_t>((tok + b) * kI8Channels + 4 * lane) * 4u,
+            static_cast<uint32_t>(r)));
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t m = static_cast<int64_t>(m0) + tok + b;
+      if (m >= p.M) break;
+      int s[4] = {};
+#pragma unroll
+      for (int r = 0; r < S; ++r) {
+        s[0] += static_cast<int>(v[b][r].x);
+        s[1] += static_cast<int>(v[b][r].y);
+        s[2] += static_cast<int>(v[b][r].z);
+        s[3] += static_cast<int>(v[b][r].w);
+      }
+      const float sa = p.a_scale[m];
+      float o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(static_cast<float>(s[j]) * sa, sb[j], bias[j]);
+      act_array<T>(o, p.act, p.alpha);
+      T *c = C + m * p.ldc + n;
+      if (whole) {
+        store_pack(c, pack<T, 4>(o));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) c[j] = from_float<T>(o[j]);
+      }
+    }
+  }
+}
+
 template <int MT, typename T>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(kSplitThreads)
     gemm_i8_split_kernel(const __grid_constant__ CUtensorMap map_w,
                          const __grid_constant__ CUtensorMap map_x, const I8Args p, T *C,
-                         int slices, int n_tiles) {
+                         int slices, int n_tiles, int stages, int area) {
   using S = SplitTraits<MT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align_smem_1024(smem_raw);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::kStages * S::kStageBytes);
-  uint64_t *empty = full + S::kStages;
-  uint64_t *acc_full = empty + S::kStages;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + area);
+  uint64_t *empty = full + S::kMostStages;
+  uint64_t *acc_full = empty + S::kMostStages;
   uint64_t *never = acc_full + 1;  // never arrived on (injected_stall)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(never + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  float *scales = reinterpret_cast<float *>(smem + S::kStages * S::kStageBytes + 256);
+  float *scales = reinterpret_cast<float *>(smem + area + 256);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x) % slices;
@@ -296,7 +449,7 @@ __global__ void __launch_bounds__(192, 1)
   const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * blocks / slices);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -316,6 +469,7 @@ __global__ void __launch_bounds__(192, 1)
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
+  griddep_launch_dependents();
 
   bool have = false;  // epilogue threads: the accumulator is complete
   const int quad = warp & 3;
@@ -334,13 +488,13 @@ __global__ void __launch_bounds__(192, 1)
         tma_load_2d(&map_x, &full[stage], st + kI8WeightBytes, kb * kI8BK, m0);
         pending |= 1u << stage;
         pending_phase = (pending_phase & ~(1u << stage)) | (phase << stage);
-        if (++stage == S::kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
       // the last copy into each stage lands before the CTA can exit
-      for (int s = 0; s < S::kStages; ++s)
+      for (int s = 0; s < stages; ++s)
         if ((pending >> s) & 1u) mbar_drain(&full[s], (pending_phase >> s) & 1u);
     }
     __syncwarp();
@@ -360,7 +514,7 @@ __global__ void __launch_bounds__(192, 1)
         for (int kk = 0; kk < kI8BK / 32; ++kk)
           mma_i8_ss(tmem_base, w + 2 * kk, x + 2 * kk, idesc, kb > kb0 || kk > 0 ? 1u : 0u);
         mma_commit(&empty[stage]);
-        if (++stage == S::kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -369,30 +523,37 @@ __global__ void __launch_bounds__(192, 1)
     }
     __syncwarp();
   } else {
+    const int64_t n = static_cast<int64_t>(n0) + ch;
+    const float sb = n < p.N ? p.b_scale[n] : 0.0f;
+    const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
+    const int c_first = (warp - 2) / 4 * 32;
+    const bool by_pairs = i8_by_pairs(p, C);
+    if (slices == 1) {
+      for (int i = threadIdx.x - 64; i < MT; i += 256)
+        scales[i] = m0 + i < p.M ? p.a_scale[m0 + i] : 0.0f;
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the epilogue warps
+    }
     have = mbar_wait(acc_full, 0u, abort_flag, p.status, kStatusTimeoutEpilogue);
     __syncwarp();
     tc_fence_after_sync();
     if (have && slices == 1) {
-      const int64_t n = static_cast<int64_t>(n0) + ch;
-      const float sb = n < p.N ? p.b_scale[n] : 0.0f;
-      const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
 #pragma unroll 1
-      for (int c0 = 0; c0 < MT && m0 + c0 < p.M; c0 += 32) {
+      for (int c0 = c_first; c0 < MT && m0 + c0 < p.M; c0 += 64) {
         uint32_t acc[32];
         tmem_ld32(t_row + c0, acc);
         tmem_wait_ld(acc);
-        i8_store_chunk<T>(p, acc, m0 + c0, n, sb, bias, scales + (warp - 2) * 32, C);
+        i8_store_chunk<T>(p, acc, m0 + c0, n, sb, bias, scales + c0, by_pairs, C);
       }
     } else if (have) {
       int *part = reinterpret_cast<int *>(smem);
 #pragma unroll 1
-      for (int c0 = 0; c0 < MT; c0 += 32) {
+      for (int c0 = c_first; c0 < MT; c0 += 64) {
         uint32_t acc[32];
         tmem_ld32(t_row + c0, acc);
         tmem_wait_ld(acc);
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (c0 + j < MT) part[(c0 + j) * kI8Channels + ch] = static_cast<int>(acc[j]);
+          part[(c0 + j) * kI8Channels + ch] = static_cast<int>(acc[j]);
       }
     }
     tc_fence_before_sync();
@@ -400,22 +561,9 @@ __global__ void __launch_bounds__(192, 1)
   if (slices > 1) {
     cluster_sync();  // every CTA's partial sums are in its shared memory
     if (warp >= 2 && have) {
-      const int64_t n = static_cast<int64_t>(n0) + ch;
-      const float sb = n < p.N ? p.b_scale[n] : 0.0f;
-      const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
-      const int per = MT / slices;
-      for (int i = 0; i < per; ++i) {
-        const int tok = rank * per + i;
-        const int m = m0 + tok;
-        if (m >= p.M) break;
-        const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(tok * kI8Channels + ch) * 4u;
-        int s = 0;
-        for (int r = 0; r < slices; ++r)
-          s += static_cast<int>(ld_shared_cluster_u32(mapa_shared(at, static_cast<uint32_t>(r))));
-        float v[1] = {fmaf(static_cast<float>(s) * p.a_scale[m], sb, bias)};
-        act_array<T>(v, p.act, p.alpha);
-        if (n < p.N) C[m * p.ldc + n] = from_float<T>(v[0]);
-      }
+      if (slices == 2) i8_add_slices<MT, 2, T>(p, smem, rank, n0, m0, C);
+      else if (slices == 4) i8_add_slices<MT, 4, T>(p, smem, rank, n0, m0, C);
+      else i8_add_slices<MT, 8, T>(p, smem, rank, n0, m0, C);
     }
     __syncwarp();
     cluster_sync();  // no CTA leaves while another reads its shared memory
@@ -440,7 +588,7 @@ __global__ void __launch_bounds__(192, 1)
 constexpr int kPairTokens = 256, kPairStages = 6, kPairEpiWarps = 8;
 constexpr int kPairStage = kI8WeightBytes + kPairTokens / 2 * kI8BK;
 constexpr int kPairThreads = 64 + kPairEpiWarps * 32;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kPairEpiWarps * 32 * 4;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kPairEpiWarps * 128 * 4;
 static_assert(kPairSmem <= 232448, "shared memory budget");
 
 // Groups of 8 channel tiles sweep all token tiles, so that the pairs at work
@@ -499,6 +647,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
+  griddep_launch_dependents();
 
   const int tiles = n_tiles * m_tiles;
   const int pairs = static_cast<int>(gridDim.x >> 1), pair = static_cast<int>(blockIdx.x >> 1);
@@ -582,7 +731,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   } else {
     // ---------------- epilogue: 2 warps per lane quadrant, half the tokens each ----------------
     const int quad = warp & 3, half = (warp - 2) >> 2;
-    float *mine = scales + (warp - 2) * 32;
+    float *mine = scales + (warp - 2) * 128;
+    const bool by_pairs = i8_by_pairs(p, C);
     int local = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++local) {
       int nt, mt;
@@ -591,12 +741,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         quad * 32 + lane;
       const float sb = n < p.N ? p.b_scale[n] : 0.0f;
       const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
-      const int acc = local & 1;
+      const int acc = local & 1, m0 = mt * kPairTokens + half * 128;
+      i8_stage_scales(p, m0, 128, mine);
       if (!mbar_wait_pair(&acc_full[acc], (local >> 1) & 1, abort_flag, peer_abort, p.status,
                           kStatusTimeoutEpilogue))
         break;
+      __syncwarp();
       tc_fence_after_sync();
-      const int m0 = mt * kPairTokens + half * 128;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
                              static_cast<uint32_t>(acc * kPairTokens + half * 128);
 #pragma unroll 1
@@ -604,7 +755,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         uint32_t v[32];
         tmem_ld32(t_row + c0, v);
         tmem_wait_ld(v);
-        i8_store_chunk<T>(p, v, m0 + c0, n, sb, bias, mine, C);
+        i8_store_chunk<T>(p, v, m0 + c0, n, sb, bias, mine + c0, by_pairs, C);
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -681,7 +832,12 @@ int launch_split(cudaStream_t s, const I8Args &p, T *C, int slices) {
   rc = encode_tmap_2d_u8_sw128(&mx, p.A, p.K, p.M, p.lda, MT);
   if (rc) return rc;
   auto *fn = gemm_i8_split_kernel<MT, T>;
-  rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), Tr::kSmemBytes);
+  // As many stages as a CTA has K blocks, up to the limit: with a short K
+  // several CTAs share an SM, and one's loads run under another's stores.
+  const int blocks = static_cast<int>(ceil_div(ceil_div(p.K, kI8BK), slices));
+  const int stages = std::min(blocks, Tr::kMostStages);
+  const int smem = Tr::smem_bytes(stages, slices > 1);
+  rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), smem);
   if (rc) return rc;
   const int n_tiles = static_cast<int>(ceil_div(p.N, kI8Channels));
   const int64_t ctas = static_cast<int64_t>(n_tiles) * ceil_div(p.M, MT) * slices;
@@ -689,11 +845,12 @@ int launch_split(cudaStream_t s, const I8Args &p, T *C, int slices) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(192);
-  cfg.dynamicSmemBytes = Tr::kSmemBytes;
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = smem;
   launch_cluster(s, nullptr, cfg, static_cast<unsigned>(slices), attr);
   count_launch();
-  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, p, C, slices, n_tiles));
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, p, C, slices, n_tiles, stages,
+                                           smem - 1024 - Tr::kTailBytes));
 }
 
 template <typename T>

@@ -58,6 +58,20 @@ __device__ __forceinline__ Pack<T, V> pack(const float (&v)[V]) {
   return p;
 }
 
+// Two values rounded to 16 bits, `a` in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return reinterpret_cast<const uint32_t &>(h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return reinterpret_cast<const uint32_t &>(h);
+}
+
 // Loads with no reuse in L1 (each value is read once by one thread). Not the
 // non-coherent path: the destination may be the source.
 template <typename T, int V>
