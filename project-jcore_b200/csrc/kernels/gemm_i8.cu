@@ -15,9 +15,6 @@
 // which are consecutive in C, so its stores are whole 64- or 128-byte pieces
 // without a transpose, and b_scale and bias are one register each.
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <utility>
 
 #include "act_epilogue.cuh"
 #include "nplk_host.h"
@@ -232,22 +229,6 @@ __global__ void __launch_bounds__(kRowsWarps * 32) gemm_i8_rows_kernel(I8Args p,
 // ---------------------------------------------------------------------------
 constexpr int kI8BK = 128, kI8Channels = 128, kI8WeightBytes = kI8Channels * kI8BK;
 
-// a_scale of `count` tokens from m0 on (0 past the last token) into this
-// warp's own `scales` in shared memory.
-__device__ __forceinline__ void i8_stage_scales(const I8Args &p, int m0, int count,
-                                                float *scales) {
-  __syncwarp();  // the previous tile's have been read
-  for (int i = threadIdx.x & 31; i < count; i += 32)
-    scales[i] = m0 + i < p.M ? p.a_scale[m0 + i] : 0.0f;
-  __syncwarp();
-}
-
-// Whether C takes 16-bit results by pairs of channels.
-template <typename T>
-__device__ __forceinline__ bool i8_by_pairs(const I8Args &p, const T *C) {
-  return sizeof(T) == 2 && p.ldc % 2 == 0 && (reinterpret_cast<uintptr_t>(C) & 3u) == 0;
-}
-
 // (a0, a1) * (b0, b1) and (a0, a1) * (b0, b1) + (c0, c1), two fp32 products an instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   uint64_t r;
@@ -265,92 +246,145 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return reinterpret_cast<const float2 &>(r);
 }
 
-// 32 columns (tokens m0..) of this thread's channel n, from their integer sums
-// to C. `scales`: their a_scale in shared memory.
-//
-// 16-bit results: neighbouring lanes (channels n, n + 1) swap halves so that
-// the even lane holds both channels of the even tokens and the odd lane those
-// of the odd ones; a store instruction then writes 64 bytes of two tokens
-// instead of one, and half as many are issued.
+// Where an epilogue warp takes its results: a 32-token x 32-channel box of C,
+// staged in shared memory (2 KB for 16-bit results, 4 KB for fp32) and handed
+// to the TMA unit, which clips it at C's edges; or, where C or its pitch is not
+// 16-byte aligned, stores of single values. Staging takes the addresses and
+// edge checks off the warps: with a store per value an epilogue warp issued
+// about 250 instructions a box, and their issue bound the kernels at small K.
 template <typename T>
-__device__ __forceinline__ void i8_store_chunk(const I8Args &p, const uint32_t (&acc)[32], int m0,
-                                               int64_t n, float sb, float bias,
-                                               const float *scales, bool by_pairs, T *C) {
-  float v[32];
-  const float2 sb2 = make_float2(sb, sb), bias2 = make_float2(bias, bias);
+struct I8Out {
+  const CUtensorMap *map;  // null: stores of single values
+  uint8_t *box;
+  T *C;
+};
+
+// One warp's box: TMEM columns t_cols.. (tokens m0..) of its 32 lanes (channels
+// n0..). `scales`: the tokens' a_scale, in shared memory. b_scale and bias of
+// the lane's channels: sb, bias [k] of channel n0 + lane / 4 + 8 k in the mma
+// layout (16-bit box), [0] of channel n0 + lane otherwise. `release` runs once
+// the columns have been read.
+template <typename T, typename Release>
+__device__ __forceinline__ void i8_finish_box(const I8Args &p, const I8Out<T> &out,
+                                              uint32_t t_cols, int m0, int n0,
+                                              const float (&sb)[4], const float (&bias)[4],
+                                              const float *scales, Release release) {
+  const int lane = threadIdx.x & 31;
+  bool staged = false;
+  if constexpr (sizeof(T) == 2) if (out.map) {
+    staged = true;
+    // mma layout: packed pairs of tokens go to shared memory transposed
+    uint32_t r[2][16];
+    tmem_ld_frag32(t_cols, r[0]);
+    tmem_ld_frag32(t_cols + (16u << 16), r[1]);
+    tmem_wait_ld16x2(r[0], r[1]);
+    release();
+    if (m0 >= p.M) return;
+    float v[32];
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
-    const float4 s = *reinterpret_cast<const float4 *>(scales + j);
-    const float2 x = make_float2(static_cast<float>(static_cast<int>(acc[j])),
-                                 static_cast<float>(static_cast<int>(acc[j + 1])));
-    const float2 y = make_float2(static_cast<float>(static_cast<int>(acc[j + 2])),
-                                 static_cast<float>(static_cast<int>(acc[j + 3])));
-    const float2 u = fma2(mul2(x, make_float2(s.x, s.y)), sb2, bias2);
-    const float2 w = fma2(mul2(y, make_float2(s.z, s.w)), sb2, bias2);
-    v[j] = u.x;
-    v[j + 1] = u.y;
-    v[j + 2] = w.x;
-    v[j + 3] = w.y;
-  }
-  act_array<T>(v, p.act, p.alpha);
-  const int rows = p.M - m0;
-  if constexpr (sizeof(T) == 2) {
-    if (by_pairs) {
-      const uint32_t odd = threadIdx.x & 1u;
-      // byte selectors: the halves sent (the other lane's tokens); then even
-      // lanes take {own low, got low}, {own low, got high}, odd lanes
-      // {got low, own high}, {got high, own high}
-      const uint32_t send = odd ? 0x5410u : 0x7632u;
-      const uint32_t first = odd ? 0x3254u : 0x5410u, second = odd ? 0x3276u : 0x7610u;
-      uint32_t o[16];
+    for (int i = 0; i < 4; ++i) {
+      const float2 s = *reinterpret_cast<const float2 *>(scales + 8 * i + 2 * (lane & 3));
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) {
-        const uint32_t w0 = pack2<T>(v[j], v[j + 1]), w1 = pack2<T>(v[j + 2], v[j + 3]);
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(w0, w1, send), 1);
-        o[j / 2] = __byte_perm(w0, got, first);
-        o[j / 2 + 1] = __byte_perm(w1, got, second);
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t *q = &r[k >> 1][4 * i + 2 * (k & 1)];
+        const float2 x = make_float2(static_cast<float>(static_cast<int>(q[0])),
+                                     static_cast<float>(static_cast<int>(q[1])));
+        const float2 y = fma2(mul2(x, s), make_float2(sb[k], sb[k]), make_float2(bias[k], bias[k]));
+        v[8 * i + 2 * k] = y.x;
+        v[8 * i + 2 * k + 1] = y.y;
       }
-      const int64_t ne = n - odd;
-      const int64_t pitch = 2 * p.ldc;
-      T *c = C + (static_cast<int64_t>(m0) + odd) * p.ldc + ne;
-      if (rows >= 32 && ne + 1 < p.N) {
+    }
+    act_array<T>(v, p.act, p.alpha);
+    if (lane == 0) bulk_wait_group_read<0>();  // the previous box has been read
+    __syncwarp();
+    // lane l addresses row l % 8 of matrix l / 8: token 8 (i + matrix / 2) + row,
+    // 16-byte piece 2 h + matrix % 2, swizzled as the map's 64-byte swizzle
+    const uint32_t base = smem_u32(out.box);
+    const uint32_t row = 8u * (lane >> 4) + (lane & 7), piece = (lane >> 3) & 1u;
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          *reinterpret_cast<uint32_t *>(c + j * pitch) = o[j];
-      } else if (ne < p.N) {
-        const bool both = ne + 1 < p.N;
+    for (int i = 0; i < 4; i += 2)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (2 * j + static_cast<int>(odd) < rows) {
-            if (both) *reinterpret_cast<uint32_t *>(c + j * pitch) = o[j];
-            else *reinterpret_cast<uint16_t *>(c + j * pitch) = static_cast<uint16_t>(o[j]);
-          }
-        }
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t token = 8u * i + row;
+        const uint32_t at = base + token * 64u + (((2u * h + piece) ^ ((token >> 1) & 3u)) << 4);
+        stmatrix_x4_trans(at, pack2<T>(v[8 * i + 4 * h], v[8 * i + 4 * h + 1]),
+                          pack2<T>(v[8 * i + 4 * h + 2], v[8 * i + 4 * h + 3]),
+                          pack2<T>(v[8 * i + 8 + 4 * h], v[8 * i + 8 + 4 * h + 1]),
+                          pack2<T>(v[8 * i + 8 + 4 * h + 2], v[8 * i + 8 + 4 * h + 3]));
+      }
+  }
+  if (!staged) {
+    uint32_t r[32];
+    tmem_ld32(t_cols, r);
+    tmem_wait_ld(r);
+    release();
+    if (m0 >= p.M) return;
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float2 x = make_float2(static_cast<float>(static_cast<int>(r[j])),
+                                   static_cast<float>(static_cast<int>(r[j + 1])));
+      const float2 y = fma2(mul2(x, *reinterpret_cast<const float2 *>(scales + j)),
+                            make_float2(sb[0], sb[0]), make_float2(bias[0], bias[0]));
+      v[j] = y.x;
+      v[j + 1] = y.y;
+    }
+    act_array<T>(v, p.act, p.alpha);
+    if (!out.map) {
+      const int64_t n = static_cast<int64_t>(n0) + lane;
+      const int rows = p.M - m0;
+      T *c = out.C + static_cast<int64_t>(m0) * p.ldc + n;
+      if (n >= p.N) return;
+      if (rows >= 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) c[j * p.ldc] = from_float<T>(v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < rows) c[j * p.ldc] = from_float<T>(v[j]);
       }
       return;
     }
+    if (lane == 0) bulk_wait_group_read<0>();
+    __syncwarp();
+    float *box = reinterpret_cast<float *>(out.box);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) box[32 * j + lane] = v[j];
   }
-  if (n >= p.N) return;
-  T *c = C + static_cast<int64_t>(m0) * p.ldc + n;
-  if (rows >= 32) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (n0 < p.N) tma_store_2d(out.map, out.box, n0, m0);
+    bulk_commit_group();
+  }
+}
+
+// b_scale and bias of a lane's channels as i8_finish_box takes them.
+template <typename T>
+__device__ __forceinline__ void i8_channel_scales(const I8Args &p, bool boxes, int n0,
+                                                  float (&sb)[4], float (&bias)[4]) {
+  const int lane = threadIdx.x & 31;
+  const bool frag = sizeof(T) == 2 && boxes;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) c[j * p.ldc] = from_float<T>(v[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < rows) c[j * p.ldc] = from_float<T>(v[j]);
+  for (int k = 0; k < 4; ++k) {
+    const int64_t n = static_cast<int64_t>(n0) + (frag ? (lane >> 2) + 8 * k : lane);
+    const bool in = n < p.N && (frag || k == 0);
+    sb[k] = in ? p.b_scale[n] : 0.0f;
+    bias[k] = in && p.bias ? p.bias[n] : 0.0f;
   }
 }
 
 // ---------------------------------------------------------------------------
 // split: one 128-channel x MT-token tile per cluster of S CTAs, CTA r taking
-// its share of the K blocks. TMA producer, MMA issuer, 8 epilogue warps (two
-// per lane quadrant, every second 32 tokens each: one warp per scheduler alone
-// would wait out every latency of the epilogue). With S > 1 each CTA lays its partial sums in its own shared
+// its share of the K blocks. TMA producer, MMA issuer, 8 epilogue warps
+// (two per lane quadrant, every second 32 tokens each: one warp per scheduler
+// alone would wait out every latency of the epilogue; 16 warps took 1 us more a
+// launch, since two CTAs of successive launches no longer fit one SM). With S > 1 each CTA lays its partial sums in its own shared
 // memory ([token][channel], over the stages, which are read out by then), and
 // CTA r adds tokens [r MT / S, (r + 1) MT / S) of all S CTAs.
 // ---------------------------------------------------------------------------
-constexpr int kSplitThreads = 64 + 8 * 32;
+constexpr int kSplitEpiWarps = 8;
+constexpr int kSplitThreads = 64 + kSplitEpiWarps * 32;
 
 template <int MT>
 struct SplitTraits {
@@ -360,9 +394,10 @@ struct SplitTraits {
   static constexpr int kPartialBytes = MT * kI8Channels * 4;  // over the stages
   // Shared memory after the stages: barriers, then the epilogue warps' scales.
   static constexpr int kTailBytes = 256 + MT * 4;
+  static constexpr int kBoxBytes = kSplitEpiWarps * 4096;  // over the stages
   static constexpr int smem_bytes(int stages, bool partials) {
-    const int area = stages * kStageBytes;
-    return 1024 + (partials && area < kPartialBytes ? kPartialBytes : area) + kTailBytes;
+    const int area = stages * kStageBytes, least = partials ? kPartialBytes : kBoxBytes;
+    return 1024 + (area < least ? least : area) + kTailBytes;
   }
   static_assert(1024 + kMostStages * kStageBytes + kTailBytes <= 232448, "shared memory budget");
 };
@@ -372,7 +407,8 @@ struct SplitTraits {
 template <int MT, int S, typename T>
 __device__ __forceinline__ void i8_add_slices(const I8Args &p, const uint8_t *part, int rank,
                                               int n0, int m0, T *C) {
-  constexpr int kPer = MT / S, kBatch = kPer / 8 < 1 ? 1 : kPer / 8 < 4 ? kPer / 8 : 4;
+  constexpr int kPer = MT / S, kEach = kPer / kSplitEpiWarps,
+                kBatch = kEach < 1 ? 1 : kEach < 4 ? kEach : 4;
   const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - 2;
   const int64_t n = static_cast<int64_t>(n0) + 4 * lane;
   float sb[4], bias[4];
@@ -384,7 +420,7 @@ __device__ __forceinline__ void i8_add_slices(const I8Args &p, const uint8_t *pa
   const bool whole = n + 4 <= p.N && p.ldc % 4 == 0 &&
                      reinterpret_cast<uintptr_t>(C) % (4 * sizeof(T)) == 0;
 #pragma unroll 1
-  for (int i = w * kBatch; i < kPer; i += 8 * kBatch) {
+  for (int i = w * kBatch; i < kPer; i += kSplitEpiWarps * kBatch) {
     const int tok = rank * kPer + i;
     if (m0 + tok >= p.M) break;
     uint4 v[kBatch][S];  // all loads first: a round trip to another SM each
@@ -425,10 +461,11 @@ __device__ __forceinline__ void i8_add_slices(const I8Args &p, const uint8_t *pa
 }
 
 template <int MT, typename T>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kSplitThreads, 2)
     gemm_i8_split_kernel(const __grid_constant__ CUtensorMap map_w,
-                         const __grid_constant__ CUtensorMap map_x, const I8Args p, T *C,
-                         int slices, int n_tiles, int stages, int area) {
+                         const __grid_constant__ CUtensorMap map_x,
+                         const __grid_constant__ CUtensorMap map_c, const I8Args p, T *C,
+                         int boxes, int slices, int n_tiles, int stages, int area) {
   using S = SplitTraits<MT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align_smem_1024(smem_raw);
@@ -523,31 +560,29 @@ __global__ void __launch_bounds__(kSplitThreads)
     }
     __syncwarp();
   } else {
-    const int64_t n = static_cast<int64_t>(n0) + ch;
-    const float sb = n < p.N ? p.b_scale[n] : 0.0f;
-    const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
     const int c_first = (warp - 2) / 4 * 32;
-    const bool by_pairs = i8_by_pairs(p, C);
+    float sb[4], bias[4];
     if (slices == 1) {
-      for (int i = threadIdx.x - 64; i < MT; i += 256)
+      i8_channel_scales<T>(p, boxes, n0 + quad * 32, sb, bias);
+      for (int i = threadIdx.x - 64; i < MT; i += kSplitEpiWarps * 32)
         scales[i] = m0 + i < p.M ? p.a_scale[m0 + i] : 0.0f;
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // the epilogue warps
+      asm volatile("bar.sync 1, %0;" ::"n"(kSplitEpiWarps * 32) : "memory");  // epilogue warps
     }
     have = mbar_wait(acc_full, 0u, abort_flag, p.status, kStatusTimeoutEpilogue);
     __syncwarp();
     tc_fence_after_sync();
     if (have && slices == 1) {
+      // boxes over the stages, which the MMAs have read out
+      const I8Out<T> out{boxes ? &map_c : nullptr, smem + (warp - 2) * 4096, C};
 #pragma unroll 1
-      for (int c0 = c_first; c0 < MT && m0 + c0 < p.M; c0 += 64) {
-        uint32_t acc[32];
-        tmem_ld32(t_row + c0, acc);
-        tmem_wait_ld(acc);
-        i8_store_chunk<T>(p, acc, m0 + c0, n, sb, bias, scales + c0, by_pairs, C);
-      }
+      for (int c0 = c_first; c0 < MT && m0 + c0 < p.M; c0 += kSplitEpiWarps * 8)
+        i8_finish_box<T>(p, out, t_row + c0, m0 + c0, n0 + quad * 32, sb, bias, scales + c0, [] {});
+      if (boxes && lane == 0) bulk_wait_group_read<0>();  // the boxes outlive their stores
+      __syncwarp();
     } else if (have) {
       int *part = reinterpret_cast<int *>(smem);
 #pragma unroll 1
-      for (int c0 = c_first; c0 < MT; c0 += 64) {
+      for (int c0 = c_first; c0 < MT; c0 += kSplitEpiWarps * 8) {
         uint32_t acc[32];
         tmem_ld32(t_row + c0, acc);
         tmem_wait_ld(acc);
@@ -566,7 +601,7 @@ __global__ void __launch_bounds__(kSplitThreads)
       else i8_add_slices<MT, 8, T>(p, smem, rank, n0, m0, C);
     }
     __syncwarp();
-    cluster_sync();  // no CTA leaves while another reads its shared memory
+    cluster_sync_relaxed();  // no CTA leaves while another reads its shared memory
   }
   __syncthreads();
   if (warp == 1) {
@@ -585,39 +620,65 @@ __global__ void __launch_bounds__(kSplitThreads)
 //   empty, acc_full     in each CTA, by the leader's commit to both
 //   acc_empty (leader)  16 arrivals: the 8 epilogue warps of each CTA
 // ---------------------------------------------------------------------------
-constexpr int kPairTokens = 256, kPairStages = 6, kPairEpiWarps = 8;
+constexpr int kPairTokens = 256, kPairEpiWarps = 8;
+constexpr int kPairSpan = kPairTokens / (kPairEpiWarps / 4);  // tokens of an epilogue warp
 constexpr int kPairStage = kI8WeightBytes + kPairTokens / 2 * kI8BK;
 constexpr int kPairThreads = 64 + kPairEpiWarps * 32;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256 + kPairEpiWarps * 128 * 4;
-static_assert(kPairSmem <= 232448, "shared memory budget");
+// After the stages: the epilogue warps' boxes and scales, the barriers.
+template <typename T>
+struct PairTraits {
+  static constexpr int kStages = sizeof(T) == 2 ? 6 : 5;
+  static constexpr int kBox = 32 * 32 * static_cast<int>(sizeof(T));
+  static constexpr int kScaleBytes = kPairEpiWarps * kPairSpan * 4;
+  static constexpr int kSmemBytes =
+      1024 + kStages * kPairStage + kPairEpiWarps * kBox + kScaleBytes + 256;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
 
-// Groups of 8 channel tiles sweep all token tiles, so that the pairs at work
-// at one time share operand rows in L2.
-__device__ __forceinline__ void pair_tile(int tile, int n_tiles, int m_tiles, int &nt, int &mt) {
-  constexpr int kGroup = 8;
-  const int group = tile / (kGroup * m_tiles);
-  const int first = group * kGroup;
-  const int size = min(n_tiles - first, kGroup);
-  const int local = tile - group * kGroup * m_tiles;
-  nt = first + local % size;
-  mt = local / size;
+// Tile order: groups of 8 channel tiles sweep all token tiles, so that the
+// pairs at work at one time share operand rows in L2.
+struct PairOrder {
+  int tiles, full_tiles;  // all; those of the groups of 8
+  FastDiv per_group;      // 8 * token tiles
+  FastDiv rest;           // channel tiles of the last, smaller group
+};
+
+PairOrder pair_order(int n_tiles, int m_tiles) {
+  PairOrder o;
+  o.tiles = n_tiles * m_tiles;
+  o.full_tiles = n_tiles / 8 * 8 * m_tiles;
+  o.per_group = make_fastdiv(static_cast<uint32_t>(8 * m_tiles));
+  o.rest = make_fastdiv(static_cast<uint32_t>(n_tiles % 8 ? n_tiles % 8 : 1));
+  return o;
+}
+
+__device__ __forceinline__ void pair_tile(const PairOrder &o, int tile, int &nt, int &mt) {
+  const uint32_t group = fdiv(static_cast<uint32_t>(tile), o.per_group);
+  const uint32_t local = static_cast<uint32_t>(tile) - group * o.per_group.d;
+  const uint32_t m = tile < o.full_tiles ? local >> 3 : fdiv(local, o.rest);
+  mt = static_cast<int>(m);
+  nt = static_cast<int>(8 * group + local - m * (tile < o.full_tiles ? 8u : o.rest.d));
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap map_w,
-                        const __grid_constant__ CUtensorMap map_x, const I8Args p, T *C,
-                        int n_tiles, int m_tiles) {
+                        const __grid_constant__ CUtensorMap map_x,
+                        const __grid_constant__ CUtensorMap map_c, const I8Args p, T *C,
+                        int boxes, const PairOrder order) {
+  using Tr = PairTraits<T>;
+  constexpr int kPairStages = Tr::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align_smem_1024(smem_raw);
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kPairStages * kPairStage);
+  uint8_t *box_area = smem + kPairStages * kPairStage;
+  float *scales = reinterpret_cast<float *>(box_area + kPairEpiWarps * Tr::kBox);
+  uint64_t *full = reinterpret_cast<uint64_t *>(scales + kPairEpiWarps * kPairSpan);
   uint64_t *empty = full + kPairStages;
   uint64_t *acc_full = empty + kPairStages;
   uint64_t *acc_empty = acc_full + 2;
   uint64_t *never = acc_empty + 2;  // never arrived on (injected_stall)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(never + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  float *scales = reinterpret_cast<float *>(smem + kPairStages * kPairStage + 256);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -649,7 +710,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   griddep_wait();
   griddep_launch_dependents();
 
-  const int tiles = n_tiles * m_tiles;
+  const int tiles = order.tiles;
   const int pairs = static_cast<int>(gridDim.x >> 1), pair = static_cast<int>(blockIdx.x >> 1);
   const int blocks = (p.K + kI8BK - 1) / kI8BK;
 
@@ -661,11 +722,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       bool aborted = false;
       for (int tile = pair; tile < tiles && !aborted; tile += pairs) {
         int nt, mt;
-        pair_tile(tile, n_tiles, m_tiles, nt, mt);
+        pair_tile(order, tile, nt, mt);
         const int row_w = nt * 2 * kI8Channels + static_cast<int>(rank) * kI8Channels;
         const int row_x = mt * kPairTokens + static_cast<int>(rank) * (kPairTokens / 2);
         for (int kb = 0; kb < blocks; ++kb) {
-          if (!mbar_wait_pair(&empty[stage], phase ^ 1u, abort_flag, peer_abort, p.status,
+          if (!mbar_wait_pair_async(&empty[stage], phase ^ 1u, abort_flag, peer_abort, p.status,
                               kStatusTimeoutProducer)) {
             aborted = true;
             break;
@@ -704,13 +765,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!go) pair_raise_abort(peer_abort);
       for (int tile = pair; go && tile < tiles; tile += pairs, ++local) {
         const int acc = local & 1;
-        go = mbar_wait_pair(&acc_empty[acc], ((local >> 1) & 1) ^ 1u, abort_flag, peer_abort,
+        go = mbar_wait_pair_async(&acc_empty[acc], ((local >> 1) & 1) ^ 1u, abort_flag, peer_abort,
                             p.status, kStatusTimeoutAccFree);
         if (!go) break;
         tc_fence_after_sync();
         const uint32_t d = tmem_base + acc * kPairTokens;
         for (int kb = 0; kb < blocks; ++kb) {
-          go = mbar_wait_pair(&full[stage], phase, abort_flag, peer_abort, p.status,
+          go = mbar_wait_pair_async(&full[stage], phase, abort_flag, peer_abort, p.status,
                               kStatusTimeoutMma);
           if (!go) break;
           tc_fence_after_sync();
@@ -729,41 +790,44 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
   } else {
-    // ---------------- epilogue: 2 warps per lane quadrant, half the tokens each ----------------
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    float *mine = scales + (warp - 2) * 128;
-    const bool by_pairs = i8_by_pairs(p, C);
+    // ---------------- epilogue: the two warps of a lane quadrant share the tokens ----------------
+    const int quad = warp & 3, part = (warp - 2) >> 2;
+    float *mine = scales + (warp - 2) * kPairSpan;
+    const I8Out<T> out{boxes ? &map_c : nullptr, box_area + (warp - 2) * Tr::kBox, C};
     int local = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++local) {
       int nt, mt;
-      pair_tile(tile, n_tiles, m_tiles, nt, mt);
-      const int64_t n = static_cast<int64_t>(nt) * 2 * kI8Channels + rank * kI8Channels +
-                        quad * 32 + lane;
-      const float sb = n < p.N ? p.b_scale[n] : 0.0f;
-      const float bias = p.bias && n < p.N ? p.bias[n] : 0.0f;
-      const int acc = local & 1, m0 = mt * kPairTokens + half * 128;
-      i8_stage_scales(p, m0, 128, mine);
-      if (!mbar_wait_pair(&acc_full[acc], (local >> 1) & 1, abort_flag, peer_abort, p.status,
-                          kStatusTimeoutEpilogue))
+      pair_tile(order, tile, nt, mt);
+      const int n0 = nt * 2 * kI8Channels + static_cast<int>(rank) * kI8Channels + quad * 32;
+      const int acc = local & 1, m0 = mt * kPairTokens + part * kPairSpan;
+      float sb[4], bias[4];
+      i8_channel_scales<T>(p, boxes, n0, sb, bias);
+      __syncwarp();  // the previous tile's scales have been read
+#pragma unroll
+      for (int i = 0; i < kPairSpan; i += 32)
+        mine[i + lane] = m0 + i + lane < p.M ? p.a_scale[m0 + i + lane] : 0.0f;
+      __syncwarp();
+      if (!mbar_wait_pair_async(&acc_full[acc], (local >> 1) & 1, abort_flag, peer_abort,
+                                p.status, kStatusTimeoutEpilogue))
         break;
       __syncwarp();
       tc_fence_after_sync();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
-                             static_cast<uint32_t>(acc * kPairTokens + half * 128);
+                             static_cast<uint32_t>(acc * kPairTokens + part * kPairSpan);
 #pragma unroll 1
-      for (int c0 = 0; c0 < 128 && m0 + c0 < p.M; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(t_row + c0, v);
-        tmem_wait_ld(v);
-        i8_store_chunk<T>(p, v, m0 + c0, n, sb, bias, mine + c0, by_pairs, C);
-      }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0u));
+      for (int c0 = 0; c0 < kPairSpan; c0 += 32)
+        i8_finish_box<T>(p, out, t_row + c0, m0 + c0, n0, sb, bias, mine + c0, [&] {
+          if (c0 + 32 == kPairSpan) {  // the accumulator has been read: hand it back
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_tmem_read(mapa_shared(smem_u32(&acc_empty[acc]), 0u));
+          }
+        });
     }
+    if (boxes && lane == 0) bulk_wait_group_read<0>();  // the boxes outlive their stores
   }
   __syncthreads();
-  cluster_sync();  // no remote arrival, copy or MMA into either CTA is left
+  cluster_sync_relaxed();  // no remote arrival, copy or MMA into either CTA is left
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc_pair(tmem_base, 512);
@@ -780,27 +844,59 @@ struct I8Plan {
   int mt, slices;
 };
 
+template <int MT>
+constexpr int split_smem(int stages, bool partials) {
+  return SplitTraits<MT>::smem_bytes(stages, partials);
+}
+
+int split_smem(int mt, int stages, bool partials) {
+  return mt == 32    ? split_smem<32>(stages, partials)
+         : mt == 64  ? split_smem<64>(stages, partials)
+         : mt == 128 ? split_smem<128>(stages, partials)
+                     : split_smem<256>(stages, partials);
+}
+
+int split_stages(int mt, int64_t blocks) {
+  const int most = mt >= 256 ? SplitTraits<256>::kMostStages
+                   : mt >= 128 ? SplitTraits<128>::kMostStages
+                   : mt >= 64  ? SplitTraits<64>::kMostStages
+                               : SplitTraits<32>::kMostStages;
+  return static_cast<int>(std::min<int64_t>(blocks, most));
+}
+
+// The rows kernel up to 8 tokens, and up to 16 while all its CTAs (two per SM)
+// are at work at once: 16 tokens, N = K = 4096: 6.2 us against 7.0 (split); N =
+// 11008: 13.4 against 11.2. Otherwise the tile and K split of least estimated
+// time. The estimates (microseconds on 148 SMs) are a fit to 777 timings of 114
+// sizes, 1 to 8192 tokens, 45 to 16384 channels, K from 67 to 16384 (rms error
+// 17%); the choice they make took 2% longer than the best one on average and
+// 34% at worst (77 x 1280 x 1024: 5.0 us against 3.8).
+//   split: waves * (start and end + K blocks * (latency or the bytes that the
+//          CTAs of an SM share) + results) + adding the slices
+//   pair:  start + rounds * max(K blocks, epilogue) + the shorter of the two
 I8Plan choose_plan(int64_t M, int64_t N, int64_t K, bool aligned) {
   if (!aligned) return {I8Kernel::kBytes, 0, 0};
-  if (M <= 16) return {I8Kernel::kRows, 0, 0};
   const int64_t sms = sm_count(), blocks = ceil_div(K, kI8BK);
-  // Clocks, from the bytes each SM takes from L2 (about 40 a clock with all SMs
-  // at work) and a fixed cost per tile.
-  const double per_byte = 1.0 / 40;
+  if (M <= 8 || (M <= 16 && ceil_div(N, 16) <= 2 * sms)) return {I8Kernel::kRows, 0, 0};
+  const double main_us = 0.31 * static_cast<double>(blocks), end_us = 3.3;
+  const int64_t rounds = ceil_div(ceil_div(N, 256) * ceil_div(M, kPairTokens), sms / 2);
   I8Plan best{I8Kernel::kPair, 0, 0};
-  double least = static_cast<double>(ceil_div(ceil_div(N, 256) * ceil_div(M, kPairTokens), sms / 2)) *
-                     blocks * kPairStage * per_byte +
-                 5000;
+  double least = 1.1 + static_cast<double>(rounds) * std::max(main_us, end_us) +
+                 std::min(main_us, end_us);
   for (int mt : {32, 64, 128, 256}) {
     for (int s : {1, 2, 4, 8}) {
       if (s > blocks || (mt == 256 && s > 1)) continue;
+      const int64_t each = ceil_div(blocks, s);
       const int64_t ctas = ceil_div(N, kI8Channels) * ceil_div(M, mt) * s;
-      const double cost =
-          static_cast<double>(ceil_div(ctas, sms)) *
-          (3000 + (s > 1 ? 1000 : 0) +
-           static_cast<double>(ceil_div(blocks, s)) * (kI8Channels + mt) * kI8BK * per_byte);
-      if (cost < least) {
-        least = cost;
+      const int fit = 2 * (split_smem(mt, split_stages(mt, each), s > 1) + 1024) <= 228 * 1024 ? 2 : 1;
+      const double share =
+          std::min<double>(fit, std::max(1.0, static_cast<double>(ctas) / static_cast<double>(sms)));
+      const double block_us = std::max(0.25, share * (kI8Channels + mt) * kI8BK * 9.2e-6);
+      const double us = static_cast<double>(ceil_div(ctas, sms * fit)) *
+                            (2.6 + static_cast<double>(each) * block_us + 0.0096 * mt * share) +
+                        (s > 1 ? 0.1 + 0.015 * mt : 0.0);
+      if (us < least) {
+        least = us;
         best = {I8Kernel::kSplit, mt, s};
       }
     }
@@ -808,9 +904,9 @@ I8Plan choose_plan(int64_t M, int64_t N, int64_t K, bool aligned) {
   return best;
 }
 
-int launch_cluster(cudaStream_t s, const void *fn, cudaLaunchConfig_t &cfg, unsigned cluster,
-                   cudaLaunchAttribute (&attr)[2]) {
-  (void)fn;
+// Launch attributes: programmatic serialization, and clusters of `cluster` CTAs.
+void set_launch(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&attr)[2], cudaStream_t s,
+                unsigned cluster) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -820,22 +916,29 @@ int launch_cluster(cudaStream_t s, const void *fn, cudaLaunchConfig_t &cfg, unsi
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   cfg.stream = s;
-  return kOk;
+}
+
+// Whether the TMA unit can store into C.
+template <typename T>
+bool i8_boxes(const I8Args &p, const T *C) {
+  return reinterpret_cast<uintptr_t>(C) % 16 == 0 && p.ldc * sizeof(T) % 16 == 0;
 }
 
 template <int MT, typename T>
 int launch_split(cudaStream_t s, const I8Args &p, T *C, int slices) {
   using Tr = SplitTraits<MT>;
-  CUtensorMap mw, mx;
+  CUtensorMap mw, mx, mc = {};
   int rc = encode_tmap_2d_u8_sw128(&mw, p.B, p.K, p.N, p.ldb, kI8Channels);
   if (rc) return rc;
   rc = encode_tmap_2d_u8_sw128(&mx, p.A, p.K, p.M, p.lda, MT);
   if (rc) return rc;
+  const bool boxes = slices == 1 && i8_boxes(p, C);
+  if (boxes) rc = encode_tmap_2d_box32(&mc, C, p.N, p.M, p.ldc * sizeof(T), sizeof(T));
+  if (rc) return rc;
   auto *fn = gemm_i8_split_kernel<MT, T>;
   // As many stages as a CTA has K blocks, up to the limit: with a short K
   // several CTAs share an SM, and one's loads run under another's stores.
-  const int blocks = static_cast<int>(ceil_div(ceil_div(p.K, kI8BK), slices));
-  const int stages = std::min(blocks, Tr::kMostStages);
+  const int stages = split_stages(MT, ceil_div(ceil_div(p.K, kI8BK), slices));
   const int smem = Tr::smem_bytes(stages, slices > 1);
   rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), smem);
   if (rc) return rc;
@@ -847,36 +950,40 @@ int launch_split(cudaStream_t s, const I8Args &p, T *C, int slices) {
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kSplitThreads);
   cfg.dynamicSmemBytes = smem;
-  launch_cluster(s, nullptr, cfg, static_cast<unsigned>(slices), attr);
+  set_launch(cfg, attr, s, static_cast<unsigned>(slices));
   count_launch();
-  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, p, C, slices, n_tiles, stages,
-                                           smem - 1024 - Tr::kTailBytes));
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, mc, p, C, boxes ? 1 : 0, slices, n_tiles,
+                                           stages, smem - 1024 - Tr::kTailBytes));
 }
 
 template <typename T>
 int launch_pair(cudaStream_t s, const I8Args &p, T *C) {
-  CUtensorMap mw, mx;
+  CUtensorMap mw, mx, mc = {};
   int rc = encode_tmap_2d_u8_sw128(&mw, p.B, p.K, p.N, p.ldb, kI8Channels);
   if (rc) return rc;
   rc = encode_tmap_2d_u8_sw128(&mx, p.A, p.K, p.M, p.lda, kPairTokens / 2);
   if (rc) return rc;
+  const bool boxes = i8_boxes(p, C);
+  if (boxes) rc = encode_tmap_2d_box32(&mc, C, p.N, p.M, p.ldc * sizeof(T), sizeof(T));
+  if (rc) return rc;
   auto *fn = gemm_i8_pair_kernel<T>;
-  rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), kPairSmem);
+  rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), PairTraits<T>::kSmemBytes);
   if (rc) return rc;
   const int64_t n_tiles = ceil_div(p.N, 2 * kI8Channels), m_tiles = ceil_div(p.M, kPairTokens);
-  if (n_tiles * m_tiles >= (int64_t(1) << 30)) return kErrUnsupported;
+  if (n_tiles * m_tiles >= (int64_t(1) << 27)) return kErrUnsupported;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
-  launch_cluster(s, nullptr, cfg, 2, attr);
+  cfg.dynamicSmemBytes = PairTraits<T>::kSmemBytes;
+  set_launch(cfg, attr, s, 2);
   // A grid beyond the pairs that fit at once would still be right (no pair
   // waits for another); all of them at once is what the tile order counts on.
   const int64_t fit = sm_count() / 2;
   cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(n_tiles * m_tiles, fit)));
   count_launch();
-  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, p, C, static_cast<int>(n_tiles),
-                                           static_cast<int>(m_tiles)));
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, mc, p, C, boxes ? 1 : 0,
+                                           pair_order(static_cast<int>(n_tiles),
+                                                      static_cast<int>(m_tiles))));
 }
 
 template <typename T>

@@ -67,6 +67,12 @@ int encode_tmap_2d_f32_sw128_atom32(CUtensorMap *map, const void *base, uint64_t
 int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
                             uint64_t row_pitch_bytes, uint32_t box_outer);
 
+// 2-D map for tensor stores of 32 x 32 boxes of 2- or 4-byte elements: dims
+// {inner, outer} elements, row pitch in bytes; 2-byte boxes (rows of 64 bytes)
+// with the 64-byte swizzle, 4-byte boxes unswizzled.
+int encode_tmap_2d_box32(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer,
+                         uint64_t row_pitch_bytes, int element_bytes);
+
 // 4-D NHWC fp32 im2col tensor map (dims {c, w, h, n}, densely packed): each
 // load gathers `pixels` output pixels x `channels` channels, walking the
 // bounding box [lower, dim-1+upper] of every image with the given traversal

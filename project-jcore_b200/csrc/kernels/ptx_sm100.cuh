@@ -371,6 +371,34 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
                : "memory");
 }
 
+// 32 consecutive 32-bit TMEM columns of 16 lanes (16x256b shape, warp-
+// collective; taddr names the first lane, 0 or 16 of the warp's quadrant), laid
+// out as mma.sync accumulators: with g = lane / 4, t = lane % 4, registers 4i
+// and 4i + 1 hold columns 8i + 2t, 8i + 2t + 1 of TMEM lane g, registers 4i + 2
+// and 4i + 3 those of TMEM lane g + 8. Valid after a tcgen05.wait::ld.
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Four 8x8 matrices of 16-bit values, transposed, into shared memory: lane l
+// gives the address of the 16 bytes of stored row l % 8 of matrix l / 8, which
+// receives column l % 8 of that matrix (register q: row lane / 4, columns
+// 2 (lane % 4) and + 1 of matrix q).
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t smem_addr, uint32_t r0, uint32_t r1,
+                                                  uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                   smem_addr),
+               "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+               : "memory");
+}
+
 // 16-column variant of tmem_ld32 (32x32b.x16).
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -481,6 +509,36 @@ __device__ __forceinline__ bool mbar_wait_pair(uint64_t *bar, uint32_t parity,
   }
 }
 
+// The same for barriers on which only TMA copies, MMA commits and threads that
+// hand back TMEM arrive: what they announce is not in the generic proxy's
+// memory, so nothing has to be made visible at cluster scope (which would
+// invalidate L1 at each wait).
+__device__ __forceinline__ bool mbar_wait_pair_async(uint64_t *bar, uint32_t parity,
+                                                     volatile int *abort, uint32_t peer_abort,
+                                                     int *status, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 31u) == 0u) {
+      if (*abort) return false;
+      if (global_timer_ns() - t0 > kWaitLimitNs) {
+        *abort = 1;
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_abort), "r"(1) : "memory");
+        atomicCAS(status, 0, code);
+        return false;
+      }
+    }
+  }
+}
+
+// Arrives once on an mbarrier of either CTA (a shared::cluster address) to hand
+// back TMEM that this warp has read (tcgen05.wait::ld done): no write of this
+// thread is released, so its global stores in flight are not waited for.
+__device__ __forceinline__ void mbar_arrive_tmem_read(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // Raises the peer CTA's abort flag (shared::cluster address).
 __device__ __forceinline__ void pair_raise_abort(uint32_t peer_abort) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_abort), "r"(1) : "memory");
@@ -490,6 +548,12 @@ __device__ __forceinline__ void pair_raise_abort(uint32_t peer_abort) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
                ::: "memory");
+}
+
+// The same without ordering any memory: all threads of both CTAs are here.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::
+                   : "memory");
 }
 
 // TMEM allocation for a CTA pair: the same warp of both CTAs executes it and
