@@ -354,7 +354,7 @@ NPL_API int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw, in
 
 /* ---- dropout ------------------------------------------------------------------ */
 /* y[i] = x[i] * 65536 / (65536 - t) where r(i) >= t, else 0, for n elements of
- * type `dtype`: t = p * 65536 rounded to the nearest integer (p in [0, 1]; t ==
+ & to the nearest integer (p in [0, 1]; t ==
  * 65536 gives all zeros) and r(i) 16 random bits that depend on seed and
  * offset + i only. The mask is never stored: the gradient is the same call on
  * dy. In place (y == x) allowed; a dropped NaN or infinity gives 0. r(i) is the

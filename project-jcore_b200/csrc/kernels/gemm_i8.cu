@@ -229,23 +229,6 @@ __global__ void __launch_bounds__(kRowsWarps * 32) gemm_i8_rows_kernel(I8Args p,
 // ---------------------------------------------------------------------------
 constexpr int kI8BK = 128, kI8Channels = 128, kI8WeightBytes = kI8Channels * kI8BK;
 
-// (a0, a1) * (b0, b1) and (a0, a1) * (b0, b1) + (c0, c1), two fp32 products an instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(r)
-      : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
-  return reinterpret_cast<const float2 &>(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(r)
-      : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)),
-        "l"(reinterpret_cast<const uint64_t &>(c)));
-  return reinterpret_cast<const float2 &>(r);
-}
-
 // Where an epilogue warp takes its results: a 32-token x 32-channel box of C,
 // staged in shared memory (2 KB for 16-bit results, 4 KB for fp32) and handed
 // to the TMA unit, which clips it at C's edges; or, where C or its pitch is not

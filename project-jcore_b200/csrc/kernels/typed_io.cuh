@@ -72,6 +72,23 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   return reinterpret_cast<const uint32_t &>(h);
 }
 
+// (a0, a1) * (b0, b1) and (a0, a1) * (b0, b1) + (c0, c1), two fp32 products an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+  return reinterpret_cast<const float2 &>(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)),
+        "l"(reinterpret_cast<const uint64_t &>(c)));
+  return reinterpret_cast<const float2 &>(r);
+}
+
 // Loads with no reuse in L1 (each value is read once by one thread). Not the
 // non-coherent path: the destination may be the source.
 template <typename T, int V>
