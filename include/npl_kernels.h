@@ -319,7 +319,8 @@ NPL_API int nplk_binary(void *stream, int op, int64_t n, const float *a, const f
  * y is rounded once. y may be x itself (then ldy == ldx). A NaN or an infinity
  * makes its group NaN and no other.
  *
- * Sizes: c a multiple of groups, c / groups <= 8192, hw < 2^31, n < 2^31; else
+ * Sizes: c a multiple of groups, c / groups <= 8192, c <= 2^24, hw < 2^31 and
+ * n * groups < 2^31; else
  * NPL_ERR_INVALID_ARG (not a multiple, a size < 1) or NPL_ERR_UNSUPPORTED (too
  * large). All alignments of an element's own size are taken; 16-byte aligned
  * pointers with ldx, ldy and c multiples of 16 bytes are the fastest.

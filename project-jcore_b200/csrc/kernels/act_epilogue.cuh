@@ -4,6 +4,7 @@
 
 #include <type_traits>
 
+#include "activation_grad.cuh"
 #include "nplk_device.cuh"
 
 namespace nplk {
@@ -53,6 +54,51 @@ __device__ __forceinline__ void act_array(float (&v)[V], int act, float alpha) {
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] = act_call(v[j], act, alpha);
+}
+
+static __device__ __noinline__ float act_slope_call(float x, int act, float alpha) {
+  return act_slope(x, act, alpha);
+}
+
+// v[j] = act'(v[j]), for gradients stored as T; 16-bit results as above.
+template <typename T, int V>
+__device__ __forceinline__ void act_slope_array(float (&v)[V], int act, float alpha) {
+  constexpr bool kFast = !std::is_same<T, float>::value;
+  switch (act) {
+    case 0:
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = 1.0f;
+      return;
+    case 1:
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = v[j] > 0.0f ? 1.0f : 0.0f;
+      return;
+    case 5:
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float x = v[j], x2 = x * x;
+        const float c = 2.0f * 0.7978845608f, k = c * 0.044715f;
+        if (kFast) {
+          const float s = __fdividef(1.0f, 1.0f + __expf(-x * fmaf(k, x2, c)));
+          v[j] = s + x * s * (1.0f - s) * fmaf(3.0f * k, x2, c);
+        } else {
+          v[j] = act_slope(x, 5, alpha);
+        }
+      }
+      return;
+    case 6:
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float x = v[j];
+        const float s = kFast ? __fdividef(1.0f, 1.0f + __expf(-x)) : 1.0f / (1.0f + expf(-x));
+        v[j] = s * fmaf(x, 1.0f - s, 1.0f);
+      }
+      return;
+    default:
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = act_slope_call(v[j], act, alpha);
+      return;
+  }
 }
 
 }  // namespace nplk

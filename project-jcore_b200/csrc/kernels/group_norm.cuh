@@ -1,0 +1,254 @@
+// What the group norm kernels share: the work split and its plan.
+//
+// An image's channels are cut into strips of whole groups; a cluster of CTAs
+// takes one strip of one image (or a run of its rows), each CTA a run of rows.
+// In a CTA, a row's strip is nv packs of V channels; thread t has pack t % nv
+// of rows t / nv, t / nv + lanes, ... (lanes = threads / nv), so that a
+// thread's channels never change and consecutive threads read consecutive
+// memory. A strip of more packs than threads takes several turns (lanes = 1).
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "nplk_device.cuh"
+#include "nplk_host.h"
+#include "ptx_sm100.cuh"
+#include "typed_io.cuh"
+
+namespace nplk {
+
+struct NormGeom {
+  int64_t ldx, ldy, lddy;  // pitches of x, of the output, of dy
+  uint32_t hw;
+  int c, groups, cg;
+  int gs, strips;       // groups of a strip; strips of an image
+  int slices;           // CTAs of a cluster
+  int chunks;           // clusters that share a strip's rows
+  uint32_t cta_rows;    // rows of a CTA
+  FastDiv div_cg;
+  const float *gamma, *beta;
+  float eps, alpha;
+  int act;
+};
+
+struct NormPlan {
+  NormGeom g;
+  int v;            // elements of a pack
+  bool keep;        // the strip stays in the cluster's shared memory
+  int threads;
+  int64_t batch;    // images of a launch
+  int apply_chunks; // second pass: CTAs per image and strip
+};
+
+// Workspace: per image and chunk, sums per channel and group.
+constexpr int kNormMostChunks = 74;
+inline int64_t norm_most_chunks(int64_t hw) {
+  const int64_t by_rows = ceil_div(hw, 64);
+  return by_rows < kNormMostChunks ? by_rows : kNormMostChunks;
+}
+
+// Floats of shared memory beside the kept strips (norm_smem below).
+inline int norm_tail_bytes(int threads, int v, int cw, int gs) {
+  const int acc = threads * v > cw ? threads * v : cw;  // per row lane and channel
+  const int teams = gs > 32 ? gs : 32;
+  return 2 * acc * 4 + 2 * cw * 4 + teams * 16 + gs * 16 + 2 * gs * 4 + 64;
+}
+
+constexpr int kNormSmemLimit = 227 * 1024;
+
+// `tensors`: strips that the kept form holds (x; or x and dy).
+inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int size, int v_fit,
+                          int tensors) {
+  NormPlan p{};
+  const int cg = static_cast<int>(c / groups);
+  auto gcd = [](int a, int b) {
+    while (b) {
+      const int t = a % b;
+      a = b;
+      b = t;
+    }
+    return a;
+  };
+  // The widest packs that the pointers allow and that fill whole groups within
+  // 8192 channels (v divides c, so v / gcd(v, cg) divides the group count).
+  int v = v_fit;
+  while (v > 1 && (c % v != 0 || v / gcd(v, cg) * cg > 8192)) v /= 2;
+  const int gs0 = v / gcd(v, cg);
+  const int sms = sm_count();
+  p.v = v;
+  p.g.hw = static_cast<uint32_t>(hw);
+  p.g.c = static_cast<int>(c);
+  p.g.groups = static_cast<int>(groups);
+  p.g.cg = cg;
+  p.g.div_cg = make_fastdiv(static_cast<uint32_t>(cg));
+
+  // Kept form: narrow strips, at least 64 bytes a row and in whole 32-byte
+  // sectors where a strip of up to 512 bytes is.
+  int gs = gs0;
+  for (int m = gs0; m <= groups; m += gs0) {
+    const int bytes = m * cg * size;
+    if (bytes > 512 && gs * cg * size >= 64) break;
+    gs = m;
+    if (bytes >= 64 && bytes % 32 == 0) break;
+  }
+  p.g.gs = gs;
+  p.g.strips = static_cast<int>(ceil_div(groups, gs));
+  p.g.chunks = 1;
+  const int cw = gs * cg;
+  const int64_t row_bytes = static_cast<int64_t>(cw) * size * tensors;
+  int s = 1;
+  auto slab = [&](int slices) { return ceil_div(hw, slices) * row_bytes; };
+  // 32 KB a CTA keeps several on an SM, so that one's loads run under another's
+  // stores; a cluster only where there are CTAs to spare or the strip asks for it.
+  const int64_t ctas = n * p.g.strips;
+  while (s < 8 && (slab(s) > 96 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sms))) s *= 2;
+  p.g.slices = s;
+  p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, s));
+  p.threads = slab(s) > 48 * 1024 ? 512 : 256;
+  p.keep = slab(s) + norm_tail_bytes(p.threads, v, cw, gs) <= kNormSmemLimit;
+  if (p.keep) {
+    const int64_t most = ((int64_t(1) << 31) - 1) / (static_cast<int64_t>(p.g.strips) * s);
+    p.batch = n < most ? n : most;
+    return p;
+  }
+
+  // Two passes: whole rows where 512 threads hold one, else as many groups.
+  gs = static_cast<int>(groups);
+  if (c > 512 * v) {
+    gs = 512 * v / (gs0 * cg) * gs0;
+  }
+  if (gs > 512) gs = 512 / gs0 * gs0;
+  if (gs < gs0) gs = gs0;
+  p.g.gs = gs;
+  p.g.strips = static_cast<int>(ceil_div(groups, gs));
+  p.threads = static_cast<int64_t>(gs) * cg > 256 * v ? 512 : 256;
+  // Images whose tensors stay in L2 between the passes (a third of its 126 MB).
+  const int64_t image = hw * c * size * tensors;
+  int64_t batch = (40 << 20) / image;
+  if (batch < 1) batch = 1;
+  p.batch = n < batch ? n : batch;
+  const int64_t wanted = static_cast<int64_t>(sms) * (p.threads == 256 ? 4 : 2);
+  int64_t chunks = wanted / (8 * p.g.strips * p.batch);
+  if (chunks < 1) chunks = 1;
+  if (chunks > norm_most_chunks(hw)) chunks = norm_most_chunks(hw);
+  p.g.slices = 8;
+  p.g.chunks = static_cast<int>(chunks);
+  p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, chunks * 8));
+  int64_t apply = ceil_div(2 * wanted, p.g.strips * p.batch);
+  if (apply > hw) apply = hw;
+  p.apply_chunks = static_cast<int>(apply);
+  return p;
+}
+
+// Elements of a pack that a pointer and pitch allow, at most 16 bytes.
+inline int norm_pack_fit(const void *ptr, int64_t ld, int size) {
+  int v = 16 / size;
+  while (v > 1 && (reinterpret_cast<uintptr_t>(ptr) % (v * size) != 0 || ld % v != 0)) v /= 2;
+  return v;
+}
+
+inline int norm_check(int64_t n, int64_t hw, int64_t c, int64_t groups) {
+  if (n < 1 || hw < 1 || c < 1 || groups < 1 || c % groups != 0) return kErrInvalidArg;
+  if (n >= (int64_t(1) << 31) || hw >= (int64_t(1) << 31) || c / groups > 8192 ||
+      c > (int64_t(1) << 24))
+    return kErrUnsupported;
+  if (n > ((int64_t(1) << 31) - 1) / groups) return kErrUnsupported;
+  return kOk;
+}
+
+inline size_t norm_workspace(int64_t n, int64_t hw, int64_t c, int64_t groups) {
+  return align_up(static_cast<size_t>(n) * norm_most_chunks(hw) * (2 * c + 2 * groups) * sizeof(float),
+                  256);
+}
+
+inline bool norm_aligned(const void *p, int bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
+// Where a CTA of the first pass is: image, strip, rows.
+struct NormPlace {
+  int64_t image, chunk;
+  int strip, rank, g0, gsl, cw, nv, lanes, col, lane;  // col, lane: of this thread
+  uint32_t r0, rows;
+  bool active;
+};
+
+template <int V>
+__device__ __forceinline__ NormPlace norm_place(const NormGeom &p) {
+  NormPlace w;
+  const uint32_t cluster = blockIdx.x / static_cast<uint32_t>(p.slices);
+  w.rank = static_cast<int>(blockIdx.x - cluster * p.slices);
+  const uint32_t at = cluster / static_cast<uint32_t>(p.chunks);
+  w.chunk = cluster - at * p.chunks;
+  w.image = at / static_cast<uint32_t>(p.strips);
+  w.strip = static_cast<int>(at - w.image * p.strips);
+  w.g0 = w.strip * p.gs;
+  w.gsl = min(p.gs, p.groups - w.g0);
+  w.cw = w.gsl * p.cg;
+  w.nv = w.cw / V;
+  const int threads = static_cast<int>(blockDim.x), t = static_cast<int>(threadIdx.x);
+  w.lanes = w.nv <= threads ? threads / w.nv : 1;
+  w.lane = w.nv <= threads ? t / w.nv : 0;
+  w.col = w.nv <= threads ? t - w.lane * w.nv : t;
+  w.active = w.lane < w.lanes && w.col < w.nv;
+  const uint64_t first =
+      (static_cast<uint64_t>(w.chunk) * p.slices + w.rank) * static_cast<uint64_t>(p.cta_rows);
+  w.r0 = first < p.hw ? static_cast<uint32_t>(first) : p.hw;
+  w.rows = min(p.cta_rows, p.hw - w.r0);
+  return w;
+}
+
+// Calls f(pack size, activation) with both as std::integral_constant: 16-byte
+// packs with the usual activations known to the compiler, everything else with
+// the activation as an argument (-1). With it as an argument the kernels hold
+// 118 registers across the calls of the rare ones instead of 40 to 80, which
+// halves the loads in flight on an SM.
+template <int kMost, typename F>
+int norm_with_pack(int v, int act, F f) {
+  using std::integral_constant;
+  if (v == kMost) {
+    constexpr integral_constant<int, kMost> pack{};
+    switch (act) {
+      case 0:
+        return f(pack, integral_constant<int, 0>{});
+      case 1:
+        return f(pack, integral_constant<int, 1>{});
+      case 5:
+        return f(pack, integral_constant<int, 5>{});
+      case 6:
+        return f(pack, integral_constant<int, 6>{});
+      default:
+        return f(pack, integral_constant<int, -1>{});
+    }
+  }
+  constexpr integral_constant<int, -1> any{};
+  if constexpr (kMost > 4)
+    if (v == 4) return f(integral_constant<int, 4>{}, any);
+  if (v == 2) return f(integral_constant<int, 2>{}, any);
+  return f(integral_constant<int, 1>{}, any);
+}
+
+template <typename... KArgs, typename... Args>
+int norm_launch(void (*kernel)(KArgs...), int64_t grid, int threads, int smem, int cluster,
+                cudaStream_t s, Args... args) {
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), smem)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = s;
+  count_launch();
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+}
+
+}  // namespace nplk

@@ -1,0 +1,474 @@
+// Gradient of group norm with an activation, channels last.
+//
+// With xh = (x - mean) * rstd, z = gamma * xh + beta, dz = dy * act'(z), per image:
+//   P[ch] = sum dz, Q[ch] = sum dz * xh over the pixels,
+//   A = sum_ch gamma P, B = sum_ch gamma Q over the group,
+//   dx = rstd * (gamma * dz - (A + xh * B) / M),
+//   dgamma = sum Q, dbeta = sum P over the images.
+//
+// The first pass sums P and Q per thread and channel, then over the CTA's rows by
+// halving, the cluster and the chunks, always in the same order. Kept form: x and
+// dy of the strip stay in the cluster's shared memory (20 bytes of traffic a
+// value less than reading them twice in fp32); otherwise two passes, image batch
+// by image batch, as in the forward kernel.
+#include "act_epilogue.cuh"
+#include "group_norm.cuh"
+
+namespace nplk {
+namespace {
+
+struct GradArgs {
+  const float *mean, *rstd;  // [n][groups]
+  float *channels;           // [n * chunks][2][c]: Q, P; or null
+  float2 *groups;            // [n * chunks][groups]: A, B (two passes)
+};
+
+// xh, z and dz of one pack's channels.
+template <typename T, int V, int kAct>
+struct Chain {
+  float mean[V], rstd[V], gamma[V], beta[V];
+
+  __device__ __forceinline__ void set(const NormGeom &p, int ch, const float *gmean,
+                                      const float *grstd, const float *ga, const float *be) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint32_t g = fdiv(static_cast<uint32_t>(ch + j), p.div_cg);
+      mean[j] = gmean[g];
+      rstd[j] = grstd[g];
+      gamma[j] = ga[ch + j];
+      beta[j] = be[ch + j];
+    }
+  }
+  __device__ __forceinline__ void operator()(const Pack<T, V> &x, const Pack<T, V> &dy,
+                                             const NormGeom &p, float (&xh)[V],
+                                             float (&dz)[V]) const {
+    unpack(x, xh);
+#pragma unroll
+    for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean[j]) * rstd[j];
+#pragma unroll
+    for (int j = 0; j < V; ++j) dz[j] = fmaf(gamma[j], xh[j], beta[j]);
+    act_slope_array<T>(dz, kAct >= 0 ? kAct : p.act, p.alpha);
+    float d[V];
+    unpack(dy, d);
+#pragma unroll
+    for (int j = 0; j < V; ++j) dz[j] *= d[j];
+  }
+};
+
+// dx of one pack from its chain and the group's sums over M.
+template <typename T, int V, int kAct>
+struct Input {
+  Chain<T, V, kAct> chain;
+  float a[V], b[V];  // A / M, B / M
+
+  __device__ __forceinline__ void set(const NormGeom &p, int ch, const float *gmean,
+                                      const float *grstd, const float *ga, const float *be,
+                                      const float2 *ab) {
+    chain.set(p, ch, gmean, grstd, ga, be);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 v = ab[fdiv(static_cast<uint32_t>(ch + j), p.div_cg)];
+      a[j] = v.x;
+      b[j] = v.y;
+    }
+  }
+  __device__ __forceinline__ Pack<T, V> operator()(const Pack<T, V> &x, const Pack<T, V> &dy,
+                                                   const NormGeom &p) const {
+    float xh[V], dz[V];
+    chain(x, dy, p, xh, dz);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      dz[j] = chain.rstd[j] * (chain.gamma[j] * dz[j] - fmaf(xh[j], b[j], a[j]));
+    return pack<T, V>(dz);
+  }
+};
+
+struct GradShared {  // the dynamic shared memory, after the kept strips
+  float *q, *p;          // [lanes][cw]
+  float *gamma, *beta;   // [cw]
+  float2 *group, *total; // A, B of the CTA's groups; of the cluster's, over M
+  float *gmean, *grstd;  // [gs]
+};
+
+template <int V>
+__device__ __forceinline__ GradShared grad_shared(uint8_t *at, const NormGeom &p) {
+  const int cw = p.gs * p.cg;
+  const int acc = max(static_cast<int>(blockDim.x) * V, cw);
+  GradShared s;
+  s.group = reinterpret_cast<float2 *>(at);
+  s.total = s.group + p.gs;
+  s.q = reinterpret_cast<float *>(s.total + p.gs);
+  s.p = s.q + acc;
+  s.gamma = s.p + acc;
+  s.beta = s.gamma + cw;
+  s.gmean = s.beta + cw;
+  s.grstd = s.gmean + p.gs;
+  return s;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, int V, int kAct, bool kKeep>
+__global__ void __launch_bounds__(512)
+    norm_grad_kernel(NormGeom p, GradArgs g, const T *dy, const T *x, T *dx) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const NormPlace w = norm_place<V>(p);
+  const size_t strip_bytes =
+      kKeep ? (static_cast<size_t>(p.cta_rows) * p.gs * p.cg * sizeof(T) + 15) / 16 * 16 : 0;
+  Pack<T, V> *xk = reinterpret_cast<Pack<T, V> *>(smem);
+  Pack<T, V> *dk = reinterpret_cast<Pack<T, V> *>(smem + strip_bytes);
+  const GradShared s = grad_shared<V>(smem + 2 * strip_bytes, p);
+  griddep_wait();
+  griddep_launch_dependents();
+  const int c0 = w.g0 * p.cg;
+  const int64_t row0 = w.image * p.hw + w.r0;
+  const T *xs = x + row0 * p.ldx + c0, *ds = dy + row0 * p.lddy + c0;
+  const uint32_t lanes = static_cast<uint32_t>(w.lanes);
+  const uint32_t mine = w.active && w.rows > static_cast<uint32_t>(w.lane)
+                            ? (w.rows - w.lane + lanes - 1) / lanes
+                            : 0;
+  const uint32_t step = (mine + 3) / 4;
+  auto ask = [&](int col) {  // the thread's rows of one pack, in four groups of copies
+#pragma unroll 1
+    for (uint32_t q = 0; q < 4; ++q) {
+      for (uint32_t k = q * step; k < (q + 1) * step && k < mine; ++k) {
+        const uint32_t r = w.lane + k * lanes;
+        const size_t at = static_cast<size_t>(r) * w.nv + col;
+        copy_pack_async<T, V>(xk + at, xs + static_cast<int64_t>(r) * p.ldx + col * V);
+        copy_pack_async<T, V>(dk + at, ds + static_cast<int64_t>(r) * p.lddy + col * V);
+      }
+      copy_async_commit();
+    }
+  };
+  if (kKeep && w.active) ask(w.col);  // the first turn's, under the loads below
+  for (int i = threadIdx.x; i < w.cw; i += blockDim.x) {
+    s.gamma[i] = p.gamma ? p.gamma[c0 + i] : 1.0f;
+    s.beta[i] = p.beta ? p.beta[c0 + i] : 0.0f;
+  }
+  for (int i = threadIdx.x; i < w.gsl; i += blockDim.x) {
+    s.gmean[i] = g.mean[w.image * p.groups + w.g0 + i];
+    s.grstd[i] = g.rstd[w.image * p.groups + w.g0 + i];
+  }
+  __syncthreads();
+  for (int col = w.active ? w.col : w.nv; col < w.nv; col += blockDim.x) {
+    Chain<T, V, kAct> chain;
+    chain.set(p, col * V, s.gmean, s.grstd, s.gamma, s.beta);
+    float sp[V], sq[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sp[j] = sq[j] = 0.0f;
+    auto add = [&](const Pack<T, V> &a, const Pack<T, V> &b) {
+      float xh[V], dz[V];
+      chain(a, b, p, xh, dz);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        sp[j] += dz[j];
+        sq[j] = fmaf(dz[j], xh[j], sq[j]);
+      }
+    };
+    if constexpr (kKeep) {
+      if (col != w.col) ask(col);
+#pragma unroll 1
+      for (uint32_t q = 0; q < 4; ++q) {
+        if (q == 0) copy_async_wait<3>();
+        else if (q == 1) copy_async_wait<2>();
+        else if (q == 2) copy_async_wait<1>();
+        else copy_async_wait<0>();
+        const uint32_t end = min((q + 1) * step, mine);
+#pragma unroll 2
+        for (uint32_t k = q * step; k < end; ++k) {
+          const size_t at = static_cast<size_t>(w.lane + k * lanes) * w.nv + col;
+          add(xk[at], dk[at]);
+        }
+      }
+    } else {
+      uint32_t r = w.lane;
+      for (; r + 3 * lanes < w.rows; r += 4 * lanes) {
+        Pack<T, V> a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          a[i] = load_pack<T, V>(xs + static_cast<int64_t>(r + i * lanes) * p.ldx + col * V);
+          b[i] = load_pack<T, V>(ds + static_cast<int64_t>(r + i * lanes) * p.lddy + col * V);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(a[i], b[i]);
+      }
+      for (; r < w.rows; r += lanes)
+        add(load_pack<T, V>(xs + static_cast<int64_t>(r) * p.ldx + col * V),
+            load_pack<T, V>(ds + static_cast<int64_t>(r) * p.lddy + col * V));
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      s.q[w.lane * w.cw + col * V + j] = sq[j];
+      s.p[w.lane * w.cw + col * V + j] = sp[j];
+    }
+  }
+  __syncthreads();
+  // The CTA's sums per channel, by halving the row lanes.
+  for (int n = w.lanes; n > 1;) {
+    const int h = (n + 1) / 2;
+    for (int i = threadIdx.x; i < (n - h) * w.cw; i += blockDim.x) {
+      s.q[i] += s.q[i + h * w.cw];
+      s.p[i] += s.p[i + h * w.cw];
+    }
+    n = h;
+    __syncthreads();
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = warp; i < w.gsl; i += static_cast<int>(blockDim.x) >> 5) {
+    float a = 0.0f, b = 0.0f;
+    for (int ch = i * p.cg + lane; ch < (i + 1) * p.cg; ch += 32) {
+      a = fmaf(s.gamma[ch], s.p[ch], a);
+      b = fmaf(s.gamma[ch], s.q[ch], b);
+    }
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (lane == 0) s.group[i] = make_float2(a, b);
+  }
+  if (p.slices > 1) cluster_sync();
+  else __syncthreads();
+  const float inv = 1.0f / (static_cast<float>(p.hw) * static_cast<float>(p.cg));
+  for (int i = threadIdx.x; i < w.gsl; i += blockDim.x) {
+    float2 t = s.group[i];
+    if (p.slices > 1) {
+      t = make_float2(0.0f, 0.0f);
+      for (int k = 0; k < p.slices; ++k) {
+        const uint32_t at = mapa_shared(smem_u32(&s.group[i]), static_cast<uint32_t>(k));
+        t.x += __uint_as_float(ld_shared_cluster_u32(at));
+        t.y += __uint_as_float(ld_shared_cluster_u32(at + 4));
+      }
+    }
+    if (kKeep) s.total[i] = make_float2(t.x * inv, t.y * inv);
+    else if (w.rank == 0)
+      g.groups[(w.image * p.chunks + w.chunk) * p.groups + w.g0 + i] = t;
+  }
+  if (g.channels) {
+    // Each CTA adds its share of the channels over the cluster.
+    float *out = g.channels + (w.image * p.chunks + w.chunk) * 2 * p.c + c0;
+    for (int ch = w.rank * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x); ch < w.cw;
+         ch += p.slices * static_cast<int>(blockDim.x)) {
+      float q = s.q[ch], b = s.p[ch];
+      if (p.slices > 1) {
+        q = b = 0.0f;
+        for (int k = 0; k < p.slices; ++k) {
+          q += __uint_as_float(ld_shared_cluster_u32(
+              mapa_shared(smem_u32(&s.q[ch]), static_cast<uint32_t>(k))));
+          b += __uint_as_float(ld_shared_cluster_u32(
+              mapa_shared(smem_u32(&s.p[ch]), static_cast<uint32_t>(k))));
+        }
+      }
+      out[ch] = q;
+      out[p.c + ch] = b;
+    }
+  }
+  if constexpr (kKeep) {
+    __syncthreads();
+    T *os = dx + row0 * p.ldy + c0;
+    for (int col = w.active ? w.col : w.nv; col < w.nv; col += blockDim.x) {
+      Input<T, V, kAct> f;
+      f.set(p, col * V, s.gmean, s.grstd, s.gamma, s.beta, s.total);
+#pragma unroll 2
+      for (uint32_t r = w.lane; r < w.rows; r += lanes) {
+        const size_t at = static_cast<size_t>(r) * w.nv + col;
+        store_pack(os + static_cast<int64_t>(r) * p.ldy + col * V, f(xk[at], dk[at], p));
+      }
+    }
+  }
+  if (p.slices > 1) cluster_sync_relaxed();  // no CTA leaves while another reads its sums
+}
+
+// Second pass, rows from the image's end.
+template <typename T, int V, int kAct>
+__global__ void __launch_bounds__(512)
+    norm_grad_apply_kernel(NormGeom p, GradArgs g, const T *dy, const T *x, T *dx,
+                           int apply_chunks, uint32_t apply_rows) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const uint32_t at = gridDim.x - 1 - blockIdx.x;
+  const uint32_t piece = at / static_cast<uint32_t>(apply_chunks);
+  const uint32_t chunk = at - piece * apply_chunks;
+  const int64_t image = piece / static_cast<uint32_t>(p.strips);
+  const int g0 = static_cast<int>(piece - image * p.strips) * p.gs;
+  const int gsl = min(p.gs, p.groups - g0), cw = gsl * p.cg, nv = cw / V, c0 = g0 * p.cg;
+  float2 *total = reinterpret_cast<float2 *>(smem);
+  float *gmean = reinterpret_cast<float *>(total + p.gs), *grstd = gmean + p.gs;
+  float *gamma = grstd + p.gs, *beta = gamma + p.gs * p.cg;
+  griddep_wait();
+  griddep_launch_dependents();
+  for (int i = threadIdx.x; i < cw; i += blockDim.x) {
+    gamma[i] = p.gamma ? p.gamma[c0 + i] : 1.0f;
+    beta[i] = p.beta ? p.beta[c0 + i] : 0.0f;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float inv = 1.0f / (static_cast<float>(p.hw) * static_cast<float>(p.cg));
+  for (int i = warp; i < gsl; i += static_cast<int>(blockDim.x) >> 5) {
+    const float2 *from = g.groups + image * p.chunks * p.groups + g0 + i;
+    float a = 0.0f, b = 0.0f;
+    for (int k = lane; k < p.chunks; k += 32) {
+      const float2 v = from[static_cast<int64_t>(k) * p.groups];
+      a += v.x;
+      b += v.y;
+    }
+    a = warp_sum(a);
+    b = warp_sum(b);
+    if (lane == 0) {
+      total[i] = make_float2(a * inv, b * inv);
+      gmean[i] = g.mean[image * p.groups + g0 + i];
+      grstd[i] = g.rstd[image * p.groups + g0 + i];
+    }
+  }
+  __syncthreads();
+  const int threads = static_cast<int>(blockDim.x), t = static_cast<int>(threadIdx.x);
+  const uint32_t lanes = nv <= threads ? threads / nv : 1;
+  const uint32_t rl = nv <= threads ? t / nv : 0;
+  const int first_col = nv <= threads ? t - static_cast<int>(rl) * nv : t;
+  const uint64_t begin = static_cast<uint64_t>(chunk) * apply_rows;
+  if (begin >= p.hw || rl >= lanes) return;
+  const uint32_t r0 = static_cast<uint32_t>(begin), rows = min(apply_rows, p.hw - r0);
+  const int64_t row0 = image * p.hw + r0;
+  for (int col = first_col; col < nv; col += threads) {
+    Input<T, V, kAct> f;
+    f.set(p, col * V, gmean, grstd, gamma, beta, total);
+    const T *xc = x + row0 * p.ldx + c0 + col * V, *dc = dy + row0 * p.lddy + c0 + col * V;
+    T *oc = dx + row0 * p.ldy + c0 + col * V;
+    uint32_t r = rl;
+    for (; r + lanes < rows; r += 2 * lanes) {
+      Pack<T, V> a[2], b[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        a[i] = load_pack<T, V>(xc + static_cast<int64_t>(r + i * lanes) * p.ldx);
+        b[i] = load_pack<T, V>(dc + static_cast<int64_t>(r + i * lanes) * p.lddy);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        store_pack(oc + static_cast<int64_t>(r + i * lanes) * p.ldy, f(a[i], b[i], p));
+    }
+    for (; r < rows; r += lanes)
+      store_pack(oc + static_cast<int64_t>(r) * p.ldy,
+                 f(load_pack<T, V>(xc + static_cast<int64_t>(r) * p.ldx),
+                   load_pack<T, V>(dc + static_cast<int64_t>(r) * p.lddy), p));
+  }
+}
+
+// dgamma and dbeta: the sums of `rows` rows [2][c]. A block takes 32 of the 2 c
+// columns, its 8 warps every eighth row.
+__global__ void __launch_bounds__(256)
+    param_grad_kernel(int64_t rows, int c, const float *from, float *dgamma, float *dbeta) {
+  __shared__ float part[8][32];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float s = 0.0f;
+  if (i < 2 * static_cast<int64_t>(c)) {
+#pragma unroll 4
+    for (int64_t r = warp; r < rows; r += 8) s += from[r * 2 * c + i];
+  }
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && i < 2 * static_cast<int64_t>(c)) {
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += part[k][lane];
+    float *out = i < c ? dgamma : dbeta;
+    if (out) out[i < c ? i : i - c] = s;
+  }
+}
+
+template <typename T>
+int run_grad(cudaStream_t s, int64_t n, const NormPlan &plan, GradArgs args, const T *dy,
+             const T *x, T *dx) {
+  const NormGeom &g = plan.g;
+  return norm_with_pack<16 / sizeof(T)>(plan.v, g.act, [&](auto pack_size, auto act) {
+    constexpr int V = decltype(pack_size)::value, kAct = decltype(act)::value;
+    const int cw = g.gs * g.cg;
+    const int tail = norm_tail_bytes(plan.threads, V, cw, g.gs);
+    for (int64_t i = 0; i < n; i += plan.batch) {
+      const int64_t count = n - i < plan.batch ? n - i : plan.batch;
+      GradArgs a = args;
+      a.mean += i * g.groups;
+      a.rstd += i * g.groups;
+      if (a.channels) a.channels += i * g.chunks * 2 * g.c;
+      const T *xi = x + i * g.hw * g.ldx, *di = dy + i * g.hw * g.lddy;
+      T *oi = dx + i * g.hw * g.ldy;
+      const int64_t ctas = count * g.strips * g.chunks * g.slices;
+      if (plan.keep) {
+        const int strip = static_cast<int>(
+            align_up(static_cast<size_t>(g.cta_rows) * cw * sizeof(T), 16));
+        if (int rc = norm_launch(norm_grad_kernel<T, V, kAct, true>, ctas, plan.threads,
+                                 2 * strip + tail, g.slices, s, g, a, di, xi, oi))
+          return rc;
+        continue;
+      }
+      if (int rc = norm_launch(norm_grad_kernel<T, V, kAct, false>, ctas, plan.threads, tail,
+                               g.slices, s, g, a, di, xi, oi))
+        return rc;
+      const uint32_t rows = static_cast<uint32_t>(ceil_div(g.hw, plan.apply_chunks));
+      const int smem = (4 * g.gs + 2 * cw) * static_cast<int>(sizeof(float));
+      if (int rc = norm_launch(norm_grad_apply_kernel<T, V, kAct>,
+                               count * g.strips * plan.apply_chunks, plan.threads, smem, 1, s, g, a,
+                               di, xi, oi, plan.apply_chunks, rows))
+        return rc;
+    }
+    return kOk;
+  });
+}
+
+}  // namespace
+}  // namespace nplk
+
+using namespace nplk;
+
+extern "C" int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw, int64_t c,
+                                            int64_t groups, int dtype, const void *dy,
+                                            int64_t lddy, const void *x, int64_t ldx,
+                                            const float *mean, const float *rstd,
+                                            const float *gamma, const float *beta, int act,
+                                            float act_alpha, void *dx, int64_t lddx,
+                                            float *dgamma, float *dbeta, void *workspace,
+                                            size_t workspace_bytes) {
+  const int size = dtype_bytes(dtype);
+  if (!size || !dy || !x || !mean || !rstd || !dx || lddy < c || ldx < c || lddx < c || act < 0 ||
+      act > 10)
+    return kErrInvalidArg;
+  if (int rc = norm_check(n, hw, c, groups)) return rc;
+  if (!norm_aligned(dy, size) || !norm_aligned(x, size) || !norm_aligned(dx, size) ||
+      (dx == dy && lddx != lddy) || (dx == x && lddx != ldx))
+    return kErrInvalidArg;
+  if (!workspace || !norm_aligned(workspace, 256) ||
+      workspace_bytes < norm_workspace(n, hw, c, groups))
+    return kErrInvalidArg;
+  int fit = norm_pack_fit(x, ldx, size);
+  fit = std::min(fit, norm_pack_fit(dy, lddy, size));
+  fit = std::min(fit, norm_pack_fit(dx, lddx, size));
+  NormPlan plan = plan_norm(n, hw, c, groups, size, fit, 2);
+  plan.g.ldx = ldx;
+  plan.g.ldy = lddx;
+  plan.g.lddy = lddy;
+  plan.g.gamma = gamma;
+  plan.g.beta = beta;
+  plan.g.act = act;
+  plan.g.alpha = act_alpha;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // The workspace: [n * chunks][2][c] channel sums, then [n * chunks][groups] A, B.
+  const int64_t rows = n * plan.g.chunks;
+  GradArgs a{mean, rstd, nullptr, nullptr};
+  float *channels = static_cast<float *>(workspace);
+  a.channels = dgamma || dbeta ? channels : nullptr;
+  a.groups = reinterpret_cast<float2 *>(channels + rows * 2 * c);
+  int rc;
+  if (dtype == NPLK_DTYPE_FP32)
+    rc = run_grad(s, n, plan, a, static_cast<const float *>(dy), static_cast<const float *>(x),
+                  static_cast<float *>(dx));
+  else if (dtype == NPLK_DTYPE_FP16)
+    rc = run_grad(s, n, plan, a, static_cast<const __half *>(dy), static_cast<const __half *>(x),
+                  static_cast<__half *>(dx));
+  else
+    rc = run_grad(s, n, plan, a, static_cast<const __nv_bfloat16 *>(dy),
+                  static_cast<const __nv_bfloat16 *>(x), static_cast<__nv_bfloat16 *>(dx));
+  if (rc || !a.channels) return rc;
+  return launch_programmatic(param_grad_kernel, dim3(static_cast<unsigned>(ceil_div(2 * c, 32))),
+                             dim3(256), 0, s, rows, static_cast<int>(c), channels, dgamma, dbeta);
+}
