@@ -36,7 +36,7 @@ struct Running {
 template <typename T, int V, int R>
 __device__ __forceinline__ void join_rows(const Pack<T, V> (&p)[R], Running<V> &run) {
   const float total = run.n + static_cast<float>(R);
-  const float share = static_cast<float>(R) / total, cross = run.n * share;
+  const float share = static_cast<float>(R) * rcp_approx(total), cross = run.n * share;
   float x[R][V];
 #pragma unroll
   for (int r = 0; r < R; ++r) unpack(p[r], x[r]);
@@ -174,7 +174,7 @@ struct Affine {
 
 // First pass, and with kKeep the whole of it.
 template <typename T, int V, int kAct, bool kKeep>
-__global__ void __launch_bounds__(512) norm_kernel(NormGeom p, const T *x, T *y, float *mean_out,
+__global__ void __launch_bounds__(norm_most_threads(V), V == 8 ? 3 : 2) norm_kernel(NormGeom p, const T *x, T *y, float *mean_out,
                                                    float *rstd_out, float2 *partial) {
   extern __shared__ __align__(16) uint8_t smem[];
   const NormPlace w = norm_place<V>(p);
@@ -211,13 +211,16 @@ __global__ void __launch_bounds__(512) norm_kernel(NormGeom p, const T *x, T *y,
                                 ? (w.rows - w.lane + lanes - 1) / lanes
                                 : 0;
       const uint32_t step = (mine + 15) / 16 * 4;
+      Pack<T, V> *own = strip + w.lane * w.nv + col;
+      const int turn = w.lanes * w.nv;  // from one of the thread's rows to the next
+      const T *from = xc + static_cast<int64_t>(w.lane) * p.ldx;
+      const int64_t pitch = static_cast<int64_t>(lanes) * p.ldx;
 #pragma unroll 1
       for (uint32_t q = 0; q < 4; ++q) {
-        for (uint32_t k = q * step; k < (q + 1) * step && k < mine; ++k) {
-          const uint32_t r = w.lane + k * lanes;
-          copy_pack_async<T, V>(strip + static_cast<size_t>(r) * w.nv + col,
-                                xc + static_cast<int64_t>(r) * p.ldx);
-        }
+        const uint32_t end = min((q + 1) * step, mine);
+#pragma unroll 4
+        for (uint32_t k = q * step; k < end; ++k)
+          copy_pack_async<T, V>(own + k * turn, from + k * pitch);
         copy_async_commit();
       }
 #pragma unroll 1
@@ -232,30 +235,39 @@ __global__ void __launch_bounds__(512) norm_kernel(NormGeom p, const T *x, T *y,
           Pack<T, V> v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            v[i] = strip[static_cast<size_t>(w.lane + (k + i) * lanes) * w.nv + col];
+            v[i] = own[(k + i) * turn];
           join_rows(v, run);
         }
         for (; k < end; ++k) {
-          const Pack<T, V> v[1] = {strip[static_cast<size_t>(w.lane + k * lanes) * w.nv + col]};
+          const Pack<T, V> v[1] = {own[k * turn]};
           join_rows(v, run);
         }
       }
     } else {
+      // Eight rows asked for at a time, joined four by four (the last ones singly).
       uint32_t r = w.lane;
-      for (; r + 7 * lanes < w.rows; r += 8 * lanes) {
+      const int64_t pitch = static_cast<int64_t>(lanes) * p.ldx;
+      const T *at = xc + static_cast<int64_t>(r) * p.ldx;
+      for (; r + 7 * lanes < w.rows; r += 8 * lanes, at += 8 * pitch) {
         Pack<T, V> a[4], b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          a[i] = load_pack<T, V>(xc + static_cast<int64_t>(r + i * lanes) * p.ldx);
+        for (int i = 0; i < 4; ++i) a[i] = load_pack<T, V>(at + i * pitch);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          b[i] = load_pack<T, V>(xc + static_cast<int64_t>(r + (4 + i) * lanes) * p.ldx);
+        for (int i = 0; i < 4; ++i) b[i] = load_pack<T, V>(at + (4 + i) * pitch);
         join_rows(a, run);
         join_rows(b, run);
       }
-      for (; r < w.rows; r += lanes) {
-        const Pack<T, V> v[1] = {load_pack<T, V>(xc + static_cast<int64_t>(r) * p.ldx)};
-        join_rows(v, run);
+      if (r < w.rows) {
+        Pack<T, V> a[7];
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          if (r + i * lanes < w.rows) a[i] = load_pack<T, V>(at + i * pitch);
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          if (r + i * lanes < w.rows) {
+            const Pack<T, V> one[1] = {a[i]};
+            join_rows(one, run);
+          }
       }
     }
 #pragma unroll
@@ -303,10 +315,13 @@ __global__ void __launch_bounds__(512) norm_kernel(NormGeom p, const T *x, T *y,
     for (int col = w.active ? w.col : w.nv; col < w.nv; col += blockDim.x) {
       Affine<T, V, kAct> f;
       f.set(p, col * V, s.gmean, s.grstd, s.gamma, s.beta);
+      const Pack<T, V> *own = strip + w.lane * w.nv + col;
+      const int turn = w.lanes * w.nv;
+      T *to = ys + static_cast<int64_t>(w.lane) * p.ldy + col * V;
+      const int64_t pitch = static_cast<int64_t>(lanes) * p.ldy;
 #pragma unroll 2
-      for (uint32_t r = w.lane; r < w.rows; r += lanes)
-        store_pack(ys + static_cast<int64_t>(r) * p.ldy + col * V,
-                   f(strip[static_cast<size_t>(r) * w.nv + col], p));
+      for (uint32_t r = w.lane; r < w.rows; r += lanes, own += turn, to += pitch)
+        store_pack(to, f(*own, p));
     }
   }
   if (p.slices > 1) cluster_sync_relaxed();  // no CTA leaves while another reads its groups
@@ -315,7 +330,7 @@ __global__ void __launch_bounds__(512) norm_kernel(NormGeom p, const T *x, T *y,
 // Second pass: joins the chunks' moments, then normalises. Rows are taken from
 // the image's end, which the first pass read last.
 template <typename T, int V, int kAct>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(norm_most_threads(V), V == 8 ? 3 : 2)
     norm_apply_kernel(NormGeom p, const T *x, T *y, float *mean_out, float *rstd_out,
                       const float2 *partial, int apply_chunks, uint32_t apply_rows) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -378,19 +393,18 @@ __global__ void __launch_bounds__(512)
     f.set(p, col * V, gmean, grstd, gamma, beta);
     const T *xc = xs + col * V;
     T *yc = ys + col * V;
-    uint32_t r = rl;
-    for (; r + 3 * lanes < rows; r += 4 * lanes) {
+    const int64_t xp = static_cast<int64_t>(lanes) * p.ldx, yp = static_cast<int64_t>(lanes) * p.ldy;
+    xc += static_cast<int64_t>(rl) * p.ldx;
+    yc += static_cast<int64_t>(rl) * p.ldy;
+    for (uint32_t r = rl; r < rows; r += 4 * lanes, xc += 4 * xp, yc += 4 * yp) {
       Pack<T, V> v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        v[i] = load_pack<T, V>(xc + static_cast<int64_t>(r + i * lanes) * p.ldx);
+        if (r + i * lanes < rows) v[i] = load_pack<T, V>(xc + i * xp);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        store_pack(yc + static_cast<int64_t>(r + i * lanes) * p.ldy, f(v[i], p));
+        if (r + i * lanes < rows) store_pack(yc + i * yp, f(v[i], p));
     }
-    for (; r < rows; r += lanes)
-      store_pack(yc + static_cast<int64_t>(r) * p.ldy,
-                 f(load_pack<T, V>(xc + static_cast<int64_t>(r) * p.ldx), p));
   }
 }
 

@@ -41,6 +41,10 @@ struct NormPlan {
   int apply_chunks; // second pass: CTAs per image and strip
 };
 
+// Threads of a CTA: packs of 8 values take 80 to 128 registers a thread (their
+// channels' constants and sums), smaller ones at most 64.
+__host__ __device__ constexpr int norm_most_threads(int v) { return v == 8 ? 256 : 512; }
+
 // Workspace: per image and chunk, sums per channel and group.
 constexpr int kNormMostChunks = 74;
 inline int64_t norm_most_chunks(int64_t hw) {
@@ -83,14 +87,17 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   p.g.cg = cg;
   p.g.div_cg = make_fastdiv(static_cast<uint32_t>(cg));
 
-  // Kept form: narrow strips, at least 64 bytes a row and in whole 32-byte
-  // sectors where a strip of up to 512 bytes is.
+  // Kept form: strips of at least 64 bytes a row; of those up to 512 bytes, the
+  // narrowest in whole 32-byte sectors if 48 KB in each of 8 CTAs hold it, else the
+  // narrowest.
+  auto row = [&](int gs) { return static_cast<int64_t>(gs) * cg * size; };
   int gs = gs0;
-  for (int m = gs0; m <= groups; m += gs0) {
-    const int bytes = m * cg * size;
-    if (bytes > 512 && gs * cg * size >= 64) break;
-    gs = m;
-    if (bytes >= 64 && bytes % 32 == 0) break;
+  while (gs + gs0 <= groups && row(gs) < 64) gs += gs0;
+  for (int m = gs; m <= groups && row(m) <= 512; m += gs0) {
+    if (row(m) % 32 == 0 && ceil_div(hw, 8) * row(m) * tensors <= 48 * 1024) {
+      gs = m;
+      break;
+    }
   }
   p.g.gs = gs;
   p.g.strips = static_cast<int>(ceil_div(groups, gs));
@@ -99,13 +106,14 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   const int64_t row_bytes = static_cast<int64_t>(cw) * size * tensors;
   int s = 1;
   auto slab = [&](int slices) { return ceil_div(hw, slices) * row_bytes; };
-  // 32 KB a CTA keeps several on an SM, so that one's loads run under another's
-  // stores; a cluster only where there are CTAs to spare or the strip asks for it.
+  // Up to 48 KB a CTA keeps four on an SM, so that one's loads run under another's
+  // stores; more CTAs while they are few.
   const int64_t ctas = n * p.g.strips;
-  while (s < 8 && (slab(s) > 96 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sms))) s *= 2;
+  while (s < 8 && (slab(s) > 48 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sms))) s *= 2;
   p.g.slices = s;
   p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, s));
-  p.threads = slab(s) > 48 * 1024 ? 512 : 256;
+  const int most = norm_most_threads(v);
+  p.threads = slab(s) > 48 * 1024 ? most : 256;
   p.keep = slab(s) + norm_tail_bytes(p.threads, v, cw, gs) <= kNormSmemLimit;
   if (p.keep) {
     const int64_t most = ((int64_t(1) << 31) - 1) / (static_cast<int64_t>(p.g.strips) * s);
@@ -113,16 +121,14 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
     return p;
   }
 
-  // Two passes: whole rows where 512 threads hold one, else as many groups.
+  // Two passes: whole rows where a CTA's threads hold one, else as many groups.
   gs = static_cast<int>(groups);
-  if (c > 512 * v) {
-    gs = 512 * v / (gs0 * cg) * gs0;
-  }
+  if (c > most * v) gs = most * v / (gs0 * cg) * gs0;
   if (gs > 512) gs = 512 / gs0 * gs0;
   if (gs < gs0) gs = gs0;
   p.g.gs = gs;
   p.g.strips = static_cast<int>(ceil_div(groups, gs));
-  p.threads = static_cast<int64_t>(gs) * cg > 256 * v ? 512 : 256;
+  p.threads = static_cast<int64_t>(gs) * cg > 256 * v ? most : 256;
   // Images whose tensors stay in L2 between the passes (a third of its 126 MB).
   const int64_t image = hw * c * size * tensors;
   int64_t batch = (40 << 20) / image;

@@ -113,7 +113,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 template <typename T, int V, int kAct, bool kKeep>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(norm_most_threads(V), 2)
     norm_grad_kernel(NormGeom p, GradArgs g, const T *dy, const T *x, T *dx) {
   extern __shared__ __align__(16) uint8_t smem[];
   const NormPlace w = norm_place<V>(p);
@@ -132,14 +132,19 @@ __global__ void __launch_bounds__(512)
                             ? (w.rows - w.lane + lanes - 1) / lanes
                             : 0;
   const uint32_t step = (mine + 3) / 4;
+  // The thread's first row, and from one of its rows to the next.
+  const int first = w.lane * w.nv, turn = w.lanes * w.nv;
+  const T *xl = xs + static_cast<int64_t>(w.lane) * p.ldx;
+  const T *dl = ds + static_cast<int64_t>(w.lane) * p.lddy;
+  const int64_t xp = static_cast<int64_t>(lanes) * p.ldx, dp = static_cast<int64_t>(lanes) * p.lddy;
   auto ask = [&](int col) {  // the thread's rows of one pack, in four groups of copies
 #pragma unroll 1
     for (uint32_t q = 0; q < 4; ++q) {
-      for (uint32_t k = q * step; k < (q + 1) * step && k < mine; ++k) {
-        const uint32_t r = w.lane + k * lanes;
-        const size_t at = static_cast<size_t>(r) * w.nv + col;
-        copy_pack_async<T, V>(xk + at, xs + static_cast<int64_t>(r) * p.ldx + col * V);
-        copy_pack_async<T, V>(dk + at, ds + static_cast<int64_t>(r) * p.lddy + col * V);
+      const uint32_t end = min((q + 1) * step, mine);
+#pragma unroll 2
+      for (uint32_t k = q * step; k < end; ++k) {
+        copy_pack_async<T, V>(xk + first + k * turn + col, xl + k * xp + col * V);
+        copy_pack_async<T, V>(dk + first + k * turn + col, dl + k * dp + col * V);
       }
       copy_async_commit();
     }
@@ -180,25 +185,24 @@ __global__ void __launch_bounds__(512)
         const uint32_t end = min((q + 1) * step, mine);
 #pragma unroll 2
         for (uint32_t k = q * step; k < end; ++k) {
-          const size_t at = static_cast<size_t>(w.lane + k * lanes) * w.nv + col;
+          const int at = first + k * turn + col;
           add(xk[at], dk[at]);
         }
       }
     } else {
-      uint32_t r = w.lane;
-      for (; r + 3 * lanes < w.rows; r += 4 * lanes) {
+      const T *xc = xl + col * V, *dc = dl + col * V;
+      for (uint32_t r = w.lane; r < w.rows; r += 4 * lanes, xc += 4 * xp, dc += 4 * dp) {
         Pack<T, V> a[4], b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] = load_pack<T, V>(xs + static_cast<int64_t>(r + i * lanes) * p.ldx + col * V);
-          b[i] = load_pack<T, V>(ds + static_cast<int64_t>(r + i * lanes) * p.lddy + col * V);
-        }
+        for (int i = 0; i < 4; ++i)
+          if (r + i * lanes < w.rows) {
+            a[i] = load_pack<T, V>(xc + i * xp);
+            b[i] = load_pack<T, V>(dc + i * dp);
+          }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) add(a[i], b[i]);
+        for (int i = 0; i < 4; ++i)
+          if (r + i * lanes < w.rows) add(a[i], b[i]);
       }
-      for (; r < w.rows; r += lanes)
-        add(load_pack<T, V>(xs + static_cast<int64_t>(r) * p.ldx + col * V),
-            load_pack<T, V>(ds + static_cast<int64_t>(r) * p.lddy + col * V));
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -270,11 +274,12 @@ __global__ void __launch_bounds__(512)
     for (int col = w.active ? w.col : w.nv; col < w.nv; col += blockDim.x) {
       Input<T, V, kAct> f;
       f.set(p, col * V, s.gmean, s.grstd, s.gamma, s.beta, s.total);
+      const Pack<T, V> *xo = xk + first + col, *dn = dk + first + col;
+      T *to = os + static_cast<int64_t>(w.lane) * p.ldy + col * V;
+      const int64_t op = static_cast<int64_t>(lanes) * p.ldy;
 #pragma unroll 2
-      for (uint32_t r = w.lane; r < w.rows; r += lanes) {
-        const size_t at = static_cast<size_t>(r) * w.nv + col;
-        store_pack(os + static_cast<int64_t>(r) * p.ldy + col * V, f(xk[at], dk[at], p));
-      }
+      for (uint32_t r = w.lane; r < w.rows; r += lanes, xo += turn, dn += turn, to += op)
+        store_pack(to, f(*xo, *dn, p));
     }
   }
   if (p.slices > 1) cluster_sync_relaxed();  // no CTA leaves while another reads its sums
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(512)
 
 // Second pass, rows from the image's end.
 template <typename T, int V, int kAct>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(norm_most_threads(V), 2)
     norm_grad_apply_kernel(NormGeom p, GradArgs g, const T *dy, const T *x, T *dx,
                            int apply_chunks, uint32_t apply_rows) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -333,22 +338,23 @@ __global__ void __launch_bounds__(512)
     f.set(p, col * V, gmean, grstd, gamma, beta, total);
     const T *xc = x + row0 * p.ldx + c0 + col * V, *dc = dy + row0 * p.lddy + c0 + col * V;
     T *oc = dx + row0 * p.ldy + c0 + col * V;
-    uint32_t r = rl;
-    for (; r + lanes < rows; r += 2 * lanes) {
+    const int64_t xp = static_cast<int64_t>(lanes) * p.ldx, dp = static_cast<int64_t>(lanes) * p.lddy,
+                  op = static_cast<int64_t>(lanes) * p.ldy;
+    xc += static_cast<int64_t>(rl) * p.ldx;
+    dc += static_cast<int64_t>(rl) * p.lddy;
+    oc += static_cast<int64_t>(rl) * p.ldy;
+    for (uint32_t r = rl; r < rows; r += 2 * lanes, xc += 2 * xp, dc += 2 * dp, oc += 2 * op) {
       Pack<T, V> a[2], b[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        a[i] = load_pack<T, V>(xc + static_cast<int64_t>(r + i * lanes) * p.ldx);
-        b[i] = load_pack<T, V>(dc + static_cast<int64_t>(r + i * lanes) * p.lddy);
-      }
+      for (int i = 0; i < 2; ++i)
+        if (r + i * lanes < rows) {
+          a[i] = load_pack<T, V>(xc + i * xp);
+          b[i] = load_pack<T, V>(dc + i * dp);
+        }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        store_pack(oc + static_cast<int64_t>(r + i * lanes) * p.ldy, f(a[i], b[i], p));
+        if (r + i * lanes < rows) store_pack(oc + i * op, f(a[i], b[i], p));
     }
-    for (; r < rows; r += lanes)
-      store_pack(oc + static_cast<int64_t>(r) * p.ldy,
-                 f(load_pack<T, V>(xc + static_cast<int64_t>(r) * p.ldx),
-                   load_pack<T, V>(dc + static_cast<int64_t>(r) * p.lddy), p));
   }
 }
 
