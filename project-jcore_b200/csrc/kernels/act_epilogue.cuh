@@ -6,6 +6,7 @@
 
 #include "activation_grad.cuh"
 #include "nplk_device.cuh"
+#include "typed_io.cuh"
 
 namespace nplk {
 
@@ -36,12 +37,35 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // The library's expf and division took 39 instructions a value in the fp32
 // norm, 70 us of 134 MB read and written that way.
 template <bool kFine>
-__device__ __forceinline__ float sigmoid(float x) {
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
   constexpr float kLog2e = 1.44269504f;
-  if (!kFine) return rcp_approx(1.0f + exp2_approx(-kLog2e * x));
-  const float d = 1.0f + exp2_approx(fminf(-kLog2e * x, 126.0f));
-  const float r = rcp_approx(d);
-  return fmaf(r, fmaf(-d, r, 1.0f), r);
+  float2 t = mul2(x, both(-kLog2e));
+  if (kFine) t = make_float2(fminf(t.x, 126.0f), fminf(t.y, 126.0f));
+  const float2 d = add2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), both(1.0f));
+  const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  if (!kFine) return r;
+  const float2 m = make_float2(-d.x, -d.y);
+  return fma2(r, fma2(m, r, both(1.0f)), r);
+}
+template <bool kFine>
+__device__ __forceinline__ float sigmoid(float x) {
+  return sigmoid2<kFine>(make_float2(x, x)).x;
+}
+
+// The two-value steps of the array forms below: f(pair) for each pair, a lone
+// value as both halves of one.
+template <int V, typename F>
+__device__ __forceinline__ void by_pairs(float (&v)[V], F f) {
+  if constexpr (V == 1) {
+    v[0] = f(make_float2(v[0], v[0])).x;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 r = f(make_float2(v[j], v[j + 1]));
+      v[j] = r.x;
+      v[j + 1] = r.y;
+    }
+  }
 }
 
 // v[j] = act(v[j]), results to be stored as T. GELU in the form
@@ -57,15 +81,14 @@ __device__ __forceinline__ void act_array(float (&v)[V], int act, float alpha) {
       for (int j = 0; j < V; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];
       return;
     case 5:
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float x = v[j], c = 2.0f * 0.7978845608f;
-        v[j] = x * sigmoid<kFine>(x * fmaf(c * 0.044715f, x * x, c));
-      }
+      by_pairs(v, [](float2 x) {
+        constexpr float c = 2.0f * 0.7978845608f;
+        const float2 u = mul2(x, fma2(both(c * 0.044715f), mul2(x, x), both(c)));
+        return mul2(x, sigmoid2<kFine>(u));
+      });
       return;
     case 6:
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] *= sigmoid<kFine>(v[j]);
+      by_pairs(v, [](float2 x) { return mul2(x, sigmoid2<kFine>(x)); });
       return;
     default:
 #pragma unroll
@@ -92,19 +115,20 @@ __device__ __forceinline__ void act_slope_array(float (&v)[V], int act, float al
       for (int j = 0; j < V; ++j) v[j] = v[j] > 0.0f ? 1.0f : 0.0f;
       return;
     case 5:
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float x = v[j], x2 = x * x, c = 2.0f * 0.7978845608f, k = c * 0.044715f;
-        const float s = sigmoid<kFine>(x * fmaf(k, x2, c));
-        v[j] = s + x * s * (1.0f - s) * fmaf(3.0f * k, x2, c);
-      }
+      by_pairs(v, [](float2 x) {
+        constexpr float c = 2.0f * 0.7978845608f, k = c * 0.044715f;
+        const float2 x2 = mul2(x, x);
+        const float2 s = sigmoid2<kFine>(mul2(x, fma2(both(k), x2, both(c))));
+        const float2 du = fma2(both(3.0f * k), x2, both(c));  // of u = c x + k x^3
+        const float2 t = mul2(mul2(x, du), fma2(s, both(-1.0f), both(1.0f)));
+        return fma2(s, t, s);  // s + x s (1 - s) u'
+      });
       return;
     case 6:
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float s = sigmoid<kFine>(v[j]);
-        v[j] = s * fmaf(v[j], 1.0f - s, 1.0f);
-      }
+      by_pairs(v, [](float2 x) {
+        const float2 s = sigmoid2<kFine>(x);
+        return mul2(s, fma2(x, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
+      });
       return;
     default:
 #pragma unroll

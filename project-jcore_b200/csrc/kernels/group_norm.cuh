@@ -26,7 +26,8 @@ struct NormGeom {
   int slices;           // CTAs of a cluster
   int chunks;           // clusters that share a strip's rows
   uint32_t cta_rows;    // rows of a CTA
-  FastDiv div_cg;
+  FastDiv div_cg, div_slices, div_chunks, div_strips;
+  FastDiv div_nv[2], div_lanes[2];  // packs and row lanes of a strip; of the last strip
   const float *gamma, *beta;
   float eps, alpha;
   int act;
@@ -41,9 +42,10 @@ struct NormPlan {
   int apply_chunks; // second pass: CTAs per image and strip
 };
 
-// Threads of a CTA: packs of 8 values take 80 to 128 registers a thread (their
-// channels' constants and sums), smaller ones at most 64.
-__host__ __device__ constexpr int norm_most_threads(int v) { return v == 8 ? 256 : 512; }
+// Most threads of a CTA. A thread keeps its channels' constants and sums in
+// registers (60 to 80 of them forward, up to 128 in the gradient), so an SM holds
+// 24 and 16 warps.
+constexpr int kNormMostThreads = 256;
 
 // Workspace: per image and chunk, sums per channel and group.
 constexpr int kNormMostChunks = 74;
@@ -52,14 +54,29 @@ inline int64_t norm_most_chunks(int64_t hw) {
   return by_rows < kNormMostChunks ? by_rows : kNormMostChunks;
 }
 
-// Floats of shared memory beside the kept strips (norm_smem below).
+// Bytes of shared memory beside the kept strips (norm_smem below).
 inline int norm_tail_bytes(int threads, int v, int cw, int gs) {
   const int acc = threads * v > cw ? threads * v : cw;  // per row lane and channel
   const int teams = gs > 32 ? gs : 32;
   return 2 * acc * 4 + 2 * cw * 4 + teams * 16 + gs * 16 + 2 * gs * 4 + 64;
 }
 
-constexpr int kNormSmemLimit = 227 * 1024;
+// Shared memory of a CTA of the kept form: two fit an SM.
+constexpr int kNormKeepLimit = 112 * 1024;
+
+// The divisions that the kernels do by multiplication, for the plan's split.
+inline void norm_divisors(NormPlan &p) {
+  NormGeom &g = p.g;
+  g.div_slices = make_fastdiv(static_cast<uint32_t>(g.slices));
+  g.div_chunks = make_fastdiv(static_cast<uint32_t>(g.chunks));
+  g.div_strips = make_fastdiv(static_cast<uint32_t>(g.strips));
+  for (int last = 0; last < 2; ++last) {
+    const int gs = last ? g.groups - (g.strips - 1) * g.gs : g.gs;
+    const int nv = gs * g.cg / p.v;
+    g.div_nv[last] = make_fastdiv(static_cast<uint32_t>(nv));
+    g.div_lanes[last] = make_fastdiv(static_cast<uint32_t>(nv <= p.threads ? p.threads / nv : 1));
+  }
+}
 
 // `tensors`: strips that the kept form holds (x; or x and dy).
 inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int size, int v_fit,
@@ -112,10 +129,15 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   while (s < 8 && (slab(s) > 48 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sms))) s *= 2;
   p.g.slices = s;
   p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, s));
-  const int most = norm_most_threads(v);
-  p.threads = slab(s) > 48 * 1024 ? most : 256;
-  p.keep = slab(s) + norm_tail_bytes(p.threads, v, cw, gs) <= kNormSmemLimit;
+  constexpr int most = kNormMostThreads;
+  // Six packs a thread: what a thread does once costs as much as 40 values.
+  const int64_t packs = p.g.cta_rows * static_cast<int64_t>(cw / v);
+  int64_t threads = ceil_div(ceil_div(packs, 6), 32) * 32;
+  if (threads < cw / v) threads = ceil_div(cw / v, 32) * 32;
+  p.threads = static_cast<int>(threads < 64 ? 64 : threads > most ? most : threads);
+  p.keep = slab(s) + norm_tail_bytes(p.threads, v, cw, gs) <= kNormKeepLimit;
   if (p.keep) {
+    norm_divisors(p);
     const int64_t most = ((int64_t(1) << 31) - 1) / (static_cast<int64_t>(p.g.strips) * s);
     p.batch = n < most ? n : most;
     return p;
@@ -128,22 +150,24 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   if (gs < gs0) gs = gs0;
   p.g.gs = gs;
   p.g.strips = static_cast<int>(ceil_div(groups, gs));
-  p.threads = static_cast<int64_t>(gs) * cg > 256 * v ? most : 256;
+  p.threads = most;
   // Images whose tensors stay in L2 between the passes (a third of its 126 MB).
   const int64_t image = hw * c * size * tensors;
   int64_t batch = (40 << 20) / image;
   if (batch < 1) batch = 1;
   p.batch = n < batch ? n : batch;
-  const int64_t wanted = static_cast<int64_t>(sms) * (p.threads == 256 ? 4 : 2);
+  const int64_t wanted = static_cast<int64_t>(sms) * (tensors == 1 ? 3 : 2);
   int64_t chunks = wanted / (8 * p.g.strips * p.batch);
   if (chunks < 1) chunks = 1;
   if (chunks > norm_most_chunks(hw)) chunks = norm_most_chunks(hw);
+  if (chunks > 1 && chunks * gs > 8192) chunks = 8192 / gs;  // 64 KB where they are joined
   p.g.slices = 8;
   p.g.chunks = static_cast<int>(chunks);
   p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, chunks * 8));
-  int64_t apply = ceil_div(2 * wanted, p.g.strips * p.batch);
+  int64_t apply = ceil_div(wanted, p.g.strips * p.batch);
   if (apply > hw) apply = hw;
   p.apply_chunks = static_cast<int>(apply);
+  norm_divisors(p);
   return p;
 }
 
@@ -176,32 +200,41 @@ inline bool norm_aligned(const void *p, int bytes) {
 struct NormPlace {
   int64_t image, chunk;
   int strip, rank, g0, gsl, cw, nv, lanes, col, lane;  // col, lane: of this thread
-  uint32_t r0, rows;
+  uint32_t r0, rows, mine;  // the CTA's rows; how many are this thread's
+  uint32_t base, rest;      // rows of a row lane: base, and one more in the first `rest`
   bool active;
 };
+
+__device__ __forceinline__ uint32_t lane_rows(const NormPlace &w, uint32_t lane) {
+  return w.base + (lane < w.rest ? 1u : 0u);
+}
 
 template <int V>
 __device__ __forceinline__ NormPlace norm_place(const NormGeom &p) {
   NormPlace w;
-  const uint32_t cluster = blockIdx.x / static_cast<uint32_t>(p.slices);
+  const uint32_t cluster = fdiv(blockIdx.x, p.div_slices);
   w.rank = static_cast<int>(blockIdx.x - cluster * p.slices);
-  const uint32_t at = cluster / static_cast<uint32_t>(p.chunks);
+  const uint32_t at = fdiv(cluster, p.div_chunks);
   w.chunk = cluster - at * p.chunks;
-  w.image = at / static_cast<uint32_t>(p.strips);
-  w.strip = static_cast<int>(at - w.image * p.strips);
+  w.image = fdiv(at, p.div_strips);
+  w.strip = static_cast<int>(at - static_cast<uint32_t>(w.image) * p.strips);
   w.g0 = w.strip * p.gs;
   w.gsl = min(p.gs, p.groups - w.g0);
   w.cw = w.gsl * p.cg;
-  w.nv = w.cw / V;
+  const int last = w.gsl < p.gs ? 1 : 0;
+  w.nv = static_cast<int>(p.div_nv[last].d);
+  w.lanes = static_cast<int>(p.div_lanes[last].d);
   const int threads = static_cast<int>(blockDim.x), t = static_cast<int>(threadIdx.x);
-  w.lanes = w.nv <= threads ? threads / w.nv : 1;
-  w.lane = w.nv <= threads ? t / w.nv : 0;
-  w.col = w.nv <= threads ? t - w.lane * w.nv : t;
+  w.lane = w.nv <= threads ? static_cast<int>(fdiv(t, p.div_nv[last])) : 0;
+  w.col = t - w.lane * w.nv;
   w.active = w.lane < w.lanes && w.col < w.nv;
   const uint64_t first =
       (static_cast<uint64_t>(w.chunk) * p.slices + w.rank) * static_cast<uint64_t>(p.cta_rows);
   w.r0 = first < p.hw ? static_cast<uint32_t>(first) : p.hw;
   w.rows = min(p.cta_rows, p.hw - w.r0);
+  w.base = fdiv(w.rows, p.div_lanes[last]);
+  w.rest = w.rows - w.base * w.lanes;
+  w.mine = w.active ? lane_rows(w, w.lane) : 0;
   return w;
 }
 

@@ -23,63 +23,104 @@ struct GradArgs {
   float2 *groups;            // [n * chunks][groups]: A, B (two passes)
 };
 
-// xh, z and dz of one pack's channels.
+template <typename T, int V>
+__device__ __forceinline__ void unpack_pairs(const Pack<T, V> &p, float2 (&v)[(V + 1) / 2]) {
+  if constexpr (V == 1) {
+    v[0] = both(to_float(p.e[0]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) v[j / 2] = make_float2(to_float(p.e[j]), to_float(p.e[j + 1]));
+  }
+}
+
+// xh and dz of one pack's channels, pairs of channels together.
 template <typename T, int V, int kAct>
 struct Chain {
-  float mean[V], rstd[V], gamma[V], beta[V];
+  static constexpr int kPairs = (V + 1) / 2;
+  float2 minus_mean[kPairs], rstd[kPairs], gamma[kPairs], beta[kPairs];
 
+  // `each(j, group)` is called for the pack's channels with their groups.
+  template <typename F>
   __device__ __forceinline__ void set(const NormGeom &p, int ch, const float *gmean,
-                                      const float *grstd, const float *ga, const float *be) {
+                                      const float *grstd, const float *ga, const float *be,
+                                      F each) {
+    float m[V], r[V];
+    int g = static_cast<int>(fdiv(static_cast<uint32_t>(ch), p.div_cg)), left = (g + 1) * p.cg - ch;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const uint32_t g = fdiv(static_cast<uint32_t>(ch + j), p.div_cg);
-      mean[j] = gmean[g];
-      rstd[j] = grstd[g];
-      gamma[j] = ga[ch + j];
-      beta[j] = be[ch + j];
+      m[j] = -gmean[g];
+      r[j] = grstd[g];
+      each(j, g);
+      if (--left == 0) {
+        left = p.cg;
+        if (j + 1 < V) ++g;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      const int k = V == 1 ? 0 : 2 * j + 1;
+      minus_mean[j] = make_float2(m[2 * j], m[k]);
+      rstd[j] = make_float2(r[2 * j], r[k]);
+      gamma[j] = make_float2(ga[ch + 2 * j], ga[ch + k]);
+      beta[j] = make_float2(be[ch + 2 * j], be[ch + k]);
     }
   }
   __device__ __forceinline__ void operator()(const Pack<T, V> &x, const Pack<T, V> &dy,
-                                             const NormGeom &p, float (&xh)[V],
-                                             float (&dz)[V]) const {
-    unpack(x, xh);
+                                             const NormGeom &p, float2 (&xh)[kPairs],
+                                             float2 (&dz)[kPairs]) const {
+    unpack_pairs(x, xh);
+    float z[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean[j]) * rstd[j];
+    for (int j = 0; j < kPairs; ++j) {
+      xh[j] = mul2(add2(xh[j], minus_mean[j]), rstd[j]);
+      const float2 v = fma2(gamma[j], xh[j], beta[j]);
+      z[2 * j] = v.x;
+      if (V > 1) z[2 * j + (V > 1 ? 1 : 0)] = v.y;
+    }
+    act_slope_array<T>(z, kAct >= 0 ? kAct : p.act, p.alpha);
+    unpack_pairs(dy, dz);
 #pragma unroll
-    for (int j = 0; j < V; ++j) dz[j] = fmaf(gamma[j], xh[j], beta[j]);
-    act_slope_array<T>(dz, kAct >= 0 ? kAct : p.act, p.alpha);
-    float d[V];
-    unpack(dy, d);
-#pragma unroll
-    for (int j = 0; j < V; ++j) dz[j] *= d[j];
+    for (int j = 0; j < kPairs; ++j)
+      dz[j] = mul2(dz[j], make_float2(z[2 * j], z[V == 1 ? 0 : 2 * j + 1]));
   }
 };
 
-// dx of one pack from its chain and the group's sums over M.
+// dx of one pack from its chain and the group's sums over M:
+// rstd gamma * dz - (rstd A + xh rstd B).
 template <typename T, int V, int kAct>
 struct Input {
+  static constexpr int kPairs = (V + 1) / 2;
   Chain<T, V, kAct> chain;
-  float a[V], b[V];  // A / M, B / M
+  float2 a[kPairs], b[kPairs];  // -rstd A / M, -rstd B / M
 
   __device__ __forceinline__ void set(const NormGeom &p, int ch, const float *gmean,
                                       const float *grstd, const float *ga, const float *be,
                                       const float2 *ab) {
-    chain.set(p, ch, gmean, grstd, ga, be);
+    float u[V], v[V];
+    chain.set(p, ch, gmean, grstd, ga, be, [&](int j, int g) {
+      u[j] = -grstd[g] * ab[g].x;
+      v[j] = -grstd[g] * ab[g].y;
+    });
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float2 v = ab[fdiv(static_cast<uint32_t>(ch + j), p.div_cg)];
-      a[j] = v.x;
-      b[j] = v.y;
+    for (int j = 0; j < kPairs; ++j) {
+      const int k = V == 1 ? 0 : 2 * j + 1;
+      a[j] = make_float2(u[2 * j], u[k]);
+      b[j] = make_float2(v[2 * j], v[k]);
     }
   }
   __device__ __forceinline__ Pack<T, V> operator()(const Pack<T, V> &x, const Pack<T, V> &dy,
                                                    const NormGeom &p) const {
-    float xh[V], dz[V];
+    float2 xh[kPairs], dz[kPairs];
     chain(x, dy, p, xh, dz);
+    float o[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      dz[j] = chain.rstd[j] * (chain.gamma[j] * dz[j] - fmaf(xh[j], b[j], a[j]));
-    return pack<T, V>(dz);
+    for (int j = 0; j < kPairs; ++j) {
+      const float2 d =
+          fma2(mul2(chain.rstd[j], chain.gamma[j]), dz[j], fma2(xh[j], b[j], a[j]));
+      o[2 * j] = d.x;
+      if (V > 1) o[2 * j + (V > 1 ? 1 : 0)] = d.y;
+    }
+    return pack<T, V>(o);
   }
 };
 
@@ -113,7 +154,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 template <typename T, int V, int kAct, bool kKeep>
-__global__ void __launch_bounds__(norm_most_threads(V), 2)
+__global__ void __launch_bounds__(kNormMostThreads, 2)
     norm_grad_kernel(NormGeom p, GradArgs g, const T *dy, const T *x, T *dx) {
   extern __shared__ __align__(16) uint8_t smem[];
   const NormPlace w = norm_place<V>(p);
@@ -128,9 +169,7 @@ __global__ void __launch_bounds__(norm_most_threads(V), 2)
   const int64_t row0 = w.image * p.hw + w.r0;
   const T *xs = x + row0 * p.ldx + c0, *ds = dy + row0 * p.lddy + c0;
   const uint32_t lanes = static_cast<uint32_t>(w.lanes);
-  const uint32_t mine = w.active && w.rows > static_cast<uint32_t>(w.lane)
-                            ? (w.rows - w.lane + lanes - 1) / lanes
-                            : 0;
+  const uint32_t mine = w.mine;
   const uint32_t step = (mine + 3) / 4;
   // The thread's first row, and from one of its rows to the next.
   const int first = w.lane * w.nv, turn = w.lanes * w.nv;
@@ -161,17 +200,18 @@ __global__ void __launch_bounds__(norm_most_threads(V), 2)
   __syncthreads();
   for (int col = w.active ? w.col : w.nv; col < w.nv; col += blockDim.x) {
     Chain<T, V, kAct> chain;
-    chain.set(p, col * V, s.gmean, s.grstd, s.gamma, s.beta);
-    float sp[V], sq[V];
+    chain.set(p, col * V, s.gmean, s.grstd, s.gamma, s.beta, [](int, int) {});
+    constexpr int kPairs = (V + 1) / 2;
+    float2 sp[kPairs], sq[kPairs];
 #pragma unroll
-    for (int j = 0; j < V; ++j) sp[j] = sq[j] = 0.0f;
+    for (int j = 0; j < kPairs; ++j) sp[j] = sq[j] = both(0.0f);
     auto add = [&](const Pack<T, V> &a, const Pack<T, V> &b) {
-      float xh[V], dz[V];
+      float2 xh[kPairs], dz[kPairs];
       chain(a, b, p, xh, dz);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        sp[j] += dz[j];
-        sq[j] = fmaf(dz[j], xh[j], sq[j]);
+      for (int j = 0; j < kPairs; ++j) {
+        sp[j] = add2(sp[j], dz[j]);
+        sq[j] = fma2(dz[j], xh[j], sq[j]);
       }
     };
     if constexpr (kKeep) {
@@ -206,8 +246,8 @@ __global__ void __launch_bounds__(norm_most_threads(V), 2)
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      s.q[w.lane * w.cw + col * V + j] = sq[j];
-      s.p[w.lane * w.cw + col * V + j] = sp[j];
+      s.q[w.lane * w.cw + col * V + j] = (j & 1) ? sq[j / 2].y : sq[j / 2].x;
+      s.p[w.lane * w.cw + col * V + j] = (j & 1) ? sp[j / 2].y : sp[j / 2].x;
     }
   }
   __syncthreads();
@@ -235,37 +275,42 @@ __global__ void __launch_bounds__(norm_most_threads(V), 2)
   if (p.slices > 1) cluster_sync();
   else __syncthreads();
   const float inv = 1.0f / (static_cast<float>(p.hw) * static_cast<float>(p.cg));
-  for (int i = threadIdx.x; i < w.gsl; i += blockDim.x) {
-    float2 t = s.group[i];
-    if (p.slices > 1) {
-      t = make_float2(0.0f, 0.0f);
-      for (int k = 0; k < p.slices; ++k) {
-        const uint32_t at = mapa_shared(smem_u32(&s.group[i]), static_cast<uint32_t>(k));
-        t.x += __uint_as_float(ld_shared_cluster_u32(at));
-        t.y += __uint_as_float(ld_shared_cluster_u32(at + 4));
-      }
+  // 8 lanes a group: one round trip to all CTAs of the cluster.
+  for (int i = threadIdx.x; i < (w.gsl * 8 + 31) / 32 * 32; i += blockDim.x) {
+    const int at = i >> 3, k = i & 7;
+    float2 t = make_float2(0.0f, 0.0f);
+    if (at < w.gsl && k < p.slices) {
+      const uint32_t from = mapa_shared(smem_u32(&s.group[at]), static_cast<uint32_t>(k));
+      t = make_float2(__uint_as_float(ld_shared_cluster_u32(from)),
+                      __uint_as_float(ld_shared_cluster_u32(from + 4)));
     }
-    if (kKeep) s.total[i] = make_float2(t.x * inv, t.y * inv);
-    else if (w.rank == 0)
-      g.groups[(w.image * p.chunks + w.chunk) * p.groups + w.g0 + i] = t;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) {
+      t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+      t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+    }
+    if (at < w.gsl && k == 0) {
+      if (kKeep) s.total[at] = make_float2(t.x * inv, t.y * inv);
+      else if (w.rank == 0)
+        g.groups[(w.image * p.chunks + w.chunk) * p.groups + w.g0 + at] = t;
+    }
   }
   if (g.channels) {
     // Each CTA adds its share of the channels over the cluster.
     float *out = g.channels + (w.image * p.chunks + w.chunk) * 2 * p.c + c0;
     for (int ch = w.rank * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x); ch < w.cw;
          ch += p.slices * static_cast<int>(blockDim.x)) {
-      float q = s.q[ch], b = s.p[ch];
-      if (p.slices > 1) {
-        q = b = 0.0f;
-        for (int k = 0; k < p.slices; ++k) {
-          q += __uint_as_float(ld_shared_cluster_u32(
-              mapa_shared(smem_u32(&s.q[ch]), static_cast<uint32_t>(k))));
-          b += __uint_as_float(ld_shared_cluster_u32(
-              mapa_shared(smem_u32(&s.p[ch]), static_cast<uint32_t>(k))));
-        }
+      float q[8], b[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool in = k < p.slices;
+        const uint32_t r = in ? static_cast<uint32_t>(k) : 0u;
+        q[k] = __uint_as_float(ld_shared_cluster_u32(mapa_shared(smem_u32(&s.q[ch]), r)));
+        b[k] = __uint_as_float(ld_shared_cluster_u32(mapa_shared(smem_u32(&s.p[ch]), r)));
+        if (!in) q[k] = b[k] = 0.0f;
       }
-      out[ch] = q;
-      out[p.c + ch] = b;
+      out[ch] = ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+      out[p.c + ch] = ((b[0] + b[1]) + (b[2] + b[3])) + ((b[4] + b[5]) + (b[6] + b[7]));
     }
   }
   if constexpr (kKeep) {
@@ -285,75 +330,95 @@ __global__ void __launch_bounds__(norm_most_threads(V), 2)
   if (p.slices > 1) cluster_sync_relaxed();  // no CTA leaves while another reads its sums
 }
 
-// Second pass, rows from the image's end.
+// Second pass, rows from the image's end; the first ones are asked for before the
+// chunks' sums are added.
 template <typename T, int V, int kAct>
-__global__ void __launch_bounds__(norm_most_threads(V), 2)
+__global__ void __launch_bounds__(kNormMostThreads, 2)
     norm_grad_apply_kernel(NormGeom p, GradArgs g, const T *dy, const T *x, T *dx,
-                           int apply_chunks, uint32_t apply_rows) {
+                           FastDiv apply_chunks, uint32_t apply_rows) {
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t at = gridDim.x - 1 - blockIdx.x;
-  const uint32_t piece = at / static_cast<uint32_t>(apply_chunks);
-  const uint32_t chunk = at - piece * apply_chunks;
-  const int64_t image = piece / static_cast<uint32_t>(p.strips);
-  const int g0 = static_cast<int>(piece - image * p.strips) * p.gs;
-  const int gsl = min(p.gs, p.groups - g0), cw = gsl * p.cg, nv = cw / V, c0 = g0 * p.cg;
-  float2 *total = reinterpret_cast<float2 *>(smem);
+  const uint32_t piece = fdiv(at, apply_chunks);
+  const uint32_t chunk = at - piece * apply_chunks.d;
+  const int64_t image = fdiv(piece, p.div_strips);
+  const int g0 = static_cast<int>(piece - static_cast<uint32_t>(image) * p.strips) * p.gs;
+  const int gsl = min(p.gs, p.groups - g0), cw = gsl * p.cg, c0 = g0 * p.cg;
+  const int last = gsl < p.gs ? 1 : 0;
+  const int nv = static_cast<int>(p.div_nv[last].d);
+  const uint32_t lanes = p.div_lanes[last].d;
+  float2 *chunks = reinterpret_cast<float2 *>(smem);  // [chunks][gsl]
+  float2 *total = chunks + p.chunks * p.gs;
   float *gmean = reinterpret_cast<float *>(total + p.gs), *grstd = gmean + p.gs;
   float *gamma = grstd + p.gs, *beta = gamma + p.gs * p.cg;
+  const int threads = static_cast<int>(blockDim.x), t = static_cast<int>(threadIdx.x);
+  const uint32_t rl = nv <= threads ? fdiv(t, p.div_nv[last]) : 0;
+  int col = t - static_cast<int>(rl) * nv;
+  const uint64_t begin = static_cast<uint64_t>(chunk) * apply_rows;
+  const uint32_t r0 = begin < p.hw ? static_cast<uint32_t>(begin) : p.hw;
+  const uint32_t rows = min(apply_rows, p.hw - r0);
+  const int64_t row = image * p.hw + r0 + rl;
+  const int64_t xp = static_cast<int64_t>(lanes) * p.ldx, dp = static_cast<int64_t>(lanes) * p.lddy,
+                op = static_cast<int64_t>(lanes) * p.ldy;
+  const T *xc = x + row * p.ldx + c0 + col * V, *dc = dy + row * p.lddy + c0 + col * V;
+  T *oc = dx + row * p.ldy + c0 + col * V;
+  if (rl >= lanes) col = nv;
   griddep_wait();
   griddep_launch_dependents();
-  for (int i = threadIdx.x; i < cw; i += blockDim.x) {
+  Pack<T, V> xv[2], dv[2];
+  auto ask = [&](const T *xf, const T *df, uint32_t r) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (r + i * lanes < rows) {
+        xv[i] = load_pack<T, V>(xf + i * xp);
+        dv[i] = load_pack<T, V>(df + i * dp);
+      }
+  };
+  if (col < nv) ask(xc, dc, rl);
+  for (int i = t; i < cw; i += threads) {
     gamma[i] = p.gamma ? p.gamma[c0 + i] : 1.0f;
     beta[i] = p.beta ? p.beta[c0 + i] : 0.0f;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = t; i < gsl; i += threads) {
+    gmean[i] = g.mean[image * p.groups + g0 + i];
+    grstd[i] = g.rstd[image * p.groups + g0 + i];
+  }
+  const int warp = t >> 5, lane = t & 31, warps = threads >> 5;
+  for (int k = warp; k < p.chunks; k += warps)
+    for (int i = lane; i < gsl; i += 32)
+      chunks[k * gsl + i] = g.groups[(image * p.chunks + k) * p.groups + g0 + i];
+  __syncthreads();
   const float inv = 1.0f / (static_cast<float>(p.hw) * static_cast<float>(p.cg));
-  for (int i = warp; i < gsl; i += static_cast<int>(blockDim.x) >> 5) {
-    const float2 *from = g.groups + image * p.chunks * p.groups + g0 + i;
+  for (int i = warp; i < gsl; i += warps) {
     float a = 0.0f, b = 0.0f;
     for (int k = lane; k < p.chunks; k += 32) {
-      const float2 v = from[static_cast<int64_t>(k) * p.groups];
-      a += v.x;
-      b += v.y;
+      a += chunks[k * gsl + i].x;
+      b += chunks[k * gsl + i].y;
     }
     a = warp_sum(a);
     b = warp_sum(b);
-    if (lane == 0) {
-      total[i] = make_float2(a * inv, b * inv);
-      gmean[i] = g.mean[image * p.groups + g0 + i];
-      grstd[i] = g.rstd[image * p.groups + g0 + i];
-    }
+    if (lane == 0) total[i] = make_float2(a * inv, b * inv);
   }
   __syncthreads();
-  const int threads = static_cast<int>(blockDim.x), t = static_cast<int>(threadIdx.x);
-  const uint32_t lanes = nv <= threads ? threads / nv : 1;
-  const uint32_t rl = nv <= threads ? t / nv : 0;
-  const int first_col = nv <= threads ? t - static_cast<int>(rl) * nv : t;
-  const uint64_t begin = static_cast<uint64_t>(chunk) * apply_rows;
-  if (begin >= p.hw || rl >= lanes) return;
-  const uint32_t r0 = static_cast<uint32_t>(begin), rows = min(apply_rows, p.hw - r0);
-  const int64_t row0 = image * p.hw + r0;
-  for (int col = first_col; col < nv; col += threads) {
+  for (bool first = true; col < nv;
+       col += threads, xc += threads * V, dc += threads * V, oc += threads * V, first = false) {
     Input<T, V, kAct> f;
     f.set(p, col * V, gmean, grstd, gamma, beta, total);
-    const T *xc = x + row0 * p.ldx + c0 + col * V, *dc = dy + row0 * p.lddy + c0 + col * V;
-    T *oc = dx + row0 * p.ldy + c0 + col * V;
-    const int64_t xp = static_cast<int64_t>(lanes) * p.ldx, dp = static_cast<int64_t>(lanes) * p.lddy,
-                  op = static_cast<int64_t>(lanes) * p.ldy;
-    xc += static_cast<int64_t>(rl) * p.ldx;
-    dc += static_cast<int64_t>(rl) * p.lddy;
-    oc += static_cast<int64_t>(rl) * p.ldy;
-    for (uint32_t r = rl; r < rows; r += 2 * lanes, xc += 2 * xp, dc += 2 * dp, oc += 2 * op) {
+    if (!first) ask(xc, dc, rl);
+    const T *xf = xc, *df = dc;
+    T *to = oc;
+    for (uint32_t r = rl; r < rows; r += 2 * lanes, to += 2 * op) {
       Pack<T, V> a[2], b[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (r + i * lanes < rows) {
-          a[i] = load_pack<T, V>(xc + i * xp);
-          b[i] = load_pack<T, V>(dc + i * dp);
-        }
+      for (int i = 0; i < 2; ++i) {
+        a[i] = xv[i];
+        b[i] = dv[i];
+      }
+      xf += 2 * xp;
+      df += 2 * dp;
+      if (r + 2 * lanes < rows) ask(xf, df, r + 2 * lanes);  // the next ones, under these
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (r + i * lanes < rows) store_pack(oc + i * op, f(a[i], b[i], p));
+        if (r + i * lanes < rows) store_pack(to + i * op, f(a[i], b[i], p));
     }
   }
 }
@@ -412,10 +477,11 @@ int run_grad(cudaStream_t s, int64_t n, const NormPlan &plan, GradArgs args, con
                                g.slices, s, g, a, di, xi, oi))
         return rc;
       const uint32_t rows = static_cast<uint32_t>(ceil_div(g.hw, plan.apply_chunks));
-      const int smem = (4 * g.gs + 2 * cw) * static_cast<int>(sizeof(float));
+      const int smem =
+          (2 * g.chunks * g.gs + 4 * g.gs + 2 * cw) * static_cast<int>(sizeof(float));
       if (int rc = norm_launch(norm_grad_apply_kernel<T, V, kAct>,
                                count * g.strips * plan.apply_chunks, plan.threads, smem, 1, s, g, a,
-                               di, xi, oi, plan.apply_chunks, rows))
+                               di, xi, oi, make_fastdiv(static_cast<uint32_t>(plan.apply_chunks)), rows))
         return rc;
     }
     return kOk;

@@ -89,6 +89,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return reinterpret_cast<const float2 &>(r);
 }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+  return reinterpret_cast<const float2 &>(r);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // Loads with no reuse in L1 (each value is read once by one thread). Not the
 // non-coherent path: the destination may be the source.
 template <typename T, int V>
