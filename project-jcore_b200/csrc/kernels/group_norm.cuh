@@ -1,11 +1,13 @@
-// What the group norm kernels share: the work split and its plan.
+// What the group norm kernels share: the work split, its plan, and how a CTA's
+// rows come into shared memory.
 //
 // An image's channels are cut into strips of whole groups; a cluster of CTAs
-// takes one strip of one image (or a run of its rows), each CTA a run of rows.
-// In a CTA, a row's strip is nv packs of V channels; thread t has pack t % nv
-// of rows t / nv, t / nv + lanes, ... (lanes = threads / nv), so that a
-// thread's channels never change and consecutive threads read consecutive
-// memory. A strip of more packs than threads takes several turns (lanes = 1).
+// takes a strip of an image (or of a run of its rows), each CTA a run of rows,
+// which come into its shared memory as [row][pitch]. A row's strip is nv packs of
+// V channels; thread t has pack t % nv of rows t / nv, t / nv + lanes, ... (lanes =
+// threads / nv), so that a thread's channels never change and consecutive threads
+// read consecutive memory. A strip of more packs than threads takes several turns
+// (lanes = 1).
 #pragma once
 
 #include <algorithm>
@@ -18,54 +20,51 @@
 
 namespace nplk {
 
+constexpr int kNormThreads = 256;  // at most
+constexpr int kNormStages = 4;     // steps in which a CTA's rows arrive
+
 struct NormGeom {
   int64_t ldx, ldy, lddy;  // pitches of x, of the output, of dy
   uint32_t hw;
   int c, groups, cg;
-  int gs, strips;       // groups of a strip; strips of an image
-  int slices;           // CTAs of a cluster
-  int chunks;           // clusters that share a strip's rows
-  uint32_t cta_rows;    // rows of a CTA
+  int gs, strips;      // groups of a strip; strips of an image
+  int slices, chunks;  // CTAs of a cluster; clusters that share a strip's rows
+  uint32_t cta_rows;   // rows of a CTA
+  int pitch;           // channels of a full strip: a row's elements in shared memory
+  int box_rows, boxes; // rows of a TMA box and boxes of a stage; 0: copied by the threads
+  uint32_t stage_rows;
   FastDiv div_cg, div_slices, div_chunks, div_strips;
   FastDiv div_nv[2], div_lanes[2];  // packs and row lanes of a strip; of the last strip
   const float *gamma, *beta;
   float eps, alpha;
   int act;
+  int *status;
 };
 
 struct NormPlan {
   NormGeom g;
-  int v;            // elements of a pack
-  bool keep;        // the strip stays in the cluster's shared memory
+  int v;          // elements of a pack
+  bool keep;      // a cluster holds the strip's rows: one launch
   int threads;
-  int64_t batch;    // images of a launch
-  int apply_chunks; // second pass: CTAs per image and strip
+  int64_t batch;  // images of a launch
 };
 
-// Most threads of a CTA. A thread keeps its channels' constants and sums in
-// registers (60 to 80 of them forward, up to 128 in the gradient), so an SM holds
-// 24 and 16 warps.
-constexpr int kNormMostThreads = 256;
-
-// Workspace: per image and chunk, sums per channel and group.
-constexpr int kNormMostChunks = 74;
+// Clusters that share a strip's rows when it is not kept, at most.
 inline int64_t norm_most_chunks(int64_t hw) {
   const int64_t by_rows = ceil_div(hw, 64);
-  return by_rows < kNormMostChunks ? by_rows : kNormMostChunks;
+  return by_rows < 512 ? by_rows : 512;
 }
 
-// Bytes of shared memory beside the kept strips (norm_smem below).
+// Bytes of shared memory beside the rows (the layouts of both kernels fit it).
 inline int norm_tail_bytes(int threads, int v, int cw, int gs) {
-  const int acc = threads * v > cw ? threads * v : cw;  // per row lane and channel
-  const int teams = gs > 32 ? gs : 32;
-  return 2 * acc * 4 + 2 * cw * 4 + teams * 16 + gs * 16 + 2 * gs * 4 + 64;
+  const int acc = threads * v > cw ? threads * v : cw;
+  return 2 * acc * 4 + 4 * cw * 4 + (gs > 32 ? gs : 32) * 16 + 9 * gs * 16 + 2 * gs * 4 + 256;
 }
-
-// Shared memory of a CTA of the kept form: two fit an SM.
+// Of a CTA that keeps its rows: two fit an SM.
 constexpr int kNormKeepLimit = 112 * 1024;
 
-// The divisions that the kernels do by multiplication, for the plan's split.
-inline void norm_divisors(NormPlan &p) {
+// The divisions that the kernels do by multiplication, and how rows arrive.
+inline void norm_finish(NormPlan &p, int64_t n, int size) {
   NormGeom &g = p.g;
   g.div_slices = make_fastdiv(static_cast<uint32_t>(g.slices));
   g.div_chunks = make_fastdiv(static_cast<uint32_t>(g.chunks));
@@ -76,9 +75,26 @@ inline void norm_divisors(NormPlan &p) {
     g.div_nv[last] = make_fastdiv(static_cast<uint32_t>(nv));
     g.div_lanes[last] = make_fastdiv(static_cast<uint32_t>(nv <= p.threads ? p.threads / nv : 1));
   }
+  g.pitch = g.gs * g.cg;
+  // TMA boxes where packs are of 16 bytes (then pitches and strips are too), a row
+  // fits a box and row numbers 32 bits; boxes of whole 8 rows start 128-byte aligned.
+  const int64_t each = ceil_div(g.cta_rows, kNormStages);
+  g.boxes = 0;
+  g.stage_rows = static_cast<uint32_t>(each);
+  if (p.v * size == 16 && g.pitch <= 256 && n * g.hw < (int64_t(1) << 31) - 1024) {
+    g.boxes = static_cast<int>(ceil_div(each, 256));
+    g.box_rows = static_cast<int>(ceil_div(ceil_div(each, g.boxes), 8) * 8);
+    g.stage_rows = static_cast<uint32_t>(g.box_rows * g.boxes);
+  }
 }
 
-// `tensors`: strips that the kept form holds (x; or x and dy).
+// Bytes of a CTA's rows of one tensor.
+inline int64_t norm_rows_bytes(const NormGeom &g, int size) {
+  const int64_t rows = g.boxes ? static_cast<int64_t>(g.stage_rows) * kNormStages : g.cta_rows;
+  return (rows * g.pitch * size + 127) / 128 * 128;
+}
+
+// `tensors`: what is read (x; or x and dy).
 inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int size, int v_fit,
                           int tensors) {
   NormPlan p{};
@@ -103,11 +119,18 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   p.g.groups = static_cast<int>(groups);
   p.g.cg = cg;
   p.g.div_cg = make_fastdiv(static_cast<uint32_t>(cg));
+  auto row = [&](int gs) { return static_cast<int64_t>(gs) * cg * size; };
+  auto threads_for = [&](int64_t rows, int cw) {
+    // Six packs a thread: what a thread does once costs as much as some packs.
+    int64_t t = ceil_div(ceil_div(rows * (cw / v), 6), 32) * 32;
+    t = std::max<int64_t>(t, ceil_div(cw / v, 32) * 32);
+    return static_cast<int>(std::min<int64_t>(std::max<int64_t>(t, 64), kNormThreads));
+  };
 
   // Kept form: strips of at least 64 bytes a row; of those up to 512 bytes, the
   // narrowest in whole 32-byte sectors if 48 KB in each of 8 CTAs hold it, else the
-  // narrowest.
-  auto row = [&](int gs) { return static_cast<int64_t>(gs) * cg * size; };
+  // narrowest. Up to 48 KB a CTA keeps several on an SM, so that one's loads run
+  // under another's stores; more CTAs while they are few.
   int gs = gs0;
   while (gs + gs0 <= groups && row(gs) < 64) gs += gs0;
   for (int m = gs; m <= groups && row(m) <= 512; m += gs0) {
@@ -119,55 +142,43 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   p.g.gs = gs;
   p.g.strips = static_cast<int>(ceil_div(groups, gs));
   p.g.chunks = 1;
-  const int cw = gs * cg;
-  const int64_t row_bytes = static_cast<int64_t>(cw) * size * tensors;
   int s = 1;
-  auto slab = [&](int slices) { return ceil_div(hw, slices) * row_bytes; };
-  // Up to 48 KB a CTA keeps four on an SM, so that one's loads run under another's
-  // stores; more CTAs while they are few.
+  auto slab = [&](int slices) { return ceil_div(hw, slices) * row(gs) * tensors; };
   const int64_t ctas = n * p.g.strips;
   while (s < 8 && (slab(s) > 48 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sms))) s *= 2;
   p.g.slices = s;
   p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, s));
-  constexpr int most = kNormMostThreads;
-  // Six packs a thread: what a thread does once costs as much as 40 values.
-  const int64_t packs = p.g.cta_rows * static_cast<int64_t>(cw / v);
-  int64_t threads = ceil_div(ceil_div(packs, 6), 32) * 32;
-  if (threads < cw / v) threads = ceil_div(cw / v, 32) * 32;
-  p.threads = static_cast<int>(threads < 64 ? 64 : threads > most ? most : threads);
-  p.keep = slab(s) + norm_tail_bytes(p.threads, v, cw, gs) <= kNormKeepLimit;
-  if (p.keep) {
-    norm_divisors(p);
+  p.threads = threads_for(p.g.cta_rows, gs * cg);
+  norm_finish(p, n, size);
+  if (tensors * norm_rows_bytes(p.g, size) + norm_tail_bytes(p.threads, v, gs * cg, gs) <=
+      kNormKeepLimit) {
+    p.keep = true;
     const int64_t most = ((int64_t(1) << 31) - 1) / (static_cast<int64_t>(p.g.strips) * s);
-    p.batch = n < most ? n : most;
+    p.batch = std::min(n, most);
     return p;
   }
 
-  // Two passes: whole rows where a CTA's threads hold one, else as many groups.
-  gs = static_cast<int>(groups);
-  if (c > most * v) gs = most * v / (gs0 * cg) * gs0;
-  if (gs > 512) gs = 512 / gs0 * gs0;
-  if (gs < gs0) gs = gs0;
+  // Two passes, the rows read by the threads: strips as wide as the CTA, eight rows
+  // a thread at once and no more where 4096 CTAs are enough, in clusters of 8: with
+  // many short CTAs at different points the memory stays busy (with one long CTA
+  // per slot all of them loaded, then all computed: 20 us against MEASURED for
+  // 34 MB). Images in batches whose tensors stay in L2 between the passes (a third
+  // of its 126 MB).
+  gs = gs0;
+  const int64_t widest = std::min<int64_t>(kNormThreads * v, INT32_MAX);
+  while (gs + gs0 <= groups && gs + gs0 <= 256 && static_cast<int64_t>(gs + gs0) * cg <= widest)
+    gs += gs0;
   p.g.gs = gs;
   p.g.strips = static_cast<int>(ceil_div(groups, gs));
-  p.threads = most;
-  // Images whose tensors stay in L2 between the passes (a third of its 126 MB).
-  const int64_t image = hw * c * size * tensors;
-  int64_t batch = (40 << 20) / image;
-  if (batch < 1) batch = 1;
-  p.batch = n < batch ? n : batch;
-  const int64_t wanted = static_cast<int64_t>(sms) * (tensors == 1 ? 3 : 2);
-  int64_t chunks = wanted / (8 * p.g.strips * p.batch);
-  if (chunks < 1) chunks = 1;
-  if (chunks > norm_most_chunks(hw)) chunks = norm_most_chunks(hw);
-  if (chunks > 1 && chunks * gs > 8192) chunks = 8192 / gs;  // 64 KB where they are joined
+  p.batch = std::min(n, std::max<int64_t>(1, (40 << 20) / (hw * c * size * tensors)));
   p.g.slices = 8;
+  p.threads = kNormThreads;
+  const int nv = gs * cg / v;
+  const int64_t rows = 8 * (nv <= p.threads ? p.threads / nv : 1);
+  const int64_t chunks = std::max<int64_t>(1, std::min(norm_most_chunks(hw), hw / (rows * 8)));
   p.g.chunks = static_cast<int>(chunks);
   p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, chunks * 8));
-  int64_t apply = ceil_div(wanted, p.g.strips * p.batch);
-  if (apply > hw) apply = hw;
-  p.apply_chunks = static_cast<int>(apply);
-  norm_divisors(p);
+  norm_finish(p, n, size);
   return p;
 }
 
@@ -187,8 +198,10 @@ inline int norm_check(int64_t n, int64_t hw, int64_t c, int64_t groups) {
   return kOk;
 }
 
+// Per image: chunks * (2 c + 2 groups) sums, and 4 per group that the second pass reads.
 inline size_t norm_workspace(int64_t n, int64_t hw, int64_t c, int64_t groups) {
-  return align_up(static_cast<size_t>(n) * norm_most_chunks(hw) * (2 * c + 2 * groups) * sizeof(float),
+  return align_up(static_cast<size_t>(n) *
+                      (norm_most_chunks(hw) * (2 * c + 2 * groups) + 4 * groups) * sizeof(float),
                   256);
 }
 
@@ -196,7 +209,7 @@ inline bool norm_aligned(const void *p, int bytes) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0;
 }
 
-// Where a CTA of the first pass is: image, strip, rows.
+// Where a CTA of the first pass is, and its thread.
 struct NormPlace {
   int64_t image, chunk;
   int strip, rank, g0, gsl, cw, nv, lanes, col, lane;  // col, lane: of this thread
@@ -209,7 +222,6 @@ __device__ __forceinline__ uint32_t lane_rows(const NormPlace &w, uint32_t lane)
   return w.base + (lane < w.rest ? 1u : 0u);
 }
 
-template <int V>
 __device__ __forceinline__ NormPlace norm_place(const NormGeom &p) {
   NormPlace w;
   const uint32_t cluster = fdiv(blockIdx.x, p.div_slices);
@@ -238,11 +250,64 @@ __device__ __forceinline__ NormPlace norm_place(const NormGeom &p) {
   return w;
 }
 
+// A CTA's rows of kTensors tensors on their way into shared memory: TMA boxes,
+// a barrier per stage, or copies by the threads that read them (counted in
+// cp.async groups, 2-byte packs at once).
+template <typename T, int V, int kTensors>
+struct RowLoads {
+  uint64_t *bars;           // [kNormStages]
+  volatile int *abort_flag;
+  int arrived;              // stages this thread has waited for
+
+  // Before griddep_wait; ends with a barrier.
+  __device__ __forceinline__ void prepare(const NormGeom &p, uint8_t *at) {
+    bars = reinterpret_cast<uint64_t *>(at);
+    abort_flag = reinterpret_cast<volatile int *>(bars + kNormStages);
+    arrived = 0;
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < kNormStages; ++s) mbar_init(&bars[s], 1);
+      *abort_flag = 0;
+      fence_mbar_init();
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ void start(const NormGeom &p, const NormPlace &w,
+                                        const CUtensorMap *const (&maps)[kTensors],
+                                        uint8_t *const (&to)[kTensors], int64_t first_image_row) {
+    if (!p.boxes || threadIdx.x != 0) return;
+    for (int s = 0; s < kNormStages; ++s) {
+      const uint32_t from = s * p.stage_rows;
+      if (from >= w.rows) break;
+      mbar_arrive_expect_tx(&bars[s], kTensors * p.stage_rows * p.pitch * sizeof(T));
+      for (int b = 0; b < p.boxes; ++b) {
+        const uint32_t r = from + b * p.box_rows;
+#pragma unroll
+        for (int k = 0; k < kTensors; ++k)
+          tma_load_2d(maps[k], &bars[s], to[k] + static_cast<size_t>(r) * p.pitch * sizeof(T),
+                      w.g0 * p.cg, static_cast<int>(first_image_row + w.r0 + r));
+      }
+    }
+  }
+  // Row r (of the CTA) and those before it have arrived.
+  __device__ __forceinline__ void wait(const NormGeom &p, uint32_t r) {
+    while (arrived < kNormStages && r >= arrived * p.stage_rows) {
+      mbar_wait(&bars[arrived], 0u, abort_flag, p.status, kStatusTimeoutStage);
+      ++arrived;
+    }
+  }
+  // Before the CTA's end: nothing is in flight (the threads have waited unless a
+  // wait expired).
+  __device__ __forceinline__ void drain(const NormGeom &p, const NormPlace &w) {
+    if (!p.boxes || threadIdx.x != 0 || !*abort_flag) return;
+    for (int s = 0; s < kNormStages; ++s)
+      if (s * p.stage_rows < w.rows) mbar_drain(&bars[s], 0u);
+  }
+};
+
 // Calls f(pack size, activation) with both as std::integral_constant: 16-byte
 // packs with the usual activations known to the compiler, everything else with
 // the activation as an argument (-1). With it as an argument the kernels hold
-// 118 registers across the calls of the rare ones instead of 40 to 80, which
-// halves the loads in flight on an SM.
+// 118 registers across the calls of the rare ones instead of 40 to 80.
 template <int kMost, typename F>
 int norm_with_pack(int v, int act, F f) {
   using std::integral_constant;
@@ -269,9 +334,11 @@ int norm_with_pack(int v, int act, F f) {
 }
 
 template <typename... KArgs, typename... Args>
-int norm_launch(void (*kernel)(KArgs...), int64_t grid, int threads, int smem, int cluster,
-                cudaStream_t s, Args... args) {
-  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), smem)) return rc;
+int norm_launch(void (*kernel)(KArgs...), int64_t grid, int threads, int64_t smem, int cluster,
+                cudaStream_t s, const Args &...args) {
+  if (grid > INT32_MAX) return kErrUnsupported;
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), static_cast<int>(smem)))
+    return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -180,6 +180,25 @@ int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, 
   return r == CUDA_SUCCESS ? kOk : kErrInternal;
 }
 
+int encode_tmap_2d_plain(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                         uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer,
+                         int element_bytes) {
+  auto fn = encode_fn();
+  if (!fn) return kErrInternal;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (row_pitch_bytes & 15u) != 0)
+    return kErrInvalidArg;
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {row_pitch_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, element_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                                          : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                  2, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? kOk : kErrInternal;
+}
+
 int encode_tmap_2d_box32(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer,
                          uint64_t row_pitch_bytes, int element_bytes) {
   auto fn = encode_fn();

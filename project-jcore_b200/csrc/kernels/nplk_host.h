@@ -67,6 +67,13 @@ int encode_tmap_2d_f32_sw128_atom32(CUtensorMap *map, const void *base, uint64_t
 int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
                             uint64_t row_pitch_bytes, uint32_t box_outer);
 
+// 2-D map for tensor loads of box_inner x box_outer boxes of 2- or 4-byte
+// elements, unswizzled: dims {inner, outer} elements, row pitch in bytes, zero
+// fill out of bounds. box_inner * element_bytes a multiple of 16.
+int encode_tmap_2d_plain(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                         uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer,
+                         int element_bytes);
+
 // 2-D map for tensor stores of 32 x 32 boxes of 2- or 4-byte elements: dims
 // {inner, outer} elements, row pitch in bytes; 2-byte boxes (rows of 64 bytes)
 // with the 64-byte swizzle, 4-byte boxes unswizzled.

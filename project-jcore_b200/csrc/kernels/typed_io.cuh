@@ -98,6 +98,17 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// The pack's values two by two (a lone one as both halves of one pair).
+template <typename T, int V>
+__device__ __forceinline__ void unpack_pairs(const Pack<T, V> &p, float2 (&v)[(V + 1) / 2]) {
+  if constexpr (V == 1) {
+    v[0] = both(to_float(p.e[0]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) v[j / 2] = make_float2(to_float(p.e[j]), to_float(p.e[j + 1]));
+  }
+}
+
 // Loads with no reuse in L1 (each value is read once by one thread). Not the
 // non-coherent path: the destination may be the source.
 template <typename T, int V>
