@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   const NormPlace w = norm_place(p);
   Pack<T, V> *strip = reinterpret_cast<Pack<T, V> *>(smem);
   const int64_t held = p.boxes ? static_cast<int64_t>(p.stage_rows) * kNormStages : p.cta_rows;
-  const size_t strip_bytes = kKeep ? (held * p.pitch * sizeof(T) + 127) / 128 * 128 : 0;
+  const size_t strip_bytes = kKeep ? (held * p.pitch * sizeof(T) + 127) / 128 * 128
+                                   : kNormRing * kNormThreads * sizeof(Pack<T, V>);
   const Shared s = norm_shared<V>(smem + strip_bytes, p);
   const int c0 = w.g0 * p.cg;
   const int64_t row0 = w.image * p.hw + w.r0;
@@ -331,35 +332,17 @@ __global__ void __launch_bounds__(kNormThreads, 3)
         join_rows(v, run);
       }
     } else {
-      // Eight rows asked for at a time, joined four by four.
-      uint32_t left = w.mine;
-      for (; left >= 8; left -= 8, from += 8 * pitch) {
-        Pack<T, V> a[4], b[4];
+      stream_rows<T, V, 1>(w.mine, {from}, {pitch}, strip, [&](const Pack<T, V>(&v)[1][4], int rows) {
+        if (rows == 4) {
+          join_rows(v[0], run);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = load_pack<T, V>(from + i * pitch);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = load_pack<T, V>(from + (4 + i) * pitch);
-        join_rows(a, run);
-        join_rows(b, run);
-      }
-      if (left) {
-        Pack<T, V> a[4], b[2], c[1];
-        const bool four = left & 4u, two = left & 2u, one = left & 1u;
-        if (four) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = load_pack<T, V>(from + i * pitch);
-          from += 4 * pitch;
+          for (int i = 0; i < 3; ++i) {
+            const Pack<T, V> one[1] = {v[0][i]};
+            if (i < rows) join_rows(one, run);
+          }
         }
-        if (two) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) b[i] = load_pack<T, V>(from + i * pitch);
-          from += 2 * pitch;
-        }
-        if (one) c[0] = load_pack<T, V>(from);
-        if (four) join_rows(a, run);
-        if (two) join_rows(b, run);
-        if (one) join_rows(c, run);
-      }
+      });
     }
     put_moments<V>(p, w, s, run, col);
   }
@@ -402,33 +385,37 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   }
 }
 
-// Joins the chunks' moments: a warp per image and group. mean and rstd to the
+// Joins the chunks' moments: a CTA per image and group. mean and rstd to the
 // caller and to stats.
-__global__ void __launch_bounds__(256)
-    norm_join_kernel(const NormGeom p, int64_t count, const float2 *partial, float *mean_out,
-                     float *rstd_out, float2 *stats) {
+__global__ void __launch_bounds__(128)
+    norm_join_kernel(const NormGeom p, const float2 *partial, float *mean_out, float *rstd_out,
+                     float2 *stats) {
+  __shared__ float4 warps[4];
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (at >= count) return;
-  const int64_t image = at / p.groups;
+  const int64_t at = blockIdx.x, image = at / p.groups;
   const float2 *from = partial + image * p.chunks * p.groups + (at - image * p.groups);
-  const uint64_t chunk_rows = static_cast<uint64_t>(p.cta_rows) * p.slices;
   Moments t{0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int k = lane; k < p.chunks; k += 32) {
-    const uint64_t first = k * chunk_rows;
-    const uint64_t rows = first < p.hw ? min(chunk_rows, p.hw - first) : 0;
+  for (int k = threadIdx.x; k < p.chunks; k += 128) {
+    const uint64_t first = static_cast<uint64_t>(k) * p.cta_rows;
+    const uint64_t rows = first < p.hw ? min(static_cast<uint64_t>(p.cta_rows), p.hw - first) : 0;
     const float2 v = from[static_cast<int64_t>(k) * p.groups];
     join_one(t, {static_cast<float>(rows) * static_cast<float>(p.cg), v.x, v.y});
   }
   t = join_lanes<32>(t);
-  if (lane == 0) {
-    const float rstd = 1.0f / sqrtf(t.m2 / t.n + p.eps);
-    if (mean_out) mean_out[at] = t.mean;
-    if (rstd_out) rstd_out[at] = rstd;
-    stats[at] = make_float2(t.mean, rstd);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) warps[warp] = make_float4(t.n, t.mean, t.m2, 0.0f);
+  __syncthreads();
+  if (warp == 0) {
+    const float4 v = lane < 4 ? warps[lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    t = join_lanes<32>({v.x, v.y, v.z});
+    if (lane == 0) {
+      const float rstd = 1.0f / sqrtf(t.m2 / t.n + p.eps);
+      if (mean_out) mean_out[at] = t.mean;
+      if (rstd_out) rstd_out[at] = rstd;
+      stats[at] = make_float2(t.mean, rstd);
+    }
   }
 }
 
@@ -490,7 +477,7 @@ int run_norm(cudaStream_t s, int64_t n, const NormPlan &plan, const T *x, T *y, 
   }
   return norm_with_pack<16 / sizeof(T)>(plan.v, g.act, [&](auto pack_size, auto act) {
     constexpr int V = decltype(pack_size)::value, kAct = decltype(act)::value;
-    const int tail = norm_tail_bytes(plan.threads, V, g.pitch, g.gs);
+    const int tail = norm_tail_bytes(plan.threads, V, g.pitch, g.gs, plan.keep);
     float2 *stats = work, *partial = work + plan.batch * g.groups;
     for (int64_t i = 0; i < n; i += plan.batch) {
       const int64_t count = std::min(n - i, plan.batch);
@@ -510,11 +497,11 @@ int run_norm(cudaStream_t s, int64_t n, const NormPlan &plan, const T *x, T *y, 
           return rc;
         continue;
       }
-      if (int rc = norm_launch(norm_kernel<T, V, 0, false>, ctas, plan.threads, tail, g.slices, s,
-                               map, g, xi, yi, nullptr, nullptr, partial))
+      if (int rc = norm_launch(norm_kernel<T, V, 0, false>, ctas, plan.threads,
+                               norm_ring_bytes(V, sizeof(T)) + tail, g.slices, s, map, g, xi, yi, nullptr, nullptr, partial))
         return rc;
-      if (int rc = norm_launch(norm_join_kernel, ceil_div(count * g.groups, 8), 256, 0, 1, s, g,
-                               count * g.groups, partial, mi, ri, stats))
+      if (int rc = norm_launch(norm_join_kernel, count * g.groups, 128, 0, 1, s, g, partial, mi, ri,
+                               stats))
         return rc;
       const uint32_t rows = std::min<uint32_t>(8 * g.div_lanes[0].d, g.hw);
       if (int rc = norm_launch(norm_apply_kernel<T, V, kAct>,

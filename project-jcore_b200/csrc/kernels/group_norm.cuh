@@ -28,7 +28,7 @@ struct NormGeom {
   uint32_t hw;
   int c, groups, cg;
   int gs, strips;      // groups of a strip; strips of an image
-  int slices, chunks;  // CTAs of a cluster; clusters that share a strip's rows
+  int slices, chunks;  // CTAs of a cluster; runs of rows of a strip that is not kept
   uint32_t cta_rows;   // rows of a CTA
   int pitch;           // channels of a full strip: a row's elements in shared memory
   int box_rows, boxes; // rows of a TMA box and boxes of a stage; 0: copied by the threads
@@ -49,16 +49,23 @@ struct NormPlan {
   int64_t batch;  // images of a launch
 };
 
-// Clusters that share a strip's rows when it is not kept, at most.
+// Runs of rows of a strip that is not kept, at most.
 inline int64_t norm_most_chunks(int64_t hw) {
   const int64_t by_rows = ceil_div(hw, 64);
-  return by_rows < 512 ? by_rows : 512;
+  return by_rows < 448 ? by_rows : 448;
 }
 
-// Bytes of shared memory beside the rows (the layouts of both kernels fit it).
-inline int norm_tail_bytes(int threads, int v, int cw, int gs) {
+// The passes over memory keep a ring of three batches of four packs per thread and
+// tensor in shared memory: while one batch is worked on the next two are on their way.
+constexpr int kNormRing = 12;
+inline int norm_ring_bytes(int v, int size) { return kNormRing * kNormThreads * v * size; }
+
+// Bytes of shared memory beside the rows (the layouts of both kernels fit it);
+// `shared`: in clusters, whose CTAs share out the channels' sums.
+inline int norm_tail_bytes(int threads, int v, int cw, int gs, bool shared) {
   const int acc = threads * v > cw ? threads * v : cw;
-  return 2 * acc * 4 + 4 * cw * 4 + (gs > 32 ? gs : 32) * 16 + 9 * gs * 16 + 2 * gs * 4 + 256;
+  return 2 * acc * 4 + 2 * cw * 4 + (shared ? 2 * (cw + 8) * 4 : 0) + (gs > 32 ? gs : 32) * 16 +
+         9 * gs * 16 + 2 * gs * 4 + 256;
 }
 // Of a CTA that keeps its rows: two fit an SM.
 constexpr int kNormKeepLimit = 112 * 1024;
@@ -150,7 +157,7 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, s));
   p.threads = threads_for(p.g.cta_rows, gs * cg);
   norm_finish(p, n, size);
-  if (tensors * norm_rows_bytes(p.g, size) + norm_tail_bytes(p.threads, v, gs * cg, gs) <=
+  if (tensors * norm_rows_bytes(p.g, size) + norm_tail_bytes(p.threads, v, gs * cg, gs, true) <=
       kNormKeepLimit) {
     p.keep = true;
     const int64_t most = ((int64_t(1) << 31) - 1) / (static_cast<int64_t>(p.g.strips) * s);
@@ -158,26 +165,20 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
     return p;
   }
 
-  // Two passes, the rows read by the threads: strips as wide as the CTA, eight rows
-  // a thread at once and no more where 4096 CTAs are enough, in clusters of 8: with
-  // many short CTAs at different points the memory stays busy (with one long CTA
-  // per slot all of them loaded, then all computed: 20 us against MEASURED for
-  // 34 MB). Images in batches whose tensors stay in L2 between the passes (a third
-  // of its 126 MB).
+  // Passes over memory: strips as wide as a CTA, one long run of rows for each CTA
+  // that the SMs hold at once. Images in batches whose tensors stay in L2 between
+  // the passes (a third of its 126 MB).
   gs = gs0;
-  const int64_t widest = std::min<int64_t>(kNormThreads * v, INT32_MAX);
-  while (gs + gs0 <= groups && gs + gs0 <= 256 && static_cast<int64_t>(gs + gs0) * cg <= widest)
-    gs += gs0;
+  while (gs + gs0 <= groups && gs + gs0 <= 256 && (gs + gs0) * cg <= kNormThreads * v) gs += gs0;
   p.g.gs = gs;
   p.g.strips = static_cast<int>(ceil_div(groups, gs));
   p.batch = std::min(n, std::max<int64_t>(1, (40 << 20) / (hw * c * size * tensors)));
-  p.g.slices = 8;
+  p.g.slices = 1;
   p.threads = kNormThreads;
-  const int nv = gs * cg / v;
-  const int64_t rows = 8 * (nv <= p.threads ? p.threads / nv : 1);
-  const int64_t chunks = std::max<int64_t>(1, std::min(norm_most_chunks(hw), hw / (rows * 8)));
-  p.g.chunks = static_cast<int>(chunks);
-  p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, chunks * 8));
+  const int64_t chunks =
+      static_cast<int64_t>(sms) * (tensors == 1 ? 3 : 2) / (p.g.strips * p.batch);
+  p.g.chunks = static_cast<int>(std::max<int64_t>(1, std::min(chunks, norm_most_chunks(hw))));
+  p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, p.g.chunks));
   norm_finish(p, n, size);
   return p;
 }
@@ -303,6 +304,41 @@ struct RowLoads {
       if (s * p.stage_rows < w.rows) mbar_drain(&bars[s], 0u);
   }
 };
+
+// Calls work(batch of packs, how many) for a thread's rows k = 0, 1, ... of kTensors
+// tensors, four at a time; from[i] + k * pitch[i] is row k. ring: the thread's own
+// slots are ring[i * kNormThreads + threadIdx.x], so it waits for its own copies only.
+template <typename T, int V, int kTensors, typename F>
+__device__ __forceinline__ void stream_rows(uint32_t count, const T *const (&from)[kTensors],
+                                            const int64_t (&pitch)[kTensors], Pack<T, V> *ring,
+                                            F work) {
+  auto ask = [&](uint32_t batch) {
+    const uint32_t slot = batch % 3 * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * batch + i < count)
+#pragma unroll
+        for (int t = 0; t < kTensors; ++t)
+          copy_pack_async<T, V>(ring + ((t * kNormRing + slot + i) * kNormThreads + threadIdx.x),
+                                from[t] + (4 * batch + i) * pitch[t]);
+    copy_async_commit();
+  };
+  ask(0);
+  ask(1);
+  for (uint32_t batch = 0; 4 * batch < count; ++batch) {
+    ask(batch + 2);
+    copy_async_wait<2>();
+    const uint32_t slot = batch % 3 * 4;
+    Pack<T, V> v[kTensors][4];
+#pragma unroll
+    for (int t = 0; t < kTensors; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[t][i] = ring[(t * kNormRing + slot + i) * kNormThreads + threadIdx.x];
+    work(v, static_cast<int>(min(4u, count - 4 * batch)));
+  }
+  copy_async_wait<0>();
+}
 
 // Calls f(pack size, activation) with both as std::integral_constant: 16-byte
 // packs with the usual activations known to the compiler, everything else with

@@ -127,7 +127,7 @@ struct GradShared {  // the dynamic shared memory, after the kept rows
   float2 *all;          // [8][gs]: A, B of the cluster's CTAs
   float *q, *p;         // [lanes][pitch]
   float *gamma, *beta;  // [pitch]
-  float *got;           // [8][share][2]: Q, P of this CTA's share of the channels
+  float *got;           // [slices][share][2], in clusters: Q, P of this CTA's share of the channels
 };
 
 template <int V>
@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(kNormThreads, 2)
   extern __shared__ __align__(128) uint8_t smem[];
   const NormPlace w = norm_place(p);
   const int64_t held = p.boxes ? static_cast<int64_t>(p.stage_rows) * kNormStages : p.cta_rows;
-  const size_t strip_bytes = kKeep ? (held * p.pitch * sizeof(T) + 127) / 128 * 128 : 0;
+  const size_t strip_bytes = kKeep ? (held * p.pitch * sizeof(T) + 127) / 128 * 128
+                                   : kNormRing * kNormThreads * sizeof(Pack<T, V>);
   Pack<T, V> *xk = reinterpret_cast<Pack<T, V> *>(smem);
   Pack<T, V> *dk = reinterpret_cast<Pack<T, V> *>(smem + strip_bytes);
   const GradShared s = grad_shared<V>(smem + 2 * strip_bytes, p);
@@ -222,18 +223,11 @@ __global__ void __launch_bounds__(kNormThreads, 2)
         add(xk[first + k * turn], dk[first + k * turn]);
       }
     } else {
-      for (uint32_t k = 0; k < w.mine; k += 4, xc += 4 * xp, dc += 4 * dp) {
-        Pack<T, V> a[4], b[4];
+      stream_rows<T, V, 2>(w.mine, {xc, dc}, {xp, dp}, xk, [&](const Pack<T, V>(&v)[2][4], int rows) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (k + i < w.mine) {
-            a[i] = load_pack<T, V>(xc + i * xp);
-            b[i] = load_pack<T, V>(dc + i * dp);
-          }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (k + i < w.mine) add(a[i], b[i]);
-      }
+          if (i < rows) add(v[0][i], v[1][i]);
+      });
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -269,7 +263,7 @@ __global__ void __launch_bounds__(kNormThreads, 2)
     }
   }
   const int share = (p.pitch + p.slices - 1) / p.slices;  // channels that a CTA adds up
-  if (g.channels) {
+  if (g.channels && p.slices > 1) {
     for (int ch = threadIdx.x; ch < w.cw; ch += blockDim.x) {
       const int owner = ch / share;
       const uint32_t to = mapa_shared(
@@ -301,8 +295,9 @@ __global__ void __launch_bounds__(kNormThreads, 2)
   if (g.channels) {
     float *out = g.channels + (w.image * p.chunks + w.chunk) * 2 * p.c + c0;
     for (int i = threadIdx.x; i < share && w.rank * share + i < w.cw; i += blockDim.x) {
-      float q = 0.0f, b = 0.0f;
-      for (int k = 0; k < p.slices; ++k) {
+      float q = s.q[i], b = s.p[i];  // of a CTA by itself
+      if (p.slices > 1) q = b = 0.0f;
+      for (int k = 0; p.slices > 1 && k < p.slices; ++k) {
         q += s.got[2 * (k * share + i)];
         b += s.got[2 * (k * share + i) + 1];
       }
@@ -327,27 +322,31 @@ __global__ void __launch_bounds__(kNormThreads, 2)
   }
 }
 
-// Adds the chunks' sums: a warp per image and group; with its mean and rstd to stat.
-__global__ void __launch_bounds__(256)
-    norm_grad_join_kernel(const NormGeom p, int64_t count, const GradArgs g, float4 *stat) {
+// Adds the chunks' sums: a CTA per image and group; with its mean and rstd to stat.
+__global__ void __launch_bounds__(128)
+    norm_grad_join_kernel(const NormGeom p, const GradArgs g, float4 *stat) {
+  __shared__ float2 warps[4];
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (at >= count) return;
-  const int64_t image = at / p.groups;
+  const int64_t at = blockIdx.x, image = at / p.groups;
   const float2 *from = g.groups + image * p.chunks * p.groups + (at - image * p.groups);
   float a = 0.0f, b = 0.0f;
 #pragma unroll 4
-  for (int k = lane; k < p.chunks; k += 32) {
+  for (int k = threadIdx.x; k < p.chunks; k += 128) {
     const float2 v = from[static_cast<int64_t>(k) * p.groups];
     a += v.x;
     b += v.y;
   }
   a = warp_sum(a);
   b = warp_sum(b);
-  const float inv = 1.0f / (static_cast<float>(p.hw) * static_cast<float>(p.cg));
-  if (lane == 0) stat[at] = make_float4(g.mean[at], g.rstd[at], a * inv, b * inv);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = make_float2(a, b);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const float inv = 1.0f / (static_cast<float>(p.hw) * static_cast<float>(p.cg));
+    a = (warps[0].x + warps[1].x) + (warps[2].x + warps[3].x);
+    b = (warps[0].y + warps[1].y) + (warps[2].y + warps[3].y);
+    stat[at] = make_float4(g.mean[at], g.rstd[at], a * inv, b * inv);
+  }
 }
 
 // dx: CTAs as in the sums' pass, rows from the image's end, which that pass read last.
@@ -432,7 +431,7 @@ int run_grad(cudaStream_t s, int64_t n, const NormPlan &plan, const GradArgs &ar
   const NormGeom &g = plan.g;
   return norm_with_pack<16 / sizeof(T)>(plan.v, g.act, [&](auto pack_size, auto act) {
     constexpr int V = decltype(pack_size)::value, kAct = decltype(act)::value;
-    const int tail = norm_tail_bytes(plan.threads, V, g.pitch, g.gs);
+    const int tail = norm_tail_bytes(plan.threads, V, g.pitch, g.gs, plan.keep);
     for (int64_t i = 0; i < n; i += plan.batch) {
       const int64_t count = std::min(n - i, plan.batch);
       GradArgs a = args;
@@ -458,11 +457,10 @@ int run_grad(cudaStream_t s, int64_t n, const NormPlan &plan, const GradArgs &ar
         if (rc) return rc;
         continue;
       }
-      if (int rc = norm_launch(norm_grad_kernel<T, V, kAct, false>, ctas, plan.threads, tail,
-                               g.slices, s, mx, md, g, a, di, xi, oi))
+      if (int rc = norm_launch(norm_grad_kernel<T, V, kAct, false>, ctas, plan.threads,
+                               2 * norm_ring_bytes(V, sizeof(T)) + tail, g.slices, s, mx, md, g, a, di, xi, oi))
         return rc;
-      if (int rc = norm_launch(norm_grad_join_kernel, ceil_div(count * g.groups, 8), 256, 0, 1, s,
-                               g, count * g.groups, a, stat))
+      if (int rc = norm_launch(norm_grad_join_kernel, count * g.groups, 128, 0, 1, s, g, a, stat))
         return rc;
       const uint32_t rows = std::min<uint32_t>(8 * g.div_lanes[0].d, g.hw);
       const int64_t pieces = ceil_div(g.hw, rows);
