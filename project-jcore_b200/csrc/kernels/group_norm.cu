@@ -27,6 +27,13 @@ struct Moments {
   float n, mean, m2;
 };
 
+// 1 / x within a step of 2^-23 (one Newton step on the approximate reciprocal), x in
+// the range of counts.
+__device__ __forceinline__ float rcp_fine(float x) {
+  const float r = rcp_approx(x);
+  return fmaf(r, fmaf(-x, r, 1.0f), r);
+}
+
 // Of one pack's channels; the mean negated, pairs of channels together.
 template <int V>
 struct Running {
@@ -82,7 +89,7 @@ __device__ __forceinline__ Moments join_lanes(const Moments &m) {
     n += __shfl_xor_sync(0xffffffffu, n, o);
     s += __shfl_xor_sync(0xffffffffu, s, o);
   }
-  const float mean = n > 0.0f ? s / n : 0.0f, d = m.mean - mean;
+  const float mean = n > 0.0f ? s * rcp_fine(n) : 0.0f, d = m.mean - mean;
   float q = m.n > 0.0f ? fmaf(m.n * d, d, m.m2) : 0.0f;
 #pragma unroll
   for (int o = kWidth / 2; o; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
@@ -157,32 +164,33 @@ __device__ __forceinline__ void put_moments(const NormGeom &p, const NormPlace &
 }
 
 // The moments of each of the CTA's groups, from what put_moments left, to
-// s.all[rank] of every CTA of the cluster. A warp takes a group, several where
-// there are warps to spare and more than 8 entries a lane.
-template <int V>
-__device__ __forceinline__ void cta_groups(const NormGeom &p, const NormPlace &w, const Shared &s) {
-  const int warps = static_cast<int>(blockDim.x) >> 5, warp = threadIdx.x >> 5,
-            lane = threadIdx.x & 31;
+// s.all[rank] of every CTA of the cluster. kWidth lanes take a group, all lanes of
+// several warps where there are warps to spare and more than 8 entries a lane.
+template <int V, int kWidth>
+__device__ __forceinline__ void cta_groups_by(const NormGeom &p, const NormPlace &w,
+                                              const Shared &s, int each) {
+  constexpr int kGroups = 32 / kWidth;  // of a warp at once
+  const int warps = static_cast<int>(blockDim.x) >> 5, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & (kWidth - 1), part = (threadIdx.x & 31) / kWidth;
   const bool joined = V > 1 && p.cg >= V;
-  const int most = w.lanes * (joined ? p.cg / V + 2 : p.cg);
-  int each = 1;  // warps of a group
-  while (2 * each * w.gsl <= warps && most > 256 * each) each *= 2;
-  const int teams = warps / each, team = warp / each, member = warp - team * each;
   auto send = [&](int g, const Moments &t) {  // lane k to CTA k
-    if (lane < p.slices)
+    if (lane < p.slices && g < w.gsl)
       st_shared_cluster_f32x4(mapa_shared(smem_u32(&s.all[w.rank * p.gs + g]), lane),
                               make_float4(t.n, t.mean, t.m2, 0.0f));
   };
-  if (team < teams) {
-    for (int g = team; g < w.gsl; g += teams) {
+  const int teams = each == 1 ? warps : warps / each, team = each == 1 ? warp : warp / each;
+  const int member = warp - team * each;
+  for (int g0 = team * kGroups; g0 < w.gsl && team < teams; g0 += teams * kGroups) {
+    const int g = g0 + part;
+    Moments t{0.0f, 0.0f, 0.0f};
+    if (g < w.gsl) {
       // per row lane: the group's channels, or the packs that hold some of them
       const int from = g * p.cg, to = from + p.cg;
       const int p0 = from / V, packs = joined ? (to - 1) / V - p0 + 1 : p.cg;
-      const uint32_t magic = 0xffffffffu / static_cast<uint32_t>(packs) + 1;  // packs > 1
+      const uint32_t magic = packs > 1 ? 0xffffffffu / static_cast<uint32_t>(packs) + 1 : 0u;
       const int entries = w.lanes * packs;
-      Moments t{0.0f, 0.0f, 0.0f};
 #pragma unroll 2
-      for (int e = member * 32 + lane; e < entries; e += each * 32) {
+      for (int e = member * kWidth + lane; e < entries; e += each * kWidth) {
         const uint32_t l = packs == 1 ? e : __umulhi(static_cast<uint32_t>(e), magic);
         const int k = e - static_cast<int>(l) * packs;
         const float rows = static_cast<float>(lane_rows(w, l));
@@ -196,17 +204,27 @@ __device__ __forceinline__ void cta_groups(const NormGeom &p, const NormPlace &w
           join_one(t, {rows, s.mean[at], s.m2[at]});
         }
       }
-      t = join_lanes<32>(t);
-      if (each == 1) send(g, t);
-      else if (lane == 0) s.team[g * each + member] = make_float4(t.n, t.mean, t.m2, 0.0f);
     }
+    t = join_lanes<kWidth>(t);
+    if (each == 1) send(g, t);
+    else if (lane == 0) s.team[g * each + member] = make_float4(t.n, t.mean, t.m2, 0.0f);
   }
   if (each == 1) return;
   __syncthreads();
   for (int g = warp; g < w.gsl; g += warps) {
     const float4 v = lane < each ? s.team[g * each + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    send(g, join_lanes<32>({v.x, v.y, v.z}));
+    send(g, join_lanes<kWidth>({v.x, v.y, v.z}));
   }
+}
+
+template <int V>
+__device__ __forceinline__ void cta_groups(const NormGeom &p, const NormPlace &w, const Shared &s) {
+  const int warps = static_cast<int>(blockDim.x) >> 5;
+  const int most = w.lanes * (V > 1 && p.cg >= V ? (p.cg + V - 1) / V + (p.cg % V ? 1 : 0) : p.cg);
+  if (most <= 16) return cta_groups_by<V, 8>(p, w, s, 1);
+  int each = 1;  // warps of a group
+  while (2 * each * w.gsl <= warps && most > 256 * each) each *= 2;
+  cta_groups_by<V, 32>(p, w, s, each);
 }
 
 // The normalised, scaled and activated values of one pack's channels.
@@ -276,7 +294,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
     norm_kernel(const __grid_constant__ CUtensorMap map, const NormGeom p, const T *x, T *y,
                 float *mean_out, float *rstd_out, float2 *partial) {
   extern __shared__ __align__(128) uint8_t smem[];
-  const NormPlace w = norm_place(p);
+  const NormPlace w = norm_place(p, blockIdx.x);
   Pack<T, V> *strip = reinterpret_cast<Pack<T, V> *>(smem);
   const int64_t held = p.boxes ? static_cast<int64_t>(p.stage_rows) * kNormStages : p.cta_rows;
   const size_t strip_bytes = kKeep ? (held * p.pitch * sizeof(T) + 127) / 128 * 128
@@ -336,11 +354,10 @@ __global__ void __launch_bounds__(kNormThreads, 3)
         if (rows == 4) {
           join_rows(v[0], run);
         } else {
-#pragma unroll
-          for (int i = 0; i < 3; ++i) {
-            const Pack<T, V> one[1] = {v[0][i]};
-            if (i < rows) join_rows(one, run);
-          }
+          const Pack<T, V> two[2] = {v[0][0], v[0][1]};
+          const Pack<T, V> one[1] = {rows == 1 ? v[0][0] : v[0][2]};
+          if (rows >= 2) join_rows(two, run);
+          if (rows != 2) join_rows(one, run);
         }
       });
     }
@@ -419,49 +436,38 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// Normalises: CTAs as in the moments' pass, each thread eight rows of one pack of
-// channels, from the image's end, which that pass read last.
+// Normalises: CTAs and threads as in the moments' pass, the images and rows in the
+// other order, so that what that pass read last comes first, out of L2.
 template <typename T, int V, int kAct>
 __global__ void __launch_bounds__(kNormThreads, 3)
-    norm_apply_kernel(const NormGeom p, const T *x, T *y, const float2 *stats, FastDiv chunks, uint32_t rows_each) {
-  const uint32_t at = gridDim.x - 1 - blockIdx.x;
-  const uint32_t piece = fdiv(at, chunks), chunk = at - piece * chunks.d;
-  const int64_t image = fdiv(piece, p.div_strips);
-  const int g0 = static_cast<int>(piece - static_cast<uint32_t>(image) * p.strips) * p.gs;
-  const int gsl = min(p.gs, p.groups - g0), c0 = g0 * p.cg;
-  const int last = gsl < p.gs ? 1 : 0;
-  const int nv = static_cast<int>(p.div_nv[last].d);
-  const uint32_t lanes = p.div_lanes[last].d;
-  const int threads = static_cast<int>(blockDim.x), t = static_cast<int>(threadIdx.x);
-  const uint32_t rl = nv <= threads ? fdiv(t, p.div_nv[last]) : 0;
-  int col = t - static_cast<int>(rl) * nv;
-  if (rl >= lanes) return;
-  const uint32_t r0 = chunk * rows_each, rows = min(rows_each, p.hw - r0);
-  const int64_t row = image * p.hw + r0 + rl;
-  const int64_t xp = static_cast<int64_t>(lanes) * p.ldx, yp = static_cast<int64_t>(lanes) * p.ldy;
+    norm_apply_kernel(const NormGeom p, const T *x, T *y, const float2 *stats) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  NormPlace w = norm_place(p, gridDim.x - 1 - blockIdx.x);
+  Pack<T, V> *ring = reinterpret_cast<Pack<T, V> *>(smem);
   griddep_wait();
   griddep_launch_dependents();
-  for (; col < nv; col += threads) {
-    const int ch = c0 + col * V;
-    const T *from = x + row * p.ldx + ch;
+  if (w.mine == 0) return;
+  // the thread's last row first
+  const int64_t row = w.image * p.hw + w.r0 + w.lane + static_cast<int64_t>(w.mine - 1) * w.lanes;
+  const int64_t xp = -static_cast<int64_t>(w.lanes) * p.ldx, yp = -static_cast<int64_t>(w.lanes) * p.ldy;
+  const float2 *st = stats + w.image * p.groups + w.g0;
+  for (int col = w.col; col < w.nv; col += blockDim.x) {
+    const int ch = w.g0 * p.cg + col * V;
     T *to = y + row * p.ldy + ch;
     Affine<T, V, kAct> f;
     bool ready = false;
-    for (uint32_t r = rl; r < rows; r += 4 * lanes, from += 4 * xp, to += 4 * yp) {
-      Pack<T, V> v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (r + i * lanes < rows) v[i] = load_pack<T, V>(from + i * xp);
+    stream_rows<T, V, 1>(w.mine, {x + row * p.ldx + ch}, {xp}, ring,
+                         [&](const Pack<T, V>(&v)[1][4], int rows) {
       if (!ready) {  // the channels' constants arrive under the first rows
-        const float2 *st = stats + image * p.groups + g0;
         f.set(p, col * V, p.gamma ? p.gamma + ch : nullptr, p.beta ? p.beta + ch : nullptr,
               [&](int g) { return st[g]; });
         ready = true;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (r + i * lanes < rows) store_pack(to + i * yp, f(v[i], p));
-    }
+        if (i < rows) store_pack(to + i * yp, f(v[0][i], p));
+      to += 4 * yp;
+    });
   }
 }
 
@@ -503,11 +509,8 @@ int run_norm(cudaStream_t s, int64_t n, const NormPlan &plan, const T *x, T *y, 
       if (int rc = norm_launch(norm_join_kernel, count * g.groups, 128, 0, 1, s, g, partial, mi, ri,
                                stats))
         return rc;
-      const uint32_t rows = std::min<uint32_t>(8 * g.div_lanes[0].d, g.hw);
-      if (int rc = norm_launch(norm_apply_kernel<T, V, kAct>,
-                               count * g.strips * ceil_div(g.hw, rows), plan.threads, 0, 1, s, g, xi,
-                               yi, stats, make_fastdiv(static_cast<uint32_t>(ceil_div(g.hw, rows))),
-                               rows))
+      if (int rc = norm_launch(norm_apply_kernel<T, V, kAct>, ctas, plan.threads,
+                               norm_ring_bytes(V, sizeof(T)), 1, s, g, xi, yi, stats))
         return rc;
     }
     return kOk;

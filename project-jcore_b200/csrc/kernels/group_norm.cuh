@@ -223,10 +223,10 @@ __device__ __forceinline__ uint32_t lane_rows(const NormPlace &w, uint32_t lane)
   return w.base + (lane < w.rest ? 1u : 0u);
 }
 
-__device__ __forceinline__ NormPlace norm_place(const NormGeom &p) {
+__device__ __forceinline__ NormPlace norm_place(const NormGeom &p, uint32_t block) {
   NormPlace w;
-  const uint32_t cluster = fdiv(blockIdx.x, p.div_slices);
-  w.rank = static_cast<int>(blockIdx.x - cluster * p.slices);
+  const uint32_t cluster = fdiv(block, p.div_slices);
+  w.rank = static_cast<int>(block - cluster * p.slices);
   const uint32_t at = fdiv(cluster, p.div_chunks);
   w.chunk = cluster - at * p.chunks;
   w.image = fdiv(at, p.div_strips);

@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kNormThreads, 2)
                      const __grid_constant__ CUtensorMap map_dy, const NormGeom p,
                      const GradArgs g, const T *dy, const T *x, T *dx) {
   extern __shared__ __align__(128) uint8_t smem[];
-  const NormPlace w = norm_place(p);
+  const NormPlace w = norm_place(p, blockIdx.x);
   const int64_t held = p.boxes ? static_cast<int64_t>(p.stage_rows) * kNormStages : p.cta_rows;
   const size_t strip_bytes = kKeep ? (held * p.pitch * sizeof(T) + 127) / 128 * 128
                                    : kNormRing * kNormThreads * sizeof(Pack<T, V>);
@@ -349,54 +349,40 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// dx: CTAs as in the sums' pass, rows from the image's end, which that pass read last.
+// dx: CTAs and threads as in the sums' pass, the images and rows in the other
+// order, so that what that pass read last comes first, out of L2.
 template <typename T, int V, int kAct>
 __global__ void __launch_bounds__(kNormThreads, 2)
-    norm_grad_apply_kernel(const NormGeom p, const float4 *stat, const T *dy, const T *x, T *dx,
-                           FastDiv chunks, uint32_t rows_each) {
-  const uint32_t at = gridDim.x - 1 - blockIdx.x;
-  const uint32_t piece = fdiv(at, chunks), chunk = at - piece * chunks.d;
-  const int64_t image = fdiv(piece, p.div_strips);
-  const int g0 = static_cast<int>(piece - static_cast<uint32_t>(image) * p.strips) * p.gs;
-  const int gsl = min(p.gs, p.groups - g0), c0 = g0 * p.cg;
-  const int last = gsl < p.gs ? 1 : 0;
-  const int nv = static_cast<int>(p.div_nv[last].d);
-  const uint32_t lanes = p.div_lanes[last].d;
-  const int threads = static_cast<int>(blockDim.x), t = static_cast<int>(threadIdx.x);
-  const uint32_t rl = nv <= threads ? fdiv(t, p.div_nv[last]) : 0;
-  int col = t - static_cast<int>(rl) * nv;
-  if (rl >= lanes) return;
-  const uint32_t r0 = chunk * rows_each, rows = min(rows_each, p.hw - r0);
-  const int64_t row = image * p.hw + r0 + rl;
-  const int64_t xp = static_cast<int64_t>(lanes) * p.ldx, dp = static_cast<int64_t>(lanes) * p.lddy,
-                op = static_cast<int64_t>(lanes) * p.ldy;
+    norm_grad_apply_kernel(const NormGeom p, const float4 *stat, const T *dy, const T *x, T *dx) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const NormPlace w = norm_place(p, gridDim.x - 1 - blockIdx.x);
+  Pack<T, V> *ring = reinterpret_cast<Pack<T, V> *>(smem);
   griddep_wait();
   griddep_launch_dependents();
-  for (; col < nv; col += threads) {
-    const int ch = c0 + col * V;
-    const T *xc = x + row * p.ldx + ch, *dc = dy + row * p.lddy + ch;
+  if (w.mine == 0) return;
+  // the thread's last row first
+  const int64_t row = w.image * p.hw + w.r0 + w.lane + static_cast<int64_t>(w.mine - 1) * w.lanes;
+  const int64_t xp = -static_cast<int64_t>(w.lanes) * p.ldx,
+                dp = -static_cast<int64_t>(w.lanes) * p.lddy,
+                op = -static_cast<int64_t>(w.lanes) * p.ldy;
+  const float4 *st = stat + w.image * p.groups + w.g0;
+  for (int col = w.col; col < w.nv; col += blockDim.x) {
+    const int ch = w.g0 * p.cg + col * V;
     T *to = dx + row * p.ldy + ch;
     Input<T, V, kAct> f;
     bool ready = false;
-    constexpr int kRows = V == 8 ? 2 : 4;  // asked for at a time
-    for (uint32_t r = rl; r < rows; r += kRows * lanes, xc += kRows * xp, dc += kRows * dp, to += kRows * op) {
-      Pack<T, V> a[kRows], b[kRows];
-#pragma unroll
-      for (int i = 0; i < kRows; ++i)
-        if (r + i * lanes < rows) {
-          a[i] = load_pack<T, V>(xc + i * xp);
-          b[i] = load_pack<T, V>(dc + i * dp);
-        }
+    stream_rows<T, V, 2>(w.mine, {x + row * p.ldx + ch, dy + row * p.lddy + ch}, {xp, dp}, ring,
+                         [&](const Pack<T, V>(&v)[2][4], int rows) {
       if (!ready) {  // the channels' constants arrive under the first rows
-        const float4 *st = stat + image * p.groups + g0;
         f.set(p, col * V, p.gamma ? p.gamma + ch : nullptr, p.beta ? p.beta + ch : nullptr,
               [&](int k) { return st[k]; });
         ready = true;
       }
 #pragma unroll
-      for (int i = 0; i < kRows; ++i)
-        if (r + i * lanes < rows) store_pack(to + i * op, f(a[i], b[i], p));
-    }
+      for (int i = 0; i < 4; ++i)
+        if (i < rows) store_pack(to + i * op, f(v[0][i], v[1][i], p));
+      to += 4 * op;
+    });
   }
 }
 
@@ -462,11 +448,8 @@ int run_grad(cudaStream_t s, int64_t n, const NormPlan &plan, const GradArgs &ar
         return rc;
       if (int rc = norm_launch(norm_grad_join_kernel, count * g.groups, 128, 0, 1, s, g, a, stat))
         return rc;
-      const uint32_t rows = std::min<uint32_t>(8 * g.div_lanes[0].d, g.hw);
-      const int64_t pieces = ceil_div(g.hw, rows);
-      if (int rc = norm_launch(norm_grad_apply_kernel<T, V, kAct>, count * g.strips * pieces,
-                               plan.threads, 0, 1, s, g, stat, di, xi, oi,
-                               make_fastdiv(static_cast<uint32_t>(pieces)), rows))
+      if (int rc = norm_launch(norm_grad_apply_kernel<T, V, kAct>, ctas, plan.threads,
+                               2 * norm_ring_bytes(V, sizeof(T)), 1, s, g, stat, di, xi, oi))
         return rc;
     }
     return kOk;
