@@ -127,9 +127,13 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   p.g.cg = cg;
   p.g.div_cg = make_fastdiv(static_cast<uint32_t>(cg));
   auto row = [&](int gs) { return static_cast<int64_t>(gs) * cg * size; };
-  auto threads_for = [&](int64_t rows, int cw) {
-    // Six packs a thread: what a thread does once costs as much as some packs.
-    int64_t t = ceil_div(ceil_div(rows * (cw / v), 6), 32) * 32;
+  auto threads_for = [&](int64_t rows, int cw, int64_t ctas) {
+    // What a thread does once costs as much as ten packs. Six packs a thread while
+    // there are few CTAs (2 x 1024 x 640 bf16: 8.1 us, with 20 packs 10.2); where there
+    // are many, 20 forward (8 x 4096 x 320: 18.6 us against 24.8 with six) and 12 in the
+    // gradient (3 x 961 x 510 fp32: 12.6 against 18.4).
+    const int each = 2 * ctas <= 3 * sms ? 6 : tensors == 1 ? 20 : 12;
+    int64_t t = ceil_div(ceil_div(rows * (cw / v), each), 32) * 32;
     t = std::max<int64_t>(t, ceil_div(cw / v, 32) * 32);
     return static_cast<int>(std::min<int64_t>(std::max<int64_t>(t, 64), kNormThreads));
   };
@@ -155,7 +159,7 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
   while (s < 8 && (slab(s) > 48 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sms))) s *= 2;
   p.g.slices = s;
   p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, s));
-  p.threads = threads_for(p.g.cta_rows, gs * cg);
+  p.threads = threads_for(p.g.cta_rows, gs * cg, ctas * s);
   norm_finish(p, n, size);
   if (tensors * norm_rows_bytes(p.g, size) + norm_tail_bytes(p.threads, v, gs * cg, gs, true) <=
       kNormKeepLimit) {
@@ -167,12 +171,13 @@ inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int 
 
   // Passes over memory: strips as wide as a CTA, one long run of rows for each CTA
   // that the SMs hold at once. Images in batches whose tensors stay in L2 between
-  // the passes (a third of its 126 MB).
+  // the passes (72 of its 126 MB: 4 x 16384 x 512 bf16 took 43.8 us in one batch,
+  // 53.8 in two).
   gs = gs0;
   while (gs + gs0 <= groups && gs + gs0 <= 256 && (gs + gs0) * cg <= kNormThreads * v) gs += gs0;
   p.g.gs = gs;
   p.g.strips = static_cast<int>(ceil_div(groups, gs));
-  p.batch = std::min(n, std::max<int64_t>(1, (40 << 20) / (hw * c * size * tensors)));
+  p.batch = std::min(n, std::max<int64_t>(1, (72 << 20) / (hw * c * size * tensors)));
   p.g.slices = 1;
   p.threads = kNormThreads;
   const int64_t chunks =
