@@ -3,9 +3,9 @@ of the nplk_* ABI runs them back to back on one stream. The benchmark times
 these functions and the parity tests check the same functions' outputs
 against the reference's own CPU chain, so what is timed is what is checked.
 
-All tensors are contiguous fp32 CUDA tensors on the current device; `stream`
-is a cudaStream_t as c_void_p. Each function returns 0 or the first non-zero
-library return code.
+All tensors are contiguous CUDA tensors on the current device, fp32 unless a
+function says otherwise; `stream` is a cudaStream_t as c_void_p. Each function
+returns 0 or the first non-zero library return code.
 """
 from __future__ import annotations
 
@@ -87,3 +87,64 @@ def fill_bias_rows(Cm, bias) -> None:
     """Cm[i, :] = bias for every row (the pre-fill that carries the bias
     through beta = 1)."""
     Cm.copy_(bias.expand(Cm.shape[0], Cm.shape[1]))
+
+
+def _dtype(t) -> int:
+    """The NPLK_DTYPE_* code of a torch tensor."""
+    from . import NPLK_DTYPE_BF16, NPLK_DTYPE_FP16, NPLK_DTYPE_FP32
+
+    return {"torch.float32": NPLK_DTYPE_FP32, "torch.float16": NPLK_DTYPE_FP16,
+            "torch.bfloat16": NPLK_DTYPE_BF16}[str(t.dtype)]
+
+
+def norm_act_project_i8(lib, stream, x, groups, gamma, beta, act, y, q, q_scale, w, w_scale, bias,
+                        out, work, ws: int, eps: float = 1e-5) -> int:
+    """A served block's norm and projection: group norm with its activation over
+    channels-last x, its rows (pixels) quantised to 8 bits, and their product
+    with 8-bit weights.
+
+    x, y: [N, HW, C] of one type; q: int8 [N * HW, ldq], ldq >= C (a multiple of
+    16 for the tensor-core product); q_scale: [N * HW]; w: int8 [D, ldw] with
+    w_scale [D] (nplk_quantize_rows of [D][C] weights or nplk_quantize_cols of
+    [C][D] ones, once); bias: [D] or None; out: [N, HW, D] of any of the types;
+    work: nplk_group_norm_workspace_size bytes."""
+    n, hw, c = x.shape
+    rows, d = n * hw, out.shape[2]
+    rc = lib.nplk_group_norm_act(stream, n, hw, c, groups, _dtype(x), _p(x), c, _p(gamma),
+                                 _p(beta), eps, act, 0.0, _p(y), c, None, None, _p(work), ws)
+    if rc != 0:
+        return rc
+    rc = lib.nplk_quantize_rows(stream, rows, c, _dtype(y), _p(y), c, _p(q), q.stride(0),
+                                _p(q_scale))
+    if rc != 0:
+        return rc
+    return lib.nplk_gemm_i8(stream, rows, d, c, _p(q), q.stride(0), _p(q_scale), _p(w),
+                            w.stride(0), _p(w_scale), _p(bias) if bias is not None else None, 0,
+                            0.0, _dtype(out), _p(out), d, None)
+
+
+def norm_act_dropout(lib, stream, x, groups, gamma, beta, act, p, seed, offset, y, mean, rstd,
+                     work, ws: int, eps: float = 1e-5) -> int:
+    """A trained block's norm, activation and dropout, y in place of both steps'
+    results: y = dropout(act(group_norm(x))). x, y: [N, HW, C] of one type; mean,
+    rstd: [N, groups], kept for the gradient."""
+    n, hw, c = x.shape
+    rc = lib.nplk_group_norm_act(stream, n, hw, c, groups, _dtype(x), _p(x), c, _p(gamma),
+                                 _p(beta), eps, act, 0.0, _p(y), c, _p(mean), _p(rstd), _p(work),
+                                 ws)
+    if rc != 0:
+        return rc
+    return lib.nplk_dropout(stream, y.numel(), _dtype(y), _p(y), _p(y), p, seed, offset, None)
+
+
+def norm_act_dropout_backward(lib, stream, dy, x, groups, mean, rstd, gamma, beta, act, p, seed,
+                              offset, dx, dgamma, dbeta, work, ws: int) -> int:
+    """The gradient of norm_act_dropout from the same seed and offset, in dx
+    (which also holds the masked dy in between)."""
+    n, hw, c = x.shape
+    rc = lib.nplk_dropout(stream, dy.numel(), _dtype(dy), _p(dy), _p(dx), p, seed, offset, None)
+    if rc != 0:
+        return rc
+    return lib.nplk_group_norm_act_backward(stream, n, hw, c, groups, _dtype(x), _p(dx), c, _p(x),
+                                            c, _p(mean), _p(rstd), _p(gamma), _p(beta), act, 0.0,
+                                            _p(dx), c, _p(dgamma), _p(dbeta), _p(work), ws)
