@@ -51,7 +51,7 @@ struct NormPlan {
 
 // Runs of rows of a strip that is not kept, at most.
 inline int64_t norm_most_chunks(int64_t hw) {
-  const int64_t by_rows = ceil_div(hw, 64);
+  const int64_t by_rows = ceil_div(hw, 8);
   return by_rows < 448 ? by_rows : 448;
 }
 
