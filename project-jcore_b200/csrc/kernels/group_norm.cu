@@ -327,8 +327,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
     if constexpr (kKeep) {
       Pack<T, V> *own = strip + w.lane * (p.pitch / V) + col;
       if (!p.boxes) {
-#pragma unroll 4
-        for (uint32_t k = 0; k < w.mine; ++k) copy_pack_async<T, V>(own + k * turn, from + k * pitch);
+        copy_rows(own, turn, from, pitch, w.mine);
         copy_async_commit();
         copy_async_wait<0>();  // its own copies are all that a thread reads: no barrier
       }

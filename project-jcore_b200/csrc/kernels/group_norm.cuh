@@ -310,6 +310,27 @@ struct RowLoads {
   }
 };
 
+// Copies packs from + k * pitch to `to` + k * step, k < count, in cp.async groups;
+// 2-byte packs, which cp.async does not take, by eight loads at a time.
+template <typename T, int V>
+__device__ __forceinline__ void copy_rows(Pack<T, V> *to, int step, const T *from, int64_t pitch,
+                                          uint32_t count) {
+  if constexpr (sizeof(Pack<T, V>) == 2) {
+    for (uint32_t k = 0; k < count; k += 8) {
+      Pack<T, V> v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < count) v[i] = load_pack<T, V>(from + (k + i) * pitch);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < count) to[(k + i) * step] = v[i];
+    }
+  } else {
+#pragma unroll 4
+    for (uint32_t k = 0; k < count; ++k) copy_pack_async<T, V>(to + k * step, from + k * pitch);
+  }
+}
+
 // Calls work(batch of packs, how many) for a thread's rows k = 0, 1, ... of kTensors
 // tensors, four at a time; from[i] + k * pitch[i] is row k. ring: the thread's own
 // slots are ring[i * kNormThreads + threadIdx.x], so it waits for its own copies only.
@@ -318,14 +339,11 @@ __device__ __forceinline__ void stream_rows(uint32_t count, const T *const (&fro
                                             const int64_t (&pitch)[kTensors], Pack<T, V> *ring,
                                             F work) {
   auto ask = [&](uint32_t batch) {
-    const uint32_t slot = batch % 3 * 4;
+    const uint32_t at = 4 * batch;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * batch + i < count)
-#pragma unroll
-        for (int t = 0; t < kTensors; ++t)
-          copy_pack_async<T, V>(ring + ((t * kNormRing + slot + i) * kNormThreads + threadIdx.x),
-                                from[t] + (4 * batch + i) * pitch[t]);
+    for (int t = 0; t < kTensors; ++t)
+      copy_rows(ring + ((t * kNormRing + batch % 3 * 4) * kNormThreads + threadIdx.x), kNormThreads,
+                from[t] + at * pitch[t], pitch[t], at < count ? min(4u, count - at) : 0u);
     copy_async_commit();
   };
   ask(0);

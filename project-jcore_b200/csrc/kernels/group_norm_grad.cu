@@ -194,11 +194,8 @@ __global__ void __launch_bounds__(kNormThreads, 2)
     const int first = w.lane * (p.pitch / V) + col;
     const T *xc = xl + col * V, *dc = dl + col * V;
     if (kKeep && !p.boxes) {
-#pragma unroll 2
-      for (uint32_t k = 0; k < w.mine; ++k) {
-        copy_pack_async<T, V>(xk + first + k * turn, xc + k * xp);
-        copy_pack_async<T, V>(dk + first + k * turn, dc + k * dp);
-      }
+      copy_rows(xk + first, turn, xc, xp, w.mine);
+      copy_rows(dk + first, turn, dc, dp, w.mine);
       copy_async_commit();
     }
     {
