@@ -69,6 +69,22 @@ def test_quantize_pitches_and_offsets(dtype, axis):
 
 
 @pytest.mark.parametrize("axis", ["rows", "cols"])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("length", [2, 5, 509, 1001, 2049, 4095, 16383, 20479])
+def test_quantize_at_any_address(length, dtype, axis):
+    # x ends with its allocation; q starts at odd bytes and keeps its surroundings
+    lib = S.gpu_lib()
+    rows, cols = (5, length) if axis == "rows" else (length, 5)
+    for skip in range(0, 8, 1 if length < 5000 else 3):
+        flat = torch.randn(skip + rows * cols, device="cuda", generator=gen(length + skip))
+        x = flat.to(TYPES[dtype][0])[skip:].view(rows, cols)
+        around = torch.full((skip + 5 * (length + 3) + 32,), 111, device="cuda", dtype=torch.int8)
+        q = around[skip + 1:skip + 1 + 5 * (length + 3)].view(5, length + 3)
+        check_quantized(x, axis, *quantize(lib, x, axis, q=q))
+        assert (around[:skip + 1] == 111).all() and (around[-31:] == 111).all()
+
+
+@pytest.mark.parametrize("axis", ["rows", "cols"])
 def test_quantize_borders(axis):
     # quotients a hair from the halves that round either way, in fp32 and bf16
     lib = S.gpu_lib()
