@@ -27,15 +27,25 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-// 1 / (1 + exp(-x)) of two values, exp(-x) as 2^t with t = -x log2 e, for x
-// multiplied on afterwards (a NaN then stays one, and stays in its half).
+// The larger of x and `low`; a NaN stays.
+__device__ __forceinline__ float at_least(float x, float low) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
+  return r;
+}
+__device__ __forceinline__ float2 at_least(float2 x, float low) {
+  return make_float2(at_least(x.x, low), at_least(x.y, low));
+}
+
+// 1 / (1 + exp(-x)) of two values that are at least -42, exp(-x) as 2^t with
+// t = -x log2 e.
 //
-// With kShare one reciprocal serves both: 1 / a = b (1 / ab). The exponential and
-// reciprocal units (16 a clock and SM) are near the bound of the norm: two per
-// value are 4.6 us for 10.5 M values, whose 42 MB move in 6.4 us (1 x 65536 x 256
-// bf16: 27.4 us against 28.7). The gradient, with more other work a value, is 3%
-// faster with two. t stops at 60, so that ab stays finite: below x = -41 the
-// result is 2^-60 instead of less.
+// With kShare one reciprocal serves both: 1 / a = b (1 / ab), ab below 2^122. The
+// exponential and reciprocal units (16 a clock and SM) are near the bound of the
+// norm: two per value are 4.6 us for 10.5 M values, whose 42 MB move in 6.4 us
+// (1 x 65536 x 256 bf16: 27.4 us against 28.7). The gradient, with more other work a
+// value, is 3% faster with two. A NaN would make both results
+// NaN then: the caller passes fmaxf(x, limit), which drops it.
 // kFine = false: 2^t and the reciprocal are within 2^-22 relative and t rounds by
 // |t| 2^-24: below a hundredth of the half steps of fp16 (2^-11) and bf16 (2^-8).
 // kFine = true, for fp32 results: one Newton step on the reciprocal; the error
@@ -46,8 +56,7 @@ template <bool kFine, bool kShare>
 __device__ __forceinline__ float2 sigmoid2(float2 x) {
   constexpr float kLog2e = 1.44269504f;
   const float2 t = mul2(x, both(-kLog2e));
-  const float2 d = add2(make_float2(exp2_approx(fminf(t.x, 60.0f)), exp2_approx(fminf(t.y, 60.0f))),
-                        both(1.0f));
+  const float2 d = add2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), both(1.0f));
   if (!kShare) {
     const float2 r = make_float2(rcp_approx(d.x), rcp_approx(d.y));
     return kFine ? fma2(r, fma2(make_float2(-d.x, -d.y), r, both(1.0f)), r) : r;
@@ -74,6 +83,10 @@ __device__ __forceinline__ void by_pairs(float (&v)[V], F f) {
   }
 }
 
+// Below these the sigmoid of x, and of GELU's 2 u, is under 2^-58: x stops there, so
+// that x * sigmoid stays under 4e-17 and nothing overflows, -infinity included.
+constexpr float kSwishLow = -41.5f, kGeluLow = -7.4f;
+
 // v[j] = act(v[j]), results to be stored as T. GELU in the form
 // 0.5 x (1 + tanh u) = x * sigmoid(2 u), u = c (x + a x^3).
 template <typename T, int V>
@@ -89,12 +102,16 @@ __device__ __forceinline__ void act_array(float (&v)[V], int act, float alpha) {
     case 5:
       by_pairs(v, [](float2 x) {
         constexpr float c = 2.0f * 0.7978845608f;
-        const float2 u = mul2(x, fma2(both(c * 0.044715f), mul2(x, x), both(c)));
-        return mul2(x, sigmoid2<kFine, true>(u));
+        const float2 w = make_float2(fmaxf(x.x, kGeluLow), fmaxf(x.y, kGeluLow));
+        const float2 u = mul2(w, fma2(both(c * 0.044715f), mul2(w, w), both(c)));
+        return mul2(at_least(x, kGeluLow), sigmoid2<kFine, true>(u));
       });
       return;
     case 6:
-      by_pairs(v, [](float2 x) { return mul2(x, sigmoid2<kFine, true>(x)); });
+      by_pairs(v, [](float2 x) {
+        const float2 w = make_float2(fmaxf(x.x, kSwishLow), fmaxf(x.y, kSwishLow));
+        return mul2(at_least(x, kSwishLow), sigmoid2<kFine, true>(w));
+      });
       return;
     default:
 #pragma unroll
@@ -107,7 +124,7 @@ static __device__ __noinline__ float act_slope_call(float x, int act, float alph
   return act_slope(x, act, alpha);
 }
 
-// v[j] = act'(v[j]), for gradients stored as T; 16-bit results as above.
+// v[j] = act'(v[j]), for gradients stored as T.
 template <typename T, int V>
 __device__ __forceinline__ void act_slope_array(float (&v)[V], int act, float alpha) {
   constexpr bool kFine = std::is_same<T, float>::value;
@@ -123,6 +140,8 @@ __device__ __forceinline__ void act_slope_array(float (&v)[V], int act, float al
     case 5:
       by_pairs(v, [](float2 x) {
         constexpr float c = 2.0f * 0.7978845608f, k = c * 0.044715f;
+        x = at_least(x, kGeluLow);
+        x = make_float2(-at_least(-x.x, -30.0f), -at_least(-x.y, -30.0f));  // the slope is 1 there
         const float2 x2 = mul2(x, x);
         const float2 s = sigmoid2<kFine, false>(mul2(x, fma2(both(k), x2, both(c))));
         const float2 du = fma2(both(3.0f * k), x2, both(c));  // of u = c x + k x^3
@@ -132,6 +151,7 @@ __device__ __forceinline__ void act_slope_array(float (&v)[V], int act, float al
       return;
     case 6:
       by_pairs(v, [](float2 x) {
+        x = at_least(x, kSwishLow);
         const float2 s = sigmoid2<kFine, false>(x);
         return mul2(s, fma2(x, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
       });

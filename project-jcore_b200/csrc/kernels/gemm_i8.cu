@@ -253,48 +253,49 @@ __device__ __forceinline__ void i8_finish_box(const I8Args &p, const I8Out<T> &o
                                               const float (&sb)[4], const float (&bias)[4],
                                               const float *scales, Release release) {
   const int lane = threadIdx.x & 31;
-  bool staged = false;
-  if constexpr (sizeof(T) == 2) if (out.map) {
-    staged = true;
-    // mma layout: packed pairs of tokens go to shared memory transposed
-    uint32_t r[2][16];
-    tmem_ld_frag32(t_cols, r[0]);
-    tmem_ld_frag32(t_cols + (16u << 16), r[1]);
-    tmem_wait_ld16x2(r[0], r[1]);
-    release();
-    if (m0 >= p.M) return;
-    float v[32];
+  const bool staged = sizeof(T) == 2 && out.map;
+  if constexpr (sizeof(T) == 2) {
+    if (staged) {
+      // mma layout: packed pairs of tokens go to shared memory transposed
+      uint32_t r[2][16];
+      tmem_ld_frag32(t_cols, r[0]);
+      tmem_ld_frag32(t_cols + (16u << 16), r[1]);
+      tmem_wait_ld16x2(r[0], r[1]);
+      release();
+      if (m0 >= p.M) return;
+      float v[32];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 s = *reinterpret_cast<const float2 *>(scales + 8 * i + 2 * (lane & 3));
+      for (int i = 0; i < 4; ++i) {
+        const float2 s = *reinterpret_cast<const float2 *>(scales + 8 * i + 2 * (lane & 3));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t *q = &r[k >> 1][4 * i + 2 * (k & 1)];
-        const float2 x = make_float2(static_cast<float>(static_cast<int>(q[0])),
-                                     static_cast<float>(static_cast<int>(q[1])));
-        const float2 y = fma2(mul2(x, s), make_float2(sb[k], sb[k]), make_float2(bias[k], bias[k]));
-        v[8 * i + 2 * k] = y.x;
-        v[8 * i + 2 * k + 1] = y.y;
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t *q = &r[k >> 1][4 * i + 2 * (k & 1)];
+          const float2 x = make_float2(static_cast<float>(static_cast<int>(q[0])),
+                                       static_cast<float>(static_cast<int>(q[1])));
+          const float2 y = fma2(mul2(x, s), both(sb[k]), both(bias[k]));
+          v[8 * i + 2 * k] = y.x;
+          v[8 * i + 2 * k + 1] = y.y;
+        }
       }
+      act_array<T>(v, p.act, p.alpha);
+      if (lane == 0) bulk_wait_group_read<0>();  // the previous box has been read
+      __syncwarp();
+      // lane l addresses row l % 8 of matrix l / 8: token 8 (i + matrix / 2) + row,
+      // 16-byte piece 2 h + matrix % 2, swizzled as the map's 64-byte swizzle
+      const uint32_t base = smem_u32(out.box);
+      const uint32_t row = 8u * (lane >> 4) + (lane & 7), piece = (lane >> 3) & 1u;
+#pragma unroll
+      for (int i = 0; i < 4; i += 2)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t token = 8u * i + row;
+          const uint32_t at = base + token * 64u + (((2u * h + piece) ^ ((token >> 1) & 3u)) << 4);
+          stmatrix_x4_trans(at, pack2<T>(v[8 * i + 4 * h], v[8 * i + 4 * h + 1]),
+                            pack2<T>(v[8 * i + 4 * h + 2], v[8 * i + 4 * h + 3]),
+                            pack2<T>(v[8 * i + 8 + 4 * h], v[8 * i + 8 + 4 * h + 1]),
+                            pack2<T>(v[8 * i + 8 + 4 * h + 2], v[8 * i + 8 + 4 * h + 3]));
+        }
     }
-    act_array<T>(v, p.act, p.alpha);
-    if (lane == 0) bulk_wait_group_read<0>();  // the previous box has been read
-    __syncwarp();
-    // lane l addresses row l % 8 of matrix l / 8: token 8 (i + matrix / 2) + row,
-    // 16-byte piece 2 h + matrix % 2, swizzled as the map's 64-byte swizzle
-    const uint32_t base = smem_u32(out.box);
-    const uint32_t row = 8u * (lane >> 4) + (lane & 7), piece = (lane >> 3) & 1u;
-#pragma unroll
-    for (int i = 0; i < 4; i += 2)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t token = 8u * i + row;
-        const uint32_t at = base + token * 64u + (((2u * h + piece) ^ ((token >> 1) & 3u)) << 4);
-        stmatrix_x4_trans(at, pack2<T>(v[8 * i + 4 * h], v[8 * i + 4 * h + 1]),
-                          pack2<T>(v[8 * i + 4 * h + 2], v[8 * i + 4 * h + 3]),
-                          pack2<T>(v[8 * i + 8 + 4 * h], v[8 * i + 8 + 4 * h + 1]),
-                          pack2<T>(v[8 * i + 8 + 4 * h + 2], v[8 * i + 8 + 4 * h + 3]));
-      }
   }
   if (!staged) {
     uint32_t r[32];
@@ -362,9 +363,10 @@ __device__ __forceinline__ void i8_channel_scales(const I8Args &p, bool boxes, i
 // its share of the K blocks. TMA producer, MMA issuer, 8 epilogue warps
 // (two per lane quadrant, every second 32 tokens each: one warp per scheduler
 // alone would wait out every latency of the epilogue; 16 warps took 1 us more a
-// launch, since two CTAs of successive launches no longer fit one SM). With S > 1 each CTA lays its partial sums in its own shared
-// memory ([token][channel], over the stages, which are read out by then), and
-// CTA r adds tokens [r MT / S, (r + 1) MT / S) of all S CTAs.
+// launch, since two CTAs of successive launches no longer fit one SM). With S > 1
+// each CTA lays its partial sums in its own shared memory ([token][channel], over
+// the stages, which are read out by then), and CTA r adds tokens
+// [r MT / S, (r + 1) MT / S) of all S CTAs.
 // ---------------------------------------------------------------------------
 constexpr int kSplitEpiWarps = 8;
 constexpr int kSplitThreads = 64 + kSplitEpiWarps * 32;
@@ -871,9 +873,10 @@ I8Plan choose_plan(int64_t M, int64_t N, int64_t K, bool aligned) {
       if (s > blocks || (mt == 256 && s > 1)) continue;
       const int64_t each = ceil_div(blocks, s);
       const int64_t ctas = ceil_div(N, kI8Channels) * ceil_div(M, mt) * s;
-      const int fit = 2 * (split_smem(mt, split_stages(mt, each), s > 1) + 1024) <= 228 * 1024 ? 2 : 1;
-      const double share =
-          std::min<double>(fit, std::max(1.0, static_cast<double>(ctas) / static_cast<double>(sms)));
+      const int smem = split_smem(mt, split_stages(mt, each), s > 1) + 1024;
+      const int fit = 2 * smem <= 228 * 1024 ? 2 : 1;
+      const double per_sm = static_cast<double>(ctas) / static_cast<double>(sms);
+      const double share = std::min<double>(fit, std::max(1.0, per_sm));
       const double block_us = std::max(0.25, share * (kI8Channels + mt) * kI8BK * 9.2e-6);
       const double us = static_cast<double>(ceil_div(ctas, sms * fit)) *
                             (2.6 + static_cast<double>(each) * block_us + 0.0096 * mt * share) +
@@ -935,8 +938,8 @@ int launch_split(cudaStream_t s, const I8Args &p, T *C, int slices) {
   cfg.dynamicSmemBytes = smem;
   set_launch(cfg, attr, s, static_cast<unsigned>(slices));
   count_launch();
-  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, mc, p, C, boxes ? 1 : 0, slices, n_tiles,
-                                           stages, smem - 1024 - Tr::kTailBytes));
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, mc, p, C, boxes ? 1 : 0, slices,
+                                           n_tiles, stages, smem - 1024 - Tr::kTailBytes));
 }
 
 template <typename T>

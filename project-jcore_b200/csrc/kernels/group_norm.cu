@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(kNormThreads, 3)
         join_rows(v, run);
       }
     } else {
-      stream_rows<T, V, 1>(w.mine, {from}, {pitch}, strip, [&](const Pack<T, V>(&v)[1][4], int rows) {
+      stream_rows<T, V, 1>(w.mine, {from}, {pitch}, strip,
+                           [&](const Pack<T, V>(&v)[1][4], int rows) {
         if (rows == 4) {
           join_rows(v[0], run);
         } else {
@@ -448,7 +449,8 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   if (w.mine == 0) return;
   // the thread's last row first
   const int64_t row = w.image * p.hw + w.r0 + w.lane + static_cast<int64_t>(w.mine - 1) * w.lanes;
-  const int64_t xp = -static_cast<int64_t>(w.lanes) * p.ldx, yp = -static_cast<int64_t>(w.lanes) * p.ldy;
+  const int64_t xp = -static_cast<int64_t>(w.lanes) * p.ldx,
+                yp = -static_cast<int64_t>(w.lanes) * p.ldy;
   const float2 *st = stats + w.image * p.groups + w.g0;
   for (int col = w.col; col < w.nv; col += blockDim.x) {
     const int ch = w.g0 * p.cg + col * V;
@@ -503,7 +505,8 @@ int run_norm(cudaStream_t s, int64_t n, const NormPlan &plan, const T *x, T *y, 
         continue;
       }
       if (int rc = norm_launch(norm_kernel<T, V, 0, false>, ctas, plan.threads,
-                               norm_ring_bytes(V, sizeof(T)) + tail, g.slices, s, map, g, xi, yi, nullptr, nullptr, partial))
+                               norm_ring_bytes(V, sizeof(T)) + tail, g.slices, s, map, g, xi, yi,
+                               nullptr, nullptr, partial))
         return rc;
       if (int rc = norm_launch(norm_join_kernel, count * g.groups, 128, 0, 1, s, g, partial, mi, ri,
                                stats))

@@ -365,8 +365,8 @@ __device__ __forceinline__ void stream_rows(uint32_t count, const T *const (&fro
 
 // Calls f(pack size, activation) with both as std::integral_constant: 16-byte
 // packs with the usual activations known to the compiler, everything else with
-// the activation as an argument (-1). With it as an argument the kernels hold
-// 118 registers across the calls of the rare ones instead of 40 to 80.
+// the activation as an argument (-1): the calls of the rare ones in the loops keep
+// every constant of a thread's channels in registers that calls preserve, or spill.
 template <int kMost, typename F>
 int norm_with_pack(int v, int act, F f) {
   using std::integral_constant;

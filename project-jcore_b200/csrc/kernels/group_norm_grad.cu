@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kNormThreads, 2)
         add(xk[first + k * turn], dk[first + k * turn]);
       }
     } else {
-      stream_rows<T, V, 2>(w.mine, {xc, dc}, {xp, dp}, xk, [&](const Pack<T, V>(&v)[2][4], int rows) {
+      stream_rows<T, V, 2>(w.mine, {xc, dc}, {xp, dp}, xk,
+                           [&](const Pack<T, V>(&v)[2][4], int rows) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (i < rows) add(v[0][i], v[1][i]);
@@ -441,7 +442,8 @@ int run_grad(cudaStream_t s, int64_t n, const NormPlan &plan, const GradArgs &ar
         continue;
       }
       if (int rc = norm_launch(norm_grad_kernel<T, V, kAct, false>, ctas, plan.threads,
-                               2 * norm_ring_bytes(V, sizeof(T)) + tail, g.slices, s, mx, md, g, a, di, xi, oi))
+                               2 * norm_ring_bytes(V, sizeof(T)) + tail, g.slices, s, mx, md, g,
+                               a, di, xi, oi))
         return rc;
       if (int rc = norm_launch(norm_grad_join_kernel, count * g.groups, 128, 0, 1, s, g, a, stat))
         return rc;
@@ -505,11 +507,11 @@ extern "C" int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw,
   a.channels = dgamma || dbeta ? channels : nullptr;
   int rc;
   if (dtype == NPLK_DTYPE_FP32)
-    rc = run_grad(s, n, plan, a, stat, static_cast<const float *>(dy), static_cast<const float *>(x),
-                  static_cast<float *>(dx));
+    rc = run_grad(s, n, plan, a, stat, static_cast<const float *>(dy),
+                  static_cast<const float *>(x), static_cast<float *>(dx));
   else if (dtype == NPLK_DTYPE_FP16)
-    rc = run_grad(s, n, plan, a, stat, static_cast<const __half *>(dy), static_cast<const __half *>(x),
-                  static_cast<__half *>(dx));
+    rc = run_grad(s, n, plan, a, stat, static_cast<const __half *>(dy),
+                  static_cast<const __half *>(x), static_cast<__half *>(dx));
   else
     rc = run_grad(s, n, plan, a, stat, static_cast<const __nv_bfloat16 *>(dy),
                   static_cast<const __nv_bfloat16 *>(x), static_cast<__nv_bfloat16 *>(dx));

@@ -475,12 +475,7 @@ __device__ __forceinline__ void st_shared_cluster_f32x4(uint32_t cluster_addr, f
                : "memory");
 }
 
-// 4 and 16 bytes of another CTA's shared memory (a shared::cluster address).
-__device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr));
-  return v;
-}
+// 16 bytes of another CTA's shared memory (a shared::cluster address).
 __device__ __forceinline__ uint4 ld_shared_cluster_v4(uint32_t cluster_addr) {
   uint4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"

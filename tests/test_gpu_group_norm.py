@@ -223,6 +223,30 @@ def test_every_activation(act, dtype):
     check_backward(x, dy, 48, 6, mean, rstd, gamma, beta, act, dx, dg, db)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("act", [5, 6])
+def test_gelu_and_swish_far_from_zero(act, dtype):
+    # the value and the slope tend to 0 and 0 on the left, to z and 1 on the right
+    lib = S.gpu_lib()
+    far = [7.0, 30.0, 45.0, 100.0, 1e4, 1e12, 1e19, 1e30]
+    beta = torch.tensor(far + [-v for v in far], device="cuda")
+    x, _, _, _ = inputs(2, 300, 16, dtype)
+    gamma = torch.ones(16, device="cuda")
+    y, mean, rstd = forward(lib, x, 16, 4, gamma, beta, act)
+    xh, _, _ = norm64(x, 4, gamma, beta, 1e-5)
+    z = xh + beta.double()
+    want = act64(z, act)
+    # a few roundings of z, where it is above -30; below, nothing of it is left
+    half = torch.finfo(TYPES[dtype]).eps / 2
+    assert ((y.double() - want).abs() <= want.abs() * half + z.abs().clamp(max=1e32) *
+            (z > -30) * 16 * U + 1e-11).all()
+    dx, dg, db = backward(lib, torch.ones_like(x), x, 16, 4, mean, rstd, gamma, beta, act)
+    assert torch.isfinite(dx).all() and torch.isfinite(dg).all()
+    slope = (beta > 0).double()
+    near = beta.abs() < 20  # slopes there are not yet 0 or 1
+    assert ((db.double() / 600 - slope).abs()[~near] <= 1e-6).all()
+
+
 @pytest.mark.parametrize("dtype,c,ld", [("fp32", 24, 40), ("bf16", 40, 41), ("fp16", 48, 64),
                                         ("bf16", 60, 62), ("fp16", 20, 24), ("fp32", 6, 7)])
 @pytest.mark.parametrize("hw", [10, 9000])
