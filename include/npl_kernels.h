@@ -327,7 +327,12 @@ NPL_API int nplk_binary(void *stream, int op, int64_t n, const float *a, const f
  *
  * workspace: nplk_group_norm_workspace_size bytes (the same for forward and
  * backward and every type), 256-byte aligned; 0 where the arguments are
- * refused. Calls that may overlap on the GPU need a workspace each. */
+ * refused. Calls that may overlap on the GPU, captured graphs among them, need a
+ * workspace each.
+ *
+ * A wait of the kernels that runs out (4 s) is reported by nplk_read_status(). The
+ * first call on a device allocates that status word, so it should precede any
+ * stream capture. */
 NPL_API size_t nplk_group_norm_workspace_size(int64_t n, int64_t hw, int64_t c, int64_t groups);
 NPL_API int nplk_group_norm_act(void *stream, int64_t n, int64_t hw, int64_t c, int64_t groups,
                                 int dtype, const void *x, int64_t ldx, const float *gamma,
@@ -395,7 +400,9 @@ NPL_API int nplk_quantize_cols(void *stream, int64_t rows, int64_t cols, int dty
  * as in nplk_activation; C is rounded once and must not overlap the inputs.
  * Any pitch and alignment is taken; the tensor-core kernels need A and B
  * 16-byte aligned with lda and ldb multiples of 16, other operands take a
- * slower kernel. M, N <= 2^30. No workspace. */
+ * slower kernel. M, N <= 2^30. No workspace. status as in nplk_gemm: a device
+ * int that receives a timeout code, or NULL for the library's word, which the
+ * first call on a device allocates (before any stream capture, then). */
 NPL_API int nplk_gemm_i8(void *stream, int64_t M, int64_t N, int64_t K, const int8_t *A,
                          int64_t lda, const float *a_scale, const int8_t *B, int64_t ldb,
                          const float *b_scale, const float *bias, int act, float act_alpha,

@@ -19,6 +19,11 @@ and checks the kernel status word.
     python -m npl_b200.profile_cases conv_pair # the 3x3 conv on CTA pairs
     python -m npl_b200.profile_cases conv_n256 # the 3x3 conv at N=256 (output beyond L2)
     python -m npl_b200.profile_cases stem_fused # stem conv + pool, and the fused form (N=16)
+    python -m npl_b200.profile_cases norm      # group norm + swish and its gradient, 16x4096x320 bf16
+    python -m npl_b200.profile_cases norm_wide # the same, 1x262144x128 fp32 (passes over memory)
+    python -m npl_b200.profile_cases dropout   # 25.7 M bf16 values
+    python -m npl_b200.profile_cases quantize  # rows and columns of 8192 x 4096 bf16
+    python -m npl_b200.profile_cases gemm_i8   # 4096x4096x4096 8-bit product, bf16 result
 
 Run from the package directory (``project-jcore_b200``) or with it on sys.path.
 """
@@ -223,6 +228,72 @@ def case_stem_fused(reps: int = 2, n: int = 16):
     assert torch.equal(fused, pooled)
 
 
+def case_norm(reps: int = 3, n: int = 16, hw: int = 4096, c: int = 320, groups: int = 32,
+              dtype: str = "bfloat16"):
+    from . import workloads
+    torch, lib, s = _setup()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(n, hw, c, device="cuda", generator=gen).to(getattr(torch, dtype))
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    gamma, beta = (torch.rand(c, device="cuda", generator=gen) for _ in range(2))
+    mean, rstd = (torch.empty(n, groups, device="cuda") for _ in range(2))
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
+    ws = lib.nplk_group_norm_workspace_size(n, hw, c, groups)
+    work = torch.empty(ws, device="cuda", dtype=torch.uint8)
+    code = workloads._dtype(x)
+    for _ in range(reps):
+        assert lib.nplk_group_norm_act(s, n, hw, c, groups, code, _p(x), c, _p(gamma), _p(beta),
+                                       1e-5, 6, 0.0, _p(y), c, _p(mean), _p(rstd), _p(work),
+                                       ws) == 0
+        assert lib.nplk_group_norm_act_backward(s, n, hw, c, groups, code, _p(y), c, _p(x), c,
+                                                _p(mean), _p(rstd), _p(gamma), _p(beta), 6, 0.0,
+                                                _p(dx), c, _p(dgamma), _p(dbeta), _p(work),
+                                                ws) == 0
+    torch.cuda.synchronize()
+    assert lib.nplk_read_status(s) == 0
+
+
+def case_dropout(reps: int = 3, count: int = 25690112):
+    from . import NPLK_DTYPE_BF16
+    torch, lib, s = _setup()
+    x = torch.ones(count, device="cuda", dtype=torch.bfloat16)
+    y = torch.empty_like(x)
+    for i in range(reps):
+        assert lib.nplk_dropout(s, count, NPLK_DTYPE_BF16, _p(x), _p(y), 0.1, 5, i * count,
+                                None) == 0
+    torch.cuda.synchronize()
+
+
+def case_quantize(reps: int = 3, rows: int = 8192, cols: int = 4096):
+    from . import NPLK_DTYPE_BF16
+    torch, lib, s = _setup()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(rows, cols, device="cuda", generator=gen).bfloat16()
+    q = torch.empty(rows * cols, device="cuda", dtype=torch.int8)
+    scale = torch.empty(max(rows, cols), device="cuda")
+    for _ in range(reps):
+        assert lib.nplk_quantize_rows(s, rows, cols, NPLK_DTYPE_BF16, _p(x), cols, _p(q), cols,
+                                      _p(scale)) == 0
+        assert lib.nplk_quantize_cols(s, rows, cols, NPLK_DTYPE_BF16, _p(x), cols, _p(q), rows,
+                                      _p(scale)) == 0
+    torch.cuda.synchronize()
+
+
+def case_gemm_i8(reps: int = 3, m: int = 4096, n: int = 4096, k: int = 4096):
+    from . import NPLK_DTYPE_BF16
+    torch, lib, s = _setup()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    a, b = (torch.randint(-127, 128, (r, k), device="cuda", generator=gen, dtype=torch.int8)
+            for r in (m, n))
+    sa, sb, bias = (torch.rand(r, device="cuda", generator=gen) for r in (m, n, n))
+    c = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
+    for _ in range(reps):
+        assert lib.nplk_gemm_i8(s, m, n, k, _p(a), k, _p(sa), _p(b), k, _p(sb), _p(bias), 0, 0.0,
+                                NPLK_DTYPE_BF16, _p(c), n, None) == 0
+    torch.cuda.synchronize()
+    assert lib.nplk_read_status(s) == 0
+
+
 CASES = {"conv": case_conv, "chain_fused": case_chain_fused,
          "conv_direct": lambda: case_conv(algo=1),
          "conv_window_tma": lambda: case_conv(algo=3),
@@ -235,7 +306,9 @@ CASES = {"conv": case_conv, "chain_fused": case_chain_fused,
          "bandwidth": case_bandwidth, "allgather": case_allgather,
          "conv_pair": lambda: case_conv(algo=5),
          "conv_n256": lambda: case_conv(n=256),
-         "stem_fused": case_stem_fused}
+         "stem_fused": case_stem_fused, "norm": case_norm,
+         "norm_wide": lambda: case_norm(n=1, hw=262144, c=128, dtype="float32"),
+         "dropout": case_dropout, "quantize": case_quantize, "gemm_i8": case_gemm_i8}
 
 if __name__ == "__main__":
     name = sys.argv[1] if len(sys.argv) > 1 else "conv"

@@ -118,6 +118,41 @@ def test_quantize_special_rows(axis, length):
     assert (q[3:6, :length] == 0).all()
 
 
+@pytest.mark.parametrize("axis", ["rows", "cols"])
+@pytest.mark.parametrize("rows,cols", [(40, 40), (3000, 513)])
+def test_quantize_captured_and_on_two_streams(rows, cols, axis):
+    lib = S.gpu_lib()
+    x = [torch.randn(rows, cols, device="cuda", generator=gen(i)) * (3 - i) for i in range(3)]
+    want = [quantize(lib, v, axis) for v in x]
+    held = x[0].clone()
+    q, scale = (torch.empty_like(t) for t in want[0])
+    q.fill_(111)
+
+    def call():
+        rc = getattr(lib, f"nplk_quantize_{axis}")(S.cuda_stream(), rows, cols, 0, held.data_ptr(),
+                                                   cols, q.data_ptr(), q.stride(0),
+                                                   scale.data_ptr())
+        assert rc == 0
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for v, (wq, ws) in zip(x, want):  # the scales fall from one replay to the next
+        held.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(q, wq) and torch.equal(scale, ws)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for st, v in zip(streams, x):
+        with torch.cuda.stream(st):
+            got.append(quantize(lib, v, axis))
+    torch.cuda.synchronize()
+    for (gq, gs), (wq, ws) in zip(got, want):
+        assert torch.equal(gq, wq) and torch.equal(gs, ws)
+
+
 # ---- product ------------------------------------------------------------------------
 
 def act64(z, act, alpha):
