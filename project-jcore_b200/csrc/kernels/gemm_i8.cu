@@ -367,6 +367,10 @@ __device__ __forceinline__ void i8_channel_scales(const I8Args &p, bool boxes, i
 // each CTA lays its partial sums in its own shared memory ([token][channel], over
 // the stages, which are read out by then), and CTA r adds tokens
 // [r MT / S, (r + 1) MT / S) of all S CTAs.
+// TMEM: a CTA of a cluster must not wait for columns that another cluster holds.
+// With S > 1, MT is at most 128, and those that shared memory and threads let onto
+// an SM together (3 x 128, or 3 x 128 and one of 32, or 6 smaller) ask for at most
+// 416 of its 512 columns; CTAs without a cluster give theirs back by themselves.
 // ---------------------------------------------------------------------------
 constexpr int kSplitEpiWarps = 8;
 constexpr int kSplitThreads = 64 + kSplitEpiWarps * 32;

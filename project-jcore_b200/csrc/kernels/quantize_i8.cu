@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kLongThreads)
 constexpr int kColThreads = 256, kColWarps = kColThreads / 32;
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kColThreads)
+__global__ void __launch_bounds__(kColThreads, 4)
     column_scales_kernel(int64_t rows, int64_t cols, const T *x, int64_t ldx, float *scale_out,
                          unsigned strips, int64_t rows_each) {
   __shared__ uint32_t red[kColWarps][32 * V];
@@ -317,15 +317,15 @@ __global__ void __launch_bounds__(kColThreads)
 
 // The second: a tile of 256 rows and 32 columns per CTA, a lane per column, which
 // finds x in L2 where that holds it; the q pass through shared memory so that
-// each column's 256 bytes leave together. 4096 x 4096 fp32 takes 32 us in both
-// kernels, 8192 x 4096 fp16 45 us; the second, two thirds of it, is bound by its
-// instructions (15 per value). One kernel instead, with clusters over the rows of
+// each column's 256 bytes leave together. 4096 x 4096 fp32 takes 30 us in both
+// kernels, 8192 x 4096 fp16 44 us; the second, two thirds of it, is bound by its
+// instructions (16 per value). One kernel instead, with clusters over the rows of
 // a strip of columns that kept in shared memory what fits there, read x once but
 // took 40 and 61 us: its CTAs load and compute in step.
 constexpr int kColRows = 256, kColEach = kColRows / kColWarps;  // rows: of a tile, of a lane
 
 template <typename T>
-__global__ void __launch_bounds__(kColThreads)
+__global__ void __launch_bounds__(kColThreads, 4)
     quantize_cols_kernel(int64_t rows, int64_t cols, const T *x, int64_t ldx, int8_t *q,
                          int64_t ldq, const float *scales, unsigned strips, bool words) {
   __shared__ uint32_t tile[32][kColRows / 4 + 1];
