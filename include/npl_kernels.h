@@ -386,7 +386,8 @@ NPL_API int nplk_dropout(void *stream, int64_t n, int dtype, const void *x, void
  * with the row are NaN.
  * nplk_quantize_cols: the same for the columns of x (a weight matrix [K][N],
  * as nplk_gemm takes it, laid out once): q[c*ldq + r] and scale[c] of column c.
- * ldq a multiple of 16 and q 16-byte aligned give nplk_gemm_i8 its fastest form. */
+ * ldq a multiple of 16 and q 16-byte aligned give nplk_gemm_i8 its fastest form.
+ * q and scale must not overlap x. */
 NPL_API int nplk_quantize_rows(void *stream, int64_t rows, int64_t cols, int dtype,
                                const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale);
 NPL_API int nplk_quantize_cols(void *stream, int64_t rows, int64_t cols, int dtype,

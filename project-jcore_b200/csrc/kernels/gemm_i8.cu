@@ -1020,6 +1020,9 @@ extern "C" int nplk_gemm_i8(void *stream, int64_t M, int64_t N, int64_t K, const
       ldb < K || ldc < N || act < 0 || act > 10)
     return kErrInvalidArg;
   if (reinterpret_cast<uintptr_t>(C) % size) return kErrInvalidArg;
+  for (const void *v : {static_cast<const void *>(a_scale), static_cast<const void *>(b_scale),
+                        static_cast<const void *>(bias), static_cast<const void *>(status)})
+    if (reinterpret_cast<uintptr_t>(v) % 4) return kErrInvalidArg;
   if (M > (int64_t(1) << 30) || N > (int64_t(1) << 30) || K > 131071) return kErrUnsupported;
   const bool aligned = reinterpret_cast<uintptr_t>(A) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(B) % 16 == 0 && lda % 16 == 0 &&

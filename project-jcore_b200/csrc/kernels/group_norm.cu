@@ -540,6 +540,9 @@ extern "C" int nplk_group_norm_act(void *stream, int64_t n, int64_t hw, int64_t 
   if (int rc = norm_check(n, hw, c, groups)) return rc;
   if (!norm_aligned(x, size) || !norm_aligned(y, size) || (x == y && ldx != ldy))
     return kErrInvalidArg;
+  for (const float *p : {gamma, beta, static_cast<const float *>(mean),
+                         static_cast<const float *>(rstd)})
+    if (!norm_aligned(p, 4)) return kErrInvalidArg;
   if (!workspace || !norm_aligned(workspace, 256) ||
       workspace_bytes < norm_workspace(n, hw, c, groups))
     return kErrInvalidArg;

@@ -505,6 +505,9 @@ extern "C" int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw,
   if (!norm_aligned(dy, size) || !norm_aligned(x, size) || !norm_aligned(dx, size) ||
       (dx == dy && lddx != lddy) || (dx == x && lddx != ldx))
     return kErrInvalidArg;
+  for (const float *p : {mean, rstd, gamma, beta, static_cast<const float *>(dgamma),
+                         static_cast<const float *>(dbeta)})
+    if (!norm_aligned(p, 4)) return kErrInvalidArg;
   if (!workspace || !norm_aligned(workspace, 256) ||
       workspace_bytes < norm_workspace(n, hw, c, groups))
     return kErrInvalidArg;

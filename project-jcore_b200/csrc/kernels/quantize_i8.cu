@@ -435,7 +435,8 @@ int quantize_lines(void *stream, int64_t rows, int64_t cols, int dtype, const vo
   if (rows < 1 || cols < 1 || !size || !x || !q || !scale || ldx < cols ||
       ldq < (by_rows ? cols : rows))
     return kErrInvalidArg;
-  if (reinterpret_cast<uintptr_t>(x) % size) return kErrInvalidArg;
+  if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(scale) % 4)
+    return kErrInvalidArg;
   if (rows >= (int64_t(1) << 31) || cols >= (int64_t(1) << 31)) return kErrUnsupported;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == NPLK_DTYPE_FP32)

@@ -96,3 +96,19 @@ def test_gemm_i8_refuses(lib):
     assert call(k=131072, lda=131072, ldb=131072) == UNSUP
     assert call(m=(1 << 30) + 1) == UNSUP
     assert call(n=(1 << 30) + 1, ldc=1 << 31) == UNSUP
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_misaligned_fp32_arguments_are_refused(lib, which):
+    odd = [ODD if i == which else P for i in range(6)]
+    work, size = P, 1 << 40
+    if which < 4:
+        assert lib.nplk_group_norm_act(None, 2, 5, 6, 3, 0, P, 6, odd[0], odd[1], 1e-5, 0, 0.0, P,
+                                       6, odd[2], odd[3], work, size) == BAD
+        assert lib.nplk_gemm_i8(None, 4, 4, 16, P, 16, odd[0], P, 16, odd[1], odd[2], 0, 0.0,
+                                0, P, 4, odd[3]) == BAD
+    assert lib.nplk_group_norm_act_backward(None, 2, 5, 6, 3, 0, P, 6, P, 6, odd[0], odd[1],
+                                            odd[2], odd[3], 0, 0.0, P, 6, odd[4], odd[5], work,
+                                            size) == BAD
+    for call in (lib.nplk_quantize_rows, lib.nplk_quantize_cols):
+        assert call(None, 4, 4, 0, P, 4, P, 16, ODD) == BAD
