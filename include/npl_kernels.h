@@ -398,7 +398,8 @@ NPL_API int nplk_quantize_cols(void *stream, int64_t rows, int64_t cols, int dty
  * and ldb; a_scale [M], b_scale [N] and bias [N] (may be NULL) fp32; C row-major
  * of type c_dtype (NPLK_DTYPE_*), pitch ldc. The sums are exact 32-bit integers
  * (K <= 131071, else NPL_ERR_UNSUPPORTED), converted once to fp32; act is 0..10
- * as in nplk_activation; C is rounded once and must not overlap the inputs.
+ * as in nplk_activation; C is rounded once and must not overlap the inputs. A row of
+ * C depends on its own row of A alone, to the bit, whatever M is.
  * Any pitch and alignment is taken; the tensor-core kernels need A and B
  * 16-byte aligned with lda and ldb multiples of 16, other operands take a
  * slower kernel. M, N <= 2^30. No workspace. status as in nplk_gemm: a device

@@ -44,8 +44,8 @@ __device__ __forceinline__ float2 at_least(float2 x, float low) {
 // exponential and reciprocal units (16 a clock and SM) are near the bound of the
 // norm: two per value are 4.6 us for 10.5 M values, whose 42 MB move in 6.4 us
 // (1 x 65536 x 256 bf16: 27.4 us against 28.7). The gradient, with more other work a
-// value, is 3% faster with two. A NaN would make both results
-// NaN then: the caller passes fmaxf(x, limit), which drops it.
+// value, is 3% faster with two. A NaN would make both results NaN then: the caller
+// passes fmaxf(x, limit), which drops it. A result's last bit depends on its partner.
 // kFine = false: 2^t and the reciprocal are within 2^-22 relative and t rounds by
 // |t| 2^-24: below a hundredth of the half steps of fp16 (2^-11) and bf16 (2^-8).
 // kFine = true, for fp32 results: one Newton step on the reciprocal; the error
@@ -88,8 +88,9 @@ __device__ __forceinline__ void by_pairs(float (&v)[V], F f) {
 constexpr float kSwishLow = -41.5f, kGeluLow = -7.4f;
 
 // v[j] = act(v[j]), results to be stored as T. GELU in the form
-// 0.5 x (1 + tanh u) = x * sigmoid(2 u), u = c (x + a x^3).
-template <typename T, int V>
+// 0.5 x (1 + tanh u) = x * sigmoid(2 u), u = c (x + a x^3). kShare as above; without it
+// v[j] depends on its own input alone.
+template <typename T, bool kShare, int V>
 __device__ __forceinline__ void act_array(float (&v)[V], int act, float alpha) {
   constexpr bool kFine = std::is_same<T, float>::value;
   switch (act) {
@@ -102,15 +103,19 @@ __device__ __forceinline__ void act_array(float (&v)[V], int act, float alpha) {
     case 5:
       by_pairs(v, [](float2 x) {
         constexpr float c = 2.0f * 0.7978845608f;
-        const float2 w = make_float2(fmaxf(x.x, kGeluLow), fmaxf(x.y, kGeluLow));
+        x = at_least(x, kGeluLow);
+        const float2 w =
+            kShare ? make_float2(fmaxf(x.x, kGeluLow), fmaxf(x.y, kGeluLow)) : x;
         const float2 u = mul2(w, fma2(both(c * 0.044715f), mul2(w, w), both(c)));
-        return mul2(at_least(x, kGeluLow), sigmoid2<kFine, true>(u));
+        return mul2(x, sigmoid2<kFine, kShare>(u));
       });
       return;
     case 6:
       by_pairs(v, [](float2 x) {
-        const float2 w = make_float2(fmaxf(x.x, kSwishLow), fmaxf(x.y, kSwishLow));
-        return mul2(at_least(x, kSwishLow), sigmoid2<kFine, true>(w));
+        x = at_least(x, kSwishLow);
+        const float2 w =
+            kShare ? make_float2(fmaxf(x.x, kSwishLow), fmaxf(x.y, kSwishLow)) : x;
+        return mul2(x, sigmoid2<kFine, kShare>(w));
       });
       return;
     default:

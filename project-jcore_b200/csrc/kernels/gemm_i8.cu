@@ -1,6 +1,7 @@
 // Matrix product in 8-bit integers with a scale for each token and channel:
 //   C[m,n] = act((sum_k A[m,k] B[n,k]) * a_scale[m] * b_scale[n] + bias[n]).
-// |A * B| <= 2^14, so 32-bit sums are exact up to K = 131071 in any order.
+// |A * B| <= 2^14, so 32-bit sums are exact up to K = 131071 in any order, and every
+// kernel rounds the same steps: a token's results do not depend on its batch.
 //
 // Four kernels, by what bounds the product (choose_plan):
 //   rows    few tokens: the weights' bytes. Each warp streams 16 channels with
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(256) gemm_i8_bytes_kernel(I8Args p, T *C) {
                                        p.bias ? p.bias[n] : 0.0f)
                                 : 0.0f;
     }
-    act_array<T>(v, p.act, p.alpha);
+    act_array<T, false>(v, p.act, p.alpha);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t n = n0 + tx + 16 * j;
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) gemm_i8_rows_kernel(I8Args p,
       for (int w = 0; w < kRowsWarps; ++w) s += red[w][m][ch];
       float v[1] = {fmaf(static_cast<float>(s) * p.a_scale[m], p.b_scale[n],
                          p.bias ? p.bias[n] : 0.0f)};
-      act_array<T>(v, p.act, p.alpha);
+      act_array<T, false>(v, p.act, p.alpha);
       C[m * p.ldc + n] = from_float<T>(v[0]);
     }
   }
@@ -277,7 +278,7 @@ __device__ __forceinline__ void i8_finish_box(const I8Args &p, const I8Out<T> &o
           v[8 * i + 2 * k + 1] = y.y;
         }
       }
-      act_array<T>(v, p.act, p.alpha);
+      act_array<T, false>(v, p.act, p.alpha);
       if (lane == 0) bulk_wait_group_read<0>();  // the previous box has been read
       __syncwarp();
       // lane l addresses row l % 8 of matrix l / 8: token 8 (i + matrix / 2) + row,
@@ -313,7 +314,7 @@ __device__ __forceinline__ void i8_finish_box(const I8Args &p, const I8Out<T> &o
       v[j] = y.x;
       v[j + 1] = y.y;
     }
-    act_array<T>(v, p.act, p.alpha);
+    act_array<T, false>(v, p.act, p.alpha);
     if (!out.map) {
       const int64_t n = static_cast<int64_t>(n0) + lane;
       const int rows = p.M - m0;
@@ -436,7 +437,7 @@ __device__ __forceinline__ void i8_add_slices(const I8Args &p, const uint8_t *pa
       float o[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = fmaf(static_cast<float>(s[j]) * sa, sb[j], bias[j]);
-      act_array<T>(o, p.act, p.alpha);
+      act_array<T, false>(o, p.act, p.alpha);
       T *c = C + m * p.ldc + n;
       if (whole) {
         store_pack(c, pack<T, 4>(o));

@@ -299,6 +299,36 @@ def test_non_finite_scales_poison_their_row_or_column(m):
     assert torch.equal(c, clean)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("act", [1, 5, 6])
+@pytest.mark.parametrize("m,n", [(5, 70), (60, 200), (700, 640)])
+def test_non_finite_scales_with_an_activation(m, n, act, dtype):
+    lib = S.gpu_lib()
+    a, b, sa, sb, bias = operands(m, n, 256)
+    clean = product(lib, a, b, sa, sb, bias, dtype, act)
+    sa, sb = sa.clone(), sb.clone()
+    sa[2], sb[n - 3] = float("nan"), float("nan")
+    c = product(lib, a, b, sa, sb, bias, dtype, act)
+    assert torch.isnan(c[2]).all() and torch.isnan(c[:, n - 3]).all()
+    c[2], c[:, n - 3] = clean[2], clean[:, n - 3]
+    assert torch.equal(c, clean)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("act", [0, 5, 6, 8])
+def test_a_row_does_not_depend_on_its_batch(act, dtype):
+    lib = S.gpu_lib()
+    a, b, sa, sb, bias = operands(3000, 641, 1100)
+    want = product(lib, a, b, sa, sb, bias, dtype, act)
+    for first, rows in ((0, 1), (1, 7), (5, 16), (100, 40), (33, 90), (1, 300), (700, 2000)):
+        part = slice(first, first + rows)
+        got = product(lib, a[part], b, sa[part].clone(), sb, bias, dtype, act)
+        assert torch.equal(got, want[part])
+    odd = torch.empty(40 * 1101, device="cuda", dtype=torch.int8).view(40, 1101)[:, :1100]
+    odd.copy_(a[:40])  # operands that the tensor-core kernels do not take
+    assert torch.equal(product(lib, odd, b, sa[:40].clone(), sb, bias, dtype, act), want[:40])
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (50, 640, 512), (600, 800, 400)])
 def test_captured_streams_and_repeats(m, n, k):
     lib = S.gpu_lib()

@@ -321,6 +321,51 @@ def test_non_finite_values_stay_in_their_group(hw):
     assert torch.equal(y[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("act", [0, 1, 5, 6])
+@pytest.mark.parametrize("dtype,c,groups", [("bf16", 36, 6), ("fp16", 35, 7), ("bf16", 320, 32),
+                                            ("fp32", 33, 11)])
+@pytest.mark.parametrize("hw", [3, 60000])
+def test_non_finite_values_beside_groups_that_share_a_piece(hw, dtype, c, groups, act):
+    lib = S.gpu_lib()
+    x, _, gamma, beta = inputs(2, hw, c, dtype)
+    clean, _, _ = forward(lib, x, c, groups, gamma, beta, act)
+    cg = c // groups
+    x[0, hw - 1, 2 * cg - 1], x[1, 0, 3 * cg] = float("nan"), float("-inf")
+    y, _, _ = forward(lib, x, c, groups, gamma, beta, act)
+    hit = torch.zeros(2, groups, dtype=torch.bool, device="cuda")
+    hit[0, 1] = hit[1, 3] = True
+    hit = per_channel(hit, c).expand_as(y)
+    assert torch.isnan(y[hit]).all() and torch.equal(y[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("act", [0, 1, 5, 6])
+@pytest.mark.parametrize("hw", [3, 200, 60000])
+def test_non_finite_gradients_stay_in_their_group(hw, act):
+    lib = S.gpu_lib()
+    for dtype, c, groups in (("fp32", 30, 10), ("bf16", 36, 6), ("bf16", 320, 32)):
+        cg = c // groups
+        x, dy, gamma, beta = inputs(2, hw, c, dtype)
+        _, mean, rstd = forward(lib, x, c, groups, gamma, beta, act)
+        clean = backward(lib, dy, x, c, groups, mean, rstd, gamma, beta, act)
+        dy[0, hw // 2, cg + 1], dy[1, 0, 4 * cg] = float("nan"), float("inf")
+        x[1, hw - 1, 3 * cg - 1] = float("nan")
+        dx, dg, db = backward(lib, dy, x, c, groups, mean, rstd, gamma, beta, act)
+        hit = torch.zeros(2, groups, dtype=torch.bool, device="cuda")
+        hit[0, 1] = hit[1, 4] = hit[1, 2] = True
+        reached = per_channel(hit, c).expand_as(dx)
+        # ReLU's zero slope makes the infinity a NaN or keeps it: not finite either way
+        assert torch.equal(dx[~reached], clean[0][~reached])
+        where = (cg + 1, 3 * cg - 1, 4 * cg)
+        other = torch.ones(c, dtype=torch.bool, device="cuda")
+        other[list(where)] = False
+        assert torch.equal(dg[other], clean[1][other]) and torch.equal(db[other], clean[2][other])
+        assert torch.isnan(dx[0, :, cg:2 * cg]).all() and torch.isnan(db[cg + 1])
+        if act:  # z is NaN there, and its slope with it, but ReLU's, which is 0
+            assert torch.isnan(dg[3 * cg - 1])
+        if hw > 3:
+            assert not torch.isfinite(db[4 * cg])
+
+
 def test_constant_groups_give_beta():
     lib = S.gpu_lib()
     x = torch.full((2, 77, 12), 3.25, device="cuda")
