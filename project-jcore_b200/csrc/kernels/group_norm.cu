@@ -283,7 +283,7 @@ struct Affine {
       v[2 * j] = z.x;
       if (V > 1) v[2 * j + (V > 1 ? 1 : 0)] = z.y;
     }
-    act_array<T, true>(v, kAct >= 0 ? kAct : p.act, p.alpha);
+    act_array<T, (V > 1)>(v, kAct >= 0 ? kAct : p.act, p.alpha);
     return pack<T, V>(v);
   }
 };
