@@ -131,6 +131,7 @@ __device__ __forceinline__ uint32_t low_bytes(const uint32_t *b) {
 // belong to the row before; the q pass through shared memory and leave as the
 // aligned words of their own row. 8192 x 4095 bf16 takes 31 us so; a thread per
 // element took 50 us.
+// The bounds of 1024 threads are for 64 registers: two blocks of 512 on an SM.
 template <typename T, int NV, bool kWarpRows, bool kShift>
 __global__ void __launch_bounds__(kWarpRows ? 128 : 1024)
     quantize_rows_kernel(int64_t rows, int cols, const T *x, int64_t ldx, int8_t *q, int64_t ldq,
@@ -373,9 +374,11 @@ __global__ void __launch_bounds__(kColThreads, 4)
 template <typename T, bool kShift>
 int run_rows(cudaStream_t s, int64_t rows, int64_t cols, const T *x, int64_t ldx, int8_t *q,
              int64_t ldq, float *scale) {
-  constexpr int V = 16 / sizeof(T), kNV = kShift ? 5 : 4;  // packs of a thread in a block
+  // Packs of a thread in a block: four (and one for the first pack's head), or eight
+  // where that took more than 512 threads.
+  constexpr int V = 16 / sizeof(T), kFew = kShift ? 5 : 4, kMany = kShift ? 9 : 8;
   const int64_t packs = ceil_div(cols + (kShift ? V - 1 : 0), V);
-  if (packs > 1024 * kNV) {
+  if (packs > 512 * kMany) {
     return launch_programmatic(quantize_long_rows_kernel<T>, dim3(static_cast<unsigned>(rows)),
                                dim3(kLongThreads), 0, s, cols, x, ldx, q, ldq, scale);
   }
@@ -390,8 +393,15 @@ int run_rows(cudaStream_t s, int64_t rows, int64_t cols, const T *x, int64_t ldx
     return go(quantize_rows_kernel<T, 4, true, kShift>, ceil_div(rows, 4), 128, 4);
   if (packs <= 32 * 8)
     return go(quantize_rows_kernel<T, 8, true, kShift>, ceil_div(rows, 4), 128, 8);
-  const int threads = static_cast<int>(ceil_div(ceil_div(packs, kNV), 32) * 32);
-  return go(quantize_rows_kernel<T, kNV, false, kShift>, rows, threads, kNV);
+  // A block of 1024 threads has an SM to itself: 4096 x 16384 fp32 took 78.5 us with
+  // four packs a thread, 57.0 with eight. Up to 512 threads four are faster (8192 x
+  // 4096 bf16: 20.0 us against 21.4).
+  auto block = [&](int each) {
+    return static_cast<int>(ceil_div(ceil_div(packs, each), 32) * 32);
+  };
+  if (packs <= 512 * kFew)
+    return go(quantize_rows_kernel<T, kFew, false, kShift>, rows, block(kFew), kFew);
+  return go(quantize_rows_kernel<T, kMany, false, kShift>, rows, block(kMany), kMany);
 }
 
 template <typename T>
