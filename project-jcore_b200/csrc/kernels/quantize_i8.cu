@@ -122,7 +122,7 @@ __device__ __forceinline__ uint32_t low_bytes(const uint32_t *b) {
   return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
-// One row per block, or per warp (kWarpRows), held in registers between the
+// One row per block, or per kLanes lanes of a warp, held in registers between the
 // two passes: each byte is read once. Thread t of the row's `threads` takes the
 // 16-byte packs t, t + threads, ... Bound by memory: 8192 x 4096 bf16 takes 20.1 us,
 // 5.0 TB/s, fp32 29 us, 5.7 TB/s.
@@ -132,25 +132,29 @@ __device__ __forceinline__ uint32_t low_bytes(const uint32_t *b) {
 // aligned words of their own row. 8192 x 4095 bf16 takes 30 us so; a thread per
 // element took 50 us.
 // The bounds of 1024 threads are for 64 registers: two blocks of 512 on an SM.
-template <typename T, int NV, bool kWarpRows, bool kShift>
-__global__ void __launch_bounds__(kWarpRows ? 128 : 1024)
+template <typename T, int NV, int kLanes, bool kShift>
+__global__ void __launch_bounds__(kLanes ? 128 : 1024)
     quantize_rows_kernel(int64_t rows, int cols, const T *x, int64_t ldx, int8_t *q, int64_t ldq,
                          float *scale_out) {
   constexpr int V = 16 / sizeof(T);
   // Whether packs past the row are told apart: warps have many (16384 x 320 fp16 with
   // four a lane: 7.2 us against 8.4), blocks of aligned rows next to none (8192 x 4096
   // bf16: 20.5 against 19.9).
-  constexpr bool kSkip = kWarpRows || kShift;
+  constexpr bool kSkip = kLanes || kShift;
   extern __shared__ __align__(16) uint32_t bytes[];  // kShift: V bytes for each pack
   __shared__ uint32_t red[32];
   griddep_wait();
   griddep_launch_dependents();
-  const int threads = kWarpRows ? 32 : static_cast<int>(blockDim.x);
-  const int t = kWarpRows ? static_cast<int>(threadIdx.x) & 31 : static_cast<int>(threadIdx.x);
-  const int64_t row = kWarpRows ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) +
-                                      (threadIdx.x >> 5)
-                                : static_cast<int64_t>(blockIdx.x);
-  if (kWarpRows && row >= rows) return;
+  constexpr int kRow = kLanes ? kLanes : 128;
+  const int threads = kLanes ? kLanes : static_cast<int>(blockDim.x);
+  const int t = kLanes ? static_cast<int>(threadIdx.x) % kRow : static_cast<int>(threadIdx.x);
+  const int part = kLanes ? static_cast<int>(threadIdx.x) / kRow : 0;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * (128 / kRow) + part;
+  const bool live = !kLanes || row < rows;
+  if (!live) {  // beside the last rows: an empty one
+    row = 0;
+    cols = 0;
+  }
   const T *xr = x + row * ldx;
   const int head =
       kShift ? static_cast<int>(reinterpret_cast<uintptr_t>(xr) % 16 / sizeof(T)) : 0;
@@ -171,17 +175,22 @@ __global__ void __launch_bounds__(kWarpRows ? 128 : 1024)
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) top = max(top, top_of(v[i]));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (!kWarpRows) {
+  if constexpr (kLanes % 32 == 0) {
+    top = __reduce_max_sync(0xffffffffu, top);
+  } else {
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if (!kLanes) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
     const int warps = static_cast<int>(blockDim.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
     top = __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
   }
   const Scale scale = make_scale(top);
-  if (t == 0) scale_out[row] = scale.value;
+  if (t == 0 && live) scale_out[row] = scale.value;
   int8_t *qr = q + row * ldq;
-  uint32_t *line = bytes + (kWarpRows ? (threadIdx.x >> 5) * (32 * NV * V / 4) : 0);
+  uint32_t *line = bytes + (kLanes ? part * (kLanes * NV * V / 4) : 0);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int at = t + i * threads, c = at * V - head;
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(kWarpRows ? 128 : 1024)
     }
   }
   if constexpr (kShift) {
-    if (kWarpRows) __syncwarp();
+    if (kLanes) __syncwarp();
     else __syncthreads();
     const int8_t *byte = reinterpret_cast<const int8_t *>(line);
     const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(qr) % 4);
@@ -394,14 +403,17 @@ int run_rows(cudaStream_t s, int64_t rows, int64_t cols, const T *x, int64_t ldx
                                kShift ? static_cast<size_t>(threads) * each * V : 0, s, rows,
                                static_cast<int>(cols), x, ldx, q, ldq, scale);
   };
-  // A warp per row, without a barrier, while few registers hold the row (two packs a
-  // lane where they do: 16384 x 320 fp16: 6.3 us against 7.3 with four).
-  if (packs <= 32 * 2)
-    return go(quantize_rows_kernel<T, 2, true, kShift>, ceil_div(rows, 4), 128, 2);
-  if (packs <= 32 * 4)
-    return go(quantize_rows_kernel<T, 4, true, kShift>, ceil_div(rows, 4), 128, 4);
-  if (packs <= 32 * 8)
-    return go(quantize_rows_kernel<T, 8, true, kShift>, ceil_div(rows, 4), 128, 8);
+  // A warp per row, without a barrier, while few registers hold the row; two packs a
+  // lane where they do (16384 x 320 fp16: 6.3 us against 7.3 with four), then of a part
+  // of the warp (65536 x 64 bf16: 5.5 us against 17.7).
+  auto lanes = [&](auto *fn, int each, int per_row) {
+    return go(fn, ceil_div(rows, 128 / per_row), 128, each);
+  };
+  if (packs <= 8 * 2) return lanes(quantize_rows_kernel<T, 2, 8, kShift>, 2, 8);
+  if (packs <= 16 * 2) return lanes(quantize_rows_kernel<T, 2, 16, kShift>, 2, 16);
+  if (packs <= 32 * 2) return lanes(quantize_rows_kernel<T, 2, 32, kShift>, 2, 32);
+  if (packs <= 32 * 4) return lanes(quantize_rows_kernel<T, 4, 32, kShift>, 4, 32);
+  if (packs <= 32 * 8) return lanes(quantize_rows_kernel<T, 8, 32, kShift>, 8, 32);
   // A block of 1024 threads has an SM to itself: 4096 x 16384 fp32 took 78.5 us with
   // four packs a thread, 57.0 with eight. Up to 512 threads four are faster (8192 x
   // 4096 bf16: 20.0 us against 21.4).
@@ -409,8 +421,8 @@ int run_rows(cudaStream_t s, int64_t rows, int64_t cols, const T *x, int64_t ldx
     return static_cast<int>(ceil_div(ceil_div(packs, each), 32) * 32);
   };
   if (packs <= 512 * kFew)
-    return go(quantize_rows_kernel<T, kFew, false, kShift>, rows, block(kFew), kFew);
-  return go(quantize_rows_kernel<T, kMany, false, kShift>, rows, block(kMany), kMany);
+    return go(quantize_rows_kernel<T, kFew, 0, kShift>, rows, block(kFew), kFew);
+  return go(quantize_rows_kernel<T, kMany, 0, kShift>, rows, block(kMany), kMany);
 }
 
 template <typename T>

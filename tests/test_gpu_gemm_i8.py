@@ -68,6 +68,19 @@ def test_quantize_pitches_and_offsets(dtype, axis):
         check_quantized(x, axis, *quantize(lib, x, axis, ldq=ldq))
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("cols", [7, 8, 9, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257])
+def test_quantize_narrow_rows(cols, dtype):
+    # rows that share a warp: counts that do not fill the last one, pitches of any size
+    lib = S.gpu_lib()
+    for rows, pitch in ((1, cols), (15, cols), (16, cols + 8 - cols % 8), (333, cols), (70, 300)):
+        flat = torch.randn(rows * pitch, device="cuda", generator=gen(rows + cols))
+        x = flat.to(TYPES[dtype][0]).view(rows, pitch)[:, :cols]
+        around = torch.full((rows + 2, 320), 111, device="cuda", dtype=torch.int8)
+        check_quantized(x, "rows", *quantize(lib, x, "rows", q=around[1:-1]))
+        assert (around[0] == 111).all() and (around[-1] == 111).all()
+
+
 @pytest.mark.parametrize("axis", ["rows", "cols"])
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("length", [2, 5, 509, 1001, 2049, 4095, 16383, 20479])
