@@ -412,19 +412,23 @@ __device__ __forceinline__ void i8_add_slices(const I8Args &p, const uint8_t *pa
 #pragma unroll 1
   for (int i = w * kBatch; i < kPer; i += kSplitEpiWarps * kBatch) {
     const int tok = rank * kPer + i;
-    if (m0 + tok >= p.M) break;
-    uint4 v[kBatch][S];  // all loads first: a round trip to another SM each
+    const int here = min(kBatch, p.M - m0 - tok);  // of the batch; the others lie past M
+    if (here <= 0) break;
+    // All loads first: a round trip to another SM each. None that no sum below waits for:
+    // it could still be under way when that SM's CTA ends.
+    uint4 v[kBatch][S];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
+      if (b < here)
 #pragma unroll
-      for (int r = 0; r < S; ++r)
-        v[b][r] = ld_shared_cluster_v4(mapa_shared(
-            smem_u32(part) + static_cast<uint32_t>((tok + b) * kI8Channels + 4 * lane) * 4u,
-            static_cast<uint32_t>(r)));
+        for (int r = 0; r < S; ++r)
+          v[b][r] = ld_shared_cluster_v4(mapa_shared(
+              smem_u32(part) + static_cast<uint32_t>((tok + b) * kI8Channels + 4 * lane) * 4u,
+              static_cast<uint32_t>(r)));
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int64_t m = static_cast<int64_t>(m0) + tok + b;
-      if (m >= p.M) break;
+      if (b >= here) break;
       int s[4] = {};
 #pragma unroll
       for (int r = 0; r < S; ++r) {
@@ -591,7 +595,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       else i8_add_slices<MT, 8, T>(p, smem, rank, n0, m0, C);
     }
     __syncwarp();
-    cluster_sync_relaxed();  // no CTA leaves while another reads its shared memory
+    // No CTA leaves while another reads its shared memory. Ordering: the relaxed form
+    // says nothing of loads issued before it.
+    cluster_sync();
   }
   __syncthreads();
   if (warp == 1) {

@@ -1,0 +1,32 @@
+"""The barriers that end kernels whose CTAs use each other's shared memory, read
+from the source: such a fault (a CTA gone while another still reads it) must not be
+looked for by running it."""
+import re
+
+import pytest
+
+from support import PKG
+
+KERNELS = PKG / "csrc" / "kernels"
+
+
+def body(text, name):
+    """The text of kernel `name` from its name to the end of its function."""
+    at = text.index(name + "(")
+    return text[at:text.index("\n}\n", at)]
+
+
+@pytest.mark.parametrize("source,kernel", [("gemm_i8.cu", "gemm_i8_split_kernel")])
+def test_the_last_cluster_barrier_orders_what_came_before(source, kernel):
+    barriers = re.findall(r"\bcluster_sync\w*\(", body((KERNELS / source).read_text(), kernel))
+    assert barriers and barriers[-1] == "cluster_sync("
+
+
+def test_no_load_from_another_cta_goes_unused():
+    # the slices' sums: tokens that are loaded are those that are added up
+    text = (KERNELS / "gemm_i8.cu").read_text()
+    adder = text[text.index("void i8_add_slices("):]
+    adder = adder[:adder.index("\n}\n")]
+    load = adder.index("ld_shared_cluster_v4")
+    assert "if (b < here)" in adder[:load] and "if (b >= here) break" in adder[load:]
+    assert re.search(r"here = min\(kBatch, p\.M - m0 - tok\)", adder)
