@@ -740,6 +740,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
       }
+      // the MMAs' last commits have arrived here too, in both CTAs
+      for (int s = 0; s < kPairStages && !aborted; ++s)
+        if ((issued >> s) & 1u)
+          aborted = !mbar_wait_pair_async(&empty[s], (issued_phase >> s) & 1u, abort_flag,
+                                          peer_abort, p.status, kStatusTimeoutProducer);
       if (rank == 0) {
         // both CTAs' copies complete on the leader's barriers: every issued
         // phase lands before the pair can exit
@@ -823,7 +828,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (boxes && lane == 0) bulk_wait_group_read<0>();  // the boxes outlive their stores
   }
   __syncthreads();
-  cluster_sync_relaxed();  // no remote arrival, copy or MMA into either CTA is left
+  cluster_sync();  // no remote arrival, copy or MMA into either CTA is left
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc_pair(tmem_base, 512);

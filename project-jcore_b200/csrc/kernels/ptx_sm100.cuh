@@ -560,14 +560,9 @@ __device__ __forceinline__ void cluster_sync() {
                ::: "memory");
 }
 
-// The same without ordering any memory: all threads of both CTAs are here.
-__device__ __forceinline__ void cluster_sync_relaxed() {
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::
-                   : "memory");
-}
-
-// Its two halves: arriving at a kernel's start and waiting before the first access
-// to another CTA's shared memory (a CTA of the cluster may not have started yet).
+// The two halves of a cluster barrier that orders no memory, for a kernel's start:
+// arriving, then waiting before the first access to another CTA's shared memory (a CTA of
+// the cluster may not have started yet).
 __device__ __forceinline__ void cluster_arrive_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }

@@ -16,7 +16,9 @@ def body(text, name):
     return text[at:text.index("\n}\n", at)]
 
 
-@pytest.mark.parametrize("source,kernel", [("gemm_i8.cu", "gemm_i8_split_kernel")])
+@pytest.mark.parametrize("source,kernel", [("gemm_i8.cu", "gemm_i8_split_kernel"),
+                                           ("gemm_i8.cu", "gemm_i8_pair_kernel"),
+                                           ("conv_window_pair.cu", "conv_window_pair_kernel")])
 def test_the_last_cluster_barrier_orders_what_came_before(source, kernel):
     barriers = re.findall(r"\bcluster_sync\w*\(", body((KERNELS / source).read_text(), kernel))
     assert barriers and barriers[-1] == "cluster_sync("
@@ -30,3 +32,12 @@ def test_no_load_from_another_cta_goes_unused():
     load = adder.index("ld_shared_cluster_v4")
     assert "if (b < here)" in adder[:load] and "if (b >= here) break" in adder[load:]
     assert re.search(r"here = min\(kBatch, p\.M - m0 - tok\)", adder)
+
+
+def test_a_pair_waits_for_the_arrivals_of_its_mma_commits():
+    # the leader's commits arrive in both CTAs: each producer ends with a wait for the
+    # last one on every stage, so none reaches a CTA that has ended
+    text = body((KERNELS / "gemm_i8.cu").read_text(), "gemm_i8_pair_kernel")
+    producer = text[text.index("TMA producer"):text.index("MMA issuer")]
+    tail = producer[producer.index("tma_load_2d_pair(&map_x"):]
+    assert "mbar_wait_pair_async(&empty[s]" in tail
