@@ -77,6 +77,7 @@ constexpr int kPairAccCols = 2 * kPairBNC;
 constexpr int kPairTmemCols = kPairPipes * 2 * kPairAccCols;
 static_assert(kPairTmemCols == 512, "TMEM budget");
 static_assert(kPairSmemBytes <= 232448, "shared memory budget");
+static_assert(tmem_excludes_clusters(kPairSmemBytes), "no other cluster's TMEM beside a pair");
 static_assert(kPairSlabBOff % 1024 == 0 && kPairSlabBytes % 1024 == 0 &&
                   kPairWinBytes % 1024 == 0,
               "128-byte-swizzle atoms stay 1024-byte aligned");

@@ -370,8 +370,9 @@ __device__ __forceinline__ void i8_channel_scales(const I8Args &p, bool boxes, i
 // [r MT / S, (r + 1) MT / S) of all S CTAs.
 // TMEM: a CTA of a cluster must not wait for columns that another cluster holds.
 // With S > 1, MT is at most 128, and those that shared memory and threads let onto
-// an SM together (3 x 128, or 3 x 128 and one of 32, or 6 smaller) ask for at most
-// 416 of its 512 columns; CTAs without a cluster give theirs back by themselves.
+// an SM together (3 x 128, or 6 smaller) ask for at most 384 of its 512 columns; the
+// kernels of CTA pairs, which take all 512, leave too little shared memory for one
+// (kTmemClusterSmem); CTAs without a cluster give theirs back by themselves.
 // ---------------------------------------------------------------------------
 constexpr int kSplitEpiWarps = 8;
 constexpr int kSplitThreads = 64 + kSplitEpiWarps * 32;
@@ -386,9 +387,11 @@ struct SplitTraits {
   static constexpr int kTailBytes = 256 + MT * 4;
   static constexpr int kBoxBytes = kSplitEpiWarps * 4096;  // over the stages
   static constexpr int smem_bytes(int stages, bool partials) {
-    const int area = stages * kStageBytes, least = partials ? kPartialBytes : kBoxBytes;
+    const int area = stages * kStageBytes;
+    const int least = partials && kPartialBytes > kBoxBytes ? kPartialBytes : kBoxBytes;
     return 1024 + (area < least ? least : area) + kTailBytes;
   }
+  static_assert(1024 + kBoxBytes + kTailBytes >= kTmemClusterSmem, "no CTA pair beside a cluster");
   static_assert(1024 + kMostStages * kStageBytes + kTailBytes <= 232448, "shared memory budget");
 };
 
@@ -629,6 +632,7 @@ struct PairTraits {
   static constexpr int kSmemBytes =
       1024 + kStages * kPairStage + kPairEpiWarps * kBox + kScaleBytes + 256;
   static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static_assert(tmem_excludes_clusters(kSmemBytes), "no other cluster's TMEM beside a pair");
 };
 
 // Tile order: groups of 8 channel tiles sweep all token tiles, so that the

@@ -570,6 +570,17 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
+// A CTA of a cluster must not wait for TMEM that a CTA of another cluster holds: each
+// could hold what the other's partner waits for, and neither would end. So the cluster
+// kernels that take all of an SM's columns leave less than kTmemClusterSmem of its shared
+// memory, and those that take a part ask for that much at least: no two such CTAs meet on
+// an SM, whatever registers they need.
+constexpr int kSmSharedBytes = 228 * 1024, kCtaReservedBytes = 1024;
+constexpr int kTmemClusterSmem = 32 * 1024;
+constexpr bool tmem_excludes_clusters(int smem_bytes) {
+  return kSmSharedBytes - (smem_bytes + kCtaReservedBytes) < kTmemClusterSmem + kCtaReservedBytes;
+}
+
 // TMEM allocation for a CTA pair: the same warp of both CTAs executes it and
 // both receive the same base address.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst_smem, uint32_t ncols) {
