@@ -565,8 +565,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         scales[i] = m0 + i < p.M ? p.a_scale[m0 + i] : 0.0f;
       asm volatile("bar.sync 1, %0;" ::"n"(kSplitEpiWarps * 32) : "memory");  // epilogue warps
     }
-    have = mbar_wait(acc_full, 0u, abort_flag, p.status, kStatusTimeoutEpilogue);
-    __syncwarp();
+    // by the whole warp or not at all: TMEM loads are for whole warps
+    have = __all_sync(0xffffffffu, mbar_wait(acc_full, 0u, abort_flag, p.status,
+                                             kStatusTimeoutEpilogue));
     tc_fence_after_sync();
     if (have && slices == 1) {
       // boxes over the stages, which the MMAs have read out
@@ -812,10 +813,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int i = 0; i < kPairSpan; i += 32)
         mine[i + lane] = m0 + i + lane < p.M ? p.a_scale[m0 + i + lane] : 0.0f;
       __syncwarp();
-      if (!mbar_wait_pair_async(&acc_full[acc], (local >> 1) & 1, abort_flag, peer_abort,
-                                p.status, kStatusTimeoutEpilogue))
+      // by the whole warp or not at all: TMEM loads are for whole warps
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait_pair_async(&acc_full[acc], (local >> 1) & 1, abort_flag,
+                                           peer_abort, p.status, kStatusTimeoutEpilogue)))
         break;
-      __syncwarp();
       tc_fence_after_sync();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
                              static_cast<uint32_t>(acc * kPairTokens + part * kPairSpan);

@@ -41,3 +41,11 @@ def test_a_pair_waits_for_the_arrivals_of_its_mma_commits():
     producer = text[text.index("TMA producer"):text.index("MMA issuer")]
     tail = producer[producer.index("tma_load_2d_pair(&map_x"):]
     assert "mbar_wait_pair_async(&empty[s]" in tail
+
+
+@pytest.mark.parametrize("kernel", ["gemm_i8_split_kernel", "gemm_i8_pair_kernel"])
+def test_a_warp_reads_its_accumulator_as_a_whole_or_not_at_all(kernel):
+    # a wait that expires may end differently from lane to lane
+    text = re.sub(r"\s+", " ", body((KERNELS / "gemm_i8.cu").read_text(), kernel))
+    waits = re.findall(r"(__all_sync\(0xffffffffu, )?mbar_wait(?:_pair_async)?\(&?acc_full", text)
+    assert waits and all(waits)
