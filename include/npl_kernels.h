@@ -359,9 +359,10 @@ NPL_API int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw, in
                                          size_t workspace_bytes);
 
 /* ---- dropout ------------------------------------------------------------------ */
-/* y[i] = x[i] * 65536 / (65536 - t) where r(i) >= t, else 0, for n elements of
- & to the nearest integer (p in [0, 1]; t ==
- * 65536 gives all zeros) and r(i) 16 random bits that depend on seed and
+/* y[i] = x[i] * s where r(i) >= t, else 0, for n elements of type `dtype`: t is
+ * p * 65536 rounded to the nearest integer (p in [0, 1], as fp32; halves up), the
+ * scale s = 65536 / (65536 - t) in fp32 (t == 65536 gives all zeros; the product is
+ * fp32 and rounded once) and r(i) 16 random bits that depend on seed and
  * offset + i only. The mask is never stored: the gradient is the same call on
  * dy. In place (y == x) allowed; a dropped NaN or infinity gives 0. r(i) is the
  * 16-bit number j % 8 (the low half of word 0 first) of Philox4x32-10 with key
