@@ -325,10 +325,11 @@ NPL_API int nplk_binary(void *stream, int op, int64_t n, const float *a, const f
  * large). All alignments of an element's own size are taken; 16-byte aligned
  * pointers with ldx, ldy and c multiples of 16 bytes are the fastest.
  *
- * workspace: nplk_group_norm_workspace_size bytes (the same for forward and
- * backward and every type), 256-byte aligned; 0 where the arguments are
- * refused. Calls that may overlap on the GPU, captured graphs among them, need a
- * workspace each.
+ * workspace: nplk_group_norm_workspace_size bytes, 256-byte aligned: enough for forward
+ * and backward, every type and alignment, and for fewer images of the same size; the
+ * current device's SM count goes into it. 0 where the arguments are refused. A buffer
+ * smaller than what the call uses is refused (NPL_ERR_INVALID_ARG). Calls that may
+ * overlap on the GPU, captured graphs among them, need a workspace each.
  *
  * A wait of the kernels that runs out (4 s) is reported by nplk_read_status(). The
  * first call on a device allocates that status word, so it should precede any

@@ -485,7 +485,7 @@ int run_norm(cudaStream_t s, int64_t n, const NormPlan &plan, const T *x, T *y, 
   return norm_with_pack<16 / sizeof(T)>(plan.v, g.act, [&](auto pack_size, auto act) {
     constexpr int V = decltype(pack_size)::value, kAct = decltype(act)::value;
     const int tail = norm_tail_bytes(plan.threads, V, g.pitch, g.gs, plan.keep);
-    float2 *stats = work, *partial = work + plan.batch * g.groups;
+    float2 *stats = work, *partial = work + norm_work(plan, n, 1).stats / 2;
     for (int64_t i = 0; i < n; i += plan.batch) {
       const int64_t count = std::min(n - i, plan.batch);
       const T *xi = x + i * g.hw * g.ldx;
@@ -543,11 +543,11 @@ extern "C" int nplk_group_norm_act(void *stream, int64_t n, int64_t hw, int64_t 
   for (const float *p : {gamma, beta, static_cast<const float *>(mean),
                          static_cast<const float *>(rstd)})
     if (!norm_aligned(p, 4)) return kErrInvalidArg;
-  if (!workspace || !norm_aligned(workspace, 256) ||
-      workspace_bytes < norm_workspace(n, hw, c, groups))
-    return kErrInvalidArg;
   const int fx = norm_pack_fit(x, ldx, size), fy = norm_pack_fit(y, ldy, size);
-  NormPlan plan = plan_norm(n, hw, c, groups, size, std::min(fx, fy), 1);
+  NormPlan plan = plan_norm({n, hw, c, groups, size, std::min(fx, fy), 1});
+  if (!workspace || !norm_aligned(workspace, 256) ||
+      workspace_bytes < std::max(kNormWorkLeast, norm_work(plan, n, 1).bytes()))
+    return kErrInvalidArg;
   plan.g.ldx = ldx;
   plan.g.ldy = ldy;
   plan.g.gamma = gamma;

@@ -101,91 +101,122 @@ inline int64_t norm_rows_bytes(const NormGeom &g, int size) {
   return (rows * g.pitch * size + 127) / 128 * 128;
 }
 
-// `tensors`: what is read (x; or x and dy).
-inline NormPlan plan_norm(int64_t n, int64_t hw, int64_t c, int64_t groups, int size, int v_fit,
-                          int tensors) {
+// What a plan is made from. `tensors`: what is read (x; or x and dy). v: elements of a
+// pack; gs0: the fewest groups that fill whole packs.
+struct NormSize {
+  int64_t n, hw, c, groups;
+  int size, tensors, cg, v, gs0;
+
+  NormSize(int64_t n_, int64_t hw_, int64_t c_, int64_t groups_, int size_, int v_fit,
+           int tensors_)
+      : n(n_), hw(hw_), c(c_), groups(groups_), size(size_), tensors(tensors_),
+        cg(static_cast<int>(c_ / groups_)), v(v_fit) {
+    auto gcd = [](int a, int b) {
+      while (b) {
+        const int t = a % b;
+        a = b;
+        b = t;
+      }
+      return a;
+    };
+    // The widest packs that the pointers allow and that fill whole groups within
+    // 8192 channels (v divides c, so v / gcd(v, cg) divides the group count).
+    while (v > 1 && (c % v != 0 || v / gcd(v, cg) * cg > 8192)) v /= 2;
+    gs0 = v / gcd(v, cg);
+  }
+  int64_t row(int gs) const { return static_cast<int64_t>(gs) * cg * size; }
+  // Images whose tensors stay in L2 between two passes (72 of its 126 MB: 4 x 16384 x 512
+  // bf16 took 43.8 us in one batch, 53.8 in two).
+  int64_t l2_images() const {
+    return std::max<int64_t>(1, (72 << 20) / (hw * c * size * tensors));
+  }
+  // CTAs of a pass over memory that the SMs hold at once.
+  int64_t ctas_at_once() const { return static_cast<int64_t>(sm_count()) * (tensors == 1 ? 3 : 2); }
+  // Runs of rows, where `images` images share the SMs.
+  int64_t chunks(int strips, int64_t images) const {
+    return std::max<int64_t>(1, std::min(ctas_at_once() / (strips * images), norm_most_chunks(hw)));
+  }
+};
+
+inline NormPlan norm_plan_base(const NormSize &z) {
   NormPlan p{};
-  const int cg = static_cast<int>(c / groups);
-  auto gcd = [](int a, int b) {
-    while (b) {
-      const int t = a % b;
-      a = b;
-      b = t;
-    }
-    return a;
-  };
-  // The widest packs that the pointers allow and that fill whole groups within
-  // 8192 channels (v divides c, so v / gcd(v, cg) divides the group count).
-  int v = v_fit;
-  while (v > 1 && (c % v != 0 || v / gcd(v, cg) * cg > 8192)) v /= 2;
-  const int gs0 = v / gcd(v, cg);
-  const int sms = sm_count();
-  p.v = v;
-  p.g.hw = static_cast<uint32_t>(hw);
-  p.g.c = static_cast<int>(c);
-  p.g.groups = static_cast<int>(groups);
-  p.g.cg = cg;
-  p.g.div_cg = make_fastdiv(static_cast<uint32_t>(cg));
-  auto row = [&](int gs) { return static_cast<int64_t>(gs) * cg * size; };
+  p.v = z.v;
+  p.g.hw = static_cast<uint32_t>(z.hw);
+  p.g.c = static_cast<int>(z.c);
+  p.g.groups = static_cast<int>(z.groups);
+  p.g.cg = z.cg;
+  p.g.div_cg = make_fastdiv(static_cast<uint32_t>(z.cg));
+  return p;
+}
+
+// Kept form: strips of at least 64 bytes a row; of those up to 512 bytes, the
+// narrowest in whole 32-byte sectors if 48 KB in each of 8 CTAs hold it, else the
+// narrowest. Up to 48 KB a CTA keeps several on an SM, so that one's loads run
+// under another's stores; more CTAs while they are few.
+inline NormPlan plan_norm_kept(const NormSize &z) {
+  NormPlan p = norm_plan_base(z);
   auto threads_for = [&](int64_t rows, int cw, int64_t ctas) {
     // What a thread does once costs as much as ten packs. Six packs a thread while
     // there are few CTAs (2 x 1024 x 640 bf16: 8.1 us, with 20 packs 10.2); where there
     // are many, 20 forward (8 x 4096 x 320: 18.6 us against 24.8 with six) and 12 in the
     // gradient (3 x 961 x 510 fp32: 12.6 against 18.4).
-    const int each = 2 * ctas <= 3 * sms ? 6 : tensors == 1 ? 20 : 12;
-    int64_t t = ceil_div(ceil_div(rows * (cw / v), each), 32) * 32;
-    t = std::max<int64_t>(t, ceil_div(cw / v, 32) * 32);
+    const int each = 2 * ctas <= 3 * sm_count() ? 6 : z.tensors == 1 ? 20 : 12;
+    int64_t t = ceil_div(ceil_div(rows * (cw / z.v), each), 32) * 32;
+    t = std::max<int64_t>(t, ceil_div(cw / z.v, 32) * 32);
     return static_cast<int>(std::min<int64_t>(std::max<int64_t>(t, 64), kNormThreads));
   };
-
-  // Kept form: strips of at least 64 bytes a row; of those up to 512 bytes, the
-  // narrowest in whole 32-byte sectors if 48 KB in each of 8 CTAs hold it, else the
-  // narrowest. Up to 48 KB a CTA keeps several on an SM, so that one's loads run
-  // under another's stores; more CTAs while they are few.
-  int gs = gs0;
-  while (gs + gs0 <= groups && row(gs) < 64) gs += gs0;
-  for (int m = gs; m <= groups && row(m) <= 512; m += gs0) {
-    if (row(m) % 32 == 0 && ceil_div(hw, 8) * row(m) * tensors <= 48 * 1024) {
+  int gs = z.gs0;
+  while (gs + z.gs0 <= z.groups && z.row(gs) < 64) gs += z.gs0;
+  for (int m = gs; m <= z.groups && z.row(m) <= 512; m += z.gs0) {
+    if (z.row(m) % 32 == 0 && ceil_div(z.hw, 8) * z.row(m) * z.tensors <= 48 * 1024) {
       gs = m;
       break;
     }
   }
   p.g.gs = gs;
-  p.g.strips = static_cast<int>(ceil_div(groups, gs));
+  p.g.strips = static_cast<int>(ceil_div(z.groups, gs));
   p.g.chunks = 1;
   int s = 1;
-  auto slab = [&](int slices) { return ceil_div(hw, slices) * row(gs) * tensors; };
-  const int64_t ctas = n * p.g.strips;
-  while (s < 8 && (slab(s) > 48 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sms))) s *= 2;
+  auto slab = [&](int slices) { return ceil_div(z.hw, slices) * z.row(gs) * z.tensors; };
+  const int64_t ctas = z.n * p.g.strips;
+  while (s < 8 && (slab(s) > 48 * 1024 || (slab(s) > 16 * 1024 && ctas * s < 2 * sm_count())))
+    s *= 2;
   p.g.slices = s;
-  p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, s));
-  p.threads = threads_for(p.g.cta_rows, gs * cg, ctas * s);
-  norm_finish(p, n, size);
-  if (tensors * norm_rows_bytes(p.g, size) + norm_tail_bytes(p.threads, v, gs * cg, gs, true) <=
-      kNormKeepLimit) {
-    p.keep = true;
-    const int64_t most = ((int64_t(1) << 31) - 1) / (static_cast<int64_t>(p.g.strips) * s);
-    p.batch = std::min(n, most);
-    return p;
-  }
+  p.g.cta_rows = static_cast<uint32_t>(ceil_div(z.hw, s));
+  p.threads = threads_for(p.g.cta_rows, gs * z.cg, ctas * s);
+  const int64_t most = ((int64_t(1) << 31) - 1) / (static_cast<int64_t>(p.g.strips) * s);
+  p.batch = std::min(z.n, most);
+  p.keep = true;
+  norm_finish(p, z.n, z.size);
+  return p;
+}
+inline bool norm_fits(const NormPlan &p, const NormSize &z) {
+  return z.tensors * norm_rows_bytes(p.g, z.size) +
+             norm_tail_bytes(p.threads, z.v, p.g.gs * z.cg, p.g.gs, true) <=
+         kNormKeepLimit;
+}
 
-  // Passes over memory: strips as wide as a CTA, one long run of rows for each CTA
-  // that the SMs hold at once. Images in batches whose tensors stay in L2 between
-  // the passes (72 of its 126 MB: 4 x 16384 x 512 bf16 took 43.8 us in one batch,
-  // 53.8 in two).
-  gs = gs0;
-  while (gs + gs0 <= groups && gs + gs0 <= 256 && (gs + gs0) * cg <= kNormThreads * v) gs += gs0;
+// Passes over memory: strips as wide as a CTA, one long run of rows for each CTA
+// that the SMs hold at once, images in batches whose tensors stay in L2.
+inline NormPlan plan_norm_passes(const NormSize &z) {
+  NormPlan p = norm_plan_base(z);
+  int gs = z.gs0;
+  while (gs + z.gs0 <= z.groups && gs + z.gs0 <= 256 && (gs + z.gs0) * z.cg <= kNormThreads * z.v)
+    gs += z.gs0;
   p.g.gs = gs;
-  p.g.strips = static_cast<int>(ceil_div(groups, gs));
-  p.batch = std::min(n, std::max<int64_t>(1, (72 << 20) / (hw * c * size * tensors)));
+  p.g.strips = static_cast<int>(ceil_div(z.groups, gs));
+  p.batch = std::min(z.n, z.l2_images());
   p.g.slices = 1;
   p.threads = kNormThreads;
-  const int64_t chunks =
-      static_cast<int64_t>(sms) * (tensors == 1 ? 3 : 2) / (p.g.strips * p.batch);
-  p.g.chunks = static_cast<int>(std::max<int64_t>(1, std::min(chunks, norm_most_chunks(hw))));
-  p.g.cta_rows = static_cast<uint32_t>(ceil_div(hw, p.g.chunks));
-  norm_finish(p, n, size);
+  p.g.chunks = static_cast<int>(z.chunks(p.g.strips, p.batch));
+  p.g.cta_rows = static_cast<uint32_t>(ceil_div(z.hw, p.g.chunks));
+  norm_finish(p, z.n, z.size);
   return p;
+}
+
+inline NormPlan plan_norm(const NormSize &z) {
+  const NormPlan kept = plan_norm_kept(z);
+  return norm_fits(kept, z) ? kept : plan_norm_passes(z);
 }
 
 // Elements of a pack that a pointer and pitch allow, at most 16 bytes.
@@ -204,11 +235,53 @@ inline int norm_check(int64_t n, int64_t hw, int64_t c, int64_t groups) {
   return kOk;
 }
 
-// Per image: chunks * (2 c + 2 groups) sums, and 4 per group that the second pass reads.
+// The workspace, in floats. Forward, in passes over memory: [batch][groups] mean and
+// rstd, [batch * chunks][groups] mean and M2. Gradient: in passes over memory
+// [batch][groups] statistics of four and [batch * chunks][groups] A, B; then, in both
+// forms, [n * chunks][2][c] channel sums.
+struct NormWork {
+  int64_t stats, partial, channels;
+  size_t bytes() const { return static_cast<size_t>(stats + partial + channels) * sizeof(float); }
+};
+inline NormWork norm_work(const NormPlan &p, int64_t n, int tensors) {
+  NormWork w{};
+  if (!p.keep) {
+    w.stats = p.batch * p.g.groups * (tensors == 1 ? 2 : 4);
+    w.partial = p.batch * p.g.chunks * p.g.groups * 2;
+  }
+  if (tensors == 2) w.channels = n * p.g.chunks * 2 * p.g.c;
+  return w;
+}
+constexpr size_t kNormWorkLeast = 256;
+
+// What suffices for either direction, every type and alignment, and for fewer images.
 inline size_t norm_workspace(int64_t n, int64_t hw, int64_t c, int64_t groups) {
-  return align_up(static_cast<size_t>(n) *
-                      (norm_most_chunks(hw) * (2 * c + 2 * groups) + 4 * groups) * sizeof(float),
-                  256);
+  size_t most = kNormWorkLeast;
+  for (int size : {2, 4}) {
+    for (int v = 16 / size; v >= 1; v /= 2) {
+      for (int tensors : {1, 2}) {
+        const NormSize z(n, hw, c, groups, size, v, tensors);
+        NormPlan p = plan_norm_kept(z);
+        // Fewer images have as many slices or more, and so no more rows in a CTA, but
+        // perhaps more threads, and boxes where the rows of all would not take them.
+        p.threads = kNormThreads;
+        norm_finish(p, 1, size);
+        if (!norm_fits(p, z)) {
+          // k images have max(1, min(T / (strips min(k, B)), most)) chunks each, B = l2_images(),
+          // T = ctas_at_once(): k <= B of them max(k, min(k most, T / strips)) at most
+          p = plan_norm_passes(z);
+          const int64_t together =
+              std::max(n, std::min(n * norm_most_chunks(hw), z.ctas_at_once() / p.g.strips));
+          const int64_t runs = std::max(together, n * z.chunks(p.g.strips, z.l2_images()));
+          const NormWork w{n * groups * 4, runs * groups * 2, tensors == 2 ? runs * 2 * c : 0};
+          most = std::max(most, w.bytes());
+        } else {
+          most = std::max(most, norm_work(p, n, tensors).bytes());
+        }
+      }
+    }
+  }
+  return align_up(most, 256);
 }
 
 inline bool norm_aligned(const void *p, int bytes) {

@@ -508,9 +508,6 @@ extern "C" int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw,
   for (const float *p : {mean, rstd, gamma, beta, static_cast<const float *>(dgamma),
                          static_cast<const float *>(dbeta)})
     if (!norm_aligned(p, 4)) return kErrInvalidArg;
-  if (!workspace || !norm_aligned(workspace, 256) ||
-      workspace_bytes < norm_workspace(n, hw, c, groups))
-    return kErrInvalidArg;
   int fit = norm_pack_fit(x, ldx, size);
   fit = std::min(fit, norm_pack_fit(dy, lddy, size));
   fit = std::min(fit, norm_pack_fit(dx, lddx, size));
@@ -518,7 +515,11 @@ extern "C" int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw,
   // pack's channels leave half as many warps on an SM (8 x 4096 x 320 bf16: 41.8 us
   // against 37.5; 1 x 64 x 1280: 9.9 against 7.0).
   fit = std::min(fit, 4);
-  NormPlan plan = plan_norm(n, hw, c, groups, size, fit, 2);
+  NormPlan plan = plan_norm({n, hw, c, groups, size, fit, 2});
+  const NormWork room = norm_work(plan, n, 2);
+  if (!workspace || !norm_aligned(workspace, 256) ||
+      workspace_bytes < std::max(kNormWorkLeast, room.bytes()))
+    return kErrInvalidArg;
   plan.g.ldx = ldx;
   plan.g.ldy = lddx;
   plan.g.lddy = lddy;
@@ -529,13 +530,11 @@ extern "C" int nplk_group_norm_act_backward(void *stream, int64_t n, int64_t hw,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   plan.g.status = device_status_word();
   if (!plan.g.status) return kErrInternal;
-  // The workspace: [batch][groups] statistics, [batch * chunks][groups] A, B, then
-  // [n * chunks][2][c] channel sums.
   const int64_t rows = n * plan.g.chunks;
   GradArgs a{mean, rstd, nullptr, nullptr};
   float4 *stat = static_cast<float4 *>(workspace);
-  a.groups = reinterpret_cast<float2 *>(stat + plan.batch * groups);
-  float *channels = reinterpret_cast<float *>(a.groups + plan.batch * plan.g.chunks * groups);
+  a.groups = reinterpret_cast<float2 *>(static_cast<float *>(workspace) + room.stats);
+  float *channels = static_cast<float *>(workspace) + room.stats + room.partial;
   a.channels = dgamma || dbeta ? channels : nullptr;
   int rc;
   if (dtype == NPLK_DTYPE_FP32)
