@@ -4,7 +4,6 @@
 
 #include <type_traits>
 
-#include "activation_grad.cuh"
 #include "nplk_device.cuh"
 #include "typed_io.cuh"
 
@@ -126,11 +125,33 @@ __device__ __forceinline__ void act_array(float (&v)[V], int act, float alpha) {
   }
 }
 
+// act'(x) of the activations that act_slope_array has no form of its own for: codes 2, 3,
+// 4 and 7..10. LeakyReLU, ELU and SELU take the left-hand value at 0, ReLU6 is 0 at both
+// bends.
 static __device__ __noinline__ float act_slope_call(float x, int act, float alpha) {
-  return act_slope(x, act, alpha);
+  switch (act) {
+    case 2:
+      return x > 0.0f && x < 6.0f ? 1.0f : 0.0f;
+    case 3: {
+      const float t = tanhf(x);
+      return 1.0f - t * t;
+    }
+    case 4: {
+      const float s = 1.0f / (1.0f + expf(-x));
+      return s * (1.0f - s);
+    }
+    case 7:
+      return x > 0.0f ? 1.0f : alpha;
+    case 8:
+      return x > 0.0f ? 1.0f : expf(x);
+    case 9:
+      return 1.05070098f * (x > 0.0f ? 1.0f : 1.67326324f * expf(x));
+    default:  // 10
+      return 1.0f / (1.0f + expf(-x));
+  }
 }
 
-// v[j] = act'(v[j]), for gradients stored as T.
+// v[j] = act'(v[j]), for gradients stored as T; ReLU's left-hand value at 0.
 template <typename T, int V>
 __device__ __forceinline__ void act_slope_array(float (&v)[V], int act, float alpha) {
   constexpr bool kFine = std::is_same<T, float>::value;
