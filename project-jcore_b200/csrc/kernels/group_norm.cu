@@ -27,6 +27,11 @@ struct Moments {
   float n, mean, m2;
 };
 
+// Weights of a join use the hardware's reciprocal as it is, within 2^-23: a weight is a
+// factor of the difference of two means or of its square, and moves a mean by that much of
+// the difference, which rounds by 2^-24 as it is; the variance by that much of itself. Only
+// a whole mean is multiplied by a refined one (rcp_fine).
+
 // 1 / x within a step of 2^-23 (one Newton step on the approximate reciprocal), x in
 // the range of counts.
 __device__ __forceinline__ float rcp_fine(float x) {
@@ -142,7 +147,7 @@ __device__ __forceinline__ void put_moments(const NormGeom &p, const NormPlace &
       sum1 += j < first ? 0.0f : mean[j];
     }
     const float k0 = static_cast<float>(first < V ? first : V), k1 = V - k0;
-    const float mean0 = sum0 * rcp_approx(k0), mean1 = k1 > 0.0f ? sum1 * rcp_approx(k1) : 0.0f;
+    const float mean0 = sum0 * rcp_fine(k0), mean1 = k1 > 0.0f ? sum1 * rcp_fine(k1) : 0.0f;
     float q0 = 0.0f, q1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
