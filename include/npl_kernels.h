@@ -315,14 +315,16 @@ NPL_API int nplk_binary(void *stream, int op, int64_t n, const float *a, const f
  * slice of a wider tensor has ldx > c), and the same with ldy; x and y are of
  * type `dtype` (NPLK_DTYPE_*), gamma and beta [c] and mean and rstd [n][groups]
  * are fp32. gamma, beta (1 and 0), mean and rstd may be NULL. act is 0..10 with
- * the formulas of nplk_activation; statistics and the normalised value are fp32,
- * y is rounded once. y may be x itself (then ldy == ldx). A NaN or an infinity
- * makes its group NaN and no other.
+ * the formulas of nplk_activation, GELU and swish as x times a sigmoid by the hardware's
+ * exponential: in fp32 within 2^-21 (1 + |y|) of the formula, and within 4e-17 of it
+ * where it tends to 0 (below -41.5 for swish, -7.4 for GELU, where nplk_activation goes
+ * on to smaller values). Statistics and the normalised value are fp32, y is rounded
+ * once. y may be x itself (then ldy == ldx). A NaN or an infinity makes its group NaN
+ * and no other.
  *
  * Sizes: c a multiple of groups, c / groups <= 8192, c <= 2^24, hw < 2^31 and
- * n * groups < 2^31; else
- * NPL_ERR_INVALID_ARG (not a multiple, a size < 1) or NPL_ERR_UNSUPPORTED (too
- * large). All alignments of an element's own size are taken; 16-byte aligned
+ * n * groups < 2^31; else NPL_ERR_INVALID_ARG (not a multiple, a size < 1) or
+ * NPL_ERR_UNSUPPORTED (too large). All alignments of an element's own size are taken; 16-byte aligned
  * pointers with ldx, ldy and c multiples of 16 bytes are the fastest.
  *
  * workspace: nplk_group_norm_workspace_size bytes, 256-byte aligned: enough for forward
@@ -344,7 +346,7 @@ NPL_API int nplk_group_norm_act(void *stream, int64_t n, int64_t hw, int64_t c, 
 /* Gradient of nplk_group_norm_act for its output gradient dy, from x and the
  * mean and rstd that the forward call stored. With xh = (x - mean) * rstd,
  * z = gamma * xh + beta and dz = dy * act'(z) (act' of ReLU and LeakyReLU at 0
- * taken from the left, of ReLU6 0 at both bends):
+ * taken from the left, of ReLU6 0 at both bends; of GELU and swish within 2^-17):
  *   dgamma[ch] = sum dz * xh,  dbeta[ch] = sum dz  over images and pixels,
  *   dx = rstd * (gamma * dz - (sum gamma * dz + xh * sum gamma * dz * xh) / M),
  * the sums of dx over the group's M = hw * c / groups values. dgamma and dbeta
@@ -400,7 +402,7 @@ NPL_API int nplk_quantize_cols(void *stream, int64_t rows, int64_t cols, int dty
  * and ldb; a_scale [M], b_scale [N] and bias [N] (may be NULL) fp32; C row-major
  * of type c_dtype (NPLK_DTYPE_*), pitch ldc. The sums are exact 32-bit integers
  * (K <= 131071, else NPL_ERR_UNSUPPORTED), converted once to fp32; act is 0..10
- * as in nplk_activation; C is rounded once and must not overlap the inputs. A row of
+ * as in nplk_group_norm_act; C is rounded once and must not overlap the inputs. A row of
  * C depends on its own row of A alone, to the bit, whatever M is.
  * Any pitch and alignment is taken; the tensor-core kernels need A and B
  * 16-byte aligned with lda and ldb multiples of 16, other operands take a
