@@ -3,6 +3,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -164,57 +165,49 @@ int encode_2d_f32(CUtensorMap *map, const void *base, uint64_t inner, uint64_t o
 }
 }  // namespace
 
-int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
-                            uint64_t row_pitch_bytes, uint32_t box_outer) {
+namespace {
+int encode_2d(CUtensorMap *map, CUtensorMapDataType type, const void *base, uint64_t inner,
+              uint64_t outer, uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer,
+              CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   auto fn = encode_fn();
   if (!fn) return kErrInternal;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (row_pitch_bytes & 15u) != 0)
     return kErrInvalidArg;
+  // The pitch of a single row leads nowhere, and maps take none from 2^40 on.
+  if (outer == 1) row_pitch_bytes = std::min<uint64_t>(row_pitch_bytes, uint64_t(1) << 36);
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_pitch_bytes};
-  cuuint32_t box[2] = {128, box_outer};
+  cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides,
-                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = fn(map, type, 2, const_cast<void *>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? kOk : kErrInternal;
+}
+
+CUtensorMapDataType word_type(int element_bytes) {
+  return element_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+}
+}  // namespace
+
+int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                            uint64_t row_pitch_bytes, uint32_t box_outer) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, row_pitch_bytes, 128,
+                   box_outer, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 int encode_tmap_2d_plain(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
                          uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer,
                          int element_bytes) {
-  auto fn = encode_fn();
-  if (!fn) return kErrInternal;
-  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (row_pitch_bytes & 15u) != 0)
-    return kErrInvalidArg;
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_pitch_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, element_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32
-                                          : CU_TENSOR_MAP_DATA_TYPE_UINT16,
-                  2, const_cast<void *>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? kOk : kErrInternal;
+  return encode_2d(map, word_type(element_bytes), base, inner, outer, row_pitch_bytes, box_inner,
+                   box_outer, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 int encode_tmap_2d_box32(CUtensorMap *map, void *base, uint64_t inner, uint64_t outer,
                          uint64_t row_pitch_bytes, int element_bytes) {
-  auto fn = encode_fn();
-  if (!fn) return kErrInternal;
-  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (row_pitch_bytes & 15u) != 0)
-    return kErrInvalidArg;
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_pitch_bytes};
-  cuuint32_t box[2] = {32, 32};
-  cuuint32_t estr[2] = {1, 1};
-  const bool wide = element_bytes == 4;
-  CUresult r = fn(map, wide ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
-                  base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  wide ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B,
-                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? kOk : kErrInternal;
+  return encode_2d(map, word_type(element_bytes), base, inner, outer, row_pitch_bytes, 32, 32,
+                   element_bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
 int encode_tmap_im2col_nhwc_f32_sw128(CUtensorMap *map, const void *base, uint64_t c,

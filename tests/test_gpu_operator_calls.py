@@ -148,3 +148,37 @@ def test_a_stream_that_is_not_the_current_one():
     # rows of the identity are 127 / 127: the product gives the rounded rows back
     want = d.float().view(-1, c)
     assert ((out - want).abs() <= 0.51 * scale[:, None]).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 1, 64), (40, 1, 4096), (1000, 1, 64), (1, 200, 64)])
+def test_the_pitch_of_a_single_row_is_of_no_account(m, n, k):
+    lib, far = S.gpu_lib(), 1 << 44
+    a, b, sa, sb, bias = operands(m, n, k)
+    want = product(lib, a, b, sa, sb, bias)
+    c, status = torch.empty_like(want), torch.zeros(1, device="cuda", dtype=torch.int32)
+    assert lib.nplk_gemm_i8(S.cuda_stream(), m, n, k, a.data_ptr(), far if m == 1 else k,
+                            sa.data_ptr(), b.data_ptr(), far if n == 1 else k, sb.data_ptr(),
+                            bias.data_ptr(), 0, 0.1, 0, c.data_ptr(), far if m == 1 else n,
+                            status.data_ptr()) == 0
+    assert torch.equal(c, want) and status.item() == 0
+
+
+@pytest.mark.parametrize("c,groups", [(64, 8), (8192, 1)])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_the_pitch_of_a_single_pixel_is_of_no_account(c, groups, dtype):
+    lib, far = S.gpu_lib(), 1 << 44
+    x, dy, gamma, beta = inputs(1, 1, c, dtype)
+    y, mean, rstd = forward(lib, x, c, groups, gamma, beta, act=6)
+    dx, _, _ = backward(lib, dy, x, c, groups, mean, rstd, gamma, beta, act=6)
+    work, size = workspace(lib, 1, 1, c, groups)
+    code = {"fp32": 0, "fp16": 1, "bf16": 2}[dtype]
+    y2, dx2 = torch.zeros_like(y), torch.zeros_like(dx)
+    assert lib.nplk_group_norm_act(S.cuda_stream(), 1, 1, c, groups, code, x.data_ptr(), far,
+                                   gamma.data_ptr(), beta.data_ptr(), 1e-5, 6, 0.1, y2.data_ptr(),
+                                   far, None, None, work.data_ptr(), size) == 0
+    assert lib.nplk_group_norm_act_backward(S.cuda_stream(), 1, 1, c, groups, code, dy.data_ptr(),
+                                            far, x.data_ptr(), far, mean.data_ptr(),
+                                            rstd.data_ptr(), gamma.data_ptr(), beta.data_ptr(), 6,
+                                            0.1, dx2.data_ptr(), far, None, None, work.data_ptr(),
+                                            size) == 0
+    assert torch.equal(y2, y) and torch.equal(dx2, dx)
