@@ -600,7 +600,10 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     }
     __syncwarp();
     // No CTA leaves while another reads its shared memory. Ordering: the relaxed form
-    // says nothing of loads issued before it.
+    // says nothing of loads issued before it. Its release waits for the stores of C too,
+    // 0.2 to 0.5 us; arriving before those stores is no better in sum (333 x 1000 x 1280
+    // fp32 5.6 us against 5.4, 256 x 4096 x 4096 10.4 against 10.1, 77 x 1280 x 1024 4.9
+    // against 5.3).
     cluster_sync();
   }
   __syncthreads();
@@ -877,7 +880,8 @@ int split_stages(int mt, int64_t blocks) {
 // time. The estimates (microseconds on 148 SMs) are a fit to 777 timings of 114
 // sizes, 1 to 8192 tokens, 45 to 16384 channels, K from 67 to 16384 (rms error
 // 17%); the choice they make took 2% longer than the best one on average and
-// 34% at worst (77 x 1280 x 1024: 5.0 us against 3.8).
+// 34% at worst (77 x 1280 x 1024: 5.0 us against 3.8). The clusters' last barrier has
+// become up to 0.5 us longer since the fit.
 //   split: waves * (start and end + K blocks * (latency or the bytes that the
 //          CTAs of an SM share) + results) + adding the slices
 //   pair:  start + rounds * max(K blocks, epilogue) + the shorter of the two

@@ -157,9 +157,12 @@ inline NormPlan plan_norm_kept(const NormSize &z) {
   NormPlan p = norm_plan_base(z);
   auto threads_for = [&](int64_t rows, int cw, int64_t ctas) {
     // What a thread does once costs as much as ten packs. Six packs a thread while
-    // there are few CTAs (2 x 1024 x 640 bf16: 8.1 us, with 20 packs 10.2); where there
-    // are many, 20 forward (8 x 4096 x 320: 18.6 us against 24.8 with six) and 12 in the
-    // gradient (3 x 961 x 510 fp32: 12.6 against 18.4).
+    // there are few CTAs (2 x 1024 x 640 bf16: 7.9 us, with 20 packs 9.7); where there
+    // are many, 20 forward (8 x 4096 x 320: 18.5 us against 24.3 with six) and 12 in the
+    // gradient (3 x 961 x 510 fp32: 12.6 against 18.4). From 223 CTAs on the better
+    // choice changes with how they fill the SMs: six would be 12% faster at 384 CTAs (6 x
+    // 1024 x 640 forward: 10.7 us against 12.1) and 11% at 768, 34% slower at 512 (8 x
+    // 1024 x 640: 17.3 against 12.9) and 28% at 1024.
     const int each = 2 * ctas <= 3 * sm_count() ? 6 : z.tensors == 1 ? 20 : 12;
     int64_t t = ceil_div(ceil_div(rows * (cw / z.v), each), 32) * 32;
     t = std::max<int64_t>(t, ceil_div(cw / z.v, 32) * 32);
