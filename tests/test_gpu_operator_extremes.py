@@ -7,6 +7,7 @@ import torch
 import support as S
 from support import nb
 from test_gpu_gemm_i8 import check_product, check_quantized
+from test_gpu_group_norm import backward, check_backward, check_forward, forward, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -156,3 +157,28 @@ def test_product_of_many_tokens_or_channels(m, n):
             check_product(c[p], a[p], b, sa[p], sb, bias, "fp16")
         else:
             check_product(c[:, p], a, b[p], sa, sb[p], bias[p], "fp16")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("groups,hw", [(1 << 24, 5), (1 << 20, 3), (2048, 2), (1 << 21, 40)])
+def test_group_norm_of_the_most_channels(groups, hw, dtype):
+    lib, c = S.gpu_lib(), 1 << 24
+    x, dy, gamma, beta = inputs(1, hw, c, dtype)
+    y, mean, rstd = forward(lib, x, c, groups, gamma, beta, act=6)
+    check_forward(x, c, groups, gamma, beta, 6, 1e-5, y, mean, rstd)
+    dx, dg, db = backward(lib, dy, x, c, groups, mean, rstd, gamma, beta, act=6)
+    check_backward(x, dy, c, groups, mean, rstd, gamma, beta, 6, dx, dg, db)
+    assert lib.nplk_read_status(S.cuda_stream()) == 0
+
+
+def test_group_norm_of_the_most_groups_and_one_pixel():
+    # a group a value: x - mean is 0, y is beta, every gradient of x 0
+    lib, n, c = S.gpu_lib(), 127, 1 << 24
+    x, dy, gamma, beta = inputs(1, n, c, "bf16")
+    x, dy = x.view(n, 1, c), dy.view(n, 1, c)
+    y, mean, rstd = forward(lib, x, c, c, gamma, beta)
+    assert torch.equal(y, beta.bfloat16().expand_as(y)) and torch.equal(mean, x[:, 0].float())
+    dx, dg, db = backward(lib, dy, x, c, c, mean, rstd, gamma, beta)
+    assert (dg == 0).all()
+    # rstd (gamma dy - gamma dy): two roundings of rstd gamma dy
+    assert (dx.float().abs() <= 4 * U * rstd[:, None] * (gamma * dy.float()).abs()).all()
