@@ -324,8 +324,8 @@ NPL_API int nplk_binary(void *stream, int op, int64_t n, const float *a, const f
  *
  * Sizes: c a multiple of groups, c / groups <= 8192, c <= 2^24, hw < 2^31 and
  * n * groups < 2^31; else NPL_ERR_INVALID_ARG (not a multiple, a size < 1) or
- * NPL_ERR_UNSUPPORTED (too large). All alignments of an element's own size are taken; 16-byte aligned
- * pointers with ldx, ldy and c multiples of 16 bytes are the fastest.
+ * NPL_ERR_UNSUPPORTED (too large). All alignments of an element's own size are taken;
+ * 16-byte aligned pointers with ldx, ldy and c multiples of 16 bytes are the fastest.
  *
  * workspace: nplk_group_norm_workspace_size bytes, 256-byte aligned: enough for forward
  * and backward, every type and alignment, and for fewer images of the same size; the
