@@ -414,6 +414,79 @@ NPL_API int nplk_gemm_i8(void *stream, int64_t M, int64_t N, int64_t K, const in
                          const float *b_scale, const float *bias, int act, float act_alpha,
                          int c_dtype, void *C, int64_t ldc, int *status);
 
+/* ---- weights in 4 bits ---------------------------------------------------------- */
+/* Weights [N][K] (output channels by K) in groups of `group` (32, 64 or 128, others
+ * NPL_ERR_UNSUPPORTED) values along K, the last group of a row possibly shorter. Two
+ * 4-bit numbers to a byte, the one of even k in the low half: row n starts at q + n * ldq
+ * (bytes). The weight is scale * (nibble - zero), the scale (type scale_dtype,
+ * NPLK_DTYPE_*) at scale[n * lds + k / group], the zero at zero[n * ldz + k / group] (a
+ * byte, its low four bits), or 8 throughout where `zero` is NULL. The reference has
+ * no types below 8 bits.
+ *
+ * nplk_quantize_w4 makes them from w (type dtype, pitch ldw), once, before serving:
+ *   zero == NULL: s = max|w| / 7,            nibble = rint(w / scale) + 8,
+ *   otherwise:    s = (high - low) / 15,     zero = rint(-low / scale),
+ *                 nibble = rint(w / scale) + zero,
+ * both of a group's own values, high = max(0, max w), low = min(0, min w); s is
+ * rounded to scale_dtype and is at least that type's smallest normal number: that is
+ * `scale`, by which the quotients (fp32, rounded to nearest, ties to even) are taken.
+ * Nibbles and zeros are clamped to 0..15. The half byte behind an odd K is 0; bytes
+ * from (K + 1) / 2 to ldq are left as they are. A group that holds a NaN gets scale
+ * NaN, one whose s is infinite in scale_dtype infinity, both with equal nibbles
+ * and zeros. w and the results must not overlap. N, K <= 2^30. */
+NPL_API int nplk_quantize_w4(void *stream, int64_t N, int64_t K, int64_t group, int dtype,
+                             const void *w, int64_t ldw, uint8_t *q, int64_t ldq,
+                             int scale_dtype, void *scale, int64_t lds, uint8_t *zero,
+                             int64_t ldz);
+
+/* C[m,n] = act(sum_k x[m,k] * weight[n,k] + bias[n]): x is [M][K] (tokens) of type
+ * x_dtype, pitch ldx; C row-major of type c_dtype, pitch ldc; bias [N] fp32 or NULL;
+ * act is 0..10 as in nplk_group_norm_act. Products are exact, sums fp32 in a fixed
+ * order (the same call gives the same bits; the order depends on M), C is rounded once.
+ * Any pitch and alignment is taken; q 16-byte aligned with ldq a multiple of 16
+ * is needed for the fast kernels. M, N, K <= 2^30. No workspace. C must not overlap the
+ * inputs. status as in nplk_gemm_i8. */
+NPL_API int nplk_gemm_w4(void *stream, int64_t M, int64_t N, int64_t K, int64_t group,
+                         int x_dtype, const void *x, int64_t ldx, const uint8_t *q, int64_t ldq,
+                         int scale_dtype, const void *scale, int64_t lds, const uint8_t *zero,
+                         int64_t ldz, const float *bias, int act, float act_alpha, int c_dtype,
+                         void *C, int64_t ldc, int *status);
+
+/* ---- log probabilities of given tokens --------------------------------------------- */
+/* For each row r of logits (rows x vocab of type dtype, pitch ld), with z = scale * l
+ * (scale > 0: the reciprocal of the temperature), p = softmax(z) and t = targets[r]:
+ *   logprob[r]  = log p[t]; 0 where t is not in 0..vocab - 1 (no token asked for)
+ *   entropy[r]  = -sum p log p (a p of 0 counts 0)
+ *   stats[2r], stats[2r + 1] = m = max l and log sum exp(z - scale * m), for the
+ *                 gradient; log sum exp(z) is scale * m + stats[2r + 1]
+ *   top_ids, top_logprobs [rows][n_top] = the n_top (0..32, more NPL_ERR_UNSUPPORTED)
+ *                 largest logits' indices and log p, largest first, of equal
+ *                 ones the lower index first.
+ * logprob, entropy, stats may each be NULL, targets if logprob is; top_ids and
+ * top_logprobs if n_top is 0; something has to be asked for. A logit of -infinity is
+ * masked: it has p = 0 and is no alternative; where there are fewer alternatives than
+ * n_top, the rest have id -1 and -infinity. A row of masked logits alone has logprob
+ * -infinity, entropy 0 and stats -infinity. A row that holds a NaN or +infinity has NaN
+ * for each result (ids -1). One pass over the logits; sums are fp32 in a fixed order.
+ * Results must not overlap the logits. vocab < 2^31 - 65536. The reference's softmax
+ * (npl_activation_norm.cpp:88-112) is the nearest it has. */
+NPL_API int nplk_token_logprobs(void *stream, int64_t rows, int64_t vocab, int dtype,
+                                const void *logits, int64_t ld, float scale,
+                                const int64_t *targets, float *logprob, float *entropy,
+                                float *stats, int n_top, int64_t *top_ids, float *top_logprobs);
+
+/* Gradient into the logits for d_logprob[r] = g and d_entropy[r] = h (each may be NULL,
+ * not both), from the stats, and where d_entropy is given the entropy, of the forward call:
+ *   dlogits[r,v] = scale * (g ([v = t] - p[v]) - h p[v] (log p[v] + entropy[r])).
+ * A row without a target counts g = 0. Rows with g = h = 0, and rows of masked logits
+ * alone, get zeros, whatever else they hold. dlogits (type dtype, pitch ldd) may be
+ * logits itself (with the same pitch), overwritten. Other arguments as the forward call. */
+NPL_API int nplk_token_logprobs_backward(void *stream, int64_t rows, int64_t vocab, int dtype,
+                                         const void *logits, int64_t ld, float scale,
+                                         const int64_t *targets, const float *stats,
+                                         const float *entropy, const float *d_logprob,
+                                         const float *d_entropy, void *dlogits, int64_t ldd);
+
 /* ---- multi-GPU helpers ------------------------------------------------------ */
 /* The reference has no multi-device path: these serve npl_matmul's product
  * (npl_tensor_ops.cpp:115-153 -> ExecuteMatMulDirect :217-311) computed as

@@ -1,0 +1,24 @@
+// Weights in 4 bits by groups along K: two to a byte, the even one in the low half;
+// a weight is scale * (nibble - zero), zero 8 where none are stored.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "npl_kernels.h"
+#include "typed_io.cuh"
+
+namespace nplk {
+
+inline bool w4_group_ok(int64_t group) { return group == 32 || group == 64 || group == 128; }
+
+// A scale of type NPLK_DTYPE_* as fp32.
+__device__ __forceinline__ float load_scale(const void *scales, int dtype, int64_t at) {
+  if (dtype == NPLK_DTYPE_FP32) return __ldg(static_cast<const float *>(scales) + at);
+  if (dtype == NPLK_DTYPE_FP16) return __half2float(__ldg(static_cast<const __half *>(scales) + at));
+  return __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(scales) + at));
+}
+
+}  // namespace nplk

@@ -212,6 +212,14 @@ NPLK_SIGNATURES = {
     "nplk_quantize_cols": (C.c_int, [_VP, _I64, _I64, C.c_int, _VP, _I64, _VP, _I64, _VP]),
     "nplk_gemm_i8": (C.c_int, [_VP, _I64, _I64, _I64, _VP, _I64, _VP, _VP, _I64, _VP, _VP,
                                C.c_int, _F, C.c_int, _VP, _I64, _VP]),
+    "nplk_quantize_w4": (C.c_int, [_VP, _I64, _I64, _I64, C.c_int, _VP, _I64, _VP, _I64, C.c_int,
+                                   _VP, _I64, _VP, _I64]),
+    "nplk_gemm_w4": (C.c_int, [_VP, _I64, _I64, _I64, _I64, C.c_int, _VP, _I64, _VP, _I64, C.c_int,
+                               _VP, _I64, _VP, _I64, _VP, C.c_int, _F, C.c_int, _VP, _I64, _VP]),
+    "nplk_token_logprobs": (C.c_int, [_VP, _I64, _I64, C.c_int, _VP, _I64, _F, _VP, _VP, _VP, _VP,
+                                      C.c_int, _VP, _VP]),
+    "nplk_token_logprobs_backward": (C.c_int, [_VP, _I64, _I64, C.c_int, _VP, _I64, _F, _VP, _VP,
+                                               _VP, _VP, _VP, _VP, _I64]),
     "nplk_colshard_relayout": (C.c_int, [_VP, _I64, _I64, _I64, _VP, _VP]),
     "nplk_ipc_handle_size": (C.c_size_t, []),
     "nplk_ipc_get_handle": (C.c_int, [_VP, _VP, _P(C.c_uint64)]),
