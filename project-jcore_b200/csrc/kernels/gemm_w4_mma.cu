@@ -1,0 +1,508 @@
+// 4-bit product for more tokens, on the tensor cores' own accumulators (tcgen05).
+//
+// A tile is 128 channels (the accumulator's lanes) x NTOK tokens (its columns); K may be
+// shared by a cluster of up to 8 CTAs. Weights arrive packed by TMA, eight warps widen
+// them to whole numbers in fp16 or bf16 (exact) in the swizzled layout that the matrix
+// instructions read, and one thread issues those. A scale belongs to a channel and a group, so the
+// sums of one group go to an accumulator of their own, and eight other warps add
+// scale * accumulator to fp32 registers while the next group runs: a lane is a
+// channel, so the scale is one register. Scaling the weights before the product would
+// round them once more (2^-9 for bf16).
+//
+// x comes by TMA where it can (16-bit, 16-byte aligned rows); otherwise, and for fp32, whose
+// three bf16 parts each take a product of their own, the widening warps bring it.
+#include <algorithm>
+
+#include "gemm_w4.cuh"
+#include "ptx_sm100.cuh"
+
+namespace nplk {
+namespace {
+
+constexpr int kChannels = 128, kBK = 128;          // of a tile; values of K a stage
+constexpr int kAtom = kChannels * 128;             // 128 rows x 64 values
+constexpr int kABytes = 2 * kAtom;
+constexpr int kRawBytes = kChannels * (kBK / 2);
+constexpr int kEpiWarps = 8, kWideWarps = 8;
+constexpr int kEpiFirst = 2, kWideFirst = kEpiFirst + kEpiWarps;
+constexpr int kThreads = 32 * (kWideFirst + kWideWarps);
+constexpr int kMostRings = 8;
+
+// P parts of x; kTma: x by TMA.
+template <int NTOK, int P>
+struct MmaTraits {
+  static constexpr int kXAtom = NTOK * 128;            // NTOK rows x 64 values
+  static constexpr int kXBytes = 2 * kXAtom * P;
+  static constexpr int kA = 2;                         // rings' lengths
+  static constexpr int kX = kXBytes > 40 * 1024 ? 2 : 3;
+  static constexpr int kRaw = (200 * 1024 - kA * kABytes - kX * kXBytes) / kRawBytes > kMostRings
+                                  ? kMostRings
+                                  : (200 * 1024 - kA * kABytes - kX * kXBytes) / kRawBytes;
+  static constexpr int kAcc = 512 / NTOK > 4 ? 4 : 512 / NTOK;
+  static constexpr int kTmemCols = kAcc * NTOK;
+  static constexpr int kRings = kA * kABytes + kX * kXBytes + kRaw * kRawBytes;
+  static constexpr int kBarriers = 2 * (kA + kX + kRaw + kAcc) + 1;
+  // at least what keeps other clusters' TMEM off this SM
+  static constexpr int kNeeded = 1024 + kRings + 8 * kBarriers + 64;
+  static constexpr int kSmem = kNeeded > 200 * 1024 ? kNeeded : 200 * 1024;
+  static_assert(kRaw >= 3, "packed weights in flight");
+  static_assert(NTOK * kChannels * 4 <= kRings, "partial sums over the rings");
+  static_assert(kSmem <= 232448, "shared memory budget");
+  static_assert(tmem_excludes_clusters(kSmem), "no other cluster's TMEM beside this one's");
+};
+
+struct MmaPlan {
+  int slices, n_tiles;
+  uint32_t stall_us;  // fault injection: 0 except on an armed launch
+};
+
+// A wait's outcome for the whole warp: TMEM loads and warp barriers are for whole warps.
+__device__ __forceinline__ bool all(bool done) { return __all_sync(0xffffffffu, done); }
+
+template <typename X>
+__device__ __forceinline__ uint32_t bits16(X v) {
+  return static_cast<uint32_t>(reinterpret_cast<const uint16_t &>(v));
+}
+
+template <typename X, int NTOK, int kGroup, bool kTma>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_w4_mma_kernel(const __grid_constant__ CUtensorMap map_w,
+                       const __grid_constant__ CUtensorMap map_x, const W4Args p,
+                       const MmaPlan plan) {
+  using F = typename W4Type<X>::Frag;
+  constexpr int P = W4Type<X>::kParts;
+  using Tr = MmaTraits<NTOK, P>;
+  constexpr int kPer = kBK / kGroup;  // groups a stage
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = align_smem_1024(smem_raw);
+  uint8_t *ring_a = smem, *ring_x = ring_a + Tr::kA * kABytes,
+          *ring_raw = ring_x + Tr::kX * Tr::kXBytes;
+  uint64_t *a_full = reinterpret_cast<uint64_t *>(smem + Tr::kRings);
+  uint64_t *a_empty = a_full + Tr::kA, *x_full = a_empty + Tr::kA, *x_empty = x_full + Tr::kX,
+           *raw_full = x_empty + Tr::kX, *raw_empty = raw_full + Tr::kRaw,
+           *acc_full = raw_empty + Tr::kRaw, *acc_empty = acc_full + Tr::kAcc,
+           *never = acc_empty + Tr::kAcc;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(never + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % plan.slices;
+  const int tile = static_cast<int>(blockIdx.x) / plan.slices;
+  const int n0 = tile % plan.n_tiles * kChannels, m0 = tile / plan.n_tiles * NTOK;
+  const int blocks = (p.K + kBK - 1) / kBK;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * blocks / plan.slices);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * blocks / plan.slices);
+  const int g_begin = kb0 * kPer, g_end = min(p.groups, kb1 * kPer);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Tr::kA; ++i) {
+      mbar_init(&a_full[i], kWideWarps);
+      mbar_init(&a_empty[i], 1);
+    }
+    for (int i = 0; i < Tr::kX; ++i) {
+      mbar_init(&x_full[i], kTma ? 1 : kWideWarps);
+      mbar_init(&x_empty[i], 1);
+    }
+    for (int i = 0; i < Tr::kRaw; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], kWideWarps);
+    }
+    for (int i = 0; i < Tr::kAcc; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], kEpiWarps);
+    }
+    mbar_init(never, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_w);
+    if (kTma) tma_prefetch_desc(&map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Tr::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  bool have = false;  // epilogue warps: the sums are whole
+  if (warp == 0) {
+    // ---------------- TMA: packed weights, and x ----------------
+    if (lane == 0) {
+      int r = 0, x = 0, xb = kb0;
+      uint32_t r_phase = 0, x_phase = 0, r_used = 0, x_used = 0, r_last = 0, x_last = 0;
+      const auto load_x = [&]() -> bool {
+        if (!mbar_wait(&x_empty[x], x_phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer))
+          return false;
+        mbar_arrive_expect_tx(&x_full[x], Tr::kXBytes);
+        uint8_t *to = ring_x + x * Tr::kXBytes;
+        tma_load_2d(&map_x, &x_full[x], to, xb * (kBK * 2), m0);
+        tma_load_2d(&map_x, &x_full[x], to + Tr::kXAtom, xb * (kBK * 2) + 128, m0);
+        x_used |= 1u << x;
+        x_last = (x_last & ~(1u << x)) | (x_phase << x);
+        ++xb;
+        if (++x == Tr::kX) {
+          x = 0;
+          x_phase ^= 1u;
+        }
+        return true;
+      };
+      bool go = true;
+      for (int kb = kb0; go && kb < kb1; ++kb) {
+        // weights run ahead of x, as far as their longer ring goes
+        go = mbar_wait(&raw_empty[r], r_phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+        if (!go) break;
+        mbar_arrive_expect_tx(&raw_full[r], kRawBytes);
+        tma_load_2d(&map_w, &raw_full[r], ring_raw + r * kRawBytes, kb * (kBK / 2), n0);
+        r_used |= 1u << r;
+        r_last = (r_last & ~(1u << r)) | (r_phase << r);
+        if (++r == Tr::kRaw) {
+          r = 0;
+          r_phase ^= 1u;
+        }
+        if (kTma && kb - kb0 >= Tr::kRaw - Tr::kX) go = load_x();
+      }
+      while (kTma && go && xb < kb1) go = load_x();
+      // the last copy into each slot lands before the CTA can exit
+      for (int i = 0; i < Tr::kRaw; ++i)
+        if ((r_used >> i) & 1u) mbar_drain(&raw_full[i], (r_last >> i) & 1u);
+      for (int i = 0; kTma && i < Tr::kX; ++i)
+        if ((x_used >> i) & 1u) mbar_drain(&x_full[i], (x_last >> i) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_f16(std::is_same<F, W4Bfloat>::value, kChannels, NTOK);
+      int a = 0, x = 0, acc = 0, group = g_begin;
+      uint32_t a_phase = 0, x_phase = 0, acc_phase = 0;
+      bool go = injected_stall(never, plan.stall_us, abort_flag, p.status);
+      for (int kb = kb0; go && kb < kb1; ++kb) {
+        go = mbar_wait(&a_full[a], a_phase, abort_flag, p.status, kStatusTimeoutMma) &&
+             mbar_wait(&x_full[x], x_phase, abort_flag, p.status, kStatusTimeoutMma);
+        if (!go) break;
+        const uint32_t sa = smem_u32(ring_a + a * kABytes), sx = smem_u32(ring_x + x * Tr::kXBytes);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (group >= g_end) break;
+          go = mbar_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status,
+                         kStatusTimeoutAccFree);
+          if (!go) break;
+          tc_fence_after_sync();
+          const uint32_t d = tmem_base + static_cast<uint32_t>(acc * NTOK);
+#pragma unroll
+          for (int kk = 0; kk < kGroup / 16; ++kk) {
+            const int k = i * kGroup + kk * 16;  // of the stage
+            const uint64_t da = umma_desc_sw128(sa + k / 64 * kAtom) + (k % 64) / 8;
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+              const uint64_t dx =
+                  umma_desc_sw128(sx + (2 * q + k / 64) * Tr::kXAtom) + (k % 64) / 8;
+              mma_f16_ss(d, da, dx, idesc, kk > 0 || q > 0 ? 1u : 0u);
+            }
+          }
+          mma_commit(&acc_full[acc]);
+          ++group;
+          if (++acc == Tr::kAcc) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+        }
+        if (!go) break;
+        if (kb + 1 < kb1) {  // the last stage's slots are not filled again
+          mma_commit(&a_empty[a]);
+          mma_commit(&x_empty[x]);
+        }
+        if (++a == Tr::kA) {
+          a = 0;
+          a_phase ^= 1u;
+        }
+        if (++x == Tr::kX) {
+          x = 0;
+          x_phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp < kWideFirst) {
+    // ---------------- groups' sums: scaled and added in registers ----------------
+    constexpr int kCols = NTOK / 2;  // tokens of a warp: two warps to a lane quadrant
+    const int quad = warp & 3, half = (warp - kEpiFirst) >> 2;
+    const int64_t n = static_cast<int64_t>(n0) + quad * 32 + lane;
+    const uint32_t row =
+        tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * kCols);
+    float2 sum[kCols / 2];
+#pragma unroll
+    for (int j = 0; j < kCols / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
+    const auto scale_at = [&](int g) {
+      return n < p.N && g < g_end ? load_scale(p.scale, p.scale_type, n * p.lds + g) : 0.0f;
+    };
+    float s_now = scale_at(g_begin), s_next = scale_at(g_begin + 1);
+    int acc = 0;
+    uint32_t phase = 0;
+    have = true;
+    for (int g = g_begin; g < g_end; ++g) {
+      const float s = s_now;
+      s_now = s_next;
+      s_next = scale_at(g + 2);
+      have = all(mbar_wait(&acc_full[acc], phase, abort_flag, p.status, kStatusTimeoutEpilogue));
+      if (!have) break;
+      tc_fence_after_sync();
+      const uint32_t from = row + static_cast<uint32_t>(acc * NTOK);
+      const auto add = [&](const uint32_t *v, int at, int count) {
+#pragma unroll
+        for (int j = 0; j < count; j += 2)
+          sum[(at + j) / 2] = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])),
+                                   both(s), sum[(at + j) / 2]);
+      };
+      const auto hand_back = [&] {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      };
+      // 16 columns at a time: with 32, the 64 sums of 128-token tiles spill
+#pragma unroll
+      for (int c = 0; c < kCols; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(from + static_cast<uint32_t>(c), v);
+        tmem_wait_ld16(v);
+        if (c + 16 == kCols) hand_back();
+        add(v, c, 16);
+      }
+      if (++acc == Tr::kAcc) {
+        acc = 0;
+        phase ^= 1u;
+      }
+    }
+    // [token][channel], over the rings, which all MMAs have read out by now
+    if (have) {
+      float *part = reinterpret_cast<float *>(smem) + half * kCols * kChannels + quad * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < kCols; j += 2) {
+        part[j * kChannels] = sum[j / 2].x;
+        part[(j + 1) * kChannels] = sum[j / 2].y;
+      }
+    }
+    __syncwarp();
+    if (plan.slices == 1)
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");  // these warps
+  } else {
+    // ---------------- widening ----------------
+    const int tid = static_cast<int>(threadIdx.x) - kWideFirst * 32;
+    const int row = tid & 127, half = tid >> 7;  // a channel's 64 values: one atom's row
+    const int64_t n = static_cast<int64_t>(n0) + row;
+    constexpr int kHalfGroups = kGroup >= 64 ? 1 : 2;  // groups of a half
+    const auto zero_at = [&](int kb, int i) {
+      const int g = kb * kPer + half * 64 / kGroup + i;
+      return p.zero && n < p.N && kb < kb1 && g < p.groups ? __ldg(p.zero + n * p.ldz + g) & 15 : 8;
+    };
+    int z_next[kHalfGroups];
+#pragma unroll
+    for (int i = 0; i < kHalfGroups; ++i) z_next[i] = zero_at(kb0, i);
+    int a = 0, r = 0, x = 0;
+    uint32_t a_phase = 0, r_phase = 0, x_phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      int z[kHalfGroups];
+#pragma unroll
+      for (int i = 0; i < kHalfGroups; ++i) {
+        z[i] = z_next[i];
+        z_next[i] = zero_at(kb + 1, i);
+      }
+      if (!all(mbar_wait(&raw_full[r], r_phase, abort_flag, p.status, kStatusTimeoutStage))) break;
+      const uint8_t *from = ring_raw + r * kRawBytes + row * 64;
+      const int sw = (row >> 1) & 3;
+      const uint4 lo = *reinterpret_cast<const uint4 *>(from + ((2 * half ^ sw) << 4));
+      const uint4 hi = *reinterpret_cast<const uint4 *>(from + (((2 * half + 1) ^ sw) << 4));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[r]);
+      if (++r == Tr::kRaw) {
+        r = 0;
+        r_phase ^= 1u;
+      }
+      if (!all(mbar_wait(&a_empty[a], a_phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+        break;
+      uint8_t *to = ring_a + a * kABytes + half * kAtom;
+      const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        uint32_t v[4];
+        w4_widen<F>(words[w], w4_offset<F>(z[kHalfGroups == 2 ? w / 4 : 0]), v);
+        // pairs (0, 4), (1, 5), ... to (0, 1), (2, 3), ...
+        *reinterpret_cast<uint4 *>(to + sw128_offset(static_cast<uint32_t>(row), w)) =
+            make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                       __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[a]);
+      if (++a == Tr::kA) {
+        a = 0;
+        a_phase ^= 1u;
+      }
+      if constexpr (!kTma) {
+        if (!all(mbar_wait(&x_empty[x], x_phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+          break;
+        uint8_t *xs = ring_x + x * Tr::kXBytes;
+        const X *src = static_cast<const X *>(p.x);
+        // pieces of eight values: 16 to a token's row of the stage
+        for (int i = tid; i < NTOK * 16; i += kWideWarps * 32) {
+          const int token = i >> 4, piece = i & 15, k = kb * kBK + piece * 8;
+          uint32_t h[P][8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool in = m0 + token < p.M && k + j < p.K;
+            const int64_t at = static_cast<int64_t>(m0 + token) * p.ldx + k + j;
+            if constexpr (P == 3) {
+              uint32_t parts[3];
+              w4_split3(in ? src[at] : 0.0f, parts);
+#pragma unroll
+              for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
+            } else {
+              h[0][j] = in ? bits16(src[at]) : 0u;
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < P; ++q)
+            *reinterpret_cast<uint4 *>(xs + (2 * q + (piece >> 3)) * Tr::kXAtom +
+                                       sw128_offset(static_cast<uint32_t>(token), piece & 7)) =
+                make_uint4(h[q][0] | h[q][1] << 16, h[q][2] | h[q][3] << 16,
+                           h[q][4] | h[q][5] << 16, h[q][6] | h[q][7] << 16);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&x_full[x]);
+        if (++x == Tr::kX) {
+          x = 0;
+          x_phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  if (plan.slices > 1) cluster_sync();  // every CTA's sums are in its shared memory
+  if (warp >= kEpiFirst && warp < kWideFirst && have) {
+    // this CTA's share of the cluster's tokens: a token per warp at a time, four channels a lane
+    const int each = NTOK / plan.slices;
+    const int64_t n = static_cast<int64_t>(n0) + 4 * lane;
+    float bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[j] = p.bias && n + j < p.N ? p.bias[n + j] : 0.0f;
+    const int size = p.c_type == NPLK_DTYPE_FP32 ? 4 : 2;
+    const bool whole = p.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(p.C) % (4 * size) == 0;
+    const int count = n < p.N ? static_cast<int>(p.N - n < 4 ? p.N - n : 4) : 0;
+    for (int i = warp - kEpiFirst; i < each; i += kEpiWarps) {
+      const int token = rank * each + i;
+      // (a load from another CTA that no store waits for could be under way when that CTA ends)
+      if (m0 + token >= p.M || count == 0) break;
+      const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(token * kChannels + 4 * lane) * 4u;
+      float v[4] = {};
+      for (int s = 0; s < plan.slices; ++s) {
+        const uint4 q = plan.slices == 1
+                            ? *reinterpret_cast<const uint4 *>(smem + (token * kChannels + 4 * lane) * 4)
+                            : ld_shared_cluster_v4(mapa_shared(at, static_cast<uint32_t>(s)));
+        v[0] += __uint_as_float(q.x);
+        v[1] += __uint_as_float(q.y);
+        v[2] += __uint_as_float(q.z);
+        v[3] += __uint_as_float(q.w);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += bias[j];
+      w4_store<4>(p, static_cast<int64_t>(m0 + token) * p.ldc + n, v, count, whole);
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  if (plan.slices > 1) cluster_sync();  // no CTA leaves while another reads its shared memory
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, Tr::kTmemCols);
+  }
+}
+
+template <typename X, int NTOK, int kGroup, bool kTma>
+int launch(cudaStream_t s, const W4Args &p, MmaPlan plan) {
+  using Tr = MmaTraits<NTOK, W4Type<X>::kParts>;
+  CUtensorMap mw, mx = {};
+  int rc = encode_tmap_2d_u8_sw64(&mw, p.q, ceil_div(p.K, 2), p.N, p.ldq, kChannels);
+  if (!rc && kTma) rc = encode_tmap_2d_u8_sw128(&mx, p.x, 2 * static_cast<int64_t>(p.K), p.M, 2 * p.ldx, NTOK);
+  if (rc) return rc;
+  auto *fn = gemm_w4_mma_kernel<X, NTOK, kGroup, kTma>;
+  rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), Tr::kSmem);
+  if (rc) return rc;
+  plan.n_tiles = static_cast<int>(ceil_div(p.N, kChannels));
+  const int64_t ctas = static_cast<int64_t>(plan.n_tiles) * ceil_div(p.M, NTOK) * plan.slices;
+  if (ctas >= (int64_t(1) << 31)) return kErrUnsupported;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(plan.slices);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Tr::kSmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = plan.slices > 1 ? 2 : 1;
+  count_launch();
+  return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, mw, mx, p, plan));
+}
+
+template <typename X, int NTOK, bool kTma>
+int by_group(cudaStream_t s, const W4Args &p, const MmaPlan &plan) {
+  return p.group == 32   ? launch<X, NTOK, 32, kTma>(s, p, plan)
+         : p.group == 64 ? launch<X, NTOK, 64, kTma>(s, p, plan)
+                         : launch<X, NTOK, 128, kTma>(s, p, plan);
+}
+
+template <typename X>
+int by_tokens(cudaStream_t s, const W4Args &p, const MmaPlan &plan, int tokens, bool tma) {
+  if (!tma) return by_group<X, 64, false>(s, p, plan);
+  return tokens == 32   ? by_group<X, 32, true>(s, p, plan)
+         : tokens == 64 ? by_group<X, 64, true>(s, p, plan)
+                        : by_group<X, 128, true>(s, p, plan);
+}
+
+}  // namespace
+
+bool gemm_w4_mma_fits(const W4Args &p) {
+  return reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && (p.ldq % 16 == 0 || p.N == 1);
+}
+
+int gemm_w4_mma(cudaStream_t s, const W4Args &args) {
+  W4Args p = args;
+  if (p.N == 1) p.ldq = static_cast<int64_t>(align_up(ceil_div(p.K, 2), 16));  // a pitch that leads nowhere
+  const bool tma = p.x_type != NPLK_DTYPE_FP32 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 &&
+                   (p.ldx % 8 == 0 || p.M == 1);
+  if (p.M == 1) p.ldx = static_cast<int64_t>(align_up(p.K, 8));
+  const int tokens = !tma ? 64 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  const int64_t sms = sm_count(), blocks = ceil_div(p.K, kBK);
+  const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, tokens);
+  MmaPlan plan{1, 0, 0};
+  double least = 1e30;
+  for (int slices : {1, 2, 4, 8}) {
+    if (slices > blocks) break;
+    const double us = static_cast<double>(ceil_div(tiles * slices, sms)) *
+                          (2.5 + 0.28 * static_cast<double>(ceil_div(blocks, slices))) +
+                      (slices > 1 ? 0.5 : 0.0);
+    if (us < least) {
+      least = us;
+      plan.slices = slices;
+    }
+  }
+  if (!p.status) p.status = device_status_word();
+  if (!p.status) return kErrInternal;
+  plan.stall_us = take_armed_stall(NPLK_DEBUG_GEMM);
+  if (p.x_type == NPLK_DTYPE_FP32) return by_group<float, 64, false>(s, p, plan);
+  if (p.x_type == NPLK_DTYPE_FP16) return by_tokens<__half>(s, p, plan, tokens, tma);
+  return by_tokens<__nv_bfloat16>(s, p, plan, tokens, tma);
+}
+
+}  // namespace nplk

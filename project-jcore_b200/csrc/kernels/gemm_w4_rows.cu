@@ -1,0 +1,318 @@
+// 4-bit product for few tokens: the weights' bytes are what there is to do.
+//
+// A team of `slices` warps takes 16 channels at a time and shares K; a CTA holds `teams` of
+// them and goes round the channels with the other CTAs, one CTA to an SM. mma.sync m16n8k16
+// with the channels as its rows: lane (g, t) holds channels g and g + 8 and token g. Which
+// values of K a lane takes is free as long as weights and x agree, so a lane takes whole
+// 32-bit words of eight nibbles, which come apart as the pairs (0, 4), (1, 5) for one mma
+// and (2, 6), (3, 7) for the next; x lies in shared memory in that order. All lanes of one
+// mma must lie in one group: for groups of 32, 64, 128 lane t takes 1, 2, 4 words in a row of each
+// (its "run"), one load of shared memory each.
+//
+// Weights go by cp.async through a ring of each warp's own, across the ends of tiles: no
+// barrier but the team's own, once per 16 channels, to add its sums.
+#include <algorithm>
+
+#include "gemm_w4.cuh"
+#include "ptx_sm100.cuh"
+
+namespace nplk {
+namespace {
+
+constexpr int kStageK = 256;              // values of K a warp takes at a time
+constexpr int kStagePitch = kStageK / 2;  // bytes
+constexpr int kStageBytes = 16 * kStagePitch;
+constexpr int kDepth = 3;                 // stages in flight and at work
+constexpr int kMostWarps = 16;
+constexpr int kMostX = 96 * 1024;         // bytes of x in shared memory
+static_assert(kMostX + kMostWarps * (kDepth * kStageBytes + 2 * 2 * 512) <= 232448, "shared memory");
+
+struct RowsPlan {
+  int slices, teams;
+  int steps;    // stages of K a warp takes for 16 channels
+  int tiles;    // of 16 channels
+  int x_units;  // 16-byte units of x in shared memory
+};
+
+__device__ __forceinline__ void team_sync(int team, int threads) {
+  if (threads == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
+}
+
+template <int kWords>
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[kWords]) {
+  if constexpr (kWords == 4) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (kWords == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t *>(p);
+  }
+}
+
+template <typename X, int NT, bool kZeros, int kGroup>
+__global__ void __launch_bounds__(kMostWarps * 32)
+    gemm_w4_rows_kernel(const W4Args p, const RowsPlan plan) {
+  using F = typename W4Type<X>::Frag;
+  constexpr int P = W4Type<X>::kParts;
+  constexpr int kRun = kGroup / 32;                 // words of a lane in a group
+  constexpr int kGroups = kStageK / kGroup;         // groups of a stage
+  constexpr int kHeld = kGroups >= 2 ? kGroups / 2 : 1;  // of them, held by each half of the lanes
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warps = plan.slices * plan.teams;
+  uint4 *sx = reinterpret_cast<uint4 *>(smem);
+  uint8_t *ring = smem + static_cast<size_t>(plan.x_units) * 16;
+  float *red = reinterpret_cast<float *>(ring + warps * kDepth * kStageBytes);
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int slice = warp % plan.slices, team = warp / plan.slices;
+  const int k_begin = slice * plan.steps * kStageK;
+  const int steps = max(0, min(plan.steps, (p.K - k_begin + kStageK - 1) / kStageK));
+  const int row_bytes = (p.K + 1) >> 1;
+  const int stride = static_cast<int>(gridDim.x) * plan.teams;
+  const int tile0 = static_cast<int>(blockIdx.x) * plan.teams + team;
+  const int rounds = tile0 < plan.tiles ? (plan.tiles - tile0 + stride - 1) / stride : 0;
+  uint8_t *mine = ring + warp * (kDepth * kStageBytes);
+
+  // What is copied next: a stage of a tile, into a slot of the ring. Lane l copies the
+  // 16 bytes l % 8 of rows l / 8, + 4, + 8, + 12.
+  int c_round = steps ? 0 : rounds, c_step = 0, c_slot = 0;
+  const uint8_t *c_row[4];
+  const auto aim = [&](int round) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = static_cast<int64_t>(tile0 + round * stride) * 16 + j * 4 + (lane >> 3);
+      // rows past the last are read as the last, their results dropped
+      c_row[j] = p.q + (n < p.N ? n : p.N - 1) * p.ldq;
+    }
+  };
+  aim(0);
+  const auto issue = [&] {
+    if (c_round < rounds) {
+      const int at = (k_begin + c_step * kStageK) / 2 + (lane & 7) * 16;
+      const int valid = max(0, min(16, row_bytes - at));  // of the 16 bytes; zeros for the rest
+      uint8_t *to = mine + c_slot * kStageBytes;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = j * 4 + (lane >> 3);
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem_u32(
+                         to + r * kStagePitch + (((lane & 7) ^ (r * kRun & 7)) << 4))),
+                     "l"(c_row[j] + (valid ? at : 0)), "r"(valid)
+                     : "memory");
+      }
+      if (++c_step == steps) {
+        c_step = 0;
+        ++c_round;
+        aim(c_round);
+      }
+    }
+    c_slot = c_slot + 1 == kDepth ? 0 : c_slot + 1;
+    copy_async_commit();
+  };
+
+  // Scales (and zeros) of a stage, loaded one stage ahead: lane l holds those of channel
+  // l % 16, of the stage's first (l < 16) or second half.
+  float sc[kHeld], sc_next[kHeld];
+  int ze[kHeld], ze_next[kHeld];
+  const auto fetch = [&](int round, int step) {
+    const int64_t n = static_cast<int64_t>(tile0 + round * stride) * 16 + (lane & 15);
+    const int g0 = (k_begin + step * kStageK) / kGroup + (lane >> 4) * kHeld;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const bool in = round < rounds && n < p.N && g0 + j < p.groups;
+      sc_next[j] = in ? load_scale(p.scale, p.scale_type, n * p.lds + g0 + j) : 0.0f;
+      if (kZeros) ze_next[j] = in ? __ldg(p.zero + n * p.ldz + g0 + j) & 15 : 8;
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < kDepth - 1; ++i) issue();
+  if (steps) fetch(0, 0);
+
+  // x into shared memory: unit (block of 32 values b, word w of it) -> pairs of its eight
+  // values, zeros behind K. A lane's words of K in step r of a run: block (run's first)
+  // + its share; the unit of (chunk of 4 kRun words, r, t) lies at ((chunk kRun + r) M + m) 4 + t.
+  {
+    const X *x = static_cast<const X *>(p.x);
+    const int words = plan.x_units / (P * p.M);  // of eight values, padded to whole chunks
+    for (int u = threadIdx.x; u < words * p.M; u += blockDim.x) {
+      const int m = u / words, w = u - m * words, k = w * 8;
+      const int chunk = w / (4 * kRun), in = w % (4 * kRun), lane_t = in / kRun, r = in % kRun;
+      const X *from = x + m * p.ldx + k;
+      uint32_t h[P][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (P == 3) {
+          uint32_t parts[3];
+          w4_split3(k + j < p.K ? from[j] : 0.0f, parts);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
+        } else {
+          h[0][j] = k + j < p.K ? reinterpret_cast<const uint16_t *>(from)[j] : 0u;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+        sx[(((chunk * kRun + r) * P + q) * p.M + m) * 4 + lane_t] =
+            make_uint4(h[q][0] | h[q][4] << 16, h[q][1] | h[q][5] << 16, h[q][2] | h[q][6] << 16,
+                       h[q][3] | h[q][7] << 16);
+    }
+  }
+  __syncthreads();
+
+  int slot = 0;
+  const int chunks_all = (p.K + kGroup - 1) / kGroup;
+  for (int round = 0; round < rounds; ++round) {
+    const int tile = tile0 + round * stride;
+    const int64_t n_out = static_cast<int64_t>(tile) * 16 + (lane & 15);
+    const float bias = p.bias && n_out < p.N ? __ldg(p.bias + n_out) : 0.0f;
+    float acc[NT][4] = {};
+    for (int step = 0; step < steps; ++step) {
+      issue();
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) {
+        sc[j] = sc_next[j];
+        if (kZeros) ze[j] = ze_next[j];
+      }
+      if (step + 1 < steps) fetch(round, step + 1);
+      else fetch(round + 1, 0);
+      copy_async_wait<kDepth - 1>();
+      __syncwarp();
+      const uint8_t *st = mine + slot * kStageBytes + g * kStagePitch;
+      slot = slot + 1 == kDepth ? 0 : slot + 1;
+      const int chunk0 = (k_begin + step * kStageK) / kGroup;
+#pragma unroll
+      for (int c = 0; c < kGroups; ++c) {
+        if (chunk0 + c >= chunks_all) break;
+        const int from = c / kHeld * 16;
+        const float s0 = __shfl_sync(0xffffffffu, sc[c % kHeld], from + g);
+        const float s1 = __shfl_sync(0xffffffffu, sc[c % kHeld], from + g + 8);
+        uint32_t off0 = w4_offset<F>(8), off1 = off0;
+        if (kZeros) {
+          off0 = w4_offset<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g));
+          off1 = w4_offset<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g + 8));
+        }
+        uint32_t a[kRun], b[kRun];
+        // rows are swizzled by 16-byte pieces, so that the 8 rows of a load miss each other's banks
+        const int byte = c * (kGroup / 2) + t * (4 * kRun);
+        const int at = byte ^ (g * kRun & 7) << 4;
+        load_words<kRun>(st + at, a);
+        load_words<kRun>(st + 8 * kStagePitch + at, b);
+        float part[NT][4] = {};
+#pragma unroll
+        for (int r = 0; r < kRun; ++r) {
+          uint32_t w0[4], w1[4];
+          w4_widen<F>(a[r], off0, w0);
+          w4_widen<F>(b[r], off1, w1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (n * 8 + g < p.M)
+                v = sx[((((chunk0 + c) * kRun + r) * P + q) * p.M + n * 8 + g) * 4 + t];
+              F::mma(part[n], w0[0], w1[0], w0[1], w1[1], v.x, v.y);
+              F::mma(part[n], w0[2], w1[2], w0[3], w1[3], v.z, v.w);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
+          acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
+          acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
+          acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
+        }
+      }
+      __syncwarp();  // the stage has been read: the next issue writes over it
+    }
+    // the team's sums meet, [token][channel]; two buffers, so that one barrier a round
+    // keeps the next round's sums off this round's readers
+    float *buffer = red + (round & 1) * warps * (NT * 128);
+    float *to = buffer + warp * (NT * 128);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float *r = to + (8 * n + 2 * t) * 16 + g;
+      r[0] = acc[n][0];
+      r[16] = acc[n][1];
+      r[8] = acc[n][2];
+      r[24] = acc[n][3];
+    }
+    team_sync(team, plan.slices * 32);
+    const float *sums = buffer + team * plan.slices * (NT * 128);
+    for (int i = slice * 32 + lane; i < p.M * 16; i += plan.slices * 32) {
+      float v[1] = {0.0f};
+#pragma unroll 4
+      for (int s = 0; s < plan.slices; ++s) v[0] += sums[s * (NT * 128) + i];
+      v[0] += bias;
+      if (n_out < p.N) w4_store<1>(p, (i >> 4) * p.ldc + n_out, v, 1, false);
+    }
+  }
+  copy_async_wait<0>();
+}
+
+int parts_of(const W4Args &p) { return p.x_type == NPLK_DTYPE_FP32 ? 3 : 1; }
+int64_t x_units(const W4Args &p) {
+  return ceil_div(p.K, p.group) * (p.group / 8) * p.M * parts_of(p);
+}
+
+template <typename X, int NT>
+auto pick(const W4Args &p) {
+  switch (p.group) {
+    case 32:
+      return p.zero ? gemm_w4_rows_kernel<X, NT, true, 32> : gemm_w4_rows_kernel<X, NT, false, 32>;
+    case 64:
+      return p.zero ? gemm_w4_rows_kernel<X, NT, true, 64> : gemm_w4_rows_kernel<X, NT, false, 64>;
+    default:
+      return p.zero ? gemm_w4_rows_kernel<X, NT, true, 128>
+                    : gemm_w4_rows_kernel<X, NT, false, 128>;
+  }
+}
+
+}  // namespace
+
+bool gemm_w4_rows_fits(const W4Args &p) {
+  return p.M <= 16 && x_units(p) * 16 <= kMostX && reinterpret_cast<uintptr_t>(p.q) % 16 == 0 &&
+         (p.ldq % 16 == 0 || p.N == 1);
+}
+
+// Slices and teams: rounds of (stages of K, about 0.75 us each for 16 warps at the memory's
+// rate, and the sums' meeting and first loads).
+int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
+  RowsPlan plan{};
+  const int64_t sms = sm_count(), stages = ceil_div(p.K, kStageK);
+  plan.tiles = static_cast<int>(ceil_div(p.N, 16));
+  double least = 1e30;
+  for (int64_t want = 1; want <= std::min<int64_t>(stages, kMostWarps); ++want) {
+    const int64_t steps = ceil_div(stages, want), slices = ceil_div(stages, steps);
+    const int64_t teams = std::min<int64_t>(kMostWarps / slices, std::max<int64_t>(1, ceil_div(plan.tiles, sms)));
+    const int64_t rounds = ceil_div(plan.tiles, teams * sms);
+    const double us = static_cast<double>(rounds) *
+                      (0.046 * static_cast<double>(steps * slices * teams) + 0.3);
+    if (us < least) {
+      least = us;
+      plan.steps = static_cast<int>(steps);
+      plan.slices = static_cast<int>(slices);
+      plan.teams = static_cast<int>(teams);
+    }
+  }
+  plan.x_units = static_cast<int>(x_units(p));
+  const int warps = plan.slices * plan.teams, nt = p.M <= 8 ? 1 : 2;
+  const int smem = plan.x_units * 16 + warps * kDepth * kStageBytes + 2 * warps * nt * 512;
+  auto *fn = p.x_type == NPLK_DTYPE_FP32   ? (nt == 1 ? pick<float, 1>(p) : pick<float, 2>(p))
+             : p.x_type == NPLK_DTYPE_FP16 ? (nt == 1 ? pick<__half, 1>(p) : pick<__half, 2>(p))
+                                           : (nt == 1 ? pick<__nv_bfloat16, 1>(p)
+                                                      : pick<__nv_bfloat16, 2>(p));
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(fn), smem);
+  if (rc) return rc;
+  const int64_t grid = std::min<int64_t>(ceil_div(plan.tiles, plan.teams), sms);
+  return launch_programmatic(fn, dim3(static_cast<unsigned>(grid)),
+                             dim3(static_cast<unsigned>(warps * 32)), static_cast<size_t>(smem), s,
+                             p, plan);
+}
+
+}  // namespace nplk

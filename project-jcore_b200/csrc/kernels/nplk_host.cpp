@@ -196,6 +196,12 @@ int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, 
                    box_outer, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
+int encode_tmap_2d_u8_sw64(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                           uint64_t row_pitch_bytes, uint32_t box_outer) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, row_pitch_bytes, 64,
+                   box_outer, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
 int encode_tmap_2d_plain(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
                          uint64_t row_pitch_bytes, uint32_t box_inner, uint32_t box_outer,
                          int element_bytes) {

@@ -67,6 +67,10 @@ int encode_tmap_2d_f32_sw128_atom32(CUtensorMap *map, const void *base, uint64_t
 int encode_tmap_2d_u8_sw128(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
                             uint64_t row_pitch_bytes, uint32_t box_outer);
 
+// The same with boxes of 64 bytes x box_outer rows and the 64-byte swizzle.
+int encode_tmap_2d_u8_sw64(CUtensorMap *map, const void *base, uint64_t inner, uint64_t outer,
+                           uint64_t row_pitch_bytes, uint32_t box_outer);
+
 // 2-D map for tensor loads of box_inner x box_outer boxes of 2- or 4-byte
 // elements, unswizzled: dims {inner, outer} elements, row pitch in bytes, zero
 // fill out of bounds. box_inner * element_bytes a multiple of 16.
