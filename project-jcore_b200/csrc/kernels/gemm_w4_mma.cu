@@ -237,8 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     float2 sum[kCols / 2];
 #pragma unroll
     for (int j = 0; j < kCols / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
+    // channels past the last take its scales, their results are dropped
+    const int64_t scale_row = (n < p.N ? n : p.N - 1) * p.lds;
     const auto scale_at = [&](int g) {
-      return n < p.N && g < g_end ? load_scale(p.scale, p.scale_type, n * p.lds + g) : 0.0f;
+      return load_scale(p.scale, p.scale_type, scale_row + min(g, g_end - 1));
     };
     float s_now = scale_at(g_begin), s_next = scale_at(g_begin + 1);
     int acc = 0;
@@ -295,9 +297,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row = tid & 127, half = tid >> 7;  // a channel's 64 values: one atom's row
     const int64_t n = static_cast<int64_t>(n0) + row;
     constexpr int kHalfGroups = kGroup >= 64 ? 1 : 2;  // groups of a half
+    const int64_t zero_row = (n < p.N ? n : p.N - 1) * p.ldz;
     const auto zero_at = [&](int kb, int i) {
-      const int g = kb * kPer + half * 64 / kGroup + i;
-      return p.zero && n < p.N && kb < kb1 && g < p.groups ? __ldg(p.zero + n * p.ldz + g) & 15 : 8;
+      const int g = min(kb * kPer + half * 64 / kGroup + i, p.groups - 1);
+      return p.zero ? __ldg(p.zero + zero_row + g) & 15 : 8;
     };
     int z_next[kHalfGroups];
 #pragma unroll

@@ -12,6 +12,7 @@
 // Weights go by cp.async through a ring of each warp's own, across the ends of tiles: no
 // barrier but the team's own, once per 16 channels, to add its sums.
 #include <algorithm>
+#include <cmath>
 
 #include "gemm_w4.cuh"
 #include "ptx_sm100.cuh"
@@ -120,13 +121,16 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   float sc[kHeld], sc_next[kHeld];
   int ze[kHeld], ze_next[kHeld];
   const auto fetch = [&](int round, int step) {
-    const int64_t n = static_cast<int64_t>(tile0 + round * stride) * 16 + (lane & 15);
+    // past the last channel or group: the last one's, for results that are dropped and
+    // inputs that are 0
+    const int64_t at = static_cast<int64_t>(tile0 + round * stride) * 16 + (lane & 15);
+    const int64_t n = at < p.N ? at : p.N - 1;
     const int g0 = (k_begin + step * kStageK) / kGroup + (lane >> 4) * kHeld;
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-      const bool in = round < rounds && n < p.N && g0 + j < p.groups;
-      sc_next[j] = in ? load_scale(p.scale, p.scale_type, n * p.lds + g0 + j) : 0.0f;
-      if (kZeros) ze_next[j] = in ? __ldg(p.zero + n * p.ldz + g0 + j) & 15 : 8;
+      const int group = min(g0 + j, p.groups - 1);
+      sc_next[j] = load_scale(p.scale, p.scale_type, n * p.lds + group);
+      if (kZeros) ze_next[j] = __ldg(p.zero + n * p.ldz + group) & 15;
     }
   };
 
@@ -140,20 +144,31 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   {
     const X *x = static_cast<const X *>(p.x);
     const int words = plan.x_units / (P * p.M);  // of eight values, padded to whole chunks
+    const bool packs = reinterpret_cast<uintptr_t>(x) % 16 == 0 && p.ldx * sizeof(X) % 16 == 0;
+#pragma unroll 2
     for (int u = threadIdx.x; u < words * p.M; u += blockDim.x) {
       const int m = u / words, w = u - m * words, k = w * 8;
       const int chunk = w / (4 * kRun), in = w % (4 * kRun), lane_t = in / kRun, r = in % kRun;
       const X *from = x + m * p.ldx + k;
+      X v[8];
+      if (packs && k + 8 <= p.K) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 16 / sizeof(X))
+          *reinterpret_cast<Pack<X, 16 / sizeof(X)> *>(v + j) = load_pack<X, 16 / sizeof(X)>(from + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? from[j] : from_float<X>(0.0f);
+      }
       uint32_t h[P][8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (P == 3) {
           uint32_t parts[3];
-          w4_split3(k + j < p.K ? from[j] : 0.0f, parts);
+          w4_split3(v[j], parts);
 #pragma unroll
           for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
         } else {
-          h[0][j] = k + j < p.K ? reinterpret_cast<const uint16_t *>(from)[j] : 0u;
+          h[0][j] = reinterpret_cast<const uint16_t &>(v[j]);
         }
       }
 #pragma unroll
@@ -280,8 +295,9 @@ bool gemm_w4_rows_fits(const W4Args &p) {
          (p.ldq % 16 == 0 || p.N == 1);
 }
 
-// Slices and teams: rounds of (stages of K, about 0.75 us each for 16 warps at the memory's
-// rate, and the sums' meeting and first loads).
+// Slices and teams of least estimated time: rounds of (stages of K, 0.75 us each for 16
+// warps at the memory's rate and hardly less for few, and the sums' meeting), and x's way into
+// shared memory.
 int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
   RowsPlan plan{};
   const int64_t sms = sm_count(), stages = ceil_div(p.K, kStageK);
@@ -291,8 +307,12 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
     const int64_t steps = ceil_div(stages, want), slices = ceil_div(stages, steps);
     const int64_t teams = std::min<int64_t>(kMostWarps / slices, std::max<int64_t>(1, ceil_div(plan.tiles, sms)));
     const int64_t rounds = ceil_div(plan.tiles, teams * sms);
-    const double us = static_cast<double>(rounds) *
-                      (0.046 * static_cast<double>(steps * slices * teams) + 0.3);
+    const double warps = static_cast<double>(slices * teams);
+    const double us =
+        static_cast<double>(rounds) *
+            (std::max(0.046 * static_cast<double>(steps) * warps, 0.35 * static_cast<double>(steps)) +
+             0.3) +
+        0.6 * std::ceil(static_cast<double>(ceil_div(p.K, 8) * p.M) / (32.0 * warps));
     if (us < least) {
       least = us;
       plan.steps = static_cast<int>(steps);

@@ -14,11 +14,15 @@ namespace nplk {
 
 inline bool w4_group_ok(int64_t group) { return group == 32 || group == 64 || group == 128; }
 
-// A scale of type NPLK_DTYPE_* as fp32.
+// A scale of type NPLK_DTYPE_* as fp32. `at` has to lie in the array whatever the result is
+// used for: the headers' __ldg of __half and __nv_bfloat16 are asm statements without side
+// effects, which the compiler may run ahead of the condition they stand under (a scale
+// array at the end of its memory segment faulted so). The integer __ldg is no such asm.
 __device__ __forceinline__ float load_scale(const void *scales, int dtype, int64_t at) {
   if (dtype == NPLK_DTYPE_FP32) return __ldg(static_cast<const float *>(scales) + at);
-  if (dtype == NPLK_DTYPE_FP16) return __half2float(__ldg(static_cast<const __half *>(scales) + at));
-  return __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(scales) + at));
+  const unsigned short bits = __ldg(static_cast<const unsigned short *>(scales) + at);
+  if (dtype == NPLK_DTYPE_FP16) return __half2float(reinterpret_cast<const __half &>(bits));
+  return __uint_as_float(static_cast<uint32_t>(bits) << 16);
 }
 
 }  // namespace nplk

@@ -227,6 +227,29 @@ def test_any_address_and_the_surroundings_of_c(m):
         assert (around == 77.0).all()
 
 
+def at_the_end(t):
+    """A copy of t whose last byte is the last of a memory segment of its own."""
+    room = torch.empty(32 << 20, device="cuda", dtype=torch.uint8)
+    size = t.numel() * t.element_size()
+    return room[room.numel() - size:].view(t.dtype).view(t.shape).copy_(t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("m,n,k,group,dtype", [(1, 300, 2048, 32, "bf16"), (9, 48, 640, 64, "fp16"),
+                                               (2, 33, 96, 32, "fp32"), (40, 130, 608, 32, "bf16"),
+                                               (70, 100, 256, 128, "fp32")])
+def test_nothing_behind_the_operands_is_read(m, n, k, group, dtype, zeros):
+    lib = S.gpu_lib()
+    x, q, sc, z, b = whole_operands(m, n, k, group, dtype, TYPES[dtype][0], zeros)
+    want = product(lib, x, q, sc, z, group, n, k, b)
+    x, q, sc, b = (at_the_end(t) for t in (x, q, sc, b))
+    z = at_the_end(z) if zeros else None
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    assert torch.equal(product(lib, x, q, sc, z, group, n, k, b), want)
+
+
 def random_operands(m, n, k, group, dtype, zeros, seed=0):
     g = gen(seed + m + n + k)
     x = (torch.randn(m, k, generator=g, device="cuda") * 3).to(TYPES[dtype][0])
