@@ -30,39 +30,72 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p);
 bool gemm_w4_mma_fits(const W4Args &p);
 int gemm_w4_mma(cudaStream_t s, const W4Args &p);
 
-// fp16 and bf16. Two nibbles in the low bits of a pair of 16-bit values become the
-// numbers 1024 + n (fp16) or 128 + n (bf16) by setting the exponent; subtracting
-// 1024 + zero or 128 + zero is then exact.
+// (a & b) | c, one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// Nibbles as fp16 or bf16 pairs, less their zero, exactly, without a shift for each:
+// a nibble in bits 0-3 of 16 ("low") or in bits 4-7 ("high") is masked where it is, an
+// exponent set beside it, and one fused multiply-add brings it to its value.
+//   fp16: low 1024 + n, times 1; high 1024 + 16 n, times 1/16.
+//   bf16 has 7 bits of significand: low 128 + n, times 1/4; high without an exponent is
+//   the number 16 n 2^-133 (bit 7 is the lowest exponent bit, and exponents 0 and 1 have the
+//   same step), times 2^127. So bf16 weights are quarters, kUnit the factor left for the end.
+// Masks, shifts and permutations issue every second cycle; a shift and a subtraction for each pair
+// took 14 of those cycles a word against 10, 16 for adjacent pairs.
 struct W4Half {
-  static constexpr uint32_t kBias = 0x64006400u;
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r =
-        __hsub2(reinterpret_cast<const __half2 &>(a), reinterpret_cast<const __half2 &>(b));
-    return reinterpret_cast<const uint32_t &>(r);
+  static constexpr float kUnit = 1.0f;
+  static constexpr uint32_t kLowBias = 0x6400u, kHighBias = 0x6400u;
+  static constexpr uint32_t kLowScale = 0x3c00u, kHighScale = 0x2c00u;  // 1, 1/16
+  static __device__ __forceinline__ uint32_t low_offset(int z) {  // -(1024 + z)
+    return 0xe400u + static_cast<uint32_t>(z);
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+  static __device__ __forceinline__ uint32_t high_offset(int z) {  // -(64 + z)
+    return 0xd400u + static_cast<uint32_t>(z << 4);
+  }
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const float (&c)[4], uint32_t a0,
+                                             uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
+          "f"(c[3]));
   }
 };
 struct W4Bfloat {
-  static constexpr uint32_t kBias = 0x43004300u;
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a),
-                                     reinterpret_cast<const __nv_bfloat162 &>(b));
-    return reinterpret_cast<const uint32_t &>(r);
+  static constexpr float kUnit = 4.0f;
+  static constexpr uint32_t kLowBias = 0x4300u, kHighBias = 0u;
+  static constexpr uint32_t kLowScale = 0x3e80u, kHighScale = 0x7f00u;  // 1/4, 2^127
+  static __device__ __forceinline__ uint32_t low_offset(int z) {  // -(32 + z / 4)
+    return 0xc200u + static_cast<uint32_t>(z);
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+  static __device__ __forceinline__ uint32_t high_offset(int z) {  // -z / 4
+    return __float_as_uint(-0.25f * static_cast<float>(z)) >> 16;
+  }
+  static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const float (&c)[4], uint32_t a0,
+                                             uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
+          "f"(c[3]));
   }
 };
 
@@ -83,18 +116,45 @@ struct W4Type<float> {
   static constexpr int kParts = 3;
 };
 
-// 1024 + zero (128 + zero) in both halves.
+__device__ __forceinline__ constexpr uint32_t twice(uint32_t half) { return half * 0x00010001u; }
+
+// What the fused multiply-adds add, for one zero: to both halves of low and high pairs.
+struct W4Offsets {
+  uint32_t low, high;
+};
 template <typename F>
-__device__ __forceinline__ uint32_t w4_offset(int zero) {
-  return F::kBias + static_cast<uint32_t>(zero) * 0x00010001u;
+__device__ __forceinline__ W4Offsets w4_offsets(int zero) {
+  return {twice(F::low_offset(zero)), twice(F::high_offset(zero))};
 }
 
 // Eight weights less their zero as four pairs (0, 4), (1, 5), (2, 6), (3, 7).
 template <typename F>
-__device__ __forceinline__ void w4_widen(uint32_t word, uint32_t offset, uint32_t (&pair)[4]) {
+__device__ __forceinline__ void w4_widen(uint32_t word, const W4Offsets &off, uint32_t (&pair)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint32_t w = i ? word >> 8 : word;
+    pair[i] = F::fma(and_or(w, 0x000f000fu, twice(F::kLowBias)), twice(F::kLowScale), off.low);
+    pair[i + 1] =
+        F::fma(and_or(w, 0x00f000f0u, twice(F::kHighBias)), twice(F::kHighScale), off.high);
+  }
+}
+
+// The same as adjacent pairs (0, 1), (2, 3), (4, 5), (6, 7): byte i to both halves, its low
+// nibble taken from the low half, its high one from the high half. `off`: low_offset in
+// the low half, high_offset in the high one.
+template <typename F>
+__device__ __forceinline__ uint32_t w4_adjacent_offset(int zero) {
+  return F::low_offset(zero) | F::high_offset(zero) << 16;
+}
+template <typename F>
+__device__ __forceinline__ uint4 w4_widen_adjacent(uint32_t word, uint32_t off) {
+  uint32_t pair[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    pair[i] = F::sub((word >> (4 * i) & 0x000f000fu) | F::kBias, offset);
+    pair[i] = F::fma(and_or(__byte_perm(word, 0u, 0x4040u + static_cast<uint32_t>(i) * 0x0101u),
+                            0x00f0000fu, F::kLowBias | F::kHighBias << 16),
+                     F::kLowScale | F::kHighScale << 16, off);
+  return make_uint4(pair[0], pair[1], pair[2], pair[3]);
 }
 
 // fp32 as three bf16 parts by truncation: 8 bits of the significand each, so the last

@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float *part = reinterpret_cast<float *>(smem) + half * kCols * kChannels + quad * 32 + lane;
 #pragma unroll
       for (int j = 0; j < kCols; j += 2) {
-        part[j * kChannels] = sum[j / 2].x;
-        part[(j + 1) * kChannels] = sum[j / 2].y;
+        part[j * kChannels] = sum[j / 2].x * F::kUnit;
+        part[(j + 1) * kChannels] = sum[j / 2].y * F::kUnit;
       }
     }
     __syncwarp();
@@ -308,10 +308,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int a = 0, r = 0, x = 0;
     uint32_t a_phase = 0, r_phase = 0, x_phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      int z[kHalfGroups];
+      uint32_t off[kHalfGroups];
 #pragma unroll
       for (int i = 0; i < kHalfGroups; ++i) {
-        z[i] = z_next[i];
+        off[i] = w4_adjacent_offset<F>(z_next[i]);
         z_next[i] = zero_at(kb + 1, i);
       }
       if (!all(mbar_wait(&raw_full[r], r_phase, abort_flag, p.status, kStatusTimeoutStage))) break;
@@ -330,14 +330,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t *to = ring_a + a * kABytes + half * kAtom;
       const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        uint32_t v[4];
-        w4_widen<F>(words[w], w4_offset<F>(z[kHalfGroups == 2 ? w / 4 : 0]), v);
-        // pairs (0, 4), (1, 5), ... to (0, 1), (2, 3), ...
+      for (int w = 0; w < 8; ++w)
         *reinterpret_cast<uint4 *>(to + sw128_offset(static_cast<uint32_t>(row), w)) =
-            make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
-                       __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
-      }
+            w4_widen_adjacent<F>(words[w], off[kHalfGroups == 2 ? w / 4 : 0]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&a_full[a]);

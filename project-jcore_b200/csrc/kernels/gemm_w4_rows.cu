@@ -33,6 +33,7 @@ struct RowsPlan {
   int steps;    // stages of K a warp takes for 16 channels
   int tiles;    // of 16 channels
   int x_units;  // 16-byte units of x in shared memory
+  int x_bytes;  // their room, whole 128 bytes: the ring behind it is swizzled by address
 };
 
 __device__ __forceinline__ void team_sync(int team, int threads) {
@@ -61,10 +62,10 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   constexpr int kRun = kGroup / 32;                 // words of a lane in a group
   constexpr int kGroups = kStageK / kGroup;         // groups of a stage
   constexpr int kHeld = kGroups >= 2 ? kGroups / 2 : 1;  // of them, held by each half of the lanes
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   const int warps = plan.slices * plan.teams;
   uint4 *sx = reinterpret_cast<uint4 *>(smem);
-  uint8_t *ring = smem + static_cast<size_t>(plan.x_units) * 16;
+  uint8_t *ring = smem + plan.x_bytes;
   float *red = reinterpret_cast<float *>(ring + warps * kDepth * kStageBytes);
   griddep_wait();
   griddep_launch_dependents();
@@ -81,13 +82,16 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   uint8_t *mine = ring + warp * (kDepth * kStageBytes);
 
   // What is copied next: a stage of a tile, into a slot of the ring. Lane l copies the
-  // 16 bytes l % 8 of rows l / 8, + 4, + 8, + 12.
+  // 16 bytes l % 8 of rows l / 8, + 4, + 8, + 12; those are swizzled within their row.
+  const int piece = lane & 7, c_r = lane >> 3;
+  const uint32_t c_to = smem_u32(mine + c_r * kStagePitch + ((piece ^ (c_r * kRun & 7)) << 4));
+  const int byte0 = k_begin / 2 + piece * 16;
   int c_round = steps ? 0 : rounds, c_step = 0, c_slot = 0;
   const uint8_t *c_row[4];
   const auto aim = [&](int round) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t n = static_cast<int64_t>(tile0 + round * stride) * 16 + j * 4 + (lane >> 3);
+      const int64_t n = static_cast<int64_t>(tile0 + round * stride) * 16 + j * 4 + c_r;
       // rows past the last are read as the last, their results dropped
       c_row[j] = p.q + (n < p.N ? n : p.N - 1) * p.ldq;
     }
@@ -95,17 +99,17 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   aim(0);
   const auto issue = [&] {
     if (c_round < rounds) {
-      const int at = (k_begin + c_step * kStageK) / 2 + (lane & 7) * 16;
+      const int at = byte0 + c_step * (kStageK / 2);
       const int valid = max(0, min(16, row_bytes - at));  // of the 16 bytes; zeros for the rest
-      uint8_t *to = mine + c_slot * kStageBytes;
+      const int from = valid ? at : 0;
+      const uint32_t to = c_to + static_cast<uint32_t>(c_slot * kStageBytes);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = j * 4 + (lane >> 3);
-        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem_u32(
-                         to + r * kStagePitch + (((lane & 7) ^ (r * kRun & 7)) << 4))),
-                     "l"(c_row[j] + (valid ? at : 0)), "r"(valid)
+      for (int j = 0; j < 4; ++j)
+        // (rows 4 apart differ in their swizzle where a row's step of it is 1)
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(
+                         (kRun == 1 && (j & 1) ? to ^ 64u : to) + j * 4 * kStagePitch),
+                     "l"(c_row[j] + from), "r"(valid)
                      : "memory");
-      }
       if (++c_step == steps) {
         c_step = 0;
         ++c_round;
@@ -120,23 +124,30 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   // l % 16, of the stage's first (l < 16) or second half.
   float sc[kHeld], sc_next[kHeld];
   int ze[kHeld], ze_next[kHeld];
-  const auto fetch = [&](int round, int step) {
+  int64_t s_row = 0, z_row = 0;
+  const auto aim_scales = [&](int round) {
     // past the last channel or group: the last one's, for results that are dropped and
     // inputs that are 0
     const int64_t at = static_cast<int64_t>(tile0 + round * stride) * 16 + (lane & 15);
     const int64_t n = at < p.N ? at : p.N - 1;
-    const int g0 = (k_begin + step * kStageK) / kGroup + (lane >> 4) * kHeld;
+    s_row = n * p.lds;
+    if (kZeros) z_row = n * p.ldz;
+  };
+  const int held0 = k_begin / kGroup + (lane >> 4) * kHeld;
+  const auto fetch = [&](int step) {
+    const int g0 = held0 + step * kGroups;
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
       const int group = min(g0 + j, p.groups - 1);
-      sc_next[j] = load_scale(p.scale, p.scale_type, n * p.lds + group);
-      if (kZeros) ze_next[j] = __ldg(p.zero + n * p.ldz + group) & 15;
+      sc_next[j] = load_scale(p.scale, p.scale_type, s_row + group);
+      if (kZeros) ze_next[j] = __ldg(p.zero + z_row + group) & 15;
     }
   };
 
 #pragma unroll
   for (int i = 0; i < kDepth - 1; ++i) issue();
-  if (steps) fetch(0, 0);
+  aim_scales(0);
+  fetch(0);
 
   // x into shared memory: unit (block of 32 values b, word w of it) -> pairs of its eight
   // values, zeros behind K. A lane's words of K in step r of a run: block (run's first)
@@ -181,6 +192,11 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   __syncthreads();
 
   int slot = 0;
+  const int swizzle = (g * kRun & 7) << 4;
+  const int x_part = p.M * 4, x_chunk = kRun * P * x_part;
+  int x_at[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) x_at[n] = min(n * 8 + g, p.M - 1) * 4 + t;
   const int chunks_all = (p.K + kGroup - 1) / kGroup;
   for (int round = 0; round < rounds; ++round) {
     const int tile = tile0 + round * stride;
@@ -194,8 +210,12 @@ __global__ void __launch_bounds__(kMostWarps * 32)
         sc[j] = sc_next[j];
         if (kZeros) ze[j] = ze_next[j];
       }
-      if (step + 1 < steps) fetch(round, step + 1);
-      else fetch(round + 1, 0);
+      if (step + 1 < steps) {
+        fetch(step + 1);
+      } else {
+        aim_scales(round + 1);
+        fetch(0);
+      }
       copy_async_wait<kDepth - 1>();
       __syncwarp();
       const uint8_t *st = mine + slot * kStageBytes + g * kStagePitch;
@@ -207,18 +227,18 @@ __global__ void __launch_bounds__(kMostWarps * 32)
         const int from = c / kHeld * 16;
         const float s0 = __shfl_sync(0xffffffffu, sc[c % kHeld], from + g);
         const float s1 = __shfl_sync(0xffffffffu, sc[c % kHeld], from + g + 8);
-        uint32_t off0 = w4_offset<F>(8), off1 = off0;
+        W4Offsets off0 = w4_offsets<F>(8), off1 = off0;
         if (kZeros) {
-          off0 = w4_offset<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g));
-          off1 = w4_offset<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g + 8));
+          off0 = w4_offsets<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g));
+          off1 = w4_offsets<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g + 8));
         }
         uint32_t a[kRun], b[kRun];
         // rows are swizzled by 16-byte pieces, so that the 8 rows of a load miss each other's banks
-        const int byte = c * (kGroup / 2) + t * (4 * kRun);
-        const int at = byte ^ (g * kRun & 7) << 4;
+        const int at = (c * (kGroup / 2) + t * (4 * kRun)) ^ swizzle;
         load_words<kRun>(st + at, a);
         load_words<kRun>(st + 8 * kStagePitch + at, b);
-        float part[NT][4] = {};
+        const uint4 *xs = sx + (chunk0 + c) * x_chunk;
+        float part[NT][4];
 #pragma unroll
         for (int r = 0; r < kRun; ++r) {
           uint32_t w0[4], w1[4];
@@ -228,11 +248,15 @@ __global__ void __launch_bounds__(kMostWarps * 32)
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int q = 0; q < P; ++q) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (n * 8 + g < p.M)
-                v = sx[((((chunk0 + c) * kRun + r) * P + q) * p.M + n * 8 + g) * 4 + t];
-              F::mma(part[n], w0[0], w1[0], w0[1], w1[1], v.x, v.y);
-              F::mma(part[n], w0[2], w1[2], w0[3], w1[3], v.z, v.w);
+              // tokens past the last are read as the last, their results dropped
+              const uint4 v = xs[(r * P + q) * x_part + x_at[n]];
+              if (r == 0 && q == 0) {
+                const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                F::mma(part[n], none, w0[0], w1[0], w0[1], w1[1], v.x, v.y);
+              } else {
+                F::mma(part[n], part[n], w0[0], w1[0], w0[1], w1[1], v.x, v.y);
+              }
+              F::mma(part[n], part[n], w0[2], w1[2], w0[3], w1[3], v.z, v.w);
             }
         }
 #pragma unroll
@@ -263,7 +287,7 @@ __global__ void __launch_bounds__(kMostWarps * 32)
       float v[1] = {0.0f};
 #pragma unroll 4
       for (int s = 0; s < plan.slices; ++s) v[0] += sums[s * (NT * 128) + i];
-      v[0] += bias;
+      v[0] = fmaf(v[0], F::kUnit, bias);
       if (n_out < p.N) w4_store<1>(p, (i >> 4) * p.ldc + n_out, v, 1, false);
     }
   }
@@ -321,8 +345,9 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
     }
   }
   plan.x_units = static_cast<int>(x_units(p));
+  plan.x_bytes = static_cast<int>(align_up(static_cast<size_t>(plan.x_units) * 16, 128));
   const int warps = plan.slices * plan.teams, nt = p.M <= 8 ? 1 : 2;
-  const int smem = plan.x_units * 16 + warps * kDepth * kStageBytes + 2 * warps * nt * 512;
+  const int smem = plan.x_bytes + warps * kDepth * kStageBytes + 2 * warps * nt * 512;
   auto *fn = p.x_type == NPLK_DTYPE_FP32   ? (nt == 1 ? pick<float, 1>(p) : pick<float, 2>(p))
              : p.x_type == NPLK_DTYPE_FP16 ? (nt == 1 ? pick<__half, 1>(p) : pick<__half, 2>(p))
                                            : (nt == 1 ? pick<__nv_bfloat16, 1>(p)
