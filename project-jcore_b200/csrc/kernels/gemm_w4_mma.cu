@@ -2,15 +2,15 @@
 //
 // A tile is 128 channels (the accumulator's lanes) x NTOK tokens (its columns); K may be
 // shared by a cluster of up to 8 CTAs. Weights arrive packed by TMA, eight warps widen
-// them to whole numbers in fp16 or bf16 (exact) in the swizzled layout that the matrix
-// instructions read, and one thread issues those. A scale belongs to a channel and a group, so the
+// them to whole numbers in fp16 or bf16 (exact), into TMEM, where the matrix
+// instructions take them from. A scale belongs to a channel and a group, so the
 // sums of one group go to an accumulator of their own, and eight other warps add
 // scale * accumulator to fp32 registers while the next group runs: a lane is a
 // channel, so the scale is one register. Scaling the weights before the product would
 // round them once more (2^-9 for bf16).
 //
 // x comes by TMA where it can (16-bit, 16-byte aligned rows); otherwise, and for fp32, whose
-// three bf16 parts each take a product of their own, the widening warps bring it.
+// three bf16 parts each take a product of their own, four more warps bring it.
 #include <algorithm>
 
 #include "gemm_w4.cuh"
@@ -19,33 +19,46 @@
 namespace nplk {
 namespace {
 
-constexpr int kChannels = 128, kBK = 128;          // of a tile; values of K a stage
-constexpr int kAtom = kChannels * 128;             // 128 rows x 64 values
-constexpr int kABytes = 2 * kAtom;
+constexpr int kChannels = 128, kBK = 128;  // of a tile; values of K a stage
 constexpr int kRawBytes = kChannels * (kBK / 2);
-constexpr int kEpiWarps = 8, kWideWarps = 8;
-constexpr int kEpiFirst = 2, kWideFirst = kEpiFirst + kEpiWarps;
-constexpr int kThreads = 32 * (kWideFirst + kWideWarps);
-constexpr int kMostRings = 8;
+constexpr int kACols = kBK / 2;            // TMEM columns of a stage's widened weights
+// Warpgroups: TMA and MMA issue; epilogue (two); widening (two, every second stage each);
+// x where it does not come by TMA.
+constexpr int kEpiFirst = 4, kEpiWarps = 8, kWideFirst = kEpiFirst + kEpiWarps, kWideWarps = 8,
+              kXFirst = kWideFirst + kWideWarps, kXWarps = 4;
 
-// P parts of x; kTma: x by TMA.
+// Threads, and registers a thread: at launch, and as the warpgroups share them.
+template <bool kTma>
+struct MmaThreads {
+  static constexpr int kThreads = 32 * (kXFirst + (kTma ? 0 : kXWarps));
+  static constexpr int kLaunch = kTma ? 96 : 80;
+  static constexpr int kIssue = 40, kEpi = kTma ? 128 : 96, kWide = kTma ? 88 : 72, kX = 96;
+  static_assert(kIssue * 128 + kEpi * 32 * kEpiWarps + kWide * 32 * kWideWarps +
+                        (kTma ? 0 : kX * 32 * kXWarps) <=
+                    kLaunch * kThreads,
+                "register shares");
+  static_assert(kLaunch * kThreads <= 65536 && (kLaunch + 8) * kThreads > 65536,
+                "what the launch bounds give a thread");
+};
+
+// P parts of x.
 template <int NTOK, int P>
 struct MmaTraits {
-  static constexpr int kXAtom = NTOK * 128;            // NTOK rows x 64 values
+  static constexpr int kXAtom = NTOK * 128;  // NTOK rows x 64 values
   static constexpr int kXBytes = 2 * kXAtom * P;
-  static constexpr int kA = 2;                         // rings' lengths
-  static constexpr int kX = kXBytes > 40 * 1024 ? 2 : 3;
-  static constexpr int kRaw = (200 * 1024 - kA * kABytes - kX * kXBytes) / kRawBytes > kMostRings
-                                  ? kMostRings
-                                  : (200 * 1024 - kA * kABytes - kX * kXBytes) / kRawBytes;
-  static constexpr int kAcc = 512 / NTOK > 4 ? 4 : 512 / NTOK;
-  static constexpr int kTmemCols = kAcc * NTOK;
-  static constexpr int kRings = kA * kABytes + kX * kXBytes + kRaw * kRawBytes;
-  static constexpr int kBarriers = 2 * (kA + kX + kRaw + kAcc) + 1;
+  static constexpr int kStages = 4;  // x in shared memory, weights in TMEM
+  static constexpr int kRaw = 208 * 1024 - kStages * kXBytes > 8 * kRawBytes
+                                  ? 8
+                                  : (208 * 1024 - kStages * kXBytes) / kRawBytes;
+  static constexpr int kAcc = NTOK == 128 ? 2 : 4;
+  static constexpr int kTmemCols = 512;
+  static constexpr int kRings = kStages * kXBytes + kRaw * kRawBytes;
+  static constexpr int kBarriers = 2 * (kStages + kRaw + kAcc) + 1;
   // at least what keeps other clusters' TMEM off this SM
   static constexpr int kNeeded = 1024 + kRings + 8 * kBarriers + 64;
   static constexpr int kSmem = kNeeded > 200 * 1024 ? kNeeded : 200 * 1024;
-  static_assert(kRaw >= 3, "packed weights in flight");
+  static_assert(kAcc * NTOK + kStages * kACols <= kTmemCols, "TMEM columns");
+  static_assert(kRaw >= 2, "packed weights in flight");
   static_assert(NTOK * kChannels * 4 <= kRings, "partial sums over the rings");
   static_assert(kSmem <= 232448, "shared memory budget");
   static_assert(tmem_excludes_clusters(kSmem), "no other cluster's TMEM beside this one's");
@@ -56,32 +69,38 @@ struct MmaPlan {
   uint32_t stall_us;  // fault injection: 0 except on an armed launch
 };
 
-// A wait's outcome for the whole warp: TMEM loads and warp barriers are for whole warps.
+// A wait's outcome for the whole warp: TMEM accesses and warp barriers are for whole warps.
 __device__ __forceinline__ bool all(bool done) { return __all_sync(0xffffffffu, done); }
 
-template <typename X>
-__device__ __forceinline__ uint32_t bits16(X v) {
-  return static_cast<uint32_t>(reinterpret_cast<const uint16_t &>(v));
-}
+// A slot of a ring and the phase of its barriers.
+struct Slot {
+  int at = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int count) {
+    if (++at == count) {
+      at = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 template <typename X, int NTOK, int kGroup, bool kTma>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     gemm_w4_mma_kernel(const __grid_constant__ CUtensorMap map_w,
                        const __grid_constant__ CUtensorMap map_x, const W4Args p,
                        const MmaPlan plan) {
   using F = typename W4Type<X>::Frag;
   constexpr int P = W4Type<X>::kParts;
   using Tr = MmaTraits<NTOK, P>;
+  using Th = MmaThreads<kTma>;
   constexpr int kPer = kBK / kGroup;  // groups a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align_smem_1024(smem_raw);
-  uint8_t *ring_a = smem, *ring_x = ring_a + Tr::kA * kABytes,
-          *ring_raw = ring_x + Tr::kX * Tr::kXBytes;
-  uint64_t *a_full = reinterpret_cast<uint64_t *>(smem + Tr::kRings);
-  uint64_t *a_empty = a_full + Tr::kA, *x_full = a_empty + Tr::kA, *x_empty = x_full + Tr::kX,
-           *raw_full = x_empty + Tr::kX, *raw_empty = raw_full + Tr::kRaw,
-           *acc_full = raw_empty + Tr::kRaw, *acc_empty = acc_full + Tr::kAcc,
-           *never = acc_empty + Tr::kAcc;
+  uint8_t *ring_x = smem, *ring_raw = ring_x + Tr::kStages * Tr::kXBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Tr::kRings);
+  uint64_t *empty = full + Tr::kStages, *raw_full = empty + Tr::kStages,
+           *raw_empty = raw_full + Tr::kRaw, *acc_full = raw_empty + Tr::kRaw,
+           *acc_empty = acc_full + Tr::kAcc, *never = acc_empty + Tr::kAcc;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(never + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -95,17 +114,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int g_begin = kb0 * kPer, g_end = min(p.groups, kb1 * kPer);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < Tr::kA; ++i) {
-      mbar_init(&a_full[i], kWideWarps);
-      mbar_init(&a_empty[i], 1);
-    }
-    for (int i = 0; i < Tr::kX; ++i) {
-      mbar_init(&x_full[i], kTma ? 1 : kWideWarps);
-      mbar_init(&x_empty[i], 1);
+    for (int i = 0; i < Tr::kStages; ++i) {
+      mbar_init(&full[i], kWideWarps / 2 + (kTma ? 1 : kXWarps));
+      mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < Tr::kRaw; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], kWideWarps);
+      mbar_init(&raw_empty[i], kWideWarps / 2);
     }
     for (int i = 0; i < Tr::kAcc; ++i) {
       mbar_init(&acc_full[i], 1);
@@ -124,112 +139,102 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = *tmem_slot, tmem_a = tmem_base + Tr::kAcc * NTOK;
   griddep_wait();
   griddep_launch_dependents();
 
   bool have = false;  // epilogue warps: the sums are whole
-  if (warp == 0) {
-    // ---------------- TMA: packed weights, and x ----------------
-    if (lane == 0) {
-      int r = 0, x = 0, xb = kb0;
-      uint32_t r_phase = 0, x_phase = 0, r_used = 0, x_used = 0, r_last = 0, x_last = 0;
+  if (warp < kEpiFirst) {
+    registers_down<Th::kIssue>();
+    if (warp == 0 && lane == 0) {
+      // ---------------- TMA: packed weights, and x ----------------
+      Slot r, x;
+      int xb = kb0;
+      uint32_t r_used = 0, x_used = 0, r_last = 0, x_last = 0;
       const auto load_x = [&]() -> bool {
-        if (!mbar_wait(&x_empty[x], x_phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer))
+        if (!mbar_wait(&empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer))
           return false;
-        mbar_arrive_expect_tx(&x_full[x], Tr::kXBytes);
-        uint8_t *to = ring_x + x * Tr::kXBytes;
-        tma_load_2d(&map_x, &x_full[x], to, xb * (kBK * 2), m0);
-        tma_load_2d(&map_x, &x_full[x], to + Tr::kXAtom, xb * (kBK * 2) + 128, m0);
-        x_used |= 1u << x;
-        x_last = (x_last & ~(1u << x)) | (x_phase << x);
+        mbar_arrive_expect_tx(&full[x.at], Tr::kXBytes);
+        uint8_t *to = ring_x + x.at * Tr::kXBytes;
+        tma_load_2d(&map_x, &full[x.at], to, xb * (kBK * 2), m0);
+        tma_load_2d(&map_x, &full[x.at], to + Tr::kXAtom, xb * (kBK * 2) + 128, m0);
+        x_used |= 1u << x.at;
+        x_last = (x_last & ~(1u << x.at)) | (x.phase << x.at);
         ++xb;
-        if (++x == Tr::kX) {
-          x = 0;
-          x_phase ^= 1u;
-        }
+        x.next(Tr::kStages);
         return true;
       };
       bool go = true;
       for (int kb = kb0; go && kb < kb1; ++kb) {
-        // weights run ahead of x, as far as their longer ring goes
-        go = mbar_wait(&raw_empty[r], r_phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+        go = mbar_wait(&raw_empty[r.at], r.phase ^ 1u, abort_flag, p.status,
+                       kStatusTimeoutProducer);
         if (!go) break;
-        mbar_arrive_expect_tx(&raw_full[r], kRawBytes);
-        tma_load_2d(&map_w, &raw_full[r], ring_raw + r * kRawBytes, kb * (kBK / 2), n0);
-        r_used |= 1u << r;
-        r_last = (r_last & ~(1u << r)) | (r_phase << r);
-        if (++r == Tr::kRaw) {
-          r = 0;
-          r_phase ^= 1u;
-        }
-        if (kTma && kb - kb0 >= Tr::kRaw - Tr::kX) go = load_x();
+        mbar_arrive_expect_tx(&raw_full[r.at], kRawBytes);
+        tma_load_2d(&map_w, &raw_full[r.at], ring_raw + r.at * kRawBytes, kb * (kBK / 2), n0);
+        r_used |= 1u << r.at;
+        r_last = (r_last & ~(1u << r.at)) | (r.phase << r.at);
+        r.next(Tr::kRaw);
+        // weights run ahead of x, as far as their longer ring goes
+        if (kTma && kb - kb0 >= Tr::kRaw - Tr::kStages) go = load_x();
       }
       while (kTma && go && xb < kb1) go = load_x();
       // the last copy into each slot lands before the CTA can exit
       for (int i = 0; i < Tr::kRaw; ++i)
         if ((r_used >> i) & 1u) mbar_drain(&raw_full[i], (r_last >> i) & 1u);
-      for (int i = 0; kTma && i < Tr::kX; ++i)
-        if ((x_used >> i) & 1u) mbar_drain(&x_full[i], (x_last >> i) & 1u);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+      for (int i = 0; kTma && i < Tr::kStages; ++i)
+        if ((x_used >> i) & 1u) mbar_drain(&full[i], (x_last >> i) & 1u);
+    } else if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      // the whole warp goes round, one lane issues: addresses and descriptors then stay in
+      // uniform registers (one lane alone took 75 cycles an instruction)
       const uint32_t idesc = umma_idesc_f16(std::is_same<F, W4Bfloat>::value, kChannels, NTOK);
-      int a = 0, x = 0, acc = 0, group = g_begin;
-      uint32_t a_phase = 0, x_phase = 0, acc_phase = 0;
-      bool go = injected_stall(never, plan.stall_us, abort_flag, p.status);
+      const uint64_t desc0 = umma_desc_sw128(smem_u32(ring_x));
+      Slot st, acc;
+      int group = g_begin;
+      bool go = all(injected_stall(never, plan.stall_us, abort_flag, p.status));
       for (int kb = kb0; go && kb < kb1; ++kb) {
-        go = mbar_wait(&a_full[a], a_phase, abort_flag, p.status, kStatusTimeoutMma) &&
-             mbar_wait(&x_full[x], x_phase, abort_flag, p.status, kStatusTimeoutMma);
+        go = all(mbar_wait(&full[st.at], st.phase, abort_flag, p.status, kStatusTimeoutMma));
         if (!go) break;
-        const uint32_t sa = smem_u32(ring_a + a * kABytes), sx = smem_u32(ring_x + x * Tr::kXBytes);
+        const uint64_t desc = desc0 + static_cast<uint64_t>(st.at * (Tr::kXBytes >> 4));
+        const uint32_t a = tmem_a + static_cast<uint32_t>(st.at * kACols);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           if (group >= g_end) break;
-          go = mbar_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status,
-                         kStatusTimeoutAccFree);
+          go = all(mbar_wait(&acc_empty[acc.at], acc.phase ^ 1u, abort_flag, p.status,
+                             kStatusTimeoutAccFree));
           if (!go) break;
           tc_fence_after_sync();
-          const uint32_t d = tmem_base + static_cast<uint32_t>(acc * NTOK);
+          const uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * NTOK);
+          if (elect_lane()) {
 #pragma unroll
-          for (int kk = 0; kk < kGroup / 16; ++kk) {
-            const int k = i * kGroup + kk * 16;  // of the stage
-            const uint64_t da = umma_desc_sw128(sa + k / 64 * kAtom) + (k % 64) / 8;
+            for (int kk = 0; kk < kGroup / 16; ++kk) {
+              const int k = i * kGroup + kk * 16;  // of the stage
 #pragma unroll
-            for (int q = 0; q < P; ++q) {
-              const uint64_t dx =
-                  umma_desc_sw128(sx + (2 * q + k / 64) * Tr::kXAtom) + (k % 64) / 8;
-              mma_f16_ss(d, da, dx, idesc, kk > 0 || q > 0 ? 1u : 0u);
+              for (int q = 0; q < P; ++q)
+                mma_f16_ts(d, a + k / 2,
+                           desc + static_cast<uint64_t>(((2 * q + k / 64) * Tr::kXAtom >> 4) +
+                                                        k % 64 / 8),
+                           idesc, kk > 0 || q > 0 ? 1u : 0u);
             }
+            mma_commit(&acc_full[acc.at]);
           }
-          mma_commit(&acc_full[acc]);
+          __syncwarp();
           ++group;
-          if (++acc == Tr::kAcc) {
-            acc = 0;
-            acc_phase ^= 1u;
-          }
+          acc.next(Tr::kAcc);
         }
         if (!go) break;
-        if (kb + 1 < kb1) {  // the last stage's slots are not filled again
-          mma_commit(&a_empty[a]);
-          mma_commit(&x_empty[x]);
-        }
-        if (++a == Tr::kA) {
-          a = 0;
-          a_phase ^= 1u;
-        }
-        if (++x == Tr::kX) {
-          x = 0;
-          x_phase ^= 1u;
-        }
+        // (the last stage's slot is not filled again)
+        if (kb + 1 < kb1 && elect_lane()) mma_commit(&empty[st.at]);
+        __syncwarp();
+        st.next(Tr::kStages);
       }
     }
     __syncwarp();
   } else if (warp < kWideFirst) {
     // ---------------- groups' sums: scaled and added in registers ----------------
+    registers_up<Th::kEpi>();
     constexpr int kCols = NTOK / 2;  // tokens of a warp: two warps to a lane quadrant
+    constexpr int kLoad = kCols < 32 ? kCols : 32;
     const int quad = warp & 3, half = (warp - kEpiFirst) >> 2;
     const int64_t n = static_cast<int64_t>(n0) + quad * 32 + lane;
     const uint32_t row =
@@ -243,41 +248,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       return load_scale(p.scale, p.scale_type, scale_row + min(g, g_end - 1));
     };
     float s_now = scale_at(g_begin), s_next = scale_at(g_begin + 1);
-    int acc = 0;
-    uint32_t phase = 0;
+    Slot acc;
     have = true;
     for (int g = g_begin; g < g_end; ++g) {
       const float s = s_now;
       s_now = s_next;
       s_next = scale_at(g + 2);
-      have = all(mbar_wait(&acc_full[acc], phase, abort_flag, p.status, kStatusTimeoutEpilogue));
+      have = all(mbar_wait(&acc_full[acc.at], acc.phase, abort_flag, p.status,
+                           kStatusTimeoutEpilogue));
       if (!have) break;
       tc_fence_after_sync();
-      const uint32_t from = row + static_cast<uint32_t>(acc * NTOK);
-      const auto add = [&](const uint32_t *v, int at, int count) {
+      const uint32_t from = row + static_cast<uint32_t>(acc.at * NTOK);
 #pragma unroll
-        for (int j = 0; j < count; j += 2)
-          sum[(at + j) / 2] = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])),
-                                   both(s), sum[(at + j) / 2]);
-      };
-      const auto hand_back = [&] {
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[acc]);
-      };
-      // 16 columns at a time: with 32, the 64 sums of 128-token tiles spill
+      for (int c = 0; c < kCols; c += kLoad) {
+        uint32_t v[kLoad];
+        if constexpr (kLoad == 16) {
+          tmem_ld16(from, v);
+          tmem_wait_ld16(v);
+        } else {
+          tmem_ld32(from + static_cast<uint32_t>(c), v);
+          tmem_wait_ld(v);
+        }
+        if (c + kLoad == kCols) {  // all read: the accumulator is free again
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[acc.at]);
+        }
 #pragma unroll
-      for (int c = 0; c < kCols; c += 16) {
-        uint32_t v[16];
-        tmem_ld16(from + static_cast<uint32_t>(c), v);
-        tmem_wait_ld16(v);
-        if (c + 16 == kCols) hand_back();
-        add(v, c, 16);
+        for (int j = 0; j < kLoad; j += 2)
+          sum[(c + j) / 2] = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])),
+                                  both(s), sum[(c + j) / 2]);
       }
-      if (++acc == Tr::kAcc) {
-        acc = 0;
-        phase ^= 1u;
-      }
+      acc.next(Tr::kAcc);
     }
     // [token][channel], over the rings, which all MMAs have read out by now
     if (have) {
@@ -291,75 +293,108 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     if (plan.slices == 1)
       asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");  // these warps
-  } else {
-    // ---------------- widening ----------------
-    const int tid = static_cast<int>(threadIdx.x) - kWideFirst * 32;
-    const int row = tid & 127, half = tid >> 7;  // a channel's 64 values: one atom's row
+  } else if (warp < kXFirst) {
+    // ---------------- widening: packed rows to TMEM, every second stage ----------------
+    registers_down<Th::kWide>();
+    const int quad = warp & 3, team = (warp - kWideFirst) >> 2;
+    const int row = quad * 32 + lane;  // a channel: its lane of TMEM
     const int64_t n = static_cast<int64_t>(n0) + row;
-    constexpr int kHalfGroups = kGroup >= 64 ? 1 : 2;  // groups of a half
+    const uint32_t t_row = tmem_a + (static_cast<uint32_t>(quad * 32) << 16);
     const int64_t zero_row = (n < p.N ? n : p.N - 1) * p.ldz;
     const auto zero_at = [&](int kb, int i) {
-      const int g = min(kb * kPer + half * 64 / kGroup + i, p.groups - 1);
-      return p.zero ? __ldg(p.zero + zero_row + g) & 15 : 8;
+      return p.zero ? __ldg(p.zero + zero_row + min(kb * kPer + i, p.groups - 1)) & 15 : 8;
     };
-    int z_next[kHalfGroups];
+    int z_next[kPer];
 #pragma unroll
-    for (int i = 0; i < kHalfGroups; ++i) z_next[i] = zero_at(kb0, i);
-    int a = 0, r = 0, x = 0;
-    uint32_t a_phase = 0, r_phase = 0, x_phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      uint32_t off[kHalfGroups];
+    for (int i = 0; i < kPer; ++i) z_next[i] = zero_at(kb0 + team, i);
+    Slot st, r;
+    if (team) {
+      st.next(Tr::kStages);
+      r.next(Tr::kRaw);
+    }
+    for (int kb = kb0 + team; kb < kb1; kb += 2) {
+      uint32_t off[kPer];
 #pragma unroll
-      for (int i = 0; i < kHalfGroups; ++i) {
+      for (int i = 0; i < kPer; ++i) {
         off[i] = w4_adjacent_offset<F>(z_next[i]);
-        z_next[i] = zero_at(kb + 1, i);
+        z_next[i] = zero_at(kb + 2, i);
       }
-      if (!all(mbar_wait(&raw_full[r], r_phase, abort_flag, p.status, kStatusTimeoutStage))) break;
-      const uint8_t *from = ring_raw + r * kRawBytes + row * 64;
-      const int sw = (row >> 1) & 3;
-      const uint4 lo = *reinterpret_cast<const uint4 *>(from + ((2 * half ^ sw) << 4));
-      const uint4 hi = *reinterpret_cast<const uint4 *>(from + (((2 * half + 1) ^ sw) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_empty[r]);
-      if (++r == Tr::kRaw) {
-        r = 0;
-        r_phase ^= 1u;
-      }
-      if (!all(mbar_wait(&a_empty[a], a_phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+      if (!all(mbar_wait(&raw_full[r.at], r.phase, abort_flag, p.status, kStatusTimeoutStage)))
         break;
-      uint8_t *to = ring_a + a * kABytes + half * kAtom;
-      const uint32_t words[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      const uint8_t *from = ring_raw + r.at * kRawBytes + row * 64;
+      const int sw = (row >> 1) & 3;
+      uint4 raw[4];
 #pragma unroll
-      for (int w = 0; w < 8; ++w)
-        *reinterpret_cast<uint4 *>(to + sw128_offset(static_cast<uint32_t>(row), w)) =
-            w4_widen_adjacent<F>(words[w], off[kHalfGroups == 2 ? w / 4 : 0]);
-      fence_proxy_async_smem();
+      for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4 *>(from + ((i ^ sw) << 4));
       __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[a]);
-      if (++a == Tr::kA) {
-        a = 0;
-        a_phase ^= 1u;
+      if (lane == 0) mbar_arrive(&raw_empty[r.at]);
+      if (!all(mbar_wait(&empty[st.at], st.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+        break;
+      tc_fence_after_sync();
+      const uint32_t to = t_row + static_cast<uint32_t>(st.at * kACols);
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        uint32_t v[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint4 &q = raw[i + j / 4];
+          const uint32_t word = j % 4 == 0 ? q.x : j % 4 == 1 ? q.y : j % 4 == 2 ? q.z : q.w;
+          const uint4 w = w4_widen_adjacent<F>(word, off[(i * 32 + j * 8) / kGroup]);
+          v[4 * j] = w.x;
+          v[4 * j + 1] = w.y;
+          v[4 * j + 2] = w.z;
+          v[4 * j + 3] = w.w;
+        }
+        tmem_st32(to + i * 16, v);
       }
-      if constexpr (!kTma) {
-        if (!all(mbar_wait(&x_empty[x], x_phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+      tmem_wait_st();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st.at]);
+      st.next(Tr::kStages);
+      st.next(Tr::kStages);
+      r.next(Tr::kRaw);
+      r.next(Tr::kRaw);
+    }
+    __syncwarp();
+  } else {
+    // ---------------- x without TMA ----------------
+    if constexpr (!kTma) {
+      registers_up<Th::kX>();
+      const X *src = static_cast<const X *>(p.x);
+      const int tid = static_cast<int>(threadIdx.x) - kXFirst * 32;
+      const bool packs = reinterpret_cast<uintptr_t>(src) % 16 == 0 && p.ldx * sizeof(X) % 16 == 0;
+      constexpr int E = 16 / sizeof(X);
+      Slot x;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!all(mbar_wait(&empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
           break;
-        uint8_t *xs = ring_x + x * Tr::kXBytes;
-        const X *src = static_cast<const X *>(p.x);
+        uint8_t *xs = ring_x + x.at * Tr::kXBytes;
         // pieces of eight values: 16 to a token's row of the stage
-        for (int i = tid; i < NTOK * 16; i += kWideWarps * 32) {
+#pragma unroll 2
+        for (int i = tid; i < NTOK * 16; i += kXWarps * 32) {
           const int token = i >> 4, piece = i & 15, k = kb * kBK + piece * 8;
+          const X *from = src + static_cast<int64_t>(m0 + token) * p.ldx + k;
+          X v[8];
+          if (packs && m0 + token < p.M && k + 8 <= p.K) {
+#pragma unroll
+            for (int j = 0; j < 8; j += E)
+              *reinterpret_cast<Pack<X, E> *>(v + j) = load_pack<X, E>(from + j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[j] = m0 + token < p.M && k + j < p.K ? from[j] : from_float<X>(0.0f);
+          }
           uint32_t h[P][8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const bool in = m0 + token < p.M && k + j < p.K;
-            const int64_t at = static_cast<int64_t>(m0 + token) * p.ldx + k + j;
             if constexpr (P == 3) {
               uint32_t parts[3];
-              w4_split3(in ? src[at] : 0.0f, parts);
+              w4_split3(v[j], parts);
 #pragma unroll
               for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
             } else {
-              h[0][j] = in ? bits16(src[at]) : 0u;
+              h[0][j] = reinterpret_cast<const uint16_t &>(v[j]);
             }
           }
 #pragma unroll
@@ -371,11 +406,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&x_full[x]);
-        if (++x == Tr::kX) {
-          x = 0;
-          x_phase ^= 1u;
-        }
+        if (lane == 0) mbar_arrive(&full[x.at]);
+        x.next(Tr::kStages);
       }
     }
     __syncwarp();
@@ -444,7 +476,7 @@ int launch(cudaStream_t s, const W4Args &p, MmaPlan plan) {
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(MmaThreads<kTma>::kThreads);
   cfg.dynamicSmemBytes = Tr::kSmem;
   cfg.stream = s;
   cfg.attrs = attr;
