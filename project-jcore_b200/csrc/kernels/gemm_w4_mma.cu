@@ -32,7 +32,7 @@ template <bool kTma>
 struct MmaThreads {
   static constexpr int kThreads = 32 * (kXFirst + (kTma ? 0 : kXWarps));
   static constexpr int kLaunch = kTma ? 96 : 80;
-  static constexpr int kIssue = 40, kEpi = kTma ? 128 : 96, kWide = kTma ? 88 : 72, kX = 96;
+  static constexpr int kIssue = 40, kEpi = kTma ? 144 : 96, kWide = 72, kX = 96;
   static_assert(kIssue * 128 + kEpi * 32 * kEpiWarps + kWide * 32 * kWideWarps +
                         (kTma ? 0 : kX * 32 * kXWarps) <=
                     kLaunch * kThreads,
@@ -83,6 +83,25 @@ struct Slot {
     }
   }
 };
+
+// kCols consecutive TMEM columns of this thread's lane, awaited.
+template <int kCols>
+__device__ __forceinline__ void tmem_ld(uint32_t from, uint32_t (&v)[kCols]) {
+  if constexpr (kCols == 16) {
+    tmem_ld16(from, v);
+    tmem_wait_ld16(v);
+  } else if constexpr (kCols == 32) {
+    tmem_ld32(from, v);
+    tmem_wait_ld(v);
+  } else {
+    static_assert(kCols == 64, "columns");
+    uint32_t(&a)[32] = *reinterpret_cast<uint32_t(*)[32]>(v);
+    uint32_t(&b)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 32);
+    tmem_ld32(from, a);
+    tmem_ld32(from + 32, b);
+    tmem_wait_ld2(a, b);
+  }
+}
 
 template <typename X, int NTOK, int kGroup, bool kTma>
 __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
@@ -193,15 +212,20 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       int group = g_begin;
       bool go = all(injected_stall(never, plan.stall_us, abort_flag, p.status));
       for (int kb = kb0; go && kb < kb1; ++kb) {
-        go = all(mbar_wait(&full[st.at], st.phase, abort_flag, p.status, kStatusTimeoutMma));
+        bool ready = mbar_test(&full[st.at], st.phase),
+             free = mbar_test(&acc_empty[acc.at], acc.phase ^ 1u);
+        if (!all(ready))
+          go = all(mbar_wait(&full[st.at], st.phase, abort_flag, p.status, kStatusTimeoutMma));
         if (!go) break;
         const uint64_t desc = desc0 + static_cast<uint64_t>(st.at * (Tr::kXBytes >> 4));
         const uint32_t a = tmem_a + static_cast<uint32_t>(st.at * kACols);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           if (group >= g_end) break;
-          go = all(mbar_wait(&acc_empty[acc.at], acc.phase ^ 1u, abort_flag, p.status,
-                             kStatusTimeoutAccFree));
+          if (i > 0) free = mbar_test(&acc_empty[acc.at], acc.phase ^ 1u);
+          if (!all(free))
+            go = all(mbar_wait(&acc_empty[acc.at], acc.phase ^ 1u, abort_flag, p.status,
+                               kStatusTimeoutAccFree));
           if (!go) break;
           tc_fence_after_sync();
           const uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * NTOK);
@@ -234,7 +258,6 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     // ---------------- groups' sums: scaled and added in registers ----------------
     registers_up<Th::kEpi>();
     constexpr int kCols = NTOK / 2;  // tokens of a warp: two warps to a lane quadrant
-    constexpr int kLoad = kCols < 32 ? kCols : 32;
     const int quad = warp & 3, half = (warp - kEpiFirst) >> 2;
     const int64_t n = static_cast<int64_t>(n0) + quad * 32 + lane;
     const uint32_t row =
@@ -245,41 +268,35 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     // channels past the last take its scales, their results are dropped
     const int64_t scale_row = (n < p.N ? n : p.N - 1) * p.lds;
     const auto scale_at = [&](int g) {
-      return load_scale(p.scale, p.scale_type, scale_row + min(g, g_end - 1));
+      return load_scale_bits(p.scale, p.scale_type, scale_row + min(g, g_end - 1));
     };
-    float s_now = scale_at(g_begin), s_next = scale_at(g_begin + 1);
+    uint32_t s_next = scale_at(g_begin), s_after = scale_at(g_begin + 1);
     Slot acc;
     have = true;
+    bool ready = false;
+    // A group's chain -- the wait, the read, the sums -- is what bounds short groups: the next
+    // group's barrier is asked for and the scale brought along under this one's sums.
     for (int g = g_begin; g < g_end; ++g) {
-      const float s = s_now;
-      s_now = s_next;
-      s_next = scale_at(g + 2);
-      have = all(mbar_wait(&acc_full[acc.at], acc.phase, abort_flag, p.status,
-                           kStatusTimeoutEpilogue));
-      if (!have) break;
-      tc_fence_after_sync();
-      const uint32_t from = row + static_cast<uint32_t>(acc.at * NTOK);
-#pragma unroll
-      for (int c = 0; c < kCols; c += kLoad) {
-        uint32_t v[kLoad];
-        if constexpr (kLoad == 16) {
-          tmem_ld16(from, v);
-          tmem_wait_ld16(v);
-        } else {
-          tmem_ld32(from + static_cast<uint32_t>(c), v);
-          tmem_wait_ld(v);
-        }
-        if (c + kLoad == kCols) {  // all read: the accumulator is free again
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[acc.at]);
-        }
-#pragma unroll
-        for (int j = 0; j < kLoad; j += 2)
-          sum[(c + j) / 2] = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])),
-                                  both(s), sum[(c + j) / 2]);
+      if (!all(ready)) {
+        have = all(mbar_wait(&acc_full[acc.at], acc.phase, abort_flag, p.status,
+                             kStatusTimeoutEpilogue));
+        if (!have) break;
       }
+      tc_fence_after_sync();
+      uint32_t v[kCols];
+      tmem_ld<kCols>(row + static_cast<uint32_t>(acc.at * NTOK), v);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc.at]);  // all read: it is free again
       acc.next(Tr::kAcc);
+      ready = mbar_test(&acc_full[acc.at], acc.phase);
+      const float s = scale_value(s_next, p.scale_type);
+      s_next = s_after;
+      s_after = scale_at(g + 2);
+#pragma unroll
+      for (int j = 0; j < kCols; j += 2)
+        sum[j / 2] = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), both(s),
+                          sum[j / 2]);
     }
     // [token][channel], over the rings, which all MMAs have read out by now
     if (have) {

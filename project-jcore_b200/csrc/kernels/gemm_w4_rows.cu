@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(kMostWarps * 32)
 
   // Scales (and zeros) of a stage, loaded one stage ahead: lane l holds those of channel
   // l % 16, of the stage's first (l < 16) or second half.
-  float sc[kHeld], sc_next[kHeld];
+  float sc[kHeld];
+  uint32_t sc_next[kHeld];
   int ze[kHeld], ze_next[kHeld];
   int64_t s_row = 0, z_row = 0;
   const auto aim_scales = [&](int round) {
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kMostWarps * 32)
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
       const int group = min(g0 + j, p.groups - 1);
-      sc_next[j] = load_scale(p.scale, p.scale_type, s_row + group);
+      sc_next[j] = load_scale_bits(p.scale, p.scale_type, s_row + group);
       if (kZeros) ze_next[j] = __ldg(p.zero + z_row + group) & 15;
     }
   };
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(kMostWarps * 32)
       issue();
 #pragma unroll
       for (int j = 0; j < kHeld; ++j) {
-        sc[j] = sc_next[j];
+        sc[j] = scale_value(sc_next[j], p.scale_type);
         if (kZeros) ze[j] = ze_next[j];
       }
       if (step + 1 < steps) {

@@ -86,6 +86,20 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint64_t *bar, uint32_t parity
   return done;
 }
 
+// Whether that phase has completed, without waiting: asked early, so that the answer is there
+// when it is needed.
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
 // Waits until the phase with the given parity has completed. Returns false if
 // the CTA was told to abort or if the wait exceeded limit_ns, in which case
 // `code` is recorded in *status (first error wins) and *abort is raised.
