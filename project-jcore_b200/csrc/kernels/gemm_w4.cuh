@@ -158,20 +158,19 @@ __device__ __forceinline__ uint4 w4_widen_adjacent(uint32_t word, uint32_t off) 
 }
 
 // fp32 as three bf16 parts by truncation: 8 bits of the significand each, so the last
-// remainder fits (but for bits below the least denormal). An infinity or NaN is its first
-// part alone.
-__device__ __forceinline__ void w4_split3(float x, uint32_t (&part)[3]) {
-  const uint32_t bits = __float_as_uint(x);
-  part[0] = bits >> 16;
-  if ((bits & 0x7f800000u) == 0x7f800000u) {
-    if (bits & 0x007fffffu) part[0] |= 0x40u;  // a NaN whose set bits are all cut off
-    part[1] = part[2] = 0u;
-    return;
+// remainder fits (but for bits below the least denormal). Infinity is its first part
+// alone; of a NaN, the remainders are NaN. Two values at a time, the first in the low halves.
+__device__ __forceinline__ void w4_split3(float a, float b, uint32_t (&part)[3]) {
+  const float inf = __builtin_huge_valf();
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    part[q] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    if (q == 2) break;
+    const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u),
+                rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    a = q == 0 && fabsf(a) == inf ? 0.0f : ra;
+    b = q == 0 && fabsf(b) == inf ? 0.0f : rb;
   }
-  const float r = x - __uint_as_float(bits & 0xffff0000u);
-  const uint32_t rb = __float_as_uint(r);
-  part[1] = rb >> 16;
-  part[2] = __float_as_uint(r - __uint_as_float(rb & 0xffff0000u)) >> 16;
 }
 
 // Activation and store of V results of consecutive channels (`whole`: as one pack).

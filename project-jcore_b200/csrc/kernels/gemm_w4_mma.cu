@@ -22,17 +22,19 @@ namespace {
 constexpr int kChannels = 128, kBK = 128;  // of a tile; values of K a stage
 constexpr int kRawBytes = kChannels * (kBK / 2);
 constexpr int kACols = kBK / 2;            // TMEM columns of a stage's widened weights
-// Warpgroups: TMA and MMA issue; epilogue (two); widening (two, every second stage each);
-// x where it does not come by TMA.
+// Warpgroups: TMA and MMA issue; epilogue (two); widening (two); x where it does not
+// come by TMA (two). A stage's chain of waits, loads and stores is long against its products,
+// so roles come in two teams that take every second stage or group: MMA issue, widening
+// and, up to 64 tokens, the epilogue.
 constexpr int kEpiFirst = 4, kEpiWarps = 8, kWideFirst = kEpiFirst + kEpiWarps, kWideWarps = 8,
-              kXFirst = kWideFirst + kWideWarps, kXWarps = 4;
+              kXFirst = kWideFirst + kWideWarps, kXWarps = 8;
 
 // Threads, and registers a thread: at launch, and as the warpgroups share them.
 template <bool kTma>
 struct MmaThreads {
   static constexpr int kThreads = 32 * (kXFirst + (kTma ? 0 : kXWarps));
-  static constexpr int kLaunch = kTma ? 96 : 80;
-  static constexpr int kIssue = 40, kEpi = kTma ? 144 : 96, kWide = 72, kX = 96;
+  static constexpr int kLaunch = kTma ? 96 : 72;
+  static constexpr int kIssue = kTma ? 48 : 40, kEpi = kTma ? 136 : 88, kWide = kTma ? 80 : 64, kX = 72;
   static_assert(kIssue * 128 + kEpi * 32 * kEpiWarps + kWide * 32 * kWideWarps +
                         (kTma ? 0 : kX * 32 * kXWarps) <=
                     kLaunch * kThreads,
@@ -42,8 +44,12 @@ struct MmaThreads {
 };
 
 // P parts of x.
-template <int NTOK, int P>
+template <int NTOK, int P, bool kTma>
 struct MmaTraits {
+  // Epilogue teams, and the tokens of one of their warps. Two teams of a warp for each quadrant
+  // of lanes, or one of two warps that halve the tokens (whose sums would not fit otherwise).
+  static constexpr int kTeams = NTOK <= 64 && kTma ? 2 : 1;
+  static constexpr int kCols = kTeams == 2 ? NTOK : NTOK / 2;
   static constexpr int kXAtom = NTOK * 128;  // NTOK rows x 64 values
   static constexpr int kXBytes = 2 * kXAtom * P;
   static constexpr int kStages = 4;  // x in shared memory, weights in TMEM
@@ -58,10 +64,22 @@ struct MmaTraits {
   static constexpr int kNeeded = 1024 + kRings + 8 * kBarriers + 64;
   static constexpr int kSmem = kNeeded > 200 * 1024 ? kNeeded : 200 * 1024;
   static_assert(kAcc * NTOK + kStages * kACols <= kTmemCols, "TMEM columns");
-  static_assert(kRaw >= 2, "packed weights in flight");
-  static_assert(NTOK * kChannels * 4 <= kRings, "partial sums over the rings");
+  static_assert(kRaw >= 2 && kRaw % 2 == 0 && kStages % 2 == 0 && kAcc % 2 == 0,
+                "a slot belongs to one of two teams");
+  static_assert(kTeams * NTOK * kChannels * 4 <= kRings, "partial sums over the rings");
   static_assert(kSmem <= 232448, "shared memory budget");
   static_assert(tmem_excludes_clusters(kSmem), "no other cluster's TMEM beside this one's");
+};
+
+// Accumulators belong to issuer teams, kAcc / 2 each, taken in turn: a team's l-th group uses
+// its slot l mod (kAcc / 2) for the l / (kAcc / 2)-th time. Waits are by parity, so whoever
+// waits on a slot has to see each of its uses; the epilogue's teams are the issuers' for that.
+template <int kAcc>
+struct AccSlot {
+  int at;
+  uint32_t phase;
+  __device__ __forceinline__ AccSlot(int team, int l)
+      : at(team * (kAcc / 2) + l % (kAcc / 2)), phase(l / (kAcc / 2) & 1) {}
 };
 
 struct MmaPlan {
@@ -110,7 +128,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
                        const MmaPlan plan) {
   using F = typename W4Type<X>::Frag;
   constexpr int P = W4Type<X>::kParts;
-  using Tr = MmaTraits<NTOK, P>;
+  using Tr = MmaTraits<NTOK, P, kTma>;
   using Th = MmaThreads<kTma>;
   constexpr int kPer = kBK / kGroup;  // groups a stage
   extern __shared__ uint8_t smem_raw[];
@@ -143,7 +161,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     }
     for (int i = 0; i < Tr::kAcc; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpiWarps);
+      mbar_init(&acc_empty[i], kEpiWarps / Tr::kTeams);
     }
     mbar_init(never, 1);
     *abort_flag = 0;
@@ -202,18 +220,19 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
         if ((r_used >> i) & 1u) mbar_drain(&raw_full[i], (r_last >> i) & 1u);
       for (int i = 0; kTma && i < Tr::kStages; ++i)
         if ((x_used >> i) & 1u) mbar_drain(&full[i], (x_last >> i) & 1u);
-    } else if (warp == 1) {
-      // ---------------- MMA issuer ----------------
-      // the whole warp goes round, one lane issues: addresses and descriptors then stay in
-      // uniform registers (one lane alone took 75 cycles an instruction)
+    } else if (warp == 1 || warp == 2) {
+      // ---------------- MMA issuers ----------------
+      // The whole warp goes round, one lane issues: addresses and descriptors then stay in
+      // uniform registers (one lane alone took 75 cycles an instruction). Groups have
+      // accumulators of their own, so the two warps' products need no order.
+      const int team = warp - 1;
       const uint32_t idesc = umma_idesc_f16(std::is_same<F, W4Bfloat>::value, kChannels, NTOK);
       const uint64_t desc0 = umma_desc_sw128(smem_u32(ring_x));
-      Slot st, acc;
-      int group = g_begin;
-      bool go = all(injected_stall(never, plan.stall_us, abort_flag, p.status));
-      for (int kb = kb0; go && kb < kb1; ++kb) {
-        bool ready = mbar_test(&full[st.at], st.phase),
-             free = mbar_test(&acc_empty[acc.at], acc.phase ^ 1u);
+      Slot st;
+      if (team) st.next(Tr::kStages);
+      bool go = team || all(injected_stall(never, plan.stall_us, abort_flag, p.status));
+      for (int kb = kb0 + team; go && kb < kb1; kb += 2) {
+        const bool ready = mbar_test(&full[st.at], st.phase);
         if (!all(ready))
           go = all(mbar_wait(&full[st.at], st.phase, abort_flag, p.status, kStatusTimeoutMma));
         if (!go) break;
@@ -221,10 +240,11 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
         const uint32_t a = tmem_a + static_cast<uint32_t>(st.at * kACols);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          if (group >= g_end) break;
-          if (i > 0) free = mbar_test(&acc_empty[acc.at], acc.phase ^ 1u);
-          if (!all(free))
-            go = all(mbar_wait(&acc_empty[acc.at], acc.phase ^ 1u, abort_flag, p.status,
+          if (kb * kPer + i >= g_end) break;
+          const AccSlot<Tr::kAcc> acc(team, (kb - kb0) / 2 * kPer + i);
+          const uint32_t free = acc.phase ^ 1u;
+          if (!all(mbar_test(&acc_empty[acc.at], free)))
+            go = all(mbar_wait(&acc_empty[acc.at], free, abort_flag, p.status,
                                kStatusTimeoutAccFree));
           if (!go) break;
           tc_fence_after_sync();
@@ -243,13 +263,11 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
             mma_commit(&acc_full[acc.at]);
           }
           __syncwarp();
-          ++group;
-          acc.next(Tr::kAcc);
         }
         if (!go) break;
-        // (the last stage's slot is not filled again)
-        if (kb + 1 < kb1 && elect_lane()) mma_commit(&empty[st.at]);
+        if (kb + Tr::kStages < kb1 && elect_lane()) mma_commit(&empty[st.at]);  // to be filled again
         __syncwarp();
+        st.next(Tr::kStages);
         st.next(Tr::kStages);
       }
     }
@@ -257,8 +275,9 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
   } else if (warp < kWideFirst) {
     // ---------------- groups' sums: scaled and added in registers ----------------
     registers_up<Th::kEpi>();
-    constexpr int kCols = NTOK / 2;  // tokens of a warp: two warps to a lane quadrant
-    const int quad = warp & 3, half = (warp - kEpiFirst) >> 2;
+    constexpr int kCols = Tr::kCols;
+    const int quad = warp & 3, second = (warp - kEpiFirst) >> 2;
+    const int team = Tr::kTeams == 2 ? second : 0, half = Tr::kTeams == 2 ? 0 : second;
     const int64_t n = static_cast<int64_t>(n0) + quad * 32 + lane;
     const uint32_t row =
         tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * kCols);
@@ -270,13 +289,22 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     const auto scale_at = [&](int g) {
       return load_scale_bits(p.scale, p.scale_type, scale_row + min(g, g_end - 1));
     };
-    uint32_t s_next = scale_at(g_begin), s_after = scale_at(g_begin + 1);
-    Slot acc;
+    // this team's j-th group, and its accumulator
+    const auto group_of = [&](int j) {
+      return Tr::kTeams == 2 ? (kb0 + team + j / kPer * 2) * kPer + j % kPer : g_begin + j;
+    };
+    const auto slot_of = [&](int j) {
+      return Tr::kTeams == 2
+                 ? AccSlot<Tr::kAcc>(team, j)
+                 : AccSlot<Tr::kAcc>(j / kPer % 2, j / (2 * kPer) * kPer + j % kPer);
+    };
+    uint32_t s_next = scale_at(group_of(0)), s_after = scale_at(group_of(1));
     have = true;
     bool ready = false;
     // A group's chain -- the wait, the read, the sums -- is what bounds short groups: the next
     // group's barrier is asked for and the scale brought along under this one's sums.
-    for (int g = g_begin; g < g_end; ++g) {
+    for (int j = 0; group_of(j) < g_end; ++j) {
+      const AccSlot<Tr::kAcc> acc = slot_of(j);
       if (!all(ready)) {
         have = all(mbar_wait(&acc_full[acc.at], acc.phase, abort_flag, p.status,
                              kStatusTimeoutEpilogue));
@@ -288,19 +316,22 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[acc.at]);  // all read: it is free again
-      acc.next(Tr::kAcc);
-      ready = mbar_test(&acc_full[acc.at], acc.phase);
+      const AccSlot<Tr::kAcc> next = slot_of(j + 1);
+      ready = mbar_test(&acc_full[next.at], next.phase);
       const float s = scale_value(s_next, p.scale_type);
       s_next = s_after;
-      s_after = scale_at(g + 2);
+      s_after = scale_at(group_of(j + 2));
 #pragma unroll
-      for (int j = 0; j < kCols; j += 2)
-        sum[j / 2] = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), both(s),
-                          sum[j / 2]);
+      for (int c = 0; c < kCols; c += 2)
+        sum[c / 2] = fma2(make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), both(s),
+                          sum[c / 2]);
     }
-    // [token][channel], over the rings, which all MMAs have read out by now
+    // [team][token][channel], over the rings. Another team's groups may still be at work on
+    // them: all their MMAs have read the rings once the whole epilogue is here.
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
     if (have) {
-      float *part = reinterpret_cast<float *>(smem) + half * kCols * kChannels + quad * 32 + lane;
+      float *part = reinterpret_cast<float *>(smem) +
+                    (team * NTOK + half * kCols) * kChannels + quad * 32 + lane;
 #pragma unroll
       for (int j = 0; j < kCols; j += 2) {
         part[j * kChannels] = sum[j / 2].x * F::kUnit;
@@ -338,23 +369,24 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       }
       if (!all(mbar_wait(&raw_full[r.at], r.phase, abort_flag, p.status, kStatusTimeoutStage)))
         break;
-      const uint8_t *from = ring_raw + r.at * kRawBytes + row * 64;
-      const int sw = (row >> 1) & 3;
-      uint4 raw[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4 *>(from + ((i ^ sw) << 4));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_empty[r.at]);
       if (!all(mbar_wait(&empty[st.at], st.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
         break;
       tc_fence_after_sync();
+      const uint8_t *from = ring_raw + r.at * kRawBytes + row * 64;
+      const int sw = (row >> 1) & 3;
       const uint32_t to = t_row + static_cast<uint32_t>(st.at * kACols);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
+        const uint4 lo = *reinterpret_cast<const uint4 *>(from + ((i ^ sw) << 4));
+        const uint4 hi = *reinterpret_cast<const uint4 *>(from + (((i + 1) ^ sw) << 4));
+        if (i == 2) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&raw_empty[r.at]);
+        }
         uint32_t v[32];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint4 &q = raw[i + j / 4];
+          const uint4 &q = j < 4 ? lo : hi;
           const uint32_t word = j % 4 == 0 ? q.x : j % 4 == 1 ? q.y : j % 4 == 2 ? q.z : q.w;
           const uint4 w = w4_widen_adjacent<F>(word, off[(i * 32 + j * 8) / kGroup]);
           v[4 * j] = w.x;
@@ -381,45 +413,49 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       const X *src = static_cast<const X *>(p.x);
       const int tid = static_cast<int>(threadIdx.x) - kXFirst * 32;
       const bool packs = reinterpret_cast<uintptr_t>(src) % 16 == 0 && p.ldx * sizeof(X) % 16 == 0;
-      constexpr int E = 16 / sizeof(X);
+      constexpr int E = 16 / sizeof(X), kPieces = NTOK * 16 / (kXWarps * 32);
       Slot x;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!all(mbar_wait(&empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
-          break;
-        uint8_t *xs = ring_x + x.at * Tr::kXBytes;
-        // pieces of eight values: 16 to a token's row of the stage
-#pragma unroll 2
-        for (int i = tid; i < NTOK * 16; i += kXWarps * 32) {
-          const int token = i >> 4, piece = i & 15, k = kb * kBK + piece * 8;
+        // pieces of eight values, 16 to a token's row of the stage; all loads first, ahead of
+        // the slot
+        alignas(16) X v[kPieces][8];
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          const int i = tid + c * (kXWarps * 32), token = i >> 4, k = kb * kBK + (i & 15) * 8;
           const X *from = src + static_cast<int64_t>(m0 + token) * p.ldx + k;
-          X v[8];
           if (packs && m0 + token < p.M && k + 8 <= p.K) {
 #pragma unroll
             for (int j = 0; j < 8; j += E)
-              *reinterpret_cast<Pack<X, E> *>(v + j) = load_pack<X, E>(from + j);
+              *reinterpret_cast<Pack<X, E> *>(v[c] + j) = load_pack<X, E>(from + j);
           } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              v[j] = m0 + token < p.M && k + j < p.K ? from[j] : from_float<X>(0.0f);
+              v[c][j] = m0 + token < p.M && k + j < p.K ? from[j] : from_float<X>(0.0f);
           }
-          uint32_t h[P][8];
+        }
+        if (!all(mbar_wait(&empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+          break;
+        uint8_t *xs = ring_x + x.at * Tr::kXBytes;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+        for (int c = 0; c < kPieces; ++c) {
+          const int i = tid + c * (kXWarps * 32), token = i >> 4, piece = i & 15;
+          uint32_t h[P][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
             if constexpr (P == 3) {
               uint32_t parts[3];
-              w4_split3(v[j], parts);
+              w4_split3(v[c][2 * j], v[c][2 * j + 1], parts);
 #pragma unroll
               for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
             } else {
-              h[0][j] = reinterpret_cast<const uint16_t &>(v[j]);
+              h[0][j] = reinterpret_cast<const uint32_t &>(v[c][2 * j]);
             }
           }
 #pragma unroll
           for (int q = 0; q < P; ++q)
             *reinterpret_cast<uint4 *>(xs + (2 * q + (piece >> 3)) * Tr::kXAtom +
                                        sw128_offset(static_cast<uint32_t>(token), piece & 7)) =
-                make_uint4(h[q][0] | h[q][1] << 16, h[q][2] | h[q][3] << 16,
-                           h[q][4] | h[q][5] << 16, h[q][6] | h[q][7] << 16);
+                make_uint4(h[q][0], h[q][1], h[q][2], h[q][3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -447,10 +483,11 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       if (m0 + token >= p.M || count == 0) break;
       const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(token * kChannels + 4 * lane) * 4u;
       float v[4] = {};
-      for (int s = 0; s < plan.slices; ++s) {
+      for (int i = 0; i < plan.slices * Tr::kTeams; ++i) {
+        const int team = i % Tr::kTeams * (NTOK * kChannels * 4);
         const uint4 q = plan.slices == 1
-                            ? *reinterpret_cast<const uint4 *>(smem + (token * kChannels + 4 * lane) * 4)
-                            : ld_shared_cluster_v4(mapa_shared(at, static_cast<uint32_t>(s)));
+                            ? *reinterpret_cast<const uint4 *>(smem + team + (token * kChannels + 4 * lane) * 4)
+                            : ld_shared_cluster_v4(mapa_shared(at + team, static_cast<uint32_t>(i / Tr::kTeams)));
         v[0] += __uint_as_float(q.x);
         v[1] += __uint_as_float(q.y);
         v[2] += __uint_as_float(q.z);
@@ -473,7 +510,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
 
 template <typename X, int NTOK, int kGroup, bool kTma>
 int launch(cudaStream_t s, const W4Args &p, MmaPlan plan) {
-  using Tr = MmaTraits<NTOK, W4Type<X>::kParts>;
+  using Tr = MmaTraits<NTOK, W4Type<X>::kParts, kTma>;
   CUtensorMap mw, mx = {};
   int rc = encode_tmap_2d_u8_sw64(&mw, p.q, ceil_div(p.K, 2), p.N, p.ldq, kChannels);
   if (!rc && kTma) rc = encode_tmap_2d_u8_sw128(&mx, p.x, 2 * static_cast<int64_t>(p.K), p.M, 2 * p.ldx, NTOK);

@@ -171,23 +171,23 @@ __global__ void __launch_bounds__(kMostWarps * 32)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? from[j] : from_float<X>(0.0f);
       }
-      uint32_t h[P][8];
+      uint32_t h[P][4];  // pairs (0, 4), (1, 5), ... of each part
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
         if constexpr (P == 3) {
           uint32_t parts[3];
-          w4_split3(v[j], parts);
+          w4_split3(v[j], v[j + 4], parts);
 #pragma unroll
           for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
         } else {
-          h[0][j] = reinterpret_cast<const uint16_t &>(v[j]);
+          h[0][j] = reinterpret_cast<const uint16_t &>(v[j]) |
+                    static_cast<uint32_t>(reinterpret_cast<const uint16_t &>(v[j + 4])) << 16;
         }
       }
 #pragma unroll
       for (int q = 0; q < P; ++q)
         sx[(((chunk * kRun + r) * P + q) * p.M + m) * 4 + lane_t] =
-            make_uint4(h[q][0] | h[q][4] << 16, h[q][1] | h[q][5] << 16, h[q][2] | h[q][6] << 16,
-                       h[q][3] | h[q][7] << 16);
+            make_uint4(h[q][0], h[q][1], h[q][2], h[q][3]);
     }
   }
   __syncthreads();
