@@ -52,19 +52,20 @@ struct MmaTraits {
   static constexpr int kCols = kTeams == 2 ? NTOK : NTOK / 2;
   static constexpr int kXAtom = NTOK * 128;  // NTOK rows x 64 values
   static constexpr int kXBytes = 2 * kXAtom * P;
-  static constexpr int kStages = 4;  // x in shared memory, weights in TMEM
-  static constexpr int kRaw = 208 * 1024 - kStages * kXBytes > 8 * kRawBytes
-                                  ? 8
-                                  : (208 * 1024 - kStages * kXBytes) / kRawBytes;
+  // Rings: widened weights in TMEM, x (its loads take some 2000 cycles, of which a stage of 64
+  // tokens has 400) and packed weights in shared memory.
+  static constexpr int kA = 4, kX = kXBytes <= 16 * 1024 ? 8 : 4;
+  static constexpr int kRaw =
+      208 * 1024 - kX * kXBytes > 8 * kRawBytes ? 8 : (208 * 1024 - kX * kXBytes) / kRawBytes;
   static constexpr int kAcc = NTOK == 128 ? 2 : 4;
   static constexpr int kTmemCols = 512;
-  static constexpr int kRings = kStages * kXBytes + kRaw * kRawBytes;
-  static constexpr int kBarriers = 2 * (kStages + kRaw + kAcc) + 1;
+  static constexpr int kRings = kX * kXBytes + kRaw * kRawBytes;
+  static constexpr int kBarriers = 2 * (kA + kX + kRaw + kAcc) + 1;
   // at least what keeps other clusters' TMEM off this SM
   static constexpr int kNeeded = 1024 + kRings + 8 * kBarriers + 64;
   static constexpr int kSmem = kNeeded > 200 * 1024 ? kNeeded : 200 * 1024;
-  static_assert(kAcc * NTOK + kStages * kACols <= kTmemCols, "TMEM columns");
-  static_assert(kRaw >= 2 && kRaw % 2 == 0 && kStages % 2 == 0 && kAcc % 2 == 0,
+  static_assert(kAcc * NTOK + kA * kACols <= kTmemCols, "TMEM columns");
+  static_assert(kRaw >= 2 && kRaw % 2 == 0 && kA % 2 == 0 && kX % 2 == 0 && kAcc % 2 == 0,
                 "a slot belongs to one of two teams");
   static_assert(kTeams * NTOK * kChannels * 4 <= kRings, "partial sums over the rings");
   static_assert(kSmem <= 232448, "shared memory budget");
@@ -133,11 +134,12 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
   constexpr int kPer = kBK / kGroup;  // groups a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align_smem_1024(smem_raw);
-  uint8_t *ring_x = smem, *ring_raw = ring_x + Tr::kStages * Tr::kXBytes;
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Tr::kRings);
-  uint64_t *empty = full + Tr::kStages, *raw_full = empty + Tr::kStages,
-           *raw_empty = raw_full + Tr::kRaw, *acc_full = raw_empty + Tr::kRaw,
-           *acc_empty = acc_full + Tr::kAcc, *never = acc_empty + Tr::kAcc;
+  uint8_t *ring_x = smem, *ring_raw = ring_x + Tr::kX * Tr::kXBytes;
+  uint64_t *a_full = reinterpret_cast<uint64_t *>(smem + Tr::kRings);
+  uint64_t *a_empty = a_full + Tr::kA, *x_full = a_empty + Tr::kA, *x_empty = x_full + Tr::kX,
+           *raw_full = x_empty + Tr::kX, *raw_empty = raw_full + Tr::kRaw,
+           *acc_full = raw_empty + Tr::kRaw, *acc_empty = acc_full + Tr::kAcc,
+           *never = acc_empty + Tr::kAcc;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(never + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -151,9 +153,13 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
   const int g_begin = kb0 * kPer, g_end = min(p.groups, kb1 * kPer);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < Tr::kStages; ++i) {
-      mbar_init(&full[i], kWideWarps / 2 + (kTma ? 1 : kXWarps));
-      mbar_init(&empty[i], 1);
+    for (int i = 0; i < Tr::kA; ++i) {
+      mbar_init(&a_full[i], kWideWarps / 2);
+      mbar_init(&a_empty[i], 1);
+    }
+    for (int i = 0; i < Tr::kX; ++i) {
+      mbar_init(&x_full[i], kTma ? 1 : kXWarps);
+      mbar_init(&x_empty[i], 1);
     }
     for (int i = 0; i < Tr::kRaw; ++i) {
       mbar_init(&raw_full[i], 1);
@@ -184,42 +190,38 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
   if (warp < kEpiFirst) {
     registers_down<Th::kIssue>();
     if (warp == 0 && lane == 0) {
-      // ---------------- TMA: packed weights, and x ----------------
-      Slot r, x;
-      int xb = kb0;
-      uint32_t r_used = 0, x_used = 0, r_last = 0, x_last = 0;
-      const auto load_x = [&]() -> bool {
-        if (!mbar_wait(&empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer))
-          return false;
-        mbar_arrive_expect_tx(&full[x.at], Tr::kXBytes);
-        uint8_t *to = ring_x + x.at * Tr::kXBytes;
-        tma_load_2d(&map_x, &full[x.at], to, xb * (kBK * 2), m0);
-        tma_load_2d(&map_x, &full[x.at], to + Tr::kXAtom, xb * (kBK * 2) + 128, m0);
-        x_used |= 1u << x.at;
-        x_last = (x_last & ~(1u << x.at)) | (x.phase << x.at);
-        ++xb;
-        x.next(Tr::kStages);
-        return true;
-      };
-      bool go = true;
-      for (int kb = kb0; go && kb < kb1; ++kb) {
-        go = mbar_wait(&raw_empty[r.at], r.phase ^ 1u, abort_flag, p.status,
-                       kStatusTimeoutProducer);
-        if (!go) break;
+      // ---------------- TMA: packed weights ----------------
+      Slot r;
+      uint32_t used = 0, last = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&raw_empty[r.at], r.phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer))
+          break;
         mbar_arrive_expect_tx(&raw_full[r.at], kRawBytes);
         tma_load_2d(&map_w, &raw_full[r.at], ring_raw + r.at * kRawBytes, kb * (kBK / 2), n0);
-        r_used |= 1u << r.at;
-        r_last = (r_last & ~(1u << r.at)) | (r.phase << r.at);
+        used |= 1u << r.at;
+        last = (last & ~(1u << r.at)) | (r.phase << r.at);
         r.next(Tr::kRaw);
-        // weights run ahead of x, as far as their longer ring goes
-        if (kTma && kb - kb0 >= Tr::kRaw - Tr::kStages) go = load_x();
       }
-      while (kTma && go && xb < kb1) go = load_x();
       // the last copy into each slot lands before the CTA can exit
       for (int i = 0; i < Tr::kRaw; ++i)
-        if ((r_used >> i) & 1u) mbar_drain(&raw_full[i], (r_last >> i) & 1u);
-      for (int i = 0; kTma && i < Tr::kStages; ++i)
-        if ((x_used >> i) & 1u) mbar_drain(&full[i], (x_last >> i) & 1u);
+        if ((used >> i) & 1u) mbar_drain(&raw_full[i], (last >> i) & 1u);
+    } else if (kTma && warp == 3 && lane == 0) {
+      // ---------------- TMA: x ----------------
+      Slot x;
+      uint32_t used = 0, last = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&x_empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer))
+          break;
+        mbar_arrive_expect_tx(&x_full[x.at], Tr::kXBytes);
+        uint8_t *to = ring_x + x.at * Tr::kXBytes;
+        tma_load_2d(&map_x, &x_full[x.at], to, kb * (kBK * 2), m0);
+        tma_load_2d(&map_x, &x_full[x.at], to + Tr::kXAtom, kb * (kBK * 2) + 128, m0);
+        used |= 1u << x.at;
+        last = (last & ~(1u << x.at)) | (x.phase << x.at);
+        x.next(Tr::kX);
+      }
+      for (int i = 0; i < Tr::kX; ++i)
+        if ((used >> i) & 1u) mbar_drain(&x_full[i], (last >> i) & 1u);
     } else if (warp == 1 || warp == 2) {
       // ---------------- MMA issuers ----------------
       // The whole warp goes round, one lane issues: addresses and descriptors then stay in
@@ -228,15 +230,20 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       const int team = warp - 1;
       const uint32_t idesc = umma_idesc_f16(std::is_same<F, W4Bfloat>::value, kChannels, NTOK);
       const uint64_t desc0 = umma_desc_sw128(smem_u32(ring_x));
-      Slot st;
-      if (team) st.next(Tr::kStages);
+      Slot st, x;
+      if (team) {
+        st.next(Tr::kA);
+        x.next(Tr::kX);
+      }
       bool go = team || all(injected_stall(never, plan.stall_us, abort_flag, p.status));
       for (int kb = kb0 + team; go && kb < kb1; kb += 2) {
-        const bool ready = mbar_test(&full[st.at], st.phase);
-        if (!all(ready))
-          go = all(mbar_wait(&full[st.at], st.phase, abort_flag, p.status, kStatusTimeoutMma));
+        const bool a_ready = mbar_test(&a_full[st.at], st.phase),
+                   x_ready = mbar_test(&x_full[x.at], x.phase);
+        if (!all(a_ready && x_ready))
+          go = all(mbar_wait(&a_full[st.at], st.phase, abort_flag, p.status, kStatusTimeoutMma) &&
+                   mbar_wait(&x_full[x.at], x.phase, abort_flag, p.status, kStatusTimeoutMma));
         if (!go) break;
-        const uint64_t desc = desc0 + static_cast<uint64_t>(st.at * (Tr::kXBytes >> 4));
+        const uint64_t desc = desc0 + static_cast<uint64_t>(x.at * (Tr::kXBytes >> 4));
         const uint32_t a = tmem_a + static_cast<uint32_t>(st.at * kACols);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -265,10 +272,15 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
           __syncwarp();
         }
         if (!go) break;
-        if (kb + Tr::kStages < kb1 && elect_lane()) mma_commit(&empty[st.at]);  // to be filled again
+        if (elect_lane()) {  // slots that are to be filled again
+          if (kb + Tr::kA < kb1) mma_commit(&a_empty[st.at]);
+          if (kb + Tr::kX < kb1) mma_commit(&x_empty[x.at]);
+        }
         __syncwarp();
-        st.next(Tr::kStages);
-        st.next(Tr::kStages);
+        st.next(Tr::kA);
+        st.next(Tr::kA);
+        x.next(Tr::kX);
+        x.next(Tr::kX);
       }
     }
     __syncwarp();
@@ -281,9 +293,9 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     const int64_t n = static_cast<int64_t>(n0) + quad * 32 + lane;
     const uint32_t row =
         tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * kCols);
-    float2 sum[kCols / 2];
+    float sum[kCols];
 #pragma unroll
-    for (int j = 0; j < kCols / 2; ++j) sum[j] = make_float2(0.0f, 0.0f);
+    for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
     // channels past the last take its scales, their results are dropped
     const int64_t scale_row = (n < p.N ? n : p.N - 1) * p.lds;
     const auto scale_at = [&](int g) {
@@ -322,9 +334,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       s_next = s_after;
       s_after = scale_at(group_of(j + 2));
 #pragma unroll
-      for (int c = 0; c < kCols; c += 2)
-        sum[c / 2] = fma2(make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), both(s),
-                          sum[c / 2]);
+      for (int c = 0; c < kCols; ++c) sum[c] = fmaf(__uint_as_float(v[c]), s, sum[c]);
     }
     // [team][token][channel], over the rings. Another team's groups may still be at work on
     // them: all their MMAs have read the rings once the whole epilogue is here.
@@ -333,10 +343,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       float *part = reinterpret_cast<float *>(smem) +
                     (team * NTOK + half * kCols) * kChannels + quad * 32 + lane;
 #pragma unroll
-      for (int j = 0; j < kCols; j += 2) {
-        part[j * kChannels] = sum[j / 2].x * F::kUnit;
-        part[(j + 1) * kChannels] = sum[j / 2].y * F::kUnit;
-      }
+      for (int j = 0; j < kCols; ++j) part[j * kChannels] = sum[j] * F::kUnit;
     }
     __syncwarp();
     if (plan.slices == 1)
@@ -357,7 +364,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     for (int i = 0; i < kPer; ++i) z_next[i] = zero_at(kb0 + team, i);
     Slot st, r;
     if (team) {
-      st.next(Tr::kStages);
+      st.next(Tr::kA);
       r.next(Tr::kRaw);
     }
     for (int kb = kb0 + team; kb < kb1; kb += 2) {
@@ -369,7 +376,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       }
       if (!all(mbar_wait(&raw_full[r.at], r.phase, abort_flag, p.status, kStatusTimeoutStage)))
         break;
-      if (!all(mbar_wait(&empty[st.at], st.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+      if (!all(mbar_wait(&a_empty[st.at], st.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
         break;
       tc_fence_after_sync();
       const uint8_t *from = ring_raw + r.at * kRawBytes + row * 64;
@@ -399,9 +406,9 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st.at]);
-      st.next(Tr::kStages);
-      st.next(Tr::kStages);
+      if (lane == 0) mbar_arrive(&a_full[st.at]);
+      st.next(Tr::kA);
+      st.next(Tr::kA);
       r.next(Tr::kRaw);
       r.next(Tr::kRaw);
     }
@@ -433,7 +440,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
               v[c][j] = m0 + token < p.M && k + j < p.K ? from[j] : from_float<X>(0.0f);
           }
         }
-        if (!all(mbar_wait(&empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+        if (!all(mbar_wait(&x_empty[x.at], x.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
           break;
         uint8_t *xs = ring_x + x.at * Tr::kXBytes;
 #pragma unroll
@@ -459,8 +466,8 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[x.at]);
-        x.next(Tr::kStages);
+        if (lane == 0) mbar_arrive(&x_full[x.at]);
+        x.next(Tr::kX);
       }
     }
     __syncwarp();
