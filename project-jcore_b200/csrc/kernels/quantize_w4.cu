@@ -5,15 +5,15 @@
 // clamped to 0..15. The scale is rounded to its stored type first: the quotients are by
 // what the product will multiply with. `least` is the type's smallest normal number.
 #include <algorithm>
+#include <type_traits>
 
 #include "nplk_host.h"
 #include "ptx_sm100.cuh"
+#include "quotient.cuh"
 #include "w4_format.cuh"
 
 namespace nplk {
 namespace {
-
-constexpr float kInf = __builtin_huge_valf();
 
 struct QuantArgs {
   int64_t ldw, ldq, lds, ldz;
@@ -45,94 +45,137 @@ __device__ __forceinline__ float most_nan(float a, float b) {
   return r;
 }
 
-// A group belongs to group / 8 neighbouring lanes, eight values each. kPacks: w in whole
+// Eight values' limits: high the largest magnitude, or with zeros the largest of w and 0, and
+// low then the largest of -w and 0. 16-bit types two at a time; NaN stays.
+template <typename T, bool kZeros>
+__device__ __forceinline__ void limits(const Pack<T, 8> &v, float &high, float &low) {
+  if constexpr (std::is_same<T, float>::value) {
+    high = low = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      high = most_nan(high, kZeros ? v.e[j] : fabsf(v.e[j]));
+      if (kZeros) low = most_nan(low, -v.e[j]);
+    }
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 h{}, l{};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const T2 w = reinterpret_cast<const T2 *>(&v)[j];
+      h = __hmax2_nan(h, kZeros ? w : __habs2(w));
+      if (kZeros) l = __hmax2_nan(l, __hneg2(w));
+    }
+    high = most_nan(to_float(h.x), to_float(h.y));
+    low = most_nan(to_float(l.x), to_float(l.y));
+  }
+}
+
+// Eight 4-bit numbers, in the low bytes of b, as a word.
+__device__ __forceinline__ uint32_t pack_nibbles(const uint32_t (&b)[8]) {
+  const uint32_t even = low_bytes(b) & 0x0f0f0f0fu, odd = low_bytes(b + 4) & 0x0f0f0f0fu;
+  return __byte_perm(even | even >> 4, odd | odd >> 4, 0x6420);
+}
+
+// Eight values an item, a group to group / 8 neighbouring lanes, a row to `lanes` threads (a
+// power of two, 32 to 256), kItems items of a thread at a time: their loads come first.
+// Bound by memory: 16384 x 4096 bf16 in groups of 128 takes 30 us, 5.6 TB/s (a thread an item
+// with a division for each value and one for its place took 91 us). kPacks: w in whole
 // 16-byte pieces and q in whole words; otherwise value by value.
+constexpr int kThreads = 256, kItems = 4;
+
 template <typename T, int kGroup, bool kZeros, bool kPacks>
-__global__ void __launch_bounds__(256)
-    quantize_w4_kernel(QuantArgs p, const T *w, int64_t items) {
+__global__ void __launch_bounds__(kThreads)
+    quantize_w4_kernel(const QuantArgs p, const T *w, int lanes) {
   constexpr int kLanes = kGroup / 8;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  const int per_row = p.groups * kLanes;
+  const int t = static_cast<int>(threadIdx.x) & (lanes - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) +
+                      static_cast<int>(threadIdx.x) / lanes;
+  const bool live = row < p.n;
+  const T *x = w + (live ? row : p.n - 1) * p.ldw;
+  uint8_t *q = p.q + row * p.ldq;
+  const int items = p.groups * kLanes;
   // whole warps go round together: a group's lanes shuffle
-  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 + (threadIdx.x & ~31); i0 < items;
-       i0 += step) {
-    const int64_t item = i0 + (threadIdx.x & 31);
-    const bool live = item < items;
-    const int64_t row = live ? item / per_row : 0;
-    const int part = live ? static_cast<int>(item - row * per_row) : 0;
-    const int c = part * 8;
-    const int here = live ? min(8, p.k - c) : 0;  // may be none or negative
-    const T *x = w + row * p.ldw + c;
-    float v[8];
-    if (kPacks && here == 8) {
-      if constexpr (sizeof(T) == 2) {
-        unpack(load_pack<T, 8>(x), v);
-      } else {
-        const Pack<T, 4> a = load_pack<T, 4>(x), b = load_pack<T, 4>(x + 4);
+  for (int base = 0; base < items; base += lanes * kItems) {
+    Pack<T, 8> v[kItems];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = to_float(a.e[j]);
-          v[4 + j] = to_float(b.e[j]);
+    for (int u = 0; u < kItems; ++u) {
+      const int c = (base + u * lanes + t) * 8;
+      if (kPacks && c + 8 <= p.k) {
+        if constexpr (sizeof(T) == 2) {
+          v[u] = load_pack<T, 8>(x + c);
+        } else {
+          *reinterpret_cast<Pack<T, 4> *>(&v[u].e[0]) = load_pack<T, 4>(x + c);
+          *reinterpret_cast<Pack<T, 4> *>(&v[u].e[4]) = load_pack<T, 4>(x + c + 4);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u].e[j] = c + j < p.k ? x[c + j] : from_float<T>(0.0f);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < here ? to_float(x[j]) : 0.0f;
-    }
-    float high = 0.0f, low = 0.0f;  // low as the largest of -w
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      high = most_nan(high, kZeros ? v[j] : fabsf(v[j]));
-      if (kZeros) low = most_nan(low, -v[j]);
     }
 #pragma unroll
-    for (int o = kLanes / 2; o; o >>= 1) {
-      high = most_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
-      if (kZeros) low = most_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
-    }
-    const float s = round_scale(kZeros ? (high + low) / 15.0f : high / 7.0f, p.scale_type);
-    const bool finite = s < kInf;
-    float zero = 8.0f;
-    if (kZeros) zero = finite ? fminf(fmaxf(rintf(low / s), 0.0f), 15.0f) : 0.0f;
-    if (here > 0 && part % kLanes == 0) {
-      const int64_t g = part / kLanes;
-      store_scale(p.scale, p.scale_type, row * p.lds + g, s);
-      if (kZeros) p.zero[row * p.ldz + g] = static_cast<uint8_t>(zero);
-    }
-    if (here <= 0) continue;
-    uint32_t word = 0;
+    for (int u = 0; u < kItems; ++u) {
+      const int item = base + u * lanes + t, c = item * 8;
+      if (base + u * lanes >= items) break;
+      float high, low;
+      limits<T, kZeros>(v[u], high, low);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float q = finite ? rintf(v[j] / s) + zero : zero;
-      // values behind the row's end are 0 bits
-      const uint32_t nibble =
-          j < here ? static_cast<uint32_t>(fminf(fmaxf(q, 0.0f), 15.0f)) : 0u;
-      word |= nibble << (4 * j);
-    }
-    uint8_t *to = p.q + row * p.ldq + c / 2;
-    if (kPacks && here == 8) {
-      *reinterpret_cast<uint32_t *>(to) = word;
-    } else {
+      for (int o = kLanes / 2; o; o >>= 1) {
+        high = most_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
+        if (kZeros) low = most_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+      }
+      const Scale s =
+          split_scale(round_scale(kZeros ? (high + low) / 15.0f : high / 7.0f, p.scale_type));
+      int zero = 8;
+      if (kZeros) {
+        uint32_t z[1];
+        quotients(Pack<float, 1>{{low}}, s, z);
+        zero = min(static_cast<int>(z[0] & 0xffu), 15);
+      }
+      if (!live || c >= p.k) continue;
+      if (item % kLanes == 0) {
+        const int64_t g = item / kLanes;
+        store_scale(p.scale, p.scale_type, row * p.lds + g, s.value);
+        if (kZeros) p.zero[row * p.ldz + g] = static_cast<uint8_t>(zero);
+      }
+      uint32_t b[8];
+      quotients(v[u], s, b);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (2 * j < here) to[j] = static_cast<uint8_t>(word >> (8 * j));
+      for (int j = 0; j < 8; ++j) {
+        b[j] += zero;
+        if (kZeros) b[j] = static_cast<uint32_t>(max(0, min(15, static_cast<int>(b[j] << 24) >> 24)));
+      }
+      uint32_t word = pack_nibbles(b);
+      uint8_t *to = q + c / 2;
+      if (kPacks && c + 8 <= p.k) {
+        *reinterpret_cast<uint32_t *>(to) = word;
+      } else {
+        const int here = min(8, p.k - c);
+        if (here < 8) word &= (1u << (4 * here)) - 1u;  // the half byte behind an odd row is 0
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (2 * j < here) to[j] = static_cast<uint8_t>(word >> (8 * j));
+      }
     }
   }
 }
 
 template <typename T, int kGroup>
 int launch(cudaStream_t s, const QuantArgs &p, const T *w) {
-  const bool packs = reinterpret_cast<uintptr_t>(w) % 16 == 0 && p.ldw * sizeof(T) % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(p.q) % 4 == 0 && p.ldq % 4 == 0;
-  const int64_t items = static_cast<int64_t>(p.n) * p.groups * (kGroup / 8);
-  const int64_t ctas = std::min<int64_t>(ceil_div(items, 256), static_cast<int64_t>(sm_count()) * 64);
+  const bool packs = reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
+                     (p.ldw * sizeof(T) % 16 == 0 || p.n == 1) &&
+                     reinterpret_cast<uintptr_t>(p.q) % 4 == 0 && (p.ldq % 4 == 0 || p.n == 1);
+  const int64_t items = static_cast<int64_t>(p.groups) * (kGroup / 8);
+  int lanes = 32;
+  while (lanes < kThreads && lanes * kItems < items) lanes *= 2;
+  const int64_t ctas = ceil_div(p.n, kThreads / lanes);
   auto *fn = p.zero ? (packs ? quantize_w4_kernel<T, kGroup, true, true>
                              : quantize_w4_kernel<T, kGroup, true, false>)
                     : (packs ? quantize_w4_kernel<T, kGroup, false, true>
                              : quantize_w4_kernel<T, kGroup, false, false>);
-  return launch_programmatic(fn, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, s, p, w, items);
+  return launch_programmatic(fn, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0, s, p, w,
+                             lanes);
 }
 
 template <typename T>

@@ -7,6 +7,7 @@
 // Differences to m come first: scale * l alone may leave fp32 (masks of the type's
 // lowest value) or lose the last bits of d, and m with L keeps both for the gradient.
 #include <algorithm>
+#include <type_traits>
 
 #include "act_epilogue.cuh"
 #include "nplk_host.h"
@@ -20,7 +21,7 @@ constexpr float kInf = __builtin_huge_valf(), kLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMostTop = 32;      // alternatives: one a lane
-constexpr int kMostWarps = 16, kMostCluster = 8;
+constexpr int kMostCluster = 8;
 
 // ---------------------------------------------------------------------------
 // Forward: one pass over the logits. A row belongs to a CTA, or to a cluster of up to
@@ -31,10 +32,10 @@ constexpr int kMostWarps = 16, kMostCluster = 8;
 // The alternatives ride along. Each warp keeps the 32 best it has seen, one a lane,
 // ordered by key: the logit's order in the high half, the complemented index in the
 // low one, so that the larger key is the larger logit or, of equal ones, the lower
-// index. What a logit must reach to be looked at is `floor`, the larger of the warp's own
-// n-th key and the least of the warps' ceil(n / warps)-th keys (at least n elements of the
-// row reach that one). It is compared with the largest of a thread's 32 (16) values,
-// which the softmax needs anyway.
+// index. What a logit must reach to be looked at is the larger of the warp's own n-th key and
+// the least of the warps' ceil(n / warps)-th values (n elements of the row reach that
+// one). It is compared with the largest of a thread's 32 (16) values, which the softmax
+// needs anyway.
 // ---------------------------------------------------------------------------
 struct LogprobArgs {
   int64_t rows, ld;
@@ -47,31 +48,47 @@ struct LogprobArgs {
   float *top_logprobs;
 };
 
+// Sums relative to a maximum.
 struct Part {
   float m, s, w;
 };
 
-// Both sums relative to the larger maximum. c = scale * log2 e.
-__device__ __forceinline__ Part join(const Part &a, const Part &b, float c) {
-  Part r;
-  r.m = fmaxf(a.m, b.m);
-  const float base = r.m == -kInf ? 0.0f : r.m;  // nothing but -infinity: u stays -infinity
-  const float ua = at_least(a.m - base, kLowest), ub = at_least(b.m - base, kLowest);
-  const float ea = exp2_approx(ua * c), eb = exp2_approx(ub * c);
-  r.s = a.s * ea + b.s * eb;
+// The part relative to `m`, not below its own maximum. c = scale * log2 e.
+__device__ __forceinline__ Part rebase(const Part &a, float m, float c) {
+  // nothing but -infinity so far: u is -infinity then, as it should be
+  const float u = at_least(a.m - (m == -kInf ? 0.0f : m), kLowest), e = exp2_approx(u * c);
   // u e first: u s may leave fp32 where e is 0
-  r.w = (a.w * ea + ua * ea * a.s) + (b.w * eb + ub * eb * b.s);
-  return r;
+  return {m, a.s * e, a.w * e + u * e * a.s};
 }
 
-__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
-  const uint32_t bits = __float_as_uint(v + 0.0f);  // -0 counts as 0
-  const uint32_t order = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-  return static_cast<uint64_t>(order) << 32 | (0xffffffffu - index);
+// The parts of the 2 * `half` lanes of a group joined, in all of them.
+template <int half>
+__device__ __forceinline__ Part join_lanes(Part a, float c) {
+  float m = a.m;
+#pragma unroll
+  for (int o = half; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+  a = rebase(a, m, c);
+#pragma unroll
+  for (int o = half; o; o >>= 1) {
+    a.s += __shfl_xor_sync(kAll, a.s, o);
+    a.w += __shfl_xor_sync(kAll, a.w, o);
+  }
+  return a;
 }
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t order = static_cast<uint32_t>(key >> 32);
+
+// fp32 values (no NaN) in the order of unsigned integers; -0 counts as 0.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t bits = __float_as_uint(v + 0.0f);
+  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
   return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+  return static_cast<uint64_t>(order_of(v)) << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t key_order(uint64_t key) {
+  return static_cast<uint32_t>(key >> 32);
 }
 __device__ __forceinline__ int64_t key_index(uint64_t key) {
   return 0xffffffffu - static_cast<uint32_t>(key);
@@ -85,15 +102,14 @@ __device__ __forceinline__ void insert(uint64_t &mine, uint64_t key, int lane) {
   if (lane == at) mine = key;
 }
 
-// The rank-th largest (0 the largest) of the lanes' values, none of them NaN.
-__device__ __forceinline__ float ranked(float v, int rank, int lane) {
-  int before = 0;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float other = __shfl_sync(kAll, v, j);
-    before += other > v || (other == v && j < lane);
+// The rank-th largest (0 the largest) of the lanes' values.
+__device__ __forceinline__ uint32_t ranked(uint32_t v, int rank, int lane) {
+  uint32_t most = __reduce_max_sync(kAll, v);
+  for (; rank > 0; --rank) {
+    if (lane == __ffs(__ballot_sync(kAll, v == most)) - 1) v = 0;  // one of them out
+    most = __reduce_max_sync(kAll, v);
   }
-  return __shfl_sync(kAll, v, __ffs(__ballot_sync(kAll, before == rank)) - 1);
+  return most;
 }
 
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
@@ -102,19 +118,32 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
 
 template <typename T>
 struct Batch {
-  static constexpr int E = 16 / sizeof(T), U = 4, kValues = E * U;
+  static constexpr int E = 16 / sizeof(T), U = 4;
   Pack<T, E> p[U];
 };
 
+// Largest value of a pack, NaNs left out: 16-bit types two at a time.
+template <typename T, int E>
+__device__ __forceinline__ float most_of(const Pack<T, E> &p) {
+  if constexpr (std::is_same<T, float>::value) {
+    return fmaxf(fmaxf(p.e[0], p.e[1]), fmaxf(p.e[2], p.e[3]));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2 *v = reinterpret_cast<const T2 *>(&p);
+    const T2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+    return fmaxf(to_float(m.x), to_float(m.y));
+  }
+}
+
 // kTop: with alternatives. The launch's CTAs are whole clusters of `cluster`.
-template <typename T, bool kTop>
-__global__ void __launch_bounds__(kMostWarps * 32)
+template <typename T, bool kTop, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps >= 16 ? 1 : 24 / kWarps)
     token_logprobs_kernel(LogprobArgs p, const T *logits, int cluster) {
   using B = Batch<T>;
-  constexpr int E = B::E, U = B::U;
-  __shared__ Part warp_part[kMostWarps];
-  __shared__ uint64_t lists[kTop ? kMostWarps * kMostTop : 1];
-  __shared__ uint64_t floors[kTop ? kMostWarps : 1];
+  constexpr int E = B::E, U = B::U, kThreads = kWarps * 32;
+  __shared__ Part warp_part[kWarps];
+  __shared__ uint64_t lists[kTop ? kWarps * kMostTop : 1];
+  __shared__ uint32_t floors[kTop ? kWarps : 1];
   // what the cluster's CTAs hand to its first: two rows' worth, so that one barrier a
   // row keeps the next row's writes off this row's reads
   __shared__ Part cta_part[2][kMostCluster];
@@ -123,11 +152,10 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   griddep_wait();
   griddep_launch_dependents();
 
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int threads = blockDim.x, warps = threads >> 5;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(blockIdx.x) % cluster;
   const float c = p.scale * kLog2e;
-  const int share = kTop ? (p.top + warps - 1) / warps : 0;
+  const int share = kTop ? (p.top + kWarps - 1) / kWarps : 0;
   if (cluster > 1) {  // the first CTA has started before anything is stored into it
     cluster_arrive_relaxed();
     cluster_wait();
@@ -145,35 +173,26 @@ __global__ void __launch_bounds__(kMostWarps * 32)
     const T *xp = x + lead;
 
     Part mine{-kInf, 0.0f, 0.0f};
-    uint64_t list = 0, floor = key_of(kLowest, 0xffffffffu);  // lists hold no -infinity
-    float floor_value = kLowest;
-    const auto raise = [&](uint64_t to) {
-      if (to > floor) {
-        floor = to;
-        floor_value = key_value(to);
-      }
-    };
-
-    // one value, or none: lane's own
+    uint64_t list = 0, own = 0;  // this lane's key of the warp's list; the list's n-th
+    float floor = kLowest;       // lists hold no -infinity
+    // one value a lane, or none
     const auto offer = [&](float v, int index, bool here) {
-      uint64_t key = here && v >= floor_value ? key_of(v, index) : 0;
-      unsigned want = __ballot_sync(kAll, key >= floor);
+      const uint64_t key = here && v >= floor ? key_of(v, index) : 0;
+      unsigned want = __ballot_sync(kAll, key > own);
       while (want) {
-        const int src = __ffs(want) - 1;
+        const uint64_t k = __shfl_sync(kAll, key, __ffs(want) - 1);
         want &= want - 1;
-        const uint64_t k = __shfl_sync(kAll, key, src);
-        if (k < floor) continue;
+        if (k <= own) continue;
         insert(list, k, lane);
-        raise(__shfl_sync(kAll, list, p.top - 1));
+        own = __shfl_sync(kAll, list, p.top - 1);
       }
+      if (own) floor = fmaxf(floor, value_of(key_order(own)));
     };
 
-    bool first = true;
-    const int last_batch = j0 + ((j1 - j0) + U * threads - 1) / (U * threads) * (U * threads);
     const auto load = [&](B &b, int j) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = j + u * threads + static_cast<int>(threadIdx.x);
+        const int at = j + u * kThreads + tid;
         if (at < j1) b.p[u] = load_pack<T, E>(xp + static_cast<int64_t>(at) * E);
         else
 #pragma unroll
@@ -181,7 +200,7 @@ __global__ void __launch_bounds__(kMostWarps * 32)
       }
     };
     B next;
-    if (j0 < last_batch) load(next, j0);
+    if (j0 < j1) load(next, j0);
 
     // the lone values, by the first CTA's first warp
     if (rank == 0 && warp == 0) {
@@ -197,20 +216,13 @@ __global__ void __launch_bounds__(kMostWarps * 32)
       if (kTop) offer(v, index, here);
     }
 
-    for (int j = j0; j < last_batch; j += U * threads) {
+    for (int j = j0; j < j1; j += U * kThreads) {
       const B now = next;
-      if (j + U * threads < last_batch) load(next, j + U * threads);
+      if (j + U * kThreads < j1) load(next, j + U * kThreads);
       float most = -kInf;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e) most = fmaxf(most, to_float(now.p[u].e[e]));
-      if (most > mine.m) {
-        const float u = at_least(mine.m - most, kLowest), e = exp2_approx(u * c);
-        mine.w = mine.w * e + u * e * mine.s;
-        mine.s *= e;
-        mine.m = most;
-      }
+      for (int u = 0; u < U; ++u) most = fmaxf(most, most_of(now.p[u]));
+      if (most > mine.m) mine = rebase(mine, most, c);
       const float2 base = both(mine.m == -kInf ? 0.0f : -mine.m), cc = both(c);
       float2 s = make_float2(0.0f, 0.0f), w = s;
 #pragma unroll
@@ -229,70 +241,55 @@ __global__ void __launch_bounds__(kMostWarps * 32)
       mine.s += s.x + s.y;
       mine.w += w.x + w.y;
       if constexpr (kTop) {
-        if (first) {
+        if (j == j0) {
           // n elements reach the least of the warps' share-th largest: each is the
           // maximum of another thread's values
-          const uint64_t reach = key_of(ranked(most, share - 1, lane), 0xffffffffu);
+          const uint32_t reach = ranked(order_of(most), share - 1, lane);
           if (lane == 0) floors[warp] = reach;
           __syncthreads();
-          uint64_t least = floors[0];
-          for (int i = 1; i < warps; ++i) least = min(least, floors[i]);
-          raise(least);
-          first = false;
-        } else {
-          uint64_t least = *reinterpret_cast<volatile uint64_t *>(&floors[0]);
-          for (int i = 1; i < warps; ++i)
-            least = min(least, *reinterpret_cast<volatile uint64_t *>(&floors[i]));
-          raise(__shfl_sync(kAll, least, 0));  // the lanes may have read at different times
         }
-        unsigned some = __ballot_sync(kAll, most >= floor_value);
+        const uint32_t floor_of =
+            lane < kWarps ? *reinterpret_cast<volatile uint32_t *>(&floors[lane]) : 0xffffffffu;
+        floor = fmaxf(floor, value_of(__reduce_min_sync(kAll, floor_of)));
+        const unsigned some = __ballot_sync(kAll, most >= floor);
         if (some) {
           // many at once (rising logits): the n-th of the lanes' maxima first
-          if (__popc(some) > 8 && __popc(some) >= p.top) {
-            raise(key_of(ranked(most, p.top - 1, lane), 0xffffffffu));
-          }
+          if (__popc(some) > 8 && __popc(some) >= p.top)
+            floor = fmaxf(floor, value_of(ranked(order_of(most), p.top - 1, lane)));
           uint32_t mask = 0;
 #pragma unroll
           for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < E; ++e)
-              mask |= static_cast<uint32_t>(to_float(now.p[u].e[e]) >= floor_value) << (u * E + e);
+              mask |= static_cast<uint32_t>(to_float(now.p[u].e[e]) >= floor) << (u * E + e);
           while (__any_sync(kAll, mask != 0)) {
             const int bit = __ffs(mask) - 1;
-            const int at = j + bit / E * threads + static_cast<int>(threadIdx.x);
-            const int index = lead + at * E + bit % E;
+            const int index = lead + (j + bit / E * kThreads + tid) * E + bit % E;
             offer(mask ? to_float(x[index]) : 0.0f, index, mask != 0);
             mask &= mask - 1;
           }
-          const uint64_t reach = __shfl_sync(kAll, list, share - 1);
+          const uint32_t reach = key_order(__shfl_sync(kAll, list, share - 1));
           if (lane == 0 && reach > floors[warp])
-            *reinterpret_cast<volatile uint64_t *>(&floors[warp]) = reach;
+            *reinterpret_cast<volatile uint32_t *>(&floors[warp]) = reach;
         }
       }
     }
 
     // the warp's, then the CTA's, then the cluster's sums
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      Part other;
-      other.m = __shfl_xor_sync(kAll, mine.m, o);
-      other.s = __shfl_xor_sync(kAll, mine.s, o);
-      other.w = __shfl_xor_sync(kAll, mine.w, o);
-      mine = join(mine, other, c);
-    }
+    mine = join_lanes<16>(mine, c);
     if (lane == 0) warp_part[warp] = mine;
     if (kTop) lists[warp * kMostTop + lane] = list;
-    if (kTop && threadIdx.x < kMostTop) best[threadIdx.x] = 0;
+    if (kTop && tid < kMostTop) best[tid] = 0;
     __syncthreads();
     // the place of each key among all: those above it in its own list, and in the others
     const auto merge = [&](const uint64_t *from, int count) {
-      for (int i = threadIdx.x; i < count * kMostTop; i += threads) {
-        const int own = i / kMostTop;
+      for (int i = tid; i < count * kMostTop; i += kThreads) {
+        const int mine_at = i / kMostTop;
         const uint64_t key = from[i];
         int place = i % kMostTop;
         if (key == 0 || place >= p.top) continue;
         for (int l = 0; l < count && place < p.top; ++l) {
-          if (l == own) continue;
+          if (l == mine_at) continue;
           const uint64_t *other = from + l * kMostTop;
           for (int k = 0; k < p.top && other[k] > key; ++k) ++place;
         }
@@ -300,54 +297,67 @@ __global__ void __launch_bounds__(kMostWarps * 32)
       }
       __syncthreads();
     };
-    if (kTop) merge(lists, warps);
-    Part total = warp_part[0];
-    for (int i = 1; i < warps; ++i) total = join(total, warp_part[i], c);
+    if (kTop) merge(lists, kWarps);
+    Part total{-kInf, 0.0f, 0.0f};
+    if (warp == 0) {
+      if (lane < kWarps) total = warp_part[lane];
+      total = join_lanes<kWarps / 2>(total, c);
+    }
     if (cluster > 1) {
-      if (threadIdx.x == 0) {
+      if (tid == 0) {
         const uint32_t to = mapa_shared(smem_u32(&cta_part[parity][rank]), 0u);
         st_shared_cluster_f32(to, total.m);
         st_shared_cluster_f32(to + 4, total.s);
         st_shared_cluster_f32(to + 8, total.w);
       }
-      if (kTop && threadIdx.x < kMostTop)
-        st_cluster_u64(mapa_shared(smem_u32(&cta_list[parity][rank * kMostTop + threadIdx.x]), 0u),
-                       best[threadIdx.x]);
+      if (kTop && tid < kMostTop)
+        st_cluster_u64(mapa_shared(smem_u32(&cta_list[parity][rank * kMostTop + tid]), 0u),
+                       best[tid]);
       cluster_sync();
       if (rank != 0) continue;
-      total = cta_part[parity][0];
-      for (int i = 1; i < cluster; ++i) total = join(total, cta_part[parity][i], c);
+      if (warp == 0) {
+        total = lane < cluster ? cta_part[parity][lane] : Part{-kInf, 0.0f, 0.0f};
+        total = join_lanes<kMostCluster / 2>(total, c);
+      }
       if (kTop) {
-        if (threadIdx.x < kMostTop) best[threadIdx.x] = 0;
+        if (tid < kMostTop) best[tid] = 0;
         __syncthreads();
         merge(cta_list[parity], cluster);
       }
     }
-    const float log_sum = logf(total.s);
-    const bool bad = total.s != total.s;  // a NaN or +infinity in the row
-    if (threadIdx.x == 0) {
-      if (p.stats) {
-        p.stats[2 * row] = total.m;
-        p.stats[2 * row + 1] = log_sum;
+    if (warp == 0) {
+      if (kWarps < 32) {  // what lane 0 has
+        total.m = __shfl_sync(kAll, total.m, 0);
+        total.s = __shfl_sync(kAll, total.s, 0);
+        total.w = __shfl_sync(kAll, total.w, 0);
       }
-      if (p.entropy)
-        p.entropy[row] = total.s == 0.0f ? 0.0f : log_sum - p.scale * (total.w / total.s);
-      if (p.logprob) {
-        const int64_t t = p.targets[row];
-        float v = 0.0f;
-        if (t >= 0 && t < p.vocab) {
-          const float l = to_float(x[t]);
-          v = bad ? log_sum : l == -kInf ? -kInf : fmaf(l - total.m, p.scale, -log_sum);
+      const float log_sum = logf(total.s);
+      const bool bad = total.s != total.s;  // a NaN or +infinity in the row
+      if (lane == 0) {
+        if (p.stats) {
+          p.stats[2 * row] = total.m;
+          p.stats[2 * row + 1] = log_sum;
         }
-        p.logprob[row] = v;
+        if (p.entropy)
+          p.entropy[row] = total.s == 0.0f ? 0.0f : log_sum - p.scale * (total.w / total.s);
+        if (p.logprob) {
+          const int64_t t = p.targets[row];
+          float v = 0.0f;
+          if (t >= 0 && t < p.vocab) {
+            const float l = to_float(x[t]);
+            v = bad ? log_sum : l == -kInf ? -kInf : fmaf(l - total.m, p.scale, -log_sum);
+          }
+          p.logprob[row] = v;
+        }
       }
-    }
-    if (kTop && static_cast<int>(threadIdx.x) < p.top) {
-      const uint64_t key = best[threadIdx.x];
-      const int64_t to = row * p.top + threadIdx.x;
-      p.top_ids[to] = key && !bad ? key_index(key) : -1;
-      p.top_logprobs[to] =
-          bad ? log_sum : key ? fmaf(key_value(key) - total.m, p.scale, -log_sum) : -kInf;
+      if (kTop && lane < p.top) {
+        const uint64_t key = best[lane];
+        const int64_t to = row * p.top + lane;
+        p.top_ids[to] = key && !bad ? key_index(key) : -1;
+        p.top_logprobs[to] = bad ? log_sum
+                             : key ? fmaf(value_of(key_order(key)) - total.m, p.scale, -log_sum)
+                                   : -kInf;
+      }
     }
     __syncthreads();  // the next row's floors, lists and best
   }
@@ -449,18 +459,30 @@ __global__ void __launch_bounds__(kGradThreads)
 }
 
 template <typename T>
+auto pick_forward(bool top, int warps) {
+  switch (warps) {
+    case 1:
+      return top ? token_logprobs_kernel<T, true, 1> : token_logprobs_kernel<T, false, 1>;
+    case 4:
+      return top ? token_logprobs_kernel<T, true, 4> : token_logprobs_kernel<T, false, 4>;
+    default:
+      return top ? token_logprobs_kernel<T, true, 16> : token_logprobs_kernel<T, false, 16>;
+  }
+}
+
+// One warp for rows of up to two batches, else four, with 16 where rows do not fill the SMs;
+// then clusters too, while each CTA has two packs a thread.
+template <typename T>
 int run_forward(cudaStream_t s, const LogprobArgs &p, const T *logits) {
   constexpr int E = 16 / sizeof(T), U = Batch<T>::U;
   const int64_t packs = std::max(1, p.vocab / E), sms = sm_count();
+  const int warps = packs <= 2 * 32 * U ? 1 : p.rows <= 2 * sms ? 16 : 4;
   int cluster = 1;
-  while (cluster < kMostCluster && p.rows * cluster * 2 <= sms &&
-         packs >= 2 * cluster * 2 * 32 * U)
+  while (warps == 16 && cluster < kMostCluster && p.rows * cluster * 2 <= sms &&
+         packs >= 2 * cluster * 16 * 32 * 2)
     cluster *= 2;
-  int warps = 1;
-  while (warps < (p.rows * cluster <= sms ? 16 : 8) && ceil_div(packs, cluster) > warps * 32)
-    warps *= 2;
-  const int64_t rows = std::min<int64_t>(p.rows, sms * 32);
-  auto *fn = p.top > 0 ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>;
+  const int64_t rows = std::min<int64_t>(p.rows, sms * 128);
+  auto *fn = pick_forward<T>(p.top > 0, warps);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
