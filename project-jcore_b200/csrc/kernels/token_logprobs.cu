@@ -22,20 +22,25 @@ constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMostTop = 32;      // alternatives: one a lane
 constexpr int kMostCluster = 8;
+constexpr int kNotes = 128;       // batches a warp can note: it makes room above kNotes - 32
+constexpr int kCandidates = 512;  // elements put in order at a time
+constexpr int kTidBits = 9;       // of a note: order of the maximum, complemented batch, thread
 
 // ---------------------------------------------------------------------------
 // Forward: one pass over the logits. A row belongs to a CTA, or to a cluster of up to
 // 8 where there are fewer rows than SMs; a thread takes every (threads)-th 16-byte
 // pack and keeps its own maximum and sums, which it rescales when the maximum
-// grows: with u = l - m (its own m) s = sum e^(scale u), w = sum e^(scale u) u.
+// grows: with t = scale (l - m) log2 e (its own m) s = sum 2^t, w = sum 2^t t.
 //
-// The alternatives ride along. Each warp keeps the 32 best it has seen, one a lane,
-// ordered by key: the logit's order in the high half, the complemented index in the
-// low one, so that the larger key is the larger logit or, of equal ones, the lower
-// index. What a logit must reach to be looked at is the larger of the warp's own n-th key and
-// the least of the warps' ceil(n / warps)-th values (n elements of the row reach that
-// one). It is compared with the largest of a thread's 32 (16) values, which the softmax
-// needs anyway.
+// The alternatives ride along. A floor that n elements of the row reach is known from the
+// first batches on: the least of the warps' ceil(n / warps)-th largest thread maxima (it
+// rises with later batches). A thread whose batch reaches the floor notes that batch, in shared memory,
+// and the row's end reads the noted batches again (few more than n), takes the elements
+// that reach the floor and puts them in order as keys: the logit's order in the high half, the complemented
+// index in the low one, so that the larger key is the larger logit or, of equal ones, the
+// lower index. All that the loop has to compare is a thread's largest value of 64
+// (32), which the softmax needs anyway. (Elements put in order on the way took 30 to 60 us
+// more than no alternatives, 45 us, at 2048 x 50021 fp16.)
 // ---------------------------------------------------------------------------
 struct LogprobArgs {
   int64_t rows, ld;
@@ -55,10 +60,11 @@ struct Part {
 
 // The part relative to `m`, not below its own maximum. c = scale * log2 e.
 __device__ __forceinline__ Part rebase(const Part &a, float m, float c) {
-  // nothing but -infinity so far: u is -infinity then, as it should be
-  const float u = at_least(a.m - (m == -kInf ? 0.0f : m), kLowest), e = exp2_approx(u * c);
-  // u e first: u s may leave fp32 where e is 0
-  return {m, a.s * e, a.w * e + u * e * a.s};
+  // nothing but -infinity so far: d is -infinity then, kept finite
+  const float u = at_least(a.m - (m == -kInf ? 0.0f : m), kLowest);
+  const float d = at_least(u * c, kLowest), e = exp2_approx(d);
+  // d e first: d s may leave fp32 where e is 0
+  return {m, a.s * e, a.w * e + d * e * a.s};
 }
 
 // The parts of the 2 * `half` lanes of a group joined, in all of them.
@@ -94,14 +100,6 @@ __device__ __forceinline__ int64_t key_index(uint64_t key) {
   return 0xffffffffu - static_cast<uint32_t>(key);
 }
 
-// Puts `key` (the same in all lanes) in its place of the warp's descending list.
-__device__ __forceinline__ void insert(uint64_t &mine, uint64_t key, int lane) {
-  const int at = __popc(__ballot_sync(kAll, mine > key));
-  const uint64_t above = __shfl_up_sync(kAll, mine, 1);
-  if (lane > at) mine = above;
-  if (lane == at) mine = key;
-}
-
 // The rank-th largest (0 the largest) of the lanes' values.
 __device__ __forceinline__ uint32_t ranked(uint32_t v, int rank, int lane) {
   uint32_t most = __reduce_max_sync(kAll, v);
@@ -118,7 +116,7 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
 
 template <typename T>
 struct Batch {
-  static constexpr int E = 16 / sizeof(T), U = 4;
+  static constexpr int E = 16 / sizeof(T), U = 8;
   Pack<T, E> p[U];
 };
 
@@ -135,20 +133,40 @@ __device__ __forceinline__ float most_of(const Pack<T, E> &p) {
   }
 }
 
+// The sums of a thread's batch with its first pack at `at`, differences first and each
+// of them kept finite.
+template <typename T, int kThreads>
+__device__ __noinline__ Part careful_sums(const T *x, int lead, int at, int end, float base, float c) {
+  constexpr int E = Batch<T>::E, U = Batch<T>::U;
+  Part r{base, 0.0f, 0.0f};
+  for (int u = 0; u < U && at + u * kThreads < end; ++u)
+    for (int e = 0; e < E; ++e) {
+      const float l = to_float(x[lead + (at + u * kThreads) * E + e]);
+      const float d = at_least(at_least(l - base, kLowest) * c, kLowest);
+      const float v = exp2_approx(d);
+      r.s += v;
+      r.w += v * d;
+    }
+  return r;
+}
+
 // kTop: with alternatives. The launch's CTAs are whole clusters of `cluster`.
 template <typename T, bool kTop, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, kWarps >= 16 ? 1 : 24 / kWarps)
+__global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
     token_logprobs_kernel(LogprobArgs p, const T *logits, int cluster) {
   using B = Batch<T>;
   constexpr int E = B::E, U = B::U, kThreads = kWarps * 32;
+  static_assert(kThreads <= 1 << kTidBits && kMostCluster * kMostTop <= kCandidates, "notes, keys");
   __shared__ Part warp_part[kWarps];
-  __shared__ uint64_t lists[kTop ? kWarps * kMostTop : 1];
+  __shared__ uint64_t notes[kTop ? kWarps * kNotes : 1];
   __shared__ uint32_t floors[kTop ? kWarps : 1];
   // what the cluster's CTAs hand to its first: two rows' worth, so that one barrier a
   // row keeps the next row's writes off this row's reads
   __shared__ Part cta_part[2][kMostCluster];
   __shared__ uint64_t cta_list[2][kTop ? kMostCluster * kMostTop : 1];
   __shared__ uint64_t best[kMostTop];
+  __shared__ uint64_t candidates[kTop ? kCandidates : 1];
+  __shared__ int found;
   griddep_wait();
   griddep_launch_dependents();
 
@@ -173,104 +191,145 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 16 ? 1 : 24 / kWarps)
     const T *xp = x + lead;
 
     Part mine{-kInf, 0.0f, 0.0f};
-    uint64_t list = 0, own = 0;  // this lane's key of the warp's list; the list's n-th
-    float floor = kLowest;       // lists hold no -infinity
-    // one value a lane, or none
-    const auto offer = [&](float v, int index, bool here) {
-      const uint64_t key = here && v >= floor ? key_of(v, index) : 0;
-      unsigned want = __ballot_sync(kAll, key > own);
-      while (want) {
-        const uint64_t k = __shfl_sync(kAll, key, __ffs(want) - 1);
-        want &= want - 1;
-        if (k <= own) continue;
-        insert(list, k, lane);
-        own = __shfl_sync(kAll, list, p.top - 1);
+    float floor = kLowest;  // no -infinity among the alternatives
+    int count = 0, held = 0;  // notes; those that reach the floor since it rose
+    uint64_t *noted = notes + (kTop ? warp * kNotes : 0);
+    // The n best notes, by maximum and then by batch: the batches of a CTA follow one
+    // another, so of equal maxima the earlier batch's counts, and those of one batch stay together.
+    const auto make_room = [&] {
+      __syncwarp();
+      uint64_t note[kNotes / 32];
+      int place[kNotes / 32];
+#pragma unroll
+      for (int i = 0; i < kNotes / 32; ++i) {
+        note[i] = i * 32 + lane < count ? noted[i * 32 + lane] : 0;
+        place[i] = note[i] ? 0 : kNotes;
       }
-      if (own) floor = fmaxf(floor, value_of(key_order(own)));
+      for (int k = 0; k < count; ++k) {
+        const uint64_t other = noted[k] >> kTidBits;
+#pragma unroll
+        for (int i = 0; i < kNotes / 32; ++i) place[i] += other > note[i] >> kTidBits;
+      }
+      __syncwarp();
+      uint32_t least = 0xffffffffu;
+      count = 0;
+#pragma unroll
+      for (int i = 0; i < kNotes / 32; ++i) {
+        const bool keep = place[i] < p.top;
+        const unsigned kept = __ballot_sync(kAll, keep);
+        if (keep) {
+          noted[count + __popc(kept & ((1u << lane) - 1u))] = note[i];
+          least = min(least, static_cast<uint32_t>(note[i] >> 32));
+        }
+        count += __popc(kept);
+      }
+      __syncwarp();
+      floor = fmaxf(floor, value_of(__reduce_min_sync(kAll, least)));
+      held = count;  // at least n
     };
 
-    const auto load = [&](B &b, int j) {
+    const auto load = [&](B &b, int j, int here) {
+      const T *from = xp + static_cast<int64_t>(j + tid) * E;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = j + u * kThreads + tid;
-        if (at < j1) b.p[u] = load_pack<T, E>(xp + static_cast<int64_t>(at) * E);
-        else
-#pragma unroll
-          for (int e = 0; e < E; ++e) b.p[u].e[e] = from_float<T>(-kInf);
-      }
+      for (int u = 0; u < U; ++u)
+        if (u < here) b.p[u] = load_pack<T, E>(from + u * (kThreads * E));
     };
-    B next;
-    if (j0 < j1) load(next, j0);
 
     // the lone values, by the first CTA's first warp
-    if (rank == 0 && warp == 0) {
-      const bool here = lane < lead + p.vocab - tail;
-      const int index = lane < lead ? lane : tail + lane - lead;
-      const float v = here ? to_float(x[index]) : -kInf;
-      if (here) {
-        mine.m = v == v ? v : -kInf;  // the maximum of a NaN and nothing
-        const float u = at_least(v - (mine.m == -kInf ? 0.0f : mine.m), kLowest);
-        mine.s = exp2_approx(u * c);
-        mine.w = mine.s * u;
-      }
-      if (kTop) offer(v, index, here);
+    const int lone_index = lane < lead ? lane : tail + lane - lead;
+    const bool lone = rank == 0 && warp == 0 && lane < lead + p.vocab - tail;
+    const float lone_value = lone ? to_float(x[lone_index]) : -kInf;
+    if (lone) {
+      mine.m = fmaxf(lone_value, -kInf);  // the maximum of a NaN and nothing
+      const float u = at_least(lone_value - (mine.m == -kInf ? 0.0f : mine.m), kLowest);
+      const float d = at_least(u * c, kLowest);
+      mine.s = exp2_approx(d);
+      mine.w = mine.s * d;
     }
 
-    for (int j = j0; j < j1; j += U * kThreads) {
-      const B now = next;
-      if (j + U * kThreads < j1) load(next, j + U * kThreads);
+    for (int j = j0, batch = 0; j < j1; j += U * kThreads, ++batch) {
+      B now;
+      const bool whole = j + U * kThreads <= j1;
+      const int here = min(U, (j1 - j - tid + kThreads - 1) / kThreads);  // packs of this thread
+      load(now, j, whole ? U : here);
       float most = -kInf;
 #pragma unroll
-      for (int u = 0; u < U; ++u) most = fmaxf(most, most_of(now.p[u]));
+      for (int u = 0; u < U; ++u)
+        if (whole || u < here) most = fmaxf(most, most_of(now.p[u]));
       if (most > mine.m) mine = rebase(mine, most, c);
-      const float2 base = both(mine.m == -kInf ? 0.0f : -mine.m), cc = both(c);
-      float2 s = make_float2(0.0f, 0.0f), w = s;
+      const float base = mine.m == -kInf ? 0.0f : mine.m;
+      // t = l c - m c in one fused step: m c rounds, by `off`, the same for all, which comes out
+      // of the sums afterwards (2^off within its first two terms: |off| < 2^-24 |m c|)
+      const float bc = base * c, off = fmaf(base, c, -bc);
+      float s[2] = {}, w[2] = {};
+      const auto add = [&](const Pack<T, E> &v) {
 #pragma unroll
-      for (int q = 0; q < U; ++q) {
-        float2 v[E / 2];
-        unpack_pairs(now.p[q], v);
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
-          const float2 u = at_least(add2(v[e], base), kLowest);
-          const float2 t = mul2(u, cc);
-          const float2 r = make_float2(exp2_approx(t.x), exp2_approx(t.y));
-          s = add2(s, r);
-          w = fma2(r, u, w);
+        for (int e = 0; e < E; ++e) {
+          const float t = fmaf(to_float(v.e[e]), c, -bc);
+          const float r = exp2_approx(t);
+          s[e & 1] += r;
+          w[e & 1] = fmaf(r, t, w[e & 1]);
         }
+      };
+      if (whole) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(now.p[u]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < here) add(now.p[u]);
       }
-      mine.s += s.x + s.y;
-      mine.w += w.x + w.y;
+      s[0] += s[1];
+      w[0] += w[1];
+      const float back = 1.0f - off * kLn2;
+      Part sum{base, s[0] * back, fmaf(-off, s[0], w[0]) * back};
+      // masked logits (0 times -infinity), and maxima that l c or m c would not fit
+      if ((w[0] != w[0] && s[0] == s[0]) || fabsf(bc) > 1e30f)
+        sum = careful_sums<T, kThreads>(x, lead, j + tid, j1, base, c);
+      mine.s += sum.s;
+      mine.w += sum.w;
       if constexpr (kTop) {
-        if (j == j0) {
+        volatile uint32_t *shared_floors = floors;
+        if (batch == 0) {
           // n elements reach the least of the warps' share-th largest: each is the
           // maximum of another thread's values
           const uint32_t reach = ranked(order_of(most), share - 1, lane);
-          if (lane == 0) floors[warp] = reach;
+          if (lane == 0) shared_floors[warp] = reach;
           __syncthreads();
         }
-        const uint32_t floor_of =
-            lane < kWarps ? *reinterpret_cast<volatile uint32_t *>(&floors[lane]) : 0xffffffffu;
-        floor = fmaxf(floor, value_of(__reduce_min_sync(kAll, floor_of)));
-        const unsigned some = __ballot_sync(kAll, most >= floor);
+        const float least = value_of(
+            __reduce_min_sync(kAll, lane < kWarps ? shared_floors[lane] : 0xffffffffu));
+        if (least > floor) {
+          floor = least;
+          held = 0;
+        }
+        unsigned some = __ballot_sync(kAll, most >= floor);
         if (some) {
           // many at once (rising logits): the n-th of the lanes' maxima first
-          if (__popc(some) > 8 && __popc(some) >= p.top)
-            floor = fmaxf(floor, value_of(ranked(order_of(most), p.top - 1, lane)));
-          uint32_t mask = 0;
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              mask |= static_cast<uint32_t>(to_float(now.p[u].e[e]) >= floor) << (u * E + e);
-          while (__any_sync(kAll, mask != 0)) {
-            const int bit = __ffs(mask) - 1;
-            const int index = lead + (j + bit / E * kThreads + tid) * E + bit % E;
-            offer(mask ? to_float(x[index]) : 0.0f, index, mask != 0);
-            mask &= mask - 1;
+          if (__popc(some) > 8 && __popc(some) >= p.top) {
+            const float higher = value_of(ranked(order_of(most), p.top - 1, lane));
+            if (higher > floor) {
+              floor = higher;
+              held = 0;
+              some = __ballot_sync(kAll, most >= floor);
+            }
           }
-          const uint32_t reach = key_order(__shfl_sync(kAll, list, share - 1));
-          if (lane == 0 && reach > floors[warp])
-            *reinterpret_cast<volatile uint32_t *>(&floors[warp]) = reach;
+          if (most >= floor)
+            noted[count + __popc(some & ((1u << lane) - 1u))] =
+                static_cast<uint64_t>(order_of(most)) << 32 |
+                (0x7fffffu - static_cast<uint32_t>(batch)) << kTidBits | static_cast<uint32_t>(tid);
+          count += __popc(some);
+          held += __popc(some);
+          if (batch > 0 && __popc(some) >= share) {
+            const uint32_t reach = ranked(order_of(most), share - 1, lane);
+            if (lane == 0 && reach > shared_floors[warp]) shared_floors[warp] = reach;
+          }
+          if (count > kNotes - 32) make_room();
+          // n elements at or above the floor, all left of what comes: equal ones no longer count
+          if (held >= p.top) {
+            floor = value_of(order_of(floor) + 1);
+            held = 0;
+          }
         }
       }
     }
@@ -278,26 +337,64 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 16 ? 1 : 24 / kWarps)
     // the warp's, then the CTA's, then the cluster's sums
     mine = join_lanes<16>(mine, c);
     if (lane == 0) warp_part[warp] = mine;
-    if (kTop) lists[warp * kMostTop + lane] = list;
-    if (kTop && tid < kMostTop) best[tid] = 0;
     __syncthreads();
-    // the place of each key among all: those above it in its own list, and in the others
-    const auto merge = [&](const uint64_t *from, int count) {
-      for (int i = tid; i < count * kMostTop; i += kThreads) {
-        const int mine_at = i / kMostTop;
-        const uint64_t key = from[i];
-        int place = i % kMostTop;
-        if (key == 0 || place >= p.top) continue;
-        for (int l = 0; l < count && place < p.top; ++l) {
-          if (l == mine_at) continue;
-          const uint64_t *other = from + l * kMostTop;
-          for (int k = 0; k < p.top && other[k] > key; ++k) ++place;
+    // Keys that reach a bound come together, and each takes the place that the number above
+    // it gives. Where they are too many (long runs of equal logits), the n-th of some of them
+    // is a better bound, and they come together again.
+    const auto in_order = [&](uint64_t bound, auto gather) {
+      for (;;) {
+        if (tid == 0) found = 0;
+        if (tid < kMostTop) best[tid] = 0;
+        __syncthreads();
+        gather([&](uint64_t key) {
+          if (key < bound) return;
+          const int at = atomicAdd(&found, 1);
+          if (at < kCandidates) candidates[at] = key;
+        });
+        __syncthreads();
+        const int all = found, n = min(all, kCandidates);
+        for (int i = tid; i < n; i += kThreads) {
+          const uint64_t key = candidates[i];
+          int place = 0;
+#pragma unroll 8
+          for (int k = 0; k < n; ++k) place += candidates[k] > key;
+          if (place < p.top) best[place] = key;
         }
-        if (place < p.top) best[place] = key;
+        __syncthreads();
+        if (all <= kCandidates) break;
+        bound = best[p.top - 1];
+        __syncthreads();
       }
-      __syncthreads();
     };
-    if (kTop) merge(lists, kWarps);
+    if constexpr (kTop) {
+      uint32_t least = order_of(kLowest);
+      if (j0 < j1) {
+        uint32_t of = floors[0];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) of = min(of, floors[i]);
+        least = max(least, of);
+      }
+      const float least_value = value_of(least);
+      in_order(static_cast<uint64_t>(least) << 32, [&](auto take) {
+        if (lone && lone_value >= least_value) take(key_of(lone_value, lone_index));
+        // eight lanes to a noted batch, a pack each
+        static_assert(U == 8, "a batch's packs");
+        for (int i = lane >> 3; i < count; i += 4) {
+          const uint64_t note = noted[i];
+          if (static_cast<uint32_t>(note >> 32) < least) continue;
+          const int batch = static_cast<int>(0x7fffffu - (static_cast<uint32_t>(note) >> kTidBits));
+          const int at = j0 + batch * (U * kThreads) + (lane & 7) * kThreads +
+                         static_cast<int>(note & ((1u << kTidBits) - 1u));
+          if (at >= j1) continue;
+          const Pack<T, E> v = load_pack<T, E>(xp + static_cast<int64_t>(at) * E);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float f = to_float(v.e[e]);
+            if (f >= least_value) take(key_of(f, static_cast<uint32_t>(lead + at * E + e)));
+          }
+        }
+      });
+    }
     Part total{-kInf, 0.0f, 0.0f};
     if (warp == 0) {
       if (lane < kWarps) total = warp_part[lane];
@@ -319,10 +416,13 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 16 ? 1 : 24 / kWarps)
         total = lane < cluster ? cta_part[parity][lane] : Part{-kInf, 0.0f, 0.0f};
         total = join_lanes<kMostCluster / 2>(total, c);
       }
-      if (kTop) {
-        if (tid < kMostTop) best[tid] = 0;
-        __syncthreads();
-        merge(cta_list[parity], cluster);
+      if constexpr (kTop) {
+        uint64_t most = 0;  // n keys reach any CTA's n-th
+        for (int i = 0; i < cluster; ++i)
+          most = max(most, cta_list[parity][i * kMostTop + p.top - 1]);
+        in_order(max(most, uint64_t(1)), [&](auto take) {
+          for (int i = tid; i < cluster * kMostTop; i += kThreads) take(cta_list[parity][i]);
+        });
       }
     }
     if (warp == 0) {
@@ -339,7 +439,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps >= 16 ? 1 : 24 / kWarps)
           p.stats[2 * row + 1] = log_sum;
         }
         if (p.entropy)
-          p.entropy[row] = total.s == 0.0f ? 0.0f : log_sum - p.scale * (total.w / total.s);
+          p.entropy[row] = total.s == 0.0f ? 0.0f : log_sum - kLn2 * (total.w / total.s);
         if (p.logprob) {
           const int64_t t = p.targets[row];
           float v = 0.0f;
