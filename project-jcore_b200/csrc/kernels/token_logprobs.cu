@@ -22,9 +22,8 @@ constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMostTop = 32;      // alternatives: one a lane
 constexpr int kMostCluster = 8;
-constexpr int kNotes = 128;       // batches a warp can note: it makes room above kNotes - 32
-constexpr int kCandidates = 512;  // elements put in order at a time
-constexpr int kTidBits = 9;       // of a note: order of the maximum, complemented batch, thread
+constexpr int kCandidates = 512;  // keys put in order at a time
+constexpr int kTidBits = 9;       // of a batch's key: order of the maximum, complemented batch, thread
 
 // ---------------------------------------------------------------------------
 // Forward: one pass over the logits. A row belongs to a CTA, or to a cluster of up to
@@ -32,15 +31,14 @@ constexpr int kTidBits = 9;       // of a note: order of the maximum, complement
 // pack and keeps its own maximum and sums, which it rescales when the maximum
 // grows: with t = scale (l - m) log2 e (its own m) s = sum 2^t, w = sum 2^t t.
 //
-// The alternatives ride along. A floor that n elements of the row reach is known from the
-// first batches on: the least of the warps' ceil(n / warps)-th largest thread maxima (it
-// rises with later batches). A thread whose batch reaches the floor notes that batch, in shared memory,
-// and the row's end reads the noted batches again (few more than n), takes the elements
-// that reach the floor and puts them in order as keys: the logit's order in the high half, the complemented
-// index in the low one, so that the larger key is the larger logit or, of equal ones, the
-// lower index. All that the loop has to compare is a thread's largest value of 64
-// (32), which the softmax needs anyway. (Elements put in order on the way took 30 to 60 us
-// more than no alternatives, 45 us, at 2048 x 50021 fp16.)
+// The alternatives: a thread's batch is 64 (32) values, whose largest the softmax needs
+// anyway; the loop only leaves it in shared memory. The n best elements lie in the n
+// batches of largest maxima (of equal ones, those further left), so at the row's end
+// those batches are found, read again, and their elements put in order as keys: the
+// logit's order in the high half, the complemented index in the low one, so that the larger
+// key is the larger logit or, of equal ones, the lower index. (Elements put in order on the way took
+// 30 to 70 us more than no alternatives, 43 us, at 2048 x 50021 fp16; batches noted on
+// the way against a rising floor 20 to 70.)
 // ---------------------------------------------------------------------------
 struct LogprobArgs {
   int64_t rows, ld;
@@ -150,30 +148,136 @@ __device__ __noinline__ Part careful_sums(const T *x, int lead, int at, int end,
   return r;
 }
 
+template <int kThreads>
+struct Shelf {
+  // maxima of thread batches, kept until they are looked through
+  static constexpr int kMaxima = kThreads < 128 ? 32 * kThreads : 4096;
+  uint64_t candidates[kCandidates], best[kMostTop];
+  uint64_t carried[kMostTop];             // the best of what came before
+  float maxima[kMaxima];
+  uint32_t batches[kMostTop + kThreads];  // those to be read again
+  uint32_t floors[kThreads / 32];
+  int found;
+};
+
+// Keys that reach a bound come together, and each takes the place that the number above
+// it gives. Where they are too many (long runs of equal logits), the n-th of some of them
+// is a better bound, and they come together again.
+template <int kThreads, typename Gather>
+__device__ __forceinline__ void in_order(Shelf<kThreads> &shelf, int top, uint64_t bound,
+                                         Gather gather) {
+  const int tid = static_cast<int>(threadIdx.x);
+  for (;;) {
+    if (tid == 0) shelf.found = 0;
+    if (tid < kMostTop) shelf.best[tid] = 0;
+    __syncthreads();
+    gather([&](uint64_t key) {
+      if (key < bound) return;
+      const int at = atomicAdd(&shelf.found, 1);
+      if (at < kCandidates) shelf.candidates[at] = key;
+    });
+    __syncthreads();
+    const int all = shelf.found, n = min(all, kCandidates);
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t key = shelf.candidates[i];
+      int place = 0;
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) place += shelf.candidates[k] > key;
+      if (place < top) shelf.best[place] = key;
+    }
+    __syncthreads();
+    if (all <= kCandidates) return;
+    bound = shelf.best[top - 1];
+    __syncthreads();
+  }
+}
+
+// The n best of what came before, the lone values and the packs [from, end), whose batches'
+// maxima are in the shelf: in order in shelf.best, and carried. Out of line: the loop
+// keeps its registers.
+template <typename T, int kWarps>
+__device__ __noinline__ void collect(const T *xp, int from, int end, int lead, float lone_value,
+                                     int lone_index, int top, Shelf<kWarps * 32> &shelf) {
+  constexpr int E = Batch<T>::E, U = Batch<T>::U, kThreads = kWarps * 32;
+  static_assert(U == 8, "a batch's packs");
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  const int batches = (end - from + U * kThreads - 1) / (U * kThreads);
+  const auto key_at = [&](int b) -> uint64_t {
+    const float m = shelf.maxima[b * kThreads + tid];
+    return m == -kInf ? 0
+                      : static_cast<uint64_t>(order_of(m)) << 32 |
+                            (0x7fffffu - static_cast<uint32_t>(b)) << kTidBits |
+                            static_cast<uint32_t>(tid);
+  };
+  // n batches reach the least of the warps' ceil(n / warps)-th largest of a maximum a lane
+  uint32_t high = 0;
+  for (int b = 0; b < batches; ++b) high = max(high, static_cast<uint32_t>(key_at(b) >> 32));
+  const uint32_t reach = ranked(high, (top + kWarps - 1) / kWarps - 1, lane);
+  if (lane == 0) shelf.floors[warp] = reach;
+  __syncthreads();
+  uint32_t floor = shelf.floors[0];
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) floor = min(floor, shelf.floors[i]);
+  in_order<kThreads>(shelf, top, max(static_cast<uint64_t>(floor) << 32, uint64_t(1)),
+                     [&](auto take) {
+                       for (int b = 0; b < batches; ++b) take(key_at(b));
+                     });
+  // the n-th batch; all of its threads' batches with an equal maximum count, their
+  // elements lie between one another's
+  const uint64_t nth = shelf.best[top - 1] >> kTidBits;
+  const float least = nth ? value_of(static_cast<uint32_t>(nth >> (32 - kTidBits))) : kLowest;
+  __syncthreads();
+  if (tid == 0) shelf.found = 0;
+  __syncthreads();
+  for (int b = 0; b < batches; ++b) {
+    const uint64_t key = key_at(b);
+    if (key && key >> kTidBits >= nth) shelf.batches[atomicAdd(&shelf.found, 1)] = b * kThreads + tid;
+  }
+  __syncthreads();
+  const int count = shelf.found;
+  __syncthreads();
+  in_order<kThreads>(shelf, top, static_cast<uint64_t>(order_of(least)) << 32, [&](auto take) {
+    if (lone_value >= least) take(key_of(lone_value, lone_index));
+    if (tid < top && shelf.carried[tid]) take(shelf.carried[tid]);
+    // eight lanes to a batch, a pack each
+    for (int i = tid >> 3; i < count; i += kThreads / 8) {
+      const int batch = static_cast<int>(shelf.batches[i]) / kThreads,
+                thread = static_cast<int>(shelf.batches[i]) % kThreads;
+      const int at = from + batch * (U * kThreads) + (lane & 7) * kThreads + thread;
+      if (at >= end) continue;
+      const Pack<T, E> v = load_pack<T, E>(xp + static_cast<int64_t>(at) * E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float f = to_float(v.e[e]);
+        if (f >= least) take(key_of(f, static_cast<uint32_t>(lead + at * E + e)));
+      }
+    }
+  });
+  if (tid < kMostTop) shelf.carried[tid] = shelf.best[tid];
+  __syncthreads();
+}
+
 // kTop: with alternatives. The launch's CTAs are whole clusters of `cluster`.
 template <typename T, bool kTop, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
     token_logprobs_kernel(LogprobArgs p, const T *logits, int cluster) {
   using B = Batch<T>;
   constexpr int E = B::E, U = B::U, kThreads = kWarps * 32;
-  static_assert(kThreads <= 1 << kTidBits && kMostCluster * kMostTop <= kCandidates, "notes, keys");
+  static_assert(kThreads <= 1 << kTidBits && kMostCluster * kMostTop <= kCandidates, "keys");
+  constexpr int kLook = Shelf<kThreads>::kMaxima / kThreads;  // batches after which the maxima are looked through
   __shared__ Part warp_part[kWarps];
-  __shared__ uint64_t notes[kTop ? kWarps * kNotes : 1];
-  __shared__ uint32_t floors[kTop ? kWarps : 1];
   // what the cluster's CTAs hand to its first: two rows' worth, so that one barrier a
   // row keeps the next row's writes off this row's reads
   __shared__ Part cta_part[2][kMostCluster];
   __shared__ uint64_t cta_list[2][kTop ? kMostCluster * kMostTop : 1];
-  __shared__ uint64_t best[kMostTop];
-  __shared__ uint64_t candidates[kTop ? kCandidates : 1];
-  __shared__ int found;
+  __shared__ __align__(16) uint8_t shelf_room[kTop ? sizeof(Shelf<kThreads>) : 16];
+  Shelf<kThreads> &shelf = *reinterpret_cast<Shelf<kThreads> *>(shelf_room);
   griddep_wait();
   griddep_launch_dependents();
 
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(blockIdx.x) % cluster;
   const float c = p.scale * kLog2e;
-  const int share = kTop ? (p.top + kWarps - 1) / kWarps : 0;
   if (cluster > 1) {  // the first CTA has started before anything is stored into it
     cluster_arrive_relaxed();
     cluster_wait();
@@ -191,43 +295,6 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
     const T *xp = x + lead;
 
     Part mine{-kInf, 0.0f, 0.0f};
-    float floor = kLowest;  // no -infinity among the alternatives
-    int count = 0, held = 0;  // notes; those that reach the floor since it rose
-    uint64_t *noted = notes + (kTop ? warp * kNotes : 0);
-    // The n best notes, by maximum and then by batch: the batches of a CTA follow one
-    // another, so of equal maxima the earlier batch's counts, and those of one batch stay together.
-    const auto make_room = [&] {
-      __syncwarp();
-      uint64_t note[kNotes / 32];
-      int place[kNotes / 32];
-#pragma unroll
-      for (int i = 0; i < kNotes / 32; ++i) {
-        note[i] = i * 32 + lane < count ? noted[i * 32 + lane] : 0;
-        place[i] = note[i] ? 0 : kNotes;
-      }
-      for (int k = 0; k < count; ++k) {
-        const uint64_t other = noted[k] >> kTidBits;
-#pragma unroll
-        for (int i = 0; i < kNotes / 32; ++i) place[i] += other > note[i] >> kTidBits;
-      }
-      __syncwarp();
-      uint32_t least = 0xffffffffu;
-      count = 0;
-#pragma unroll
-      for (int i = 0; i < kNotes / 32; ++i) {
-        const bool keep = place[i] < p.top;
-        const unsigned kept = __ballot_sync(kAll, keep);
-        if (keep) {
-          noted[count + __popc(kept & ((1u << lane) - 1u))] = note[i];
-          least = min(least, static_cast<uint32_t>(note[i] >> 32));
-        }
-        count += __popc(kept);
-      }
-      __syncwarp();
-      floor = fmaxf(floor, value_of(__reduce_min_sync(kAll, least)));
-      held = count;  // at least n
-    };
-
     const auto load = [&](B &b, int j, int here) {
       const T *from = xp + static_cast<int64_t>(j + tid) * E;
 #pragma unroll
@@ -247,7 +314,9 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
       mine.w = mine.s * d;
     }
 
-    for (int j = j0, batch = 0; j < j1; j += U * kThreads, ++batch) {
+    if (kTop && tid < kMostTop) shelf.carried[tid] = 0;  // (seen by collect past its barriers)
+    int from = j0;  // of the maxima held
+    for (int j = j0; j < j1; j += U * kThreads) {
       B now;
       const bool whole = j + U * kThreads <= j1;
       const int here = min(U, (j1 - j - tid + kThreads - 1) / kThreads);  // packs of this thread
@@ -289,47 +358,11 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
       mine.s += sum.s;
       mine.w += sum.w;
       if constexpr (kTop) {
-        volatile uint32_t *shared_floors = floors;
-        if (batch == 0) {
-          // n elements reach the least of the warps' share-th largest: each is the
-          // maximum of another thread's values
-          const uint32_t reach = ranked(order_of(most), share - 1, lane);
-          if (lane == 0) shared_floors[warp] = reach;
-          __syncthreads();
-        }
-        const float least = value_of(
-            __reduce_min_sync(kAll, lane < kWarps ? shared_floors[lane] : 0xffffffffu));
-        if (least > floor) {
-          floor = least;
-          held = 0;
-        }
-        unsigned some = __ballot_sync(kAll, most >= floor);
-        if (some) {
-          // many at once (rising logits): the n-th of the lanes' maxima first
-          if (__popc(some) > 8 && __popc(some) >= p.top) {
-            const float higher = value_of(ranked(order_of(most), p.top - 1, lane));
-            if (higher > floor) {
-              floor = higher;
-              held = 0;
-              some = __ballot_sync(kAll, most >= floor);
-            }
-          }
-          if (most >= floor)
-            noted[count + __popc(some & ((1u << lane) - 1u))] =
-                static_cast<uint64_t>(order_of(most)) << 32 |
-                (0x7fffffu - static_cast<uint32_t>(batch)) << kTidBits | static_cast<uint32_t>(tid);
-          count += __popc(some);
-          held += __popc(some);
-          if (batch > 0 && __popc(some) >= share) {
-            const uint32_t reach = ranked(order_of(most), share - 1, lane);
-            if (lane == 0 && reach > shared_floors[warp]) shared_floors[warp] = reach;
-          }
-          if (count > kNotes - 32) make_room();
-          // n elements at or above the floor, all left of what comes: equal ones no longer count
-          if (held >= p.top) {
-            floor = value_of(order_of(floor) + 1);
-            held = 0;
-          }
+        const int batch = (j - from) / (U * kThreads);
+        shelf.maxima[batch * kThreads + tid] = most;
+        if (batch == kLook - 1 && j + U * kThreads < j1) {
+          collect<T, kWarps>(xp, from, j + U * kThreads, lead, -kInf, 0, p.top, shelf);
+          from = j + U * kThreads;
         }
       }
     }
@@ -338,63 +371,8 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
     mine = join_lanes<16>(mine, c);
     if (lane == 0) warp_part[warp] = mine;
     __syncthreads();
-    // Keys that reach a bound come together, and each takes the place that the number above
-    // it gives. Where they are too many (long runs of equal logits), the n-th of some of them
-    // is a better bound, and they come together again.
-    const auto in_order = [&](uint64_t bound, auto gather) {
-      for (;;) {
-        if (tid == 0) found = 0;
-        if (tid < kMostTop) best[tid] = 0;
-        __syncthreads();
-        gather([&](uint64_t key) {
-          if (key < bound) return;
-          const int at = atomicAdd(&found, 1);
-          if (at < kCandidates) candidates[at] = key;
-        });
-        __syncthreads();
-        const int all = found, n = min(all, kCandidates);
-        for (int i = tid; i < n; i += kThreads) {
-          const uint64_t key = candidates[i];
-          int place = 0;
-#pragma unroll 8
-          for (int k = 0; k < n; ++k) place += candidates[k] > key;
-          if (place < p.top) best[place] = key;
-        }
-        __syncthreads();
-        if (all <= kCandidates) break;
-        bound = best[p.top - 1];
-        __syncthreads();
-      }
-    };
-    if constexpr (kTop) {
-      uint32_t least = order_of(kLowest);
-      if (j0 < j1) {
-        uint32_t of = floors[0];
-#pragma unroll
-        for (int i = 1; i < kWarps; ++i) of = min(of, floors[i]);
-        least = max(least, of);
-      }
-      const float least_value = value_of(least);
-      in_order(static_cast<uint64_t>(least) << 32, [&](auto take) {
-        if (lone && lone_value >= least_value) take(key_of(lone_value, lone_index));
-        // eight lanes to a noted batch, a pack each
-        static_assert(U == 8, "a batch's packs");
-        for (int i = lane >> 3; i < count; i += 4) {
-          const uint64_t note = noted[i];
-          if (static_cast<uint32_t>(note >> 32) < least) continue;
-          const int batch = static_cast<int>(0x7fffffu - (static_cast<uint32_t>(note) >> kTidBits));
-          const int at = j0 + batch * (U * kThreads) + (lane & 7) * kThreads +
-                         static_cast<int>(note & ((1u << kTidBits) - 1u));
-          if (at >= j1) continue;
-          const Pack<T, E> v = load_pack<T, E>(xp + static_cast<int64_t>(at) * E);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float f = to_float(v.e[e]);
-            if (f >= least_value) take(key_of(f, static_cast<uint32_t>(lead + at * E + e)));
-          }
-        }
-      });
-    }
+    if constexpr (kTop)
+      collect<T, kWarps>(xp, from, j1, lead, lone ? lone_value : -kInf, lone_index, p.top, shelf);
     Part total{-kInf, 0.0f, 0.0f};
     if (warp == 0) {
       if (lane < kWarps) total = warp_part[lane];
@@ -409,7 +387,7 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
       }
       if (kTop && tid < kMostTop)
         st_cluster_u64(mapa_shared(smem_u32(&cta_list[parity][rank * kMostTop + tid]), 0u),
-                       best[tid]);
+                       shelf.best[tid]);
       cluster_sync();
       if (rank != 0) continue;
       if (warp == 0) {
@@ -420,7 +398,7 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
         uint64_t most = 0;  // n keys reach any CTA's n-th
         for (int i = 0; i < cluster; ++i)
           most = max(most, cta_list[parity][i * kMostTop + p.top - 1]);
-        in_order(max(most, uint64_t(1)), [&](auto take) {
+        in_order<kThreads>(shelf, p.top, max(most, uint64_t(1)), [&](auto take) {
           for (int i = tid; i < cluster * kMostTop; i += kThreads) take(cta_list[parity][i]);
         });
       }
@@ -451,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
         }
       }
       if (kTop && lane < p.top) {
-        const uint64_t key = best[lane];
+        const uint64_t key = shelf.best[lane];
         const int64_t to = row * p.top + lane;
         p.top_ids[to] = key && !bad ? key_index(key) : -1;
         p.top_logprobs[to] = bad ? log_sum
@@ -570,13 +548,16 @@ auto pick_forward(bool top, int warps) {
   }
 }
 
-// One warp for rows of up to two batches, else four, with 16 where rows do not fill the SMs;
-// then clusters too, while each CTA has two packs a thread.
+// One warp for rows of up to four packs a lane, else four, or 16 where rows do not fill the SMs;
+// then clusters too, while each CTA has two packs a thread. Eight warps a row instead of
+// four are slower (2048 x 50021 fp16 48 us against 43, with five alternatives 65 against 57; 4096 x
+// 32000 bf16 88 against 65) but for long rows with alternatives (1024 x 128000 bf16, 20 of them:
+// 73 against 76).
 template <typename T>
 int run_forward(cudaStream_t s, const LogprobArgs &p, const T *logits) {
-  constexpr int E = 16 / sizeof(T), U = Batch<T>::U;
+  constexpr int E = 16 / sizeof(T);
   const int64_t packs = std::max(1, p.vocab / E), sms = sm_count();
-  const int warps = packs <= 2 * 32 * U ? 1 : p.rows <= 2 * sms ? 16 : 4;
+  const int warps = packs <= 128 ? 1 : packs > 1024 && p.rows <= 2 * sms ? 16 : 4;
   int cluster = 1;
   while (warps == 16 && cluster < kMostCluster && p.rows * cluster * 2 <= sms &&
          packs >= 2 * cluster * 16 * 32 * 2)
