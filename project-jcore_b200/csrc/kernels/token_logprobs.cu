@@ -131,23 +131,6 @@ __device__ __forceinline__ float most_of(const Pack<T, E> &p) {
   }
 }
 
-// The sums of a thread's batch with its first pack at `at`, differences first and each
-// of them kept finite.
-template <typename T, int kThreads>
-__device__ __noinline__ Part careful_sums(const T *x, int lead, int at, int end, float base, float c) {
-  constexpr int E = Batch<T>::E, U = Batch<T>::U;
-  Part r{base, 0.0f, 0.0f};
-  for (int u = 0; u < U && at + u * kThreads < end; ++u)
-    for (int e = 0; e < E; ++e) {
-      const float l = to_float(x[lead + (at + u * kThreads) * E + e]);
-      const float d = at_least(at_least(l - base, kLowest) * c, kLowest);
-      const float v = exp2_approx(d);
-      r.s += v;
-      r.w += v * d;
-    }
-  return r;
-}
-
 template <int kThreads>
 struct Shelf {
   // maxima of thread batches, kept until they are looked through
@@ -259,7 +242,7 @@ __device__ __noinline__ void collect(const T *xp, int from, int end, int lead, f
 
 // kTop: with alternatives. The launch's CTAs are whole clusters of `cluster`.
 template <typename T, bool kTop, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 24 : 32) / kWarps)
     token_logprobs_kernel(LogprobArgs p, const T *logits, int cluster) {
   using B = Batch<T>;
   constexpr int E = B::E, U = B::U, kThreads = kWarps * 32;
@@ -327,17 +310,15 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
         if (whole || u < here) most = fmaxf(most, most_of(now.p[u]));
       if (most > mine.m) mine = rebase(mine, most, c);
       const float base = mine.m == -kInf ? 0.0f : mine.m;
-      // t = l c - m c in one fused step: m c rounds, by `off`, the same for all, which comes out
-      // of the sums afterwards (2^off within its first two terms: |off| < 2^-24 |m c|)
-      const float bc = base * c, off = fmaf(base, c, -bc);
-      float s[2] = {}, w[2] = {};
-      const auto add = [&](const Pack<T, E> &v) {
+      float ss[2] = {}, ww[2] = {};
+      const auto add = [&](const Pack<T, E> &p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float t = fmaf(to_float(v.e[e]), c, -bc);
+          // (a masked logit's t kept finite: 0 times it is 0)
+          const float t = at_least((to_float(p.e[e]) - base) * c, kLowest);
           const float r = exp2_approx(t);
-          s[e & 1] += r;
-          w[e & 1] = fmaf(r, t, w[e & 1]);
+          ss[e & 1] += r;
+          ww[e & 1] = fmaf(r, t, ww[e & 1]);
         }
       };
       if (whole) {
@@ -348,15 +329,8 @@ __global__ void __launch_bounds__(kWarps * 32, 24 / kWarps)
         for (int u = 0; u < U; ++u)
           if (u < here) add(now.p[u]);
       }
-      s[0] += s[1];
-      w[0] += w[1];
-      const float back = 1.0f - off * kLn2;
-      Part sum{base, s[0] * back, fmaf(-off, s[0], w[0]) * back};
-      // masked logits (0 times -infinity), and maxima that l c or m c would not fit
-      if ((w[0] != w[0] && s[0] == s[0]) || fabsf(bc) > 1e30f)
-        sum = careful_sums<T, kThreads>(x, lead, j + tid, j1, base, c);
-      mine.s += sum.s;
-      mine.w += sum.w;
+      mine.s += ss[0] + ss[1];
+      mine.w += ww[0] + ww[1];
       if constexpr (kTop) {
         const int batch = (j - from) / (U * kThreads);
         shelf.maxima[batch * kThreads + tid] = most;
