@@ -138,7 +138,8 @@ struct Shelf {
   uint64_t candidates[kCandidates], best[kMostTop];
   uint64_t carried[kMostTop];             // the best of what came before
   float maxima[kMaxima];
-  uint32_t batches[kMostTop + kThreads];  // those to be read again
+  static constexpr int kBatches = kMostTop + kThreads;
+  uint32_t batches[kBatches];             // those to be read again
   uint32_t floors[kThreads / 32];
   int found;
 };
@@ -185,40 +186,52 @@ __device__ __noinline__ void collect(const T *xp, int from, int end, int lead, f
   static_assert(U == 8, "a batch's packs");
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int batches = (end - from + U * kThreads - 1) / (U * kThreads);
-  const auto key_at = [&](int b) -> uint64_t {
-    const float m = shelf.maxima[b * kThreads + tid];
-    return m == -kInf ? 0
-                      : static_cast<uint64_t>(order_of(m)) << 32 |
-                            (0x7fffffu - static_cast<uint32_t>(b)) << kTidBits |
-                            static_cast<uint32_t>(tid);
-  };
   // n batches reach the least of the warps' ceil(n / warps)-th largest of a maximum a lane
-  uint32_t high = 0;
-  for (int b = 0; b < batches; ++b) high = max(high, static_cast<uint32_t>(key_at(b) >> 32));
-  const uint32_t reach = ranked(high, (top + kWarps - 1) / kWarps - 1, lane);
+  float most = -kInf;
+  for (int b = 0; b < batches; ++b) most = fmaxf(most, shelf.maxima[b * kThreads + tid]);
+  const uint32_t reach = ranked(order_of(most), (top + kWarps - 1) / kWarps - 1, lane);
   if (lane == 0) shelf.floors[warp] = reach;
+  if (tid == 0) shelf.found = 0;
   __syncthreads();
   uint32_t floor = shelf.floors[0];
 #pragma unroll
   for (int i = 1; i < kWarps; ++i) floor = min(floor, shelf.floors[i]);
-  in_order<kThreads>(shelf, top, max(static_cast<uint64_t>(floor) << 32, uint64_t(1)),
-                     [&](auto take) {
-                       for (int b = 0; b < batches; ++b) take(key_at(b));
-                     });
-  // the n-th batch; all of its threads' batches with an equal maximum count, their
-  // elements lie between one another's
-  const uint64_t nth = shelf.best[top - 1] >> kTidBits;
-  const float least = nth ? value_of(static_cast<uint32_t>(nth >> (32 - kTidBits))) : kLowest;
+  float least = fmaxf(value_of(floor), kLowest);
+  // two or three times n of them, in general
+  if (most >= least)
+    for (int b = 0; b < batches; ++b)
+      if (shelf.maxima[b * kThreads + tid] >= least) {
+        const int at = atomicAdd(&shelf.found, 1);
+        if (at < shelf.kBatches) shelf.batches[at] = b * kThreads + tid;
+      }
   __syncthreads();
-  if (tid == 0) shelf.found = 0;
+  int count = shelf.found;
   __syncthreads();
-  for (int b = 0; b < batches; ++b) {
-    const uint64_t key = key_at(b);
-    if (key && key >> kTidBits >= nth) shelf.batches[atomicAdd(&shelf.found, 1)] = b * kThreads + tid;
+  if (count > shelf.kBatches) {  // runs of equal logits
+    const auto key_at = [&](int b) -> uint64_t {
+      const float m = shelf.maxima[b * kThreads + tid];
+      return m == -kInf ? 0
+                        : static_cast<uint64_t>(order_of(m)) << 32 |
+                              (0x7fffffu - static_cast<uint32_t>(b)) << kTidBits |
+                              static_cast<uint32_t>(tid);
+    };
+    in_order<kThreads>(shelf, top, static_cast<uint64_t>(order_of(least)) << 32, [&](auto take) {
+      for (int b = 0; b < batches; ++b) take(key_at(b));
+    });
+    // the n-th batch; all of its threads' batches with an equal maximum count, their
+    // elements lie between one another's
+    const uint64_t nth = shelf.best[top - 1] >> kTidBits;
+    least = value_of(static_cast<uint32_t>(nth >> (32 - kTidBits)));
+    __syncthreads();
+    if (tid == 0) shelf.found = 0;
+    __syncthreads();
+    for (int b = 0; b < batches; ++b)
+      if (key_at(b) >> kTidBits >= nth)
+        shelf.batches[atomicAdd(&shelf.found, 1)] = b * kThreads + tid;
+    __syncthreads();
+    count = shelf.found;
+    __syncthreads();
   }
-  __syncthreads();
-  const int count = shelf.found;
-  __syncthreads();
   in_order<kThreads>(shelf, top, static_cast<uint64_t>(order_of(least)) << 32, [&](auto take) {
     if (lone_value >= least) take(key_of(lone_value, lone_index));
     if (tid < top && shelf.carried[tid]) take(shelf.carried[tid]);
@@ -285,6 +298,14 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 24 : 3
         if (u < here) b.p[u] = load_pack<T, E>(from + u * (kThreads * E));
     };
 
+    // the target's logit, long before it is needed
+    int64_t target = -1;
+    float target_logit = 0.0f;
+    if (p.logprob && rank == 0 && tid == 0) {
+      target = p.targets[row];
+      if (target >= 0 && target < p.vocab) target_logit = to_float(x[target]);
+      else target = -1;
+    }
     // the lone values, by the first CTA's first warp
     const int lone_index = lane < lead ? lane : tail + lane - lead;
     const bool lone = rank == 0 && warp == 0 && lane < lead + p.vocab - tail;
@@ -393,13 +414,10 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 24 : 3
         if (p.entropy)
           p.entropy[row] = total.s == 0.0f ? 0.0f : log_sum - kLn2 * (total.w / total.s);
         if (p.logprob) {
-          const int64_t t = p.targets[row];
-          float v = 0.0f;
-          if (t >= 0 && t < p.vocab) {
-            const float l = to_float(x[t]);
-            v = bad ? log_sum : l == -kInf ? -kInf : fmaf(l - total.m, p.scale, -log_sum);
-          }
-          p.logprob[row] = v;
+          p.logprob[row] = target < 0              ? 0.0f
+                           : bad                   ? log_sum
+                           : target_logit == -kInf ? -kInf
+                                                   : fmaf(target_logit - total.m, p.scale, -log_sum);
         }
       }
       if (kTop && lane < p.top) {
