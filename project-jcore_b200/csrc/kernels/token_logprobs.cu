@@ -435,43 +435,95 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 24 : 3
 
 // ---------------------------------------------------------------------------
 // Gradient: dl = p (A + B t) + [v = target] scale g with t = (d - L) log2 e, p = 2^t,
-// A = -scale (g + h H), B = -scale h ln 2. A CTA takes a run of packs of one row.
+// A = -scale (g + h H), B = -scale h ln 2. CTAs go round runs of packs of a row; a run's
+// logits load under the one before, and its row's numbers, which say whether they are
+// needed at all, one run earlier still. Bound by memory: 4096 x 32000 bf16 takes 92 us, of 80
+// for its bytes (121 us with a CTA a run, which waited for one and then for the other).
+// Short rows go to CTAs of one warp.
 // ---------------------------------------------------------------------------
 struct LogprobGradArgs {
-  int64_t rows, ld, ldd;
+  int64_t ld, ldd;
   int vocab;
   float scale;
   const int64_t *targets;
   const float *stats, *entropy, *d_logprob, *d_entropy;
 };
 
-constexpr int kGradThreads = 256, kGradPacks = 4;
+constexpr int kGradPacks = 4;
 
-template <typename T, int E>
-__global__ void __launch_bounds__(kGradThreads)
-    token_logprobs_grad_kernel(LogprobGradArgs p, const T *logits, T *dlogits, int64_t runs,
-                               int per_row) {
+// What a run needs to know of its row.
+struct GradRow {
+  int64_t row, target;
+  float g, h, m, log_sum, entropy;
+  int first;  // pack
+};
+
+template <typename T, int E, int kThreads>
+__global__ void __launch_bounds__(kThreads, 3 * 256 / kThreads)
+    token_logprobs_grad_kernel(LogprobGradArgs p, const T *logits, T *dlogits, uint32_t runs,
+                               FastDiv per_row) {
   griddep_wait();
   griddep_launch_dependents();
-  for (int64_t run = blockIdx.x; run < runs; run += gridDim.x) {
-    const int64_t row = run / per_row;
-    const T *x = logits + row * p.ld;
-    T *dx = dlogits + row * p.ldd;
-    const int64_t target = p.targets ? p.targets[row] : -1;
-    const bool asked = target >= 0 && target < p.vocab;
-    const float g = asked && p.d_logprob ? p.d_logprob[row] : 0.0f;
-    const float h = p.d_entropy ? p.d_entropy[row] : 0.0f;
-    const float m = p.stats[2 * row], log_sum = p.stats[2 * row + 1];
-    // nothing asked of the row, or nothing in it
-    const bool zeros = (g == 0.0f && h == 0.0f) || (m == -kInf && log_sum == -kInf);
-    const float a = -p.scale * (h != 0.0f ? fmaf(h, p.entropy[row], g) : g);
-    const float2 aa = both(a), bb = both(-p.scale * h * kLn2);
-    const float2 c = both(p.scale * kLog2e), base = both(-m), ll = both(-log_sum * kLog2e);
-    const float hot = p.scale * g;
+  const int tid = static_cast<int>(threadIdx.x);
+  const auto row_of = [&](uint32_t run) {
+    GradRow r{};
+    if (run >= runs) return r;
+    const uint32_t row = fdiv(run, per_row);
+    r.row = row;
+    r.first = static_cast<int>(run - row * per_row.d) * (kThreads * kGradPacks);
+    r.target = p.targets ? p.targets[row] : -1;
+    if (p.d_logprob) r.g = p.d_logprob[row];
+    if (p.d_entropy) {
+      r.h = p.d_entropy[row];
+      r.entropy = p.entropy[row];
+    }
+    r.m = p.stats[2 * static_cast<int64_t>(row)];
+    r.log_sum = p.stats[2 * static_cast<int64_t>(row) + 1];
+    return r;
+  };
+  const auto asked = [&](const GradRow &r) { return r.target >= 0 && r.target < p.vocab; };
+  // nothing asked of the row, or nothing in it
+  const auto zeros = [&](const GradRow &r) {
+    return ((r.g == 0.0f || !asked(r)) && r.h == 0.0f) || (r.m == -kInf && r.log_sum == -kInf);
+  };
+  const auto lead_of = [&](const T *x) {
     const int mis = E == 1 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
-    const int lead = min(mis ? E - mis : 0, p.vocab);
-    const int packs = (p.vocab - lead) / E, tail = lead + packs * E;
-    const int hit = asked ? static_cast<int>(target) : -1;
+    return min(mis ? E - mis : 0, p.vocab);
+  };
+  struct Packs {
+    Pack<T, E> v[kGradPacks];
+  };
+  const auto load = [&](const GradRow &r, uint32_t run) {
+    Packs q;
+    const T *x = logits + r.row * p.ld;
+    const int lead = lead_of(x), packs = (p.vocab - lead) / E;
+    if (run < runs && !zeros(r)) {
+#pragma unroll
+      for (int u = 0; u < kGradPacks; ++u) {
+        const int at = r.first + u * kThreads + tid;
+        if (at < packs) q.v[u] = load_pack<T, E>(x + lead + static_cast<int64_t>(at) * E);
+      }
+    }
+    return q;
+  };
+
+  const uint32_t step = gridDim.x;
+  uint32_t run = blockIdx.x;
+  GradRow now = row_of(run), next = row_of(run + step);
+  Packs in = load(now, run);
+  for (; run < runs; run += step) {
+    const Packs in_next = load(next, run + step);
+    const GradRow after = row_of(run + 2 * step);
+    const T *x = logits + now.row * p.ld;
+    T *dx = dlogits + now.row * p.ldd;
+    const bool none = zeros(now), hit_row = asked(now);
+    const float g = hit_row ? now.g : 0.0f, h = now.h;
+    const float a = -p.scale * (h != 0.0f ? fmaf(h, now.entropy, g) : g);
+    const float2 aa = both(a), bb = both(-p.scale * h * kLn2);
+    const float2 c = both(p.scale * kLog2e), base = both(-now.m), ll = both(-now.log_sum * kLog2e);
+    const float hot = p.scale * g;
+    const int lead = lead_of(x), packs = (p.vocab - lead) / E, tail = lead + packs * E;
+    const int hit = hit_row ? static_cast<int>(now.target) : -1;
     const auto pairs = [&](float2 v) {
       const float2 u = at_least(add2(v, base), kLowest);
       // (2^-1000 is 0, and 0 times a finite number too)
@@ -479,27 +531,18 @@ __global__ void __launch_bounds__(kGradThreads)
       const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
       return mul2(e, fma2(t, bb, aa));
     };
-    const int first = static_cast<int>(run % per_row) * (kGradThreads * kGradPacks);
-    Pack<T, E> in[kGradPacks];
-    if (!zeros) {
-#pragma unroll
-      for (int u = 0; u < kGradPacks; ++u) {
-        const int at = first + u * kGradThreads + static_cast<int>(threadIdx.x);
-        if (at < packs) in[u] = load_pack<T, E>(x + lead + static_cast<int64_t>(at) * E);
-      }
-    }
 #pragma unroll
     for (int u = 0; u < kGradPacks; ++u) {
-      const int at = first + u * kGradThreads + static_cast<int>(threadIdx.x);
+      const int at = now.first + u * kThreads + tid;
       if (at >= packs) break;
       const int index = lead + at * E;
       float v[E];
-      if (zeros) {
+      if (none) {
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = 0.0f;
       } else {
         float2 q[(E + 1) / 2];
-        unpack_pairs(in[u], q);
+        unpack_pairs(in.v[u], q);
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
           const float2 r = pairs(q[e / 2]);
@@ -515,16 +558,18 @@ __global__ void __launch_bounds__(kGradThreads)
       store_pack(dx + index, pack<T, E>(v));
     }
     // the lone values beside the packs, by the row's first run
-    const int lone = static_cast<int>(threadIdx.x);
-    if (first == 0 && lone < lead + p.vocab - tail) {
-      const int index = lone < lead ? lone : tail + lone - lead;
+    if (now.first == 0 && tid < lead + p.vocab - tail) {
+      const int index = tid < lead ? tid : tail + tid - lead;
       float v = 0.0f;
-      if (!zeros) {
+      if (!none) {
         v = pairs(both(to_float(x[index]))).x;
         if (index == hit) v += hot;
       }
       dx[index] = from_float<T>(v);
     }
+    now = next;
+    next = after;
+    in = in_next;
   }
 }
 
@@ -551,7 +596,7 @@ int run_forward(cudaStream_t s, const LogprobArgs &p, const T *logits) {
   const int64_t packs = std::max(1, p.vocab / E), sms = sm_count();
   const int warps = packs <= 128 ? 1 : packs > 1024 && p.rows <= 2 * sms ? 16 : 4;
   int cluster = 1;
-  while (warps == 16 && cluster < kMostCluster && p.rows * cluster * 2 <= sms &&
+  while (warps == 16 && cluster < kMostCluster && p.rows * cluster * 8 <= sms * 3 &&
          packs >= 2 * cluster * 16 * 32 * 2)
     cluster *= 2;
   const int64_t rows = std::min<int64_t>(p.rows, sms * 128);
@@ -574,23 +619,38 @@ int run_forward(cudaStream_t s, const LogprobArgs &p, const T *logits) {
 }
 
 template <typename T>
-int run_gradient(cudaStream_t s, const LogprobGradArgs &p, const T *logits, T *dlogits) {
+int run_gradient(cudaStream_t s, int64_t rows, const LogprobGradArgs &p, const T *logits,
+                 T *dlogits) {
   constexpr int E = 16 / sizeof(T);
   // Packs need rows of the same alignment on both sides. A pitch that changes it from row to
   // row changes it on both alike if the pitches differ by whole packs.
   const bool alike = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) %
                              16 == 0 &&
-                     (p.rows == 1 || (p.ld - p.ldd) % E == 0);
-  const int width = alike ? E : 1;
-  const int64_t per_row = std::max<int64_t>(1, ceil_div(p.vocab / width, kGradThreads * kGradPacks));
-  const int64_t runs = p.rows * per_row;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(runs, int64_t(1) << 30));
-  return alike ? launch_programmatic(token_logprobs_grad_kernel<T, E>, dim3(grid),
-                                     dim3(kGradThreads), 0, s, p, logits, dlogits, runs,
-                                     static_cast<int>(per_row))
-               : launch_programmatic(token_logprobs_grad_kernel<T, 1>, dim3(grid),
-                                     dim3(kGradThreads), 0, s, p, logits, dlogits, runs,
-                                     static_cast<int>(per_row));
+                     (rows == 1 || (p.ld - p.ldd) % E == 0);
+  const int packs = p.vocab / (alike ? E : 1), threads = packs <= 32 * kGradPacks ? 32 : 256;
+  const int64_t per_row = std::max<int64_t>(1, ceil_div(packs, threads * kGradPacks));
+  auto *fn = threads == 32 ? (alike ? token_logprobs_grad_kernel<T, E, 32>
+                                    : token_logprobs_grad_kernel<T, 1, 32>)
+                           : (alike ? token_logprobs_grad_kernel<T, E, 256>
+                                    : token_logprobs_grad_kernel<T, 1, 256>);
+  // rows of a launch: their runs are counted in 31 bits
+  const int64_t most = std::max<int64_t>(1, (int64_t(1) << 30) / per_row);
+  for (int64_t r = 0; r < rows; r += most) {
+    LogprobGradArgs q = p;
+    if (q.targets) q.targets += r;
+    if (q.d_logprob) q.d_logprob += r;
+    if (q.d_entropy) q.d_entropy += r;
+    if (q.entropy) q.entropy += r;
+    q.stats += 2 * r;
+    const int64_t runs = std::min(most, rows - r) * per_row;
+    const int64_t grid = std::min<int64_t>(runs, static_cast<int64_t>(sm_count()) * (3 * 256 / threads));
+    const int rc = launch_programmatic(fn, dim3(static_cast<unsigned>(grid)), dim3(static_cast<unsigned>(threads)), 0, s,
+                                       q, logits + r * p.ld, dlogits + r * p.ldd,
+                                       static_cast<uint32_t>(runs),
+                                       make_fastdiv(static_cast<uint32_t>(per_row)));
+    if (rc) return rc;
+  }
+  return kOk;
 }
 
 // Checks shared by both directions.
@@ -645,13 +705,13 @@ extern "C" int nplk_token_logprobs_backward(void *stream, int64_t rows, int64_t 
   if (misaligned(dlogits, dtype_bytes(dtype)) || misaligned(targets, 8) || misaligned(stats, 4) ||
       misaligned(entropy, 4) || misaligned(d_logprob, 4) || misaligned(d_entropy, 4))
     return kErrInvalidArg;
-  const LogprobGradArgs p{rows,    ld,      ldd,       static_cast<int>(vocab), scale, targets,
-                          stats,   entropy, d_logprob, d_entropy};
+  const LogprobGradArgs p{ld,    ldd,     static_cast<int>(vocab), scale,    targets,
+                          stats, entropy, d_logprob,               d_entropy};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == NPLK_DTYPE_FP32)
-    return run_gradient(s, p, static_cast<const float *>(logits), static_cast<float *>(dlogits));
+    return run_gradient(s, rows, p, static_cast<const float *>(logits), static_cast<float *>(dlogits));
   if (dtype == NPLK_DTYPE_FP16)
-    return run_gradient(s, p, static_cast<const __half *>(logits), static_cast<__half *>(dlogits));
-  return run_gradient(s, p, static_cast<const __nv_bfloat16 *>(logits),
+    return run_gradient(s, rows, p, static_cast<const __half *>(logits), static_cast<__half *>(dlogits));
+  return run_gradient(s, rows, p, static_cast<const __nv_bfloat16 *>(logits),
                       static_cast<__nv_bfloat16 *>(dlogits));
 }
