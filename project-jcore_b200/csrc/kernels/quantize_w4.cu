@@ -45,10 +45,40 @@ __device__ __forceinline__ float most_nan(float a, float b) {
   return r;
 }
 
-// Eight values' limits: high the largest magnitude, or with zeros the largest of w and 0, and
-// low then the largest of -w and 0. 16-bit types two at a time; NaN stays.
+// Two values in one register: two rows of 16-bit types, one of fp32 in each.
+template <typename T>
+struct Two {
+  using type = float2;
+};
+template <>
+struct Two<__half> {
+  using type = __half2;
+};
+template <>
+struct Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+__device__ __forceinline__ float2 most2(float2 a, float2 b) {
+  return make_float2(most_nan(a.x, b.x), most_nan(a.y, b.y));
+}
+__device__ __forceinline__ __half2 most2(__half2 a, __half2 b) { return __hmax2_nan(a, b); }
+__device__ __forceinline__ __nv_bfloat162 most2(__nv_bfloat162 a, __nv_bfloat162 b) {
+  return __hmax2_nan(a, b);
+}
+__device__ __forceinline__ float2 shuffle2(float2 a, int o) {
+  return make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o));
+}
+__device__ __forceinline__ __half2 shuffle2(__half2 a, int o) {
+  return __shfl_xor_sync(0xffffffffu, a, o);
+}
+__device__ __forceinline__ __nv_bfloat162 shuffle2(__nv_bfloat162 a, int o) {
+  return __shfl_xor_sync(0xffffffffu, a, o);
+}
+
+// Eight values' limits, NaN above all: high the largest magnitude, or with zeros the largest
+// of w and 0, and low then the largest of -w and 0.
 template <typename T, bool kZeros>
-__device__ __forceinline__ void limits(const Pack<T, 8> &v, float &high, float &low) {
+__device__ __forceinline__ void limits(const Pack<T, 8> &v, T &high, T &low) {
   if constexpr (std::is_same<T, float>::value) {
     high = low = 0.0f;
 #pragma unroll
@@ -57,16 +87,16 @@ __device__ __forceinline__ void limits(const Pack<T, 8> &v, float &high, float &
       if (kZeros) low = most_nan(low, -v.e[j]);
     }
   } else {
-    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    using T2 = typename Two<T>::type;
     T2 h{}, l{};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const T2 w = reinterpret_cast<const T2 *>(&v)[j];
-      h = __hmax2_nan(h, kZeros ? w : __habs2(w));
-      if (kZeros) l = __hmax2_nan(l, __hneg2(w));
+      h = most2(h, kZeros ? w : __habs2(w));
+      if (kZeros) l = most2(l, __hneg2(w));
     }
-    high = most_nan(to_float(h.x), to_float(h.y));
-    low = most_nan(to_float(l.x), to_float(l.y));
+    high = __hmax_nan(h.x, h.y);
+    if (kZeros) low = __hmax_nan(l.x, l.y);
   }
 }
 
@@ -77,32 +107,34 @@ __device__ __forceinline__ uint32_t pack_nibbles(const uint32_t (&b)[8]) {
 }
 
 // Eight values an item, a group to group / 8 neighbouring lanes, a row to `lanes` threads (a
-// power of two, 32 to 256), kItems items of a thread at a time: their loads come first.
-// Bound by memory: 16384 x 4096 bf16 in groups of 128 takes 30 us, 5.6 TB/s (a thread an item
-// with a division for each value and one for its place took 91 us). kPacks: w in whole
-// 16-byte pieces and q in whole words; otherwise value by value.
+// power of two, 32 to 256), four items of a thread at a time: their loads come first, and of
+// four lanes each works out the scale of another item (two divisions each).
+// 16384 x 4096 bf16 in groups of 128 takes 41 us, of 26 for its bytes; issue is at 71% (a
+// thread an item with a division for each value and one for its place took 91 us). kPacks:
+// w in whole 16-byte pieces and q in whole words; otherwise value by value.
 constexpr int kThreads = 256, kItems = 4;
 
 template <typename T, int kGroup, bool kZeros, bool kPacks>
 __global__ void __launch_bounds__(kThreads)
     quantize_w4_kernel(const QuantArgs p, const T *w, int lanes) {
   constexpr int kLanes = kGroup / 8;
+  using T2 = typename Two<T>::type;
   griddep_wait();
   griddep_launch_dependents();
-  const int t = static_cast<int>(threadIdx.x) & (lanes - 1);
+  const int t = static_cast<int>(threadIdx.x) & (lanes - 1), lane = static_cast<int>(threadIdx.x) & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) +
                       static_cast<int>(threadIdx.x) / lanes;
   const bool live = row < p.n;
   const T *x = w + (live ? row : p.n - 1) * p.ldw;
   uint8_t *q = p.q + row * p.ldq;
-  const int items = p.groups * kLanes;
-  // whole warps go round together: a group's lanes shuffle
-  for (int base = 0; base < items; base += lanes * kItems) {
+  // One time round. `whole`: every item lies in the row.
+  const auto go = [&](int base, auto tag) {
+    constexpr bool whole = decltype(tag)::value;
     Pack<T, 8> v[kItems];
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
       const int c = (base + u * lanes + t) * 8;
-      if (kPacks && c + 8 <= p.k) {
+      if (kPacks && (whole || c + 8 <= p.k)) {
         if constexpr (sizeof(T) == 2) {
           v[u] = load_pack<T, 8>(x + c);
         } else {
@@ -111,54 +143,86 @@ __global__ void __launch_bounds__(kThreads)
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[u].e[j] = c + j < p.k ? x[c + j] : from_float<T>(0.0f);
+        for (int j = 0; j < 8; ++j)
+          v[u].e[j] = whole || c + j < p.k ? x[c + j] : from_float<T>(0.0f);
       }
     }
+    // limits of the four items' groups, two of them together
+    T2 high[2], low[2];
 #pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const int item = base + u * lanes + t, c = item * 8;
-      if (base + u * lanes >= items) break;
-      float high, low;
-      limits<T, kZeros>(v[u], high, low);
+    for (int u = 0; u < 2; ++u) {
+      limits<T, kZeros>(v[2 * u], high[u].x, low[u].x);
+      limits<T, kZeros>(v[2 * u + 1], high[u].y, low[u].y);
 #pragma unroll
       for (int o = kLanes / 2; o; o >>= 1) {
-        high = most_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
-        if (kZeros) low = most_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high[u] = most2(high[u], shuffle2(high[u], o));
+        if (kZeros) low[u] = most2(low[u], shuffle2(low[u], o));
       }
-      const Scale s =
-          split_scale(round_scale(kZeros ? (high + low) / 15.0f : high / 7.0f, p.scale_type));
-      int zero = 8;
-      if (kZeros) {
-        uint32_t z[1];
-        quotients(Pack<float, 1>{{low}}, s, z);
-        zero = min(static_cast<int>(z[0] & 0xffu), 15);
-      }
-      if (!live || c >= p.k) continue;
-      if (item % kLanes == 0) {
-        const int64_t g = item / kLanes;
-        store_scale(p.scale, p.scale_type, row * p.lds + g, s.value);
-        if (kZeros) p.zero[row * p.ldz + g] = static_cast<uint8_t>(zero);
-      }
-      uint32_t b[8];
-      quotients(v[u], s, b);
+    }
+    // item lane % 4's
+    const auto mine = [&](const T2 (&of)[2]) {
+      const T2 pair = lane & 2 ? of[1] : of[0];
+      return to_float(lane & 1 ? pair.y : pair.x);
+    };
+    const float h = mine(high), l = kZeros ? mine(low) : 0.0f;
+    const Scale s = split_scale(round_scale(kZeros ? (h + l) / 15.0f : h / 7.0f, p.scale_type));
+    int zero = 8;
+    if (kZeros) {
+      uint32_t z[1];
+      quotients(Pack<float, 1>{{l}}, s, z);
+      zero = static_cast<int>(z[0] & 0xffu);  // at most 15: l is at most 15 scales and a rounding
+    }
+    // the group's first four lanes store their items' scales
+    const int g = (base + (lane & 3) * lanes + t) / kLanes;
+    if (lane % kLanes < 4 && live && (whole || g < p.groups)) {
+      store_scale(p.scale, p.scale_type, row * p.lds + g, s.value);
+      if (kZeros) p.zero[row * p.ldz + g] = static_cast<uint8_t>(zero);
+    }
+    const bool rare = __any_sync(0xffffffffu, s.lifted);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        b[j] += zero;
-        if (kZeros) b[j] = static_cast<uint32_t>(max(0, min(15, static_cast<int>(b[j] << 24) >> 24)));
-      }
-      uint32_t word = pack_nibbles(b);
-      uint8_t *to = q + c / 2;
-      if (kPacks && c + 8 <= p.k) {
-        *reinterpret_cast<uint32_t *>(to) = word;
+    for (int u = 0; u < kItems; ++u) {
+      const int c = (base + u * lanes + t) * 8;
+      const int from = (lane & ~3) + u;
+      Scale of;
+      of.value = of.divisor = __shfl_sync(0xffffffffu, s.value, from);
+      of.inverse = __shfl_sync(0xffffffffu, s.inverse, from);
+      of.finite = of.value < CUDART_INF_F;
+      of.lifted = false;
+      const int z = kZeros ? __shfl_sync(0xffffffffu, zero, from) : 8;
+      uint32_t b[8], word;
+      if (rare) {
+        of = split_scale(of.value);
+        quotients(v[u], of, b);
       } else {
-        const int here = min(8, p.k - c);
-        if (here < 8) word &= (1u << (4 * here)) - 1u;  // the half byte behind an odd row is 0
+        finite_quotients(v[u], of, b);
+      }
+      if (kZeros) {
+        // rounded apart, the largest value and the zero may come to 16
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          b[j] = static_cast<uint32_t>(min((static_cast<int>(b[j] << 24) >> 24) + z, 15));
+        word = pack_nibbles(b);
+      } else {
+        word = pack_nibbles(b) ^ 0x88888888u;  // plus 8 in 4 bits
+      }
+      if (!of.finite) word = kZeros ? 0u : 0x88888888u;
+      uint8_t *to = q + c / 2;
+      if (kPacks && (whole || c + 8 <= p.k)) {
+        if (live) *reinterpret_cast<uint32_t *>(to) = word;
+      } else if (live) {
+        const int here = min(8, p.k - c);  // may be none or negative
+        if (here < 8) word &= (1u << (4 * max(here, 0))) - 1u;  // the half byte behind an odd row is 0
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (2 * j < here) to[j] = static_cast<uint8_t>(word >> (8 * j));
       }
     }
-  }
+  };
+  // whole warps go round together: a group's lanes shuffle
+  const int each = lanes * kItems;
+  int base = 0;
+  for (; (base + each) * 8 <= p.k; base += each) go(base, std::true_type());
+  for (; base < p.groups * kLanes; base += each) go(base, std::false_type());
 }
 
 template <typename T, int kGroup>
