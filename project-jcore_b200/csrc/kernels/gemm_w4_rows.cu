@@ -1,16 +1,18 @@
 // 4-bit product for few tokens: the weights' bytes are what there is to do.
 //
-// A team of `slices` warps takes 16 channels at a time and shares K; a CTA holds `teams` of
+// A team of `slices` warps takes 32 channels at a time and shares K; a CTA holds `teams` of
 // them and goes round the channels with the other CTAs, one CTA to an SM. mma.sync m16n8k16
-// with the channels as its rows: lane (g, t) holds channels g and g + 8 and token g. Which
-// values of K a lane takes is free as long as weights and x agree, so a lane takes whole
-// 32-bit words of eight nibbles, which come apart as the pairs (0, 4), (1, 5) for one mma
-// and (2, 6), (3, 7) for the next; x lies in shared memory in that order. All lanes of one
-// mma must lie in one group: for groups of 32, 64, 128 lane t takes 1, 2, 4 words in a row of each
-// (its "run"), one load of shared memory each.
+// with the channels as its rows: lane (g, t) holds channels g, g + 8, g + 16 and g + 24 (two
+// products) and token g. Which values of K a lane takes is free as long as weights and x
+// agree, so a lane takes whole 32-bit words of eight nibbles, which come apart as the pairs
+// (0, 4), (1, 5) for one mma and (2, 6), (3, 7) for the next; x lies in shared memory in that
+// order. All lanes of one mma must lie in one group: for groups of 32, 64, 128 lane t takes
+// 1, 2, 4 words in a row of each (its "run"), one load of shared memory each.
 //
 // Weights go by cp.async through a ring of each warp's own, across the ends of tiles: no
-// barrier but the team's own, once per 16 channels, to add its sums.
+// barrier but the team's own, once per 32 channels, to add its sums. Beside the bytes, issue
+// is what counts: NN instructions a stage of 32 x 256 weights (16 channels a stage took 1.8 times as many
+// for the same weights).
 #include <algorithm>
 #include <cmath>
 
@@ -20,20 +22,24 @@
 namespace nplk {
 namespace {
 
+constexpr int kRows = 32;                 // channels of a tile
 constexpr int kStageK = 256;              // values of K a warp takes at a time
 constexpr int kStagePitch = kStageK / 2;  // bytes
-constexpr int kStageBytes = 16 * kStagePitch;
-constexpr int kDepth = 3;                 // stages in flight and at work
+constexpr int kStageBytes = kRows * kStagePitch;
+constexpr int kDepth = 2;                 // stages in flight and at work
 constexpr int kMostWarps = 16;
-constexpr int kMostX = 96 * 1024;         // bytes of x in shared memory
-static_assert(kMostX + kMostWarps * (kDepth * kStageBytes + 2 * 2 * 512) <= 232448, "shared memory");
+constexpr int kMostX = 64 * 1024;         // bytes of x in shared memory
+constexpr int kRedBytes = kRows * 8 * 4;  // sums of a warp and eight tokens
+static_assert(kMostX + kMostWarps * (kDepth * kStageBytes + 2 * kRedBytes) <= 232448,
+              "shared memory");
 
 struct RowsPlan {
   int slices, teams;
-  int steps;    // stages of K a warp takes for 16 channels
-  int tiles;    // of 16 channels
+  int steps;    // stages of K a warp takes for a tile
+  int tiles;
   int x_units;  // 16-byte units of x in shared memory
   int x_bytes;  // their room, whole 128 bytes: the ring behind it is swizzled by address
+  int packed;   // a stage's scales of a channel as one aligned piece
 };
 
 __device__ __forceinline__ void team_sync(int team, int threads) {
@@ -54,14 +60,15 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[kWord
   }
 }
 
+// NT: tokens in eights. Sums of a team have two buffers where NT is 1, so that one barrier a
+// round keeps the next round's sums off this round's readers; else two barriers.
 template <typename X, int NT, bool kZeros, int kGroup>
-__global__ void __launch_bounds__(kMostWarps * 32)
+__global__ void __launch_bounds__(kMostWarps * 32, 1)
     gemm_w4_rows_kernel(const W4Args p, const RowsPlan plan) {
   using F = typename W4Type<X>::Frag;
   constexpr int P = W4Type<X>::kParts;
-  constexpr int kRun = kGroup / 32;                 // words of a lane in a group
-  constexpr int kGroups = kStageK / kGroup;         // groups of a stage
-  constexpr int kHeld = kGroups >= 2 ? kGroups / 2 : 1;  // of them, held by each half of the lanes
+  constexpr int kRun = kGroup / 32;          // words of a lane in a group
+  constexpr int kGroups = kStageK / kGroup;  // groups of a stage
   extern __shared__ __align__(128) uint8_t smem[];
   const int warps = plan.slices * plan.teams;
   uint4 *sx = reinterpret_cast<uint4 *>(smem);
@@ -82,34 +89,40 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   uint8_t *mine = ring + warp * (kDepth * kStageBytes);
 
   // What is copied next: a stage of a tile, into a slot of the ring. Lane l copies the
-  // 16 bytes l % 8 of rows l / 8, + 4, + 8, + 12; those are swizzled within their row.
+  // 16 bytes l % 8 of rows l / 8, + 4, ... + 28; those are swizzled within their row.
   const int piece = lane & 7, c_r = lane >> 3;
   const uint32_t c_to = smem_u32(mine + c_r * kStagePitch + ((piece ^ (c_r * kRun & 7)) << 4));
   const int byte0 = k_begin / 2 + piece * 16;
+  const bool no_tail = (k_begin + steps * kStageK) / 2 <= row_bytes;
   int c_round = steps ? 0 : rounds, c_step = 0, c_slot = 0;
-  const uint8_t *c_row[4];
+  const uint8_t *c_row;  // of row c_r
+  int64_t c_four;        // bytes from one of the lane's rows to the next
+  int c_most;            // rows of the lane in the weights, less one
   const auto aim = [&](int round) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = static_cast<int64_t>(tile0 + round * stride) * 16 + j * 4 + c_r;
-      // rows past the last are read as the last, their results dropped
-      c_row[j] = p.q + (n < p.N ? n : p.N - 1) * p.ldq;
-    }
+    const int64_t n = static_cast<int64_t>(tile0 + round * stride) * kRows + c_r;
+    // rows past the last are read as the lane's last, or the tile's first, their results dropped
+    const int64_t left = p.N - 1 - n;
+    c_most = left < 0 ? 0 : static_cast<int>(left < 28 ? left >> 2 : 7);
+    c_row = p.q + (n < p.N ? n : p.N - 1) * p.ldq;
   };
+  c_four = 4 * p.ldq;
   aim(0);
   const auto issue = [&] {
     if (c_round < rounds) {
       const int at = byte0 + c_step * (kStageK / 2);
-      const int valid = max(0, min(16, row_bytes - at));  // of the 16 bytes; zeros for the rest
-      const int from = valid ? at : 0;
+      // of the 16 bytes; zeros for the rest
+      const int valid = no_tail ? 16 : max(0, min(16, row_bytes - at));
+      const uint8_t *from = c_row + (valid ? at : 0);
       const uint32_t to = c_to + static_cast<uint32_t>(c_slot * kStageBytes);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 8; ++j) {
         // (rows 4 apart differ in their swizzle where a row's step of it is 1)
         asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(
                          (kRun == 1 && (j & 1) ? to ^ 64u : to) + j * 4 * kStagePitch),
-                     "l"(c_row[j] + from), "r"(valid)
+                     "l"(from), "r"(valid)
                      : "memory");
+        if (j < c_most) from += c_four;
+      }
       if (++c_step == steps) {
         c_step = 0;
         ++c_round;
@@ -120,28 +133,43 @@ __global__ void __launch_bounds__(kMostWarps * 32)
     copy_async_commit();
   };
 
-  // Scales (and zeros) of a stage, loaded one stage ahead: lane l holds those of channel
-  // l % 16, of the stage's first (l < 16) or second half.
-  float sc[kHeld];
-  uint32_t sc_next[kHeld];
-  int ze[kHeld], ze_next[kHeld];
+  // Scales (and zeros) of a stage, loaded one stage ahead: lane l holds those of channel l.
+  uint32_t sc_next[kGroups];
+  int ze_next[kGroups];
   int64_t s_row = 0, z_row = 0;
   const auto aim_scales = [&](int round) {
     // past the last channel or group: the last one's, for results that are dropped and
     // inputs that are 0
-    const int64_t at = static_cast<int64_t>(tile0 + round * stride) * 16 + (lane & 15);
+    const int64_t at = static_cast<int64_t>(tile0 + round * stride) * kRows + lane;
     const int64_t n = at < p.N ? at : p.N - 1;
     s_row = n * p.lds;
     if (kZeros) z_row = n * p.ldz;
   };
-  const int held0 = k_begin / kGroup + (lane >> 4) * kHeld;
   const auto fetch = [&](int step) {
-    const int g0 = held0 + step * kGroups;
+    const int g0 = (k_begin + step * kStageK) / kGroup;
+    if (plan.packed && g0 + kGroups <= p.groups) {  // 16-bit scales, whole pieces of 2 kGroups bytes
+      const unsigned short *from = static_cast<const unsigned short *>(p.scale) + s_row + g0;
+      uint32_t w[kGroups / 2];
+      if constexpr (kGroups == 2) {
+        w[0] = __ldg(reinterpret_cast<const unsigned int *>(from));
+      } else if constexpr (kGroups == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(from));
+        w[0] = v.x, w[1] = v.y;
+      } else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(from));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      }
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      const int group = min(g0 + j, p.groups - 1);
-      sc_next[j] = load_scale_bits(p.scale, p.scale_type, s_row + group);
-      if (kZeros) ze_next[j] = __ldg(p.zero + z_row + group) & 15;
+      for (int j = 0; j < kGroups; ++j) sc_next[j] = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+        sc_next[j] = load_scale_bits(p.scale, p.scale_type, s_row + min(g0 + j, p.groups - 1));
+    }
+    if (kZeros) {
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+        ze_next[j] = __ldg(p.zero + z_row + min(g0 + j, p.groups - 1)) & 15;
     }
   };
 
@@ -200,16 +228,17 @@ __global__ void __launch_bounds__(kMostWarps * 32)
   for (int n = 0; n < NT; ++n) x_at[n] = min(n * 8 + g, p.M - 1) * 4 + t;
   const int chunks_all = (p.K + kGroup - 1) / kGroup;
   for (int round = 0; round < rounds; ++round) {
-    const int tile = tile0 + round * stride;
-    const int64_t n_out = static_cast<int64_t>(tile) * 16 + (lane & 15);
+    const int64_t n_out = static_cast<int64_t>(tile0 + round * stride) * kRows + lane;
     const float bias = p.bias && n_out < p.N ? __ldg(p.bias + n_out) : 0.0f;
-    float acc[NT][4] = {};
+    float acc[2][NT][4] = {};
     for (int step = 0; step < steps; ++step) {
       issue();
+      float sc[kGroups];
+      uint32_t offs[kGroups];  // low and high offset of the zero, a half each
 #pragma unroll
-      for (int j = 0; j < kHeld; ++j) {
+      for (int j = 0; j < kGroups; ++j) {
         sc[j] = scale_value(sc_next[j], p.scale_type);
-        if (kZeros) ze[j] = ze_next[j];
+        if (kZeros) offs[j] = F::low_offset(ze_next[j]) | F::high_offset(ze_next[j]) << 16;
       }
       if (step + 1 < steps) {
         fetch(step + 1);
@@ -222,74 +251,88 @@ __global__ void __launch_bounds__(kMostWarps * 32)
       const uint8_t *st = mine + slot * kStageBytes + g * kStagePitch;
       slot = slot + 1 == kDepth ? 0 : slot + 1;
       const int chunk0 = (k_begin + step * kStageK) / kGroup;
+      const uint4 *xs = sx + chunk0 * x_chunk;
 #pragma unroll
-      for (int c = 0; c < kGroups; ++c) {
+      for (int c = 0; c < kGroups; ++c, xs += x_chunk) {
         if (chunk0 + c >= chunks_all) break;
-        const int from = c / kHeld * 16;
-        const float s0 = __shfl_sync(0xffffffffu, sc[c % kHeld], from + g);
-        const float s1 = __shfl_sync(0xffffffffu, sc[c % kHeld], from + g + 8);
-        W4Offsets off0 = w4_offsets<F>(8), off1 = off0;
-        if (kZeros) {
-          off0 = w4_offsets<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g));
-          off1 = w4_offsets<F>(__shfl_sync(0xffffffffu, ze[c % kHeld], from + g + 8));
-        }
-        uint32_t a[kRun], b[kRun];
+        uint32_t w[4][kRun];
         // rows are swizzled by 16-byte pieces, so that the 8 rows of a load miss each other's banks
         const int at = (c * (kGroup / 2) + t * (4 * kRun)) ^ swizzle;
-        load_words<kRun>(st + at, a);
-        load_words<kRun>(st + 8 * kStagePitch + at, b);
-        const uint4 *xs = sx + (chunk0 + c) * x_chunk;
-        float part[NT][4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) load_words<kRun>(st + h * (8 * kStagePitch) + at, w[h]);
+        W4Offsets off[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          if (kZeros) {
+            const uint32_t both_of = __shfl_sync(0xffffffffu, offs[c], h * 8 + g);
+            off[h] = {__byte_perm(both_of, 0u, 0x1010), __byte_perm(both_of, 0u, 0x3232)};
+          } else {
+            off[h] = w4_offsets<F>(8);
+          }
+        }
+        float part[2][NT][4];
 #pragma unroll
         for (int r = 0; r < kRun; ++r) {
-          uint32_t w0[4], w1[4];
-          w4_widen<F>(a[r], off0, w0);
-          w4_widen<F>(b[r], off1, w1);
+          uint32_t wide[4][4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) w4_widen<F>(w[h][r], off[h], wide[h]);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int q = 0; q < P; ++q) {
               // tokens past the last are read as the last, their results dropped
               const uint4 v = xs[(r * P + q) * x_part + x_at[n]];
-              if (r == 0 && q == 0) {
-                const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                F::mma(part[n], none, w0[0], w1[0], w0[1], w1[1], v.x, v.y);
-              } else {
-                F::mma(part[n], part[n], w0[0], w1[0], w0[1], w1[1], v.x, v.y);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const auto &a = wide[2 * h], &b = wide[2 * h + 1];
+                if (r == 0 && q == 0) {
+                  const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                  F::mma(part[h][n], none, a[0], b[0], a[1], b[1], v.x, v.y);
+                } else {
+                  F::mma(part[h][n], part[h][n], a[0], b[0], a[1], b[1], v.x, v.y);
+                }
+                F::mma(part[h][n], part[h][n], a[2], b[2], a[3], b[3], v.z, v.w);
               }
-              F::mma(part[n], part[n], w0[2], w1[2], w0[3], w1[3], v.z, v.w);
             }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
-          acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
-          acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
-          acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
+        for (int h = 0; h < 2; ++h) {
+          const float s0 = __shfl_sync(0xffffffffu, sc[c], h * 16 + g);
+          const float s1 = __shfl_sync(0xffffffffu, sc[c], h * 16 + 8 + g);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[h][n][0] = fmaf(s0, part[h][n][0], acc[h][n][0]);
+            acc[h][n][1] = fmaf(s0, part[h][n][1], acc[h][n][1]);
+            acc[h][n][2] = fmaf(s1, part[h][n][2], acc[h][n][2]);
+            acc[h][n][3] = fmaf(s1, part[h][n][3], acc[h][n][3]);
+          }
         }
       }
       __syncwarp();  // the stage has been read: the next issue writes over it
     }
-    // the team's sums meet, [token][channel]; two buffers, so that one barrier a round
-    // keeps the next round's sums off this round's readers
-    float *buffer = red + (round & 1) * warps * (NT * 128);
-    float *to = buffer + warp * (NT * 128);
+    // the team's sums meet, [token][channel]
+    constexpr int kSums = NT * 8 * kRows;
+    if (NT > 1) team_sync(team, plan.slices * 32);
+    float *buffer = red + (NT == 1 ? (round & 1) * warps * kSums : 0);
+    float *to = buffer + warp * kSums;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float *r = to + (8 * n + 2 * t) * 16 + g;
-      r[0] = acc[n][0];
-      r[16] = acc[n][1];
-      r[8] = acc[n][2];
-      r[24] = acc[n][3];
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float *r = to + (8 * n + 2 * t) * kRows + h * 16 + g;
+        r[0] = acc[h][n][0];
+        r[kRows] = acc[h][n][1];
+        r[8] = acc[h][n][2];
+        r[kRows + 8] = acc[h][n][3];
+      }
     team_sync(team, plan.slices * 32);
-    const float *sums = buffer + team * plan.slices * (NT * 128);
-    for (int i = slice * 32 + lane; i < p.M * 16; i += plan.slices * 32) {
+    const float *sums = buffer + team * plan.slices * kSums + lane;
+    for (int m = slice; m < p.M; m += plan.slices) {
       float v[1] = {0.0f};
 #pragma unroll 4
-      for (int s = 0; s < plan.slices; ++s) v[0] += sums[s * (NT * 128) + i];
+      for (int s = 0; s < plan.slices; ++s) v[0] += sums[s * kSums + m * kRows];
       v[0] = fmaf(v[0], F::kUnit, bias);
-      if (n_out < p.N) w4_store<1>(p, (i >> 4) * p.ldc + n_out, v, 1, false);
+      if (n_out < p.N) w4_store<1>(p, m * p.ldc + n_out, v, 1, false);
     }
   }
   copy_async_wait<0>();
@@ -320,13 +363,13 @@ bool gemm_w4_rows_fits(const W4Args &p) {
          (p.ldq % 16 == 0 || p.N == 1);
 }
 
-// Slices and teams of least estimated time: rounds of (stages of K, 0.75 us each for 16
+// Slices and teams of least estimated time: rounds of (stages of K, 1.5 us each for 16
 // warps at the memory's rate and hardly less for few, and the sums' meeting), and x's way into
 // shared memory.
 int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
   RowsPlan plan{};
   const int64_t sms = sm_count(), stages = ceil_div(p.K, kStageK);
-  plan.tiles = static_cast<int>(ceil_div(p.N, 16));
+  plan.tiles = static_cast<int>(ceil_div(p.N, kRows));
   double least = 1e30;
   for (int64_t want = 1; want <= std::min<int64_t>(stages, kMostWarps); ++want) {
     const int64_t steps = ceil_div(stages, want), slices = ceil_div(stages, steps);
@@ -335,7 +378,7 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
     const double warps = static_cast<double>(slices * teams);
     const double us =
         static_cast<double>(rounds) *
-            (std::max(0.046 * static_cast<double>(steps) * warps, 0.35 * static_cast<double>(steps)) +
+            (std::max(0.093 * static_cast<double>(steps) * warps, 0.5 * static_cast<double>(steps)) +
              0.3) +
         0.6 * std::ceil(static_cast<double>(ceil_div(p.K, 8) * p.M) / (32.0 * warps));
     if (us < least) {
@@ -347,8 +390,12 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
   }
   plan.x_units = static_cast<int>(x_units(p));
   plan.x_bytes = static_cast<int>(align_up(static_cast<size_t>(plan.x_units) * 16, 128));
+  // pieces of 2 (256 / group) bytes
+  const int64_t piece = kStageK / p.group;
+  plan.packed = p.scale_type != NPLK_DTYPE_FP32 && p.lds % piece == 0 &&
+                reinterpret_cast<uintptr_t>(p.scale) % (2 * piece) == 0;
   const int warps = plan.slices * plan.teams, nt = p.M <= 8 ? 1 : 2;
-  const int smem = plan.x_bytes + warps * kDepth * kStageBytes + 2 * warps * nt * 512;
+  const int smem = plan.x_bytes + warps * (kDepth * kStageBytes + 2 * kRedBytes);
   auto *fn = p.x_type == NPLK_DTYPE_FP32   ? (nt == 1 ? pick<float, 1>(p) : pick<float, 2>(p))
              : p.x_type == NPLK_DTYPE_FP16 ? (nt == 1 ? pick<__half, 1>(p) : pick<__half, 2>(p))
                                            : (nt == 1 ? pick<__nv_bfloat16, 1>(p)
