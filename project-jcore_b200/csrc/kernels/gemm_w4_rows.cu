@@ -10,9 +10,14 @@
 // 1, 2, 4 words in a row of each (its "run"), one load of shared memory each.
 //
 // Weights go by cp.async through a ring of each warp's own, across the ends of tiles: no
-// barrier but the team's own, once per 32 channels, to add its sums. Beside the bytes, issue
-// is what counts: NN instructions a stage of 32 x 256 weights (16 channels a stage took 1.8 times as many
-// for the same weights).
+// barrier but the team's own, once per 32 channels, to add its sums. What bounds it: the
+// widening's instructions as much as the bytes where there are many channels (16 channels a
+// tile, with twice the loads of x and of scales to a weight, took 82 us where 32 take 67), and
+// the latencies of a start, a stage and a meeting where there are few.
+//
+// Measured (group 128, cold weights): 1 x 4096 x 4096 bf16 6.7 us, 8 tokens 8.2;
+// 4 x 128000 x 4096 fp16 67 us, of which the bytes are 43; 8 x 128000 x 4096 bf16 with groups
+// of 32 78 us.
 #include <algorithm>
 #include <cmath>
 
@@ -37,8 +42,8 @@ struct RowsPlan {
   int slices, teams;
   int steps;    // stages of K a warp takes for a tile
   int tiles;
-  int x_units;  // 16-byte units of x in shared memory
-  int x_bytes;  // their room, whole 128 bytes: the ring behind it is swizzled by address
+  FastDiv words;  // eights of a token's values, padded to whole groups
+  int x_bytes;  // room of x, whole 128 bytes: the ring behind it is swizzled by address
   int packed;   // a stage's scales of a channel as one aligned piece
 };
 
@@ -58,6 +63,18 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[kWord
   } else {
     w[0] = *reinterpret_cast<const uint32_t *>(p);
   }
+}
+
+// Zeros where there is nothing. No branch: the compiler waits for a load where its branch
+// joins, and one latency per load was half of a small call of eight tokens.
+__device__ __forceinline__ uint4 load_if(const void *p, bool there) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  asm volatile(
+      "{\n\t.reg .pred there;\n\tsetp.ne.u32 there, %5, 0;\n\t"
+      "@there ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(p), "r"(static_cast<uint32_t>(there)));
+  return v;
 }
 
 // NT: tokens in eights. Sums of a team have two buffers where NT is 1, so that one barrier a
@@ -134,9 +151,10 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1)
   };
 
   // Scales (and zeros) of a stage, loaded one stage ahead: lane l holds those of channel l.
-  uint32_t sc_next[kGroups];
+  uint32_t sc_next[kGroups];  // as loaded: packed pairs in the first half, or one each
   int ze_next[kGroups];
   int64_t s_row = 0, z_row = 0;
+  bool pairs = false;
   const auto aim_scales = [&](int round) {
     // past the last channel or group: the last one's, for results that are dropped and
     // inputs that are 0
@@ -149,19 +167,18 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1)
     const int g0 = (k_begin + step * kStageK) / kGroup;
     if (plan.packed && g0 + kGroups <= p.groups) {  // 16-bit scales, whole pieces of 2 kGroups bytes
       const unsigned short *from = static_cast<const unsigned short *>(p.scale) + s_row + g0;
-      uint32_t w[kGroups / 2];
+      pairs = true;
       if constexpr (kGroups == 2) {
-        w[0] = __ldg(reinterpret_cast<const unsigned int *>(from));
+        sc_next[0] = __ldg(reinterpret_cast<const unsigned int *>(from));
       } else if constexpr (kGroups == 4) {
         const uint2 v = __ldg(reinterpret_cast<const uint2 *>(from));
-        w[0] = v.x, w[1] = v.y;
+        sc_next[0] = v.x, sc_next[1] = v.y;
       } else {
         const uint4 v = __ldg(reinterpret_cast<const uint4 *>(from));
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        sc_next[0] = v.x, sc_next[1] = v.y, sc_next[2] = v.z, sc_next[3] = v.w;
       }
-#pragma unroll
-      for (int j = 0; j < kGroups; ++j) sc_next[j] = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
     } else {
+      pairs = false;
 #pragma unroll
       for (int j = 0; j < kGroups; ++j)
         sc_next[j] = load_scale_bits(p.scale, p.scale_type, s_row + min(g0 + j, p.groups - 1));
@@ -173,50 +190,83 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1)
     }
   };
 
+  // x into shared memory: unit w of a token holds the pairs of its eight values from 8 w on,
+  // zeros behind K, each part by itself. In a chunk of 4 kRun units lane t of a quad takes units
+  // t kRun + r, r = 0 .. kRun - 1; (chunk, r, part, token, t) lies at
+  // (((chunk kRun + r) P + part) M + token) 4 + t.
+  const X *x = static_cast<const X *>(p.x);
+  const bool packs = reinterpret_cast<uintptr_t>(x) % 16 == 0 && p.ldx * sizeof(X) % 16 == 0 &&
+                     p.K % p.group == 0;
+  const int words = static_cast<int>(plan.words.d), all_words = words * p.M;
+  struct Unit {
+    uint4 v[sizeof(X) / 2];
+  };
+  const auto load_unit = [&](int u) {
+    Unit unit;
+    const int m = static_cast<int>(fdiv(u, plan.words));
+    const X *from = x + m * p.ldx + (u - m * words) * 8;
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(X)) / 2; ++j)
+      unit.v[j] = load_if(from + j * (16 / sizeof(X)), u < all_words);
+    return unit;
+  };
+  const auto load_ragged = [&](int u) {
+    Unit unit{};
+    const int m = static_cast<int>(fdiv(u, plan.words)), k = (u - m * words) * 8;
+    const X *from = x + m * p.ldx + k;
+    X *v = reinterpret_cast<X *>(&unit);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < p.K) v[j] = from[j];
+    return unit;
+  };
+  const auto store_unit = [&](int u, const Unit &unit) {
+    const int m = static_cast<int>(fdiv(u, plan.words)), w = u - m * words;
+    const int chunk = w / (4 * kRun), in = w % (4 * kRun), lane_t = in / kRun, r = in % kRun;
+    const X *v = reinterpret_cast<const X *>(&unit);
+    uint32_t h[P][4];  // pairs (0, 4), (1, 5), ... of each part
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (P == 3) {
+        uint32_t parts[3];
+        w4_split3(v[j], v[j + 4], parts);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
+      } else {
+        h[0][j] = reinterpret_cast<const uint16_t &>(v[j]) |
+                  static_cast<uint32_t>(reinterpret_cast<const uint16_t &>(v[j + 4])) << 16;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+      sx[(((chunk * kRun + r) * P + q) * p.M + m) * 4 + lane_t] =
+          make_uint4(h[q][0], h[q][1], h[q][2], h[q][3]);
+  };
+
+  // all of the first loads before any of them is waited for: weights, x, scales
+  constexpr int kUnits = 16 / sizeof(X);
+  const int threads = static_cast<int>(blockDim.x), first = static_cast<int>(threadIdx.x);
+  Unit units[kUnits];
 #pragma unroll
   for (int i = 0; i < kDepth - 1; ++i) issue();
+  if (packs) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) units[i] = load_unit(first + i * threads);
+  }
   aim_scales(0);
   fetch(0);
-
-  // x into shared memory: unit (block of 32 values b, word w of it) -> pairs of its eight
-  // values, zeros behind K. A lane's words of K in step r of a run: block (run's first)
-  // + its share; the unit of (chunk of 4 kRun words, r, t) lies at ((chunk kRun + r) M + m) 4 + t.
-  {
-    const X *x = static_cast<const X *>(p.x);
-    const int words = plan.x_units / (P * p.M);  // of eight values, padded to whole chunks
-    const bool packs = reinterpret_cast<uintptr_t>(x) % 16 == 0 && p.ldx * sizeof(X) % 16 == 0;
-#pragma unroll 2
-    for (int u = threadIdx.x; u < words * p.M; u += blockDim.x) {
-      const int m = u / words, w = u - m * words, k = w * 8;
-      const int chunk = w / (4 * kRun), in = w % (4 * kRun), lane_t = in / kRun, r = in % kRun;
-      const X *from = x + m * p.ldx + k;
-      X v[8];
-      if (packs && k + 8 <= p.K) {
+  if (packs) {
+    for (int u = first;;) {
 #pragma unroll
-        for (int j = 0; j < 8; j += 16 / sizeof(X))
-          *reinterpret_cast<Pack<X, 16 / sizeof(X)> *>(v + j) = load_pack<X, 16 / sizeof(X)>(from + j);
-      } else {
+      for (int i = 0; i < kUnits; ++i)
+        if (u + i * threads < all_words) store_unit(u + i * threads, units[i]);
+      u += kUnits * threads;
+      if (u >= all_words) break;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? from[j] : from_float<X>(0.0f);
-      }
-      uint32_t h[P][4];  // pairs (0, 4), (1, 5), ... of each part
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (P == 3) {
-          uint32_t parts[3];
-          w4_split3(v[j], v[j + 4], parts);
-#pragma unroll
-          for (int q = 0; q < 3; ++q) h[q][j] = parts[q];
-        } else {
-          h[0][j] = reinterpret_cast<const uint16_t &>(v[j]) |
-                    static_cast<uint32_t>(reinterpret_cast<const uint16_t &>(v[j + 4])) << 16;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < P; ++q)
-        sx[(((chunk * kRun + r) * P + q) * p.M + m) * 4 + lane_t] =
-            make_uint4(h[q][0], h[q][1], h[q][2], h[q][3]);
+      for (int i = 0; i < kUnits; ++i) units[i] = load_unit(u + i * threads);
     }
+  } else {
+    for (int u = first; u < all_words; u += threads) store_unit(u, load_ragged(u));
   }
   __syncthreads();
 
@@ -237,7 +287,8 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1)
       uint32_t offs[kGroups];  // low and high offset of the zero, a half each
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) {
-        sc[j] = scale_value(sc_next[j], p.scale_type);
+        const uint32_t pair = sc_next[j / 2];
+        sc[j] = scale_value(!pairs ? sc_next[j] : j & 1 ? pair >> 16 : pair & 0xffffu, p.scale_type);
         if (kZeros) offs[j] = F::low_offset(ze_next[j]) | F::high_offset(ze_next[j]) << 16;
       }
       if (step + 1 < steps) {
@@ -358,6 +409,9 @@ auto pick(const W4Args &p) {
 
 }  // namespace
 
+// Up to 16 tokens, as far as x fits, this way is the faster or even, against the tensor cores'
+// tiles of 32 tokens: 1 and 8 x 4096 x 4096 bf16 6.7 and 8.2 us (9.1, 9.2), 1 x 16384 x 4096
+// 12 (17), 16 x 128000 x 2048 52 (77), 16 x 4096 x 2048 7.9 (7.6).
 bool gemm_w4_rows_fits(const W4Args &p) {
   return p.M <= 16 && x_units(p) * 16 <= kMostX && reinterpret_cast<uintptr_t>(p.q) % 16 == 0 &&
          (p.ldq % 16 == 0 || p.N == 1);
@@ -380,7 +434,7 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
         static_cast<double>(rounds) *
             (std::max(0.093 * static_cast<double>(steps) * warps, 0.5 * static_cast<double>(steps)) +
              0.3) +
-        0.6 * std::ceil(static_cast<double>(ceil_div(p.K, 8) * p.M) / (32.0 * warps));
+        0.15 * std::ceil(static_cast<double>(ceil_div(p.K, 8) * p.M) / (32.0 * warps));
     if (us < least) {
       least = us;
       plan.steps = static_cast<int>(steps);
@@ -388,8 +442,8 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
       plan.teams = static_cast<int>(teams);
     }
   }
-  plan.x_units = static_cast<int>(x_units(p));
-  plan.x_bytes = static_cast<int>(align_up(static_cast<size_t>(plan.x_units) * 16, 128));
+  plan.words = make_fastdiv(static_cast<uint32_t>(ceil_div(p.K, p.group) * (p.group / 8)));
+  plan.x_bytes = static_cast<int>(align_up(static_cast<size_t>(x_units(p)) * 16, 128));
   // pieces of 2 (256 / group) bytes
   const int64_t piece = kStageK / p.group;
   plan.packed = p.scale_type != NPLK_DTYPE_FP32 && p.lds % piece == 0 &&
