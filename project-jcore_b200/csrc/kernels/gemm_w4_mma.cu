@@ -22,21 +22,25 @@ namespace {
 constexpr int kChannels = 128, kBK = 128;  // of a tile; values of K a stage
 constexpr int kRawBytes = kChannels * (kBK / 2);
 constexpr int kACols = kBK / 2;            // TMEM columns of a stage's widened weights
-// Warpgroups: TMA and MMA issue; epilogue (two); widening (two); x where it does not
-// come by TMA (two). A stage's chain of waits, loads and stores is long against its products,
-// so roles come in two teams that take every second stage or group: MMA issue, widening
-// and, up to 64 tokens, the epilogue.
-constexpr int kEpiFirst = 4, kEpiWarps = 8, kWideFirst = kEpiFirst + kEpiWarps, kWideWarps = 8,
-              kXFirst = kWideFirst + kWideWarps, kXWarps = 8;
-
-// Threads, and registers a thread: at launch, and as the warpgroups share them.
-template <bool kTma>
+// Warpgroups: TMA and MMA issue; epilogue; widening (two); x where it does not come by TMA
+// (two). A stage's chain of waits, loads and stores is long against its products, so roles
+// come in two teams that take every second stage or group: MMA issue, widening and, up to 64
+// tokens, the epilogue.
+//
+// Warps, threads, and registers a thread: at launch, and as the warpgroups share them.
+template <int NTOK, int kGroup, bool kTma>
 struct MmaThreads {
-  static constexpr int kThreads = 32 * (kXFirst + (kTma ? 0 : kXWarps));
-  static constexpr int kLaunch = kTma ? 96 : 72;
-  static constexpr int kIssue = kTma ? 48 : 40, kEpi = kTma ? 136 : 88, kWide = kTma ? 80 : 64, kX = 72;
+  static constexpr bool kMany = kTma && (NTOK == 128 || kGroup < 128);
+  static constexpr int kEpiFirst = 4, kEpiWarps = kMany ? 16 : 8,
+                       kWideFirst = kEpiFirst + kEpiWarps, kWideWarps = 8,
+                       kXFirst = kWideFirst + kWideWarps, kXWarps = kTma ? 0 : 8;
+  static constexpr int kThreads = 32 * (kXFirst + kXWarps);
+  static constexpr int kLaunch = kTma && !kMany ? 96 : 72;
+  static constexpr int kIssue = kTma && !kMany ? 48 : 40,
+                       kEpi = !kTma ? 88 : kMany ? 80 : 136, kWide = kTma && !kMany ? 80 : 64,
+                       kX = 72;
   static_assert(kIssue * 128 + kEpi * 32 * kEpiWarps + kWide * 32 * kWideWarps +
-                        (kTma ? 0 : kX * 32 * kXWarps) <=
+                        kX * 32 * kXWarps <=
                     kLaunch * kThreads,
                 "register shares");
   static_assert(kLaunch * kThreads <= 65536 && (kLaunch + 8) * kThreads > 65536,
@@ -44,12 +48,12 @@ struct MmaThreads {
 };
 
 // P parts of x.
-template <int NTOK, int P, bool kTma>
+template <int NTOK, int P, int kGroup, bool kTma>
 struct MmaTraits {
-  // Epilogue teams, and the tokens of one of their warps. Two teams of a warp for each quadrant
-  // of lanes, or one of two warps that halve the tokens (whose sums would not fit otherwise).
+  // Epilogue teams, and the tokens of one of their warps, whose sums it holds.
   static constexpr int kTeams = NTOK <= 64 && kTma ? 2 : 1;
-  static constexpr int kCols = kTeams == 2 ? NTOK : NTOK / 2;
+  static constexpr int kParts = MmaThreads<NTOK, kGroup, kTma>::kEpiWarps / 4 / kTeams;
+  static constexpr int kCols = NTOK / kParts;
   static constexpr int kXAtom = NTOK * 128;  // NTOK rows x 64 values
   static constexpr int kXBytes = 2 * kXAtom * P;
   // Rings: widened weights in TMEM, x (its loads take some 2000 cycles, of which a stage of 64
@@ -123,14 +127,14 @@ __device__ __forceinline__ void tmem_ld(uint32_t from, uint32_t (&v)[kCols]) {
 }
 
 template <typename X, int NTOK, int kGroup, bool kTma>
-__global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
+__global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
     gemm_w4_mma_kernel(const __grid_constant__ CUtensorMap map_w,
                        const __grid_constant__ CUtensorMap map_x, const W4Args p,
                        const MmaPlan plan) {
   using F = typename W4Type<X>::Frag;
   constexpr int P = W4Type<X>::kParts;
-  using Tr = MmaTraits<NTOK, P, kTma>;
-  using Th = MmaThreads<kTma>;
+  using Tr = MmaTraits<NTOK, P, kGroup, kTma>;
+  using Th = MmaThreads<NTOK, kGroup, kTma>;
   constexpr int kPer = kBK / kGroup;  // groups a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align_smem_1024(smem_raw);
@@ -154,20 +158,20 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < Tr::kA; ++i) {
-      mbar_init(&a_full[i], kWideWarps / 2);
+      mbar_init(&a_full[i], Th::kWideWarps / 2);
       mbar_init(&a_empty[i], 1);
     }
     for (int i = 0; i < Tr::kX; ++i) {
-      mbar_init(&x_full[i], kTma ? 1 : kXWarps);
+      mbar_init(&x_full[i], kTma ? 1 : Th::kXWarps);
       mbar_init(&x_empty[i], 1);
     }
     for (int i = 0; i < Tr::kRaw; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], kWideWarps / 2);
+      mbar_init(&raw_empty[i], Th::kWideWarps / 2);
     }
     for (int i = 0; i < Tr::kAcc; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpiWarps / Tr::kTeams);
+      mbar_init(&acc_empty[i], Th::kEpiWarps / Tr::kTeams);
     }
     mbar_init(never, 1);
     *abort_flag = 0;
@@ -187,7 +191,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
   griddep_launch_dependents();
 
   bool have = false;  // epilogue warps: the sums are whole
-  if (warp < kEpiFirst) {
+  if (warp < Th::kEpiFirst) {
     registers_down<Th::kIssue>();
     if (warp == 0 && lane == 0) {
       // ---------------- TMA: packed weights ----------------
@@ -284,18 +288,16 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp < kWideFirst) {
+  } else if (warp < Th::kWideFirst) {
     // ---------------- groups' sums: scaled and added in registers ----------------
     registers_up<Th::kEpi>();
     constexpr int kCols = Tr::kCols;
-    const int quad = warp & 3, second = (warp - kEpiFirst) >> 2;
-    const int team = Tr::kTeams == 2 ? second : 0, half = Tr::kTeams == 2 ? 0 : second;
+    const int quad = warp & 3, of = (warp - Th::kEpiFirst) >> 2;
+    const int team = of / Tr::kParts, first = of % Tr::kParts * kCols;  // tokens from here on
     const int64_t n = static_cast<int64_t>(n0) + quad * 32 + lane;
     const uint32_t row =
-        tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(half * kCols);
-    float sum[kCols];
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
+        tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(first);
+    float2 sum[kCols / 2] = {};
     // channels past the last take its scales, their results are dropped
     const int64_t scale_row = (n < p.N ? n : p.N - 1) * p.lds;
     const auto scale_at = [&](int g) {
@@ -334,32 +336,35 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       s_next = s_after;
       s_after = scale_at(group_of(j + 2));
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) sum[c] = fmaf(__uint_as_float(v[c]), s, sum[c]);
+      for (int c = 0; c < kCols / 2; ++c)
+        sum[c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
+                      both(s), sum[c]);
     }
     // [team][token][channel], over the rings. Another team's groups may still be at work on
     // them: all their MMAs have read the rings once the whole epilogue is here.
-    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(Th::kEpiWarps * 32) : "memory");
     if (have) {
       float *part = reinterpret_cast<float *>(smem) +
-                    (team * NTOK + half * kCols) * kChannels + quad * 32 + lane;
+                    (team * NTOK + first) * kChannels + quad * 32 + lane;
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) part[j * kChannels] = sum[j] * F::kUnit;
+      for (int j = 0; j < kCols; ++j)
+        part[j * kChannels] = (j & 1 ? sum[j / 2].y : sum[j / 2].x) * F::kUnit;
     }
     __syncwarp();
     if (plan.slices == 1)
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");  // these warps
-  } else if (warp < kXFirst) {
+      asm volatile("bar.sync 1, %0;" ::"n"(Th::kEpiWarps * 32) : "memory");  // these warps
+  } else if (warp < Th::kXFirst) {
     // ---------------- widening: packed rows to TMEM, every second stage ----------------
     registers_down<Th::kWide>();
-    const int quad = warp & 3, team = (warp - kWideFirst) >> 2;
+    const int quad = warp & 3, team = (warp - Th::kWideFirst) >> 2;
     const int row = quad * 32 + lane;  // a channel: its lane of TMEM
     const int64_t n = static_cast<int64_t>(n0) + row;
     const uint32_t t_row = tmem_a + (static_cast<uint32_t>(quad * 32) << 16);
     const int64_t zero_row = (n < p.N ? n : p.N - 1) * p.ldz;
     const auto zero_at = [&](int kb, int i) {
-      return p.zero ? __ldg(p.zero + zero_row + min(kb * kPer + i, p.groups - 1)) & 15 : 8;
+      return p.zero ? load_zero_bits(p.zero, zero_row + min(kb * kPer + i, p.groups - 1)) : 8u;
     };
-    int z_next[kPer];
+    uint32_t z_next[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) z_next[i] = zero_at(kb0 + team, i);
     Slot st, r;
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
       uint32_t off[kPer];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        off[i] = w4_adjacent_offset<F>(z_next[i]);
+        off[i] = w4_adjacent_offset<F>(static_cast<int>(z_next[i] & 15u));
         z_next[i] = zero_at(kb + 2, i);
       }
       if (!all(mbar_wait(&raw_full[r.at], r.phase, abort_flag, p.status, kStatusTimeoutStage)))
@@ -418,9 +423,9 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     if constexpr (!kTma) {
       registers_up<Th::kX>();
       const X *src = static_cast<const X *>(p.x);
-      const int tid = static_cast<int>(threadIdx.x) - kXFirst * 32;
+      const int tid = static_cast<int>(threadIdx.x) - Th::kXFirst * 32;
       const bool packs = reinterpret_cast<uintptr_t>(src) % 16 == 0 && p.ldx * sizeof(X) % 16 == 0;
-      constexpr int E = 16 / sizeof(X), kPieces = NTOK * 16 / (kXWarps * 32);
+      constexpr int E = 16 / sizeof(X), kPieces = NTOK * 16 / (Th::kXWarps * 32);
       Slot x;
       for (int kb = kb0; kb < kb1; ++kb) {
         // pieces of eight values, 16 to a token's row of the stage; all loads first, ahead of
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
         alignas(16) X v[kPieces][8];
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
-          const int i = tid + c * (kXWarps * 32), token = i >> 4, k = kb * kBK + (i & 15) * 8;
+          const int i = tid + c * (Th::kXWarps * 32), token = i >> 4, k = kb * kBK + (i & 15) * 8;
           const X *from = src + static_cast<int64_t>(m0 + token) * p.ldx + k;
           if (packs && m0 + token < p.M && k + 8 <= p.K) {
 #pragma unroll
@@ -445,7 +450,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
         uint8_t *xs = ring_x + x.at * Tr::kXBytes;
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
-          const int i = tid + c * (kXWarps * 32), token = i >> 4, piece = i & 15;
+          const int i = tid + c * (Th::kXWarps * 32), token = i >> 4, piece = i & 15;
           uint32_t h[P][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
   }
 
   if (plan.slices > 1) cluster_sync();  // every CTA's sums are in its shared memory
-  if (warp >= kEpiFirst && warp < kWideFirst && have) {
+  if (warp >= Th::kEpiFirst && warp < Th::kWideFirst && have) {
     // this CTA's share of the cluster's tokens: a token per warp at a time, four channels a lane
     const int each = NTOK / plan.slices;
     const int64_t n = static_cast<int64_t>(n0) + 4 * lane;
@@ -484,7 +489,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
     const int size = p.c_type == NPLK_DTYPE_FP32 ? 4 : 2;
     const bool whole = p.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(p.C) % (4 * size) == 0;
     const int count = n < p.N ? static_cast<int>(p.N - n < 4 ? p.N - n : 4) : 0;
-    for (int i = warp - kEpiFirst; i < each; i += kEpiWarps) {
+    for (int i = warp - Th::kEpiFirst; i < each; i += Th::kEpiWarps) {
       const int token = rank * each + i;
       // (a load from another CTA that no store waits for could be under way when that CTA ends)
       if (m0 + token >= p.M || count == 0) break;
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(MmaThreads<kTma>::kThreads, 1)
 
 template <typename X, int NTOK, int kGroup, bool kTma>
 int launch(cudaStream_t s, const W4Args &p, MmaPlan plan) {
-  using Tr = MmaTraits<NTOK, W4Type<X>::kParts, kTma>;
+  using Tr = MmaTraits<NTOK, W4Type<X>::kParts, kGroup, kTma>;
   CUtensorMap mw, mx = {};
   int rc = encode_tmap_2d_u8_sw64(&mw, p.q, ceil_div(p.K, 2), p.N, p.ldq, kChannels);
   if (!rc && kTma) rc = encode_tmap_2d_u8_sw128(&mx, p.x, 2 * static_cast<int64_t>(p.K), p.M, 2 * p.ldx, NTOK);
@@ -537,7 +542,7 @@ int launch(cudaStream_t s, const W4Args &p, MmaPlan plan) {
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(MmaThreads<kTma>::kThreads);
+  cfg.blockDim = dim3(MmaThreads<NTOK, kGroup, kTma>::kThreads);
   cfg.dynamicSmemBytes = Tr::kSmem;
   cfg.stream = s;
   cfg.attrs = attr;

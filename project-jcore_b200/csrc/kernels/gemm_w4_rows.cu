@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1)
 
   // Scales (and zeros) of a stage, loaded one stage ahead: lane l holds those of channel l.
   uint32_t sc_next[kGroups];  // as loaded: packed pairs in the first half, or one each
-  int ze_next[kGroups];
+  uint32_t ze_next[kGroups];
   int64_t s_row = 0, z_row = 0;
   bool pairs = false;
   const auto aim_scales = [&](int round) {
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1)
     if (kZeros) {
 #pragma unroll
       for (int j = 0; j < kGroups; ++j)
-        ze_next[j] = __ldg(p.zero + z_row + min(g0 + j, p.groups - 1)) & 15;
+        ze_next[j] = load_zero_bits(p.zero, z_row + min(g0 + j, p.groups - 1));
     }
   };
 
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kMostWarps * 32, 1)
       for (int j = 0; j < kGroups; ++j) {
         const uint32_t pair = sc_next[j / 2];
         sc[j] = scale_value(!pairs ? sc_next[j] : j & 1 ? pair >> 16 : pair & 0xffffu, p.scale_type);
-        if (kZeros) offs[j] = F::low_offset(ze_next[j]) | F::high_offset(ze_next[j]) << 16;
+        if (kZeros) offs[j] = w4_adjacent_offset<F>(static_cast<int>(ze_next[j] & 15u));
       }
       if (step + 1 < steps) {
         fetch(step + 1);

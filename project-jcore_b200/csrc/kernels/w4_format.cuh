@@ -15,14 +15,29 @@ namespace nplk {
 inline bool w4_group_ok(int64_t group) { return group == 32 || group == 64 || group == 128; }
 
 // A scale of type NPLK_DTYPE_* as it is stored, and its value: the conversion apart from the
-// load, so that a load ahead of its use is not waited for. `at` has to lie in the array
-// whatever the result is used for: the headers' __ldg of __half and __nv_bfloat16 are asm
-// statements without side effects, which the compiler may run ahead of the condition they
-// stand under (a scale array at the end of its memory segment faulted so). The integer
-// __ldg is no such asm.
+// load, so that a load ahead of its use is not waited for (nor, in 16 bits, for its widening,
+// which the compiler puts behind the load; here the load itself widens). `at` has to lie in the
+// array whatever the result is used for, and the statements are volatile: the compiler may run
+// an asm statement without side effects, which the headers' __ldg of 16-bit floats are, ahead
+// of the condition it stands under (a scale array at the end of its memory segment faulted so).
 __device__ __forceinline__ uint32_t load_scale_bits(const void *scales, int dtype, int64_t at) {
-  return dtype == NPLK_DTYPE_FP32 ? __ldg(static_cast<const unsigned int *>(scales) + at)
-                                  : __ldg(static_cast<const unsigned short *>(scales) + at);
+  uint32_t bits;
+  if (dtype == NPLK_DTYPE_FP32) {
+    asm volatile("ld.global.nc.u32 %0, [%1];"
+                 : "=r"(bits)
+                 : "l"(static_cast<const uint32_t *>(scales) + at));
+  } else {
+    asm volatile("ld.global.nc.u16 %0, [%1];"
+                 : "=r"(bits)
+                 : "l"(static_cast<const uint16_t *>(scales) + at));
+  }
+  return bits;
+}
+// A zero's byte, of which the low half counts: taken apart where it is used, for the same reason.
+__device__ __forceinline__ uint32_t load_zero_bits(const uint8_t *zeros, int64_t at) {
+  uint32_t bits;
+  asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(bits) : "l"(zeros + at));
+  return bits;
 }
 __device__ __forceinline__ float scale_value(uint32_t bits, int dtype) {
   if (dtype == NPLK_DTYPE_FP32) return __uint_as_float(bits);
