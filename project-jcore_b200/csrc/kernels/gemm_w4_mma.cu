@@ -10,7 +10,14 @@
 // round them once more (2^-9 for bf16).
 //
 // x comes by TMA where it can (16-bit, 16-byte aligned rows); otherwise, and for fp32, whose
-// three bf16 parts each take a product of their own, four more warps bring it.
+// three bf16 parts each take a product of their own, eight more warps bring it.
+//
+// Measured (group 128, cold weights): 512 x 4096 x 4096 bf16 23.6 us, 512 x 16384 x 4096 93,
+// 48 x 16384 x 4096 with zeros 21, 256 x 4096 x 4096 fp32 47. What bounds it is instructions:
+// 66% of issue slots over the whole of a call of 512 tokens, three to a pair of weights (128
+// channels widened anew for each tile of tokens) and 70 to an epilogue warp's group, against
+// 38% of the tensor cores. Groups of 64 and 32 have two and four times the sums to add: 512 x
+// 4096 x 4096 43 and 73 us.
 #include <algorithm>
 
 #include "gemm_w4.cuh"
@@ -26,6 +33,10 @@ constexpr int kACols = kBK / 2;            // TMEM columns of a stage's widened 
 // (two). A stage's chain of waits, loads and stores is long against its products, so roles
 // come in two teams that take every second stage or group: MMA issue, widening and, up to 64
 // tokens, the epilogue.
+//
+// Epilogue: sixteen warps where groups' sums are many, 128 tokens or short groups (512 x 4096 x
+// 4096 23.6 us, 25.3 with eight; 48 x 16384 x 4096 with groups of 32 37 and 42); eight otherwise
+// (48 x 16384 x 4096 21.1 us, 22.0 with sixteen; 17 x 4096 x 4096 9.3 and 10.1).
 //
 // Warps, threads, and registers a thread: at launch, and as the warpgroups share them.
 template <int NTOK, int kGroup, bool kTma>
@@ -582,11 +593,12 @@ int gemm_w4_mma(cudaStream_t s, const W4Args &args) {
   const int64_t sms = sm_count(), blocks = ceil_div(p.K, kBK);
   const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, tokens);
   MmaPlan plan{1, 0, 0};
+  // waves of (start and end, stages of a slice), and the slices' meeting, as measured
   double least = 1e30;
   for (int slices : {1, 2, 4, 8}) {
     if (slices > blocks) break;
     const double us = static_cast<double>(ceil_div(tiles * slices, sms)) *
-                          (2.5 + 0.28 * static_cast<double>(ceil_div(blocks, slices))) +
+                          (4.5 + 0.55 * static_cast<double>(ceil_div(blocks, slices))) +
                       (slices > 1 ? 0.5 : 0.0);
     if (us < least) {
       least = us;
