@@ -467,8 +467,9 @@ NPL_API int nplk_gemm_w4(void *stream, int64_t M, int64_t N, int64_t K, int64_t 
  * masked: it has p = 0 and is no alternative; where there are fewer alternatives than
  * n_top, the rest have id -1 and -infinity. A row of masked logits alone has logprob
  * -infinity, entropy 0 and stats -infinity. A row that holds a NaN or +infinity has NaN
- * for each result (ids -1). One pass over the logits; sums are fp32 in a fixed order.
- * Results must not overlap the logits. vocab < 2^31 - 65536. The reference's softmax
+ * for each result (ids -1). One pass over the logits; sums are fp32 in a fixed order, which
+ * goes by rows, vocab, n_top and the row's alignment to 16 bytes. Results must not overlap
+ * the logits. vocab < 2^31 - 65536. The reference's softmax
  * (npl_activation_norm.cpp:88-112) is the nearest it has. */
 NPL_API int nplk_token_logprobs(void *stream, int64_t rows, int64_t vocab, int dtype,
                                 const void *logits, int64_t ld, float scale,
@@ -623,7 +624,7 @@ NPL_API int nplk_gemm_tune(void *stream, int64_t M, int64_t N, int64_t K, const 
 /* No reference counterpart: the reference's CPU loops cannot time out or run
  * out of device memory. Both hooks are off unless armed. */
 
-#define NPLK_DEBUG_GEMM 1        /* the tcgen05 GEMM kernels (split and raw forms, nplk_gemm_i8's) */
+#define NPLK_DEBUG_GEMM 1        /* the tcgen05 GEMM kernels (split and raw forms, nplk_gemm_i8, nplk_gemm_w4) */
 #define NPLK_DEBUG_CONV_WINDOW 2 /* the window conv kernels (gather and plane forms) */
 
 /* Arms the next launch of one kernel family, from any thread, to exercise its

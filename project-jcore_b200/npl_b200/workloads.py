@@ -148,3 +148,60 @@ def norm_act_dropout_backward(lib, stream, dy, x, groups, mean, rstd, gamma, bet
     return lib.nplk_group_norm_act_backward(stream, n, hw, c, groups, _dtype(x), _p(dx), c, _p(x),
                                             c, _p(mean), _p(rstd), _p(gamma), _p(beta), act, 0.0,
                                             _p(dx), c, _p(dgamma), _p(dbeta), _p(work), ws)
+
+
+def layer_norm_project_w4(lib, stream, x, gamma, beta, y, q, scale, zero, group, bias, act, out,
+                          eps: float = 1e-5) -> int:
+    """Rows of x normalised and projected by weights in 4 bits: a served layer's norm and
+    product, or, into a vocabulary, a language model's head.
+
+    x, y: fp32 [M, K]; gamma, beta: [K]; q: uint8 [N, ldq] with scale [N, groups] of any of
+    the types and zero (uint8, or None), as nplk_quantize_w4 makes them; bias: [N] or None;
+    out: [M, N] of any of the types, its pitch free."""
+    m, k = x.shape
+    rc = lib.nplk_layer_norm(stream, m, k, _p(x), _p(y), _p(gamma), _p(beta), eps)
+    if rc != 0:
+        return rc
+    return lib.nplk_gemm_w4(stream, m, out.shape[1], k, group, _dtype(y), _p(y), k, _p(q),
+                            q.stride(0), _dtype(scale), _p(scale), scale.stride(0),
+                            _p(zero) if zero is not None else None,
+                            zero.stride(0) if zero is not None else 0,
+                            _p(bias) if bias is not None else None, act, 0.0, _dtype(out), _p(out),
+                            out.stride(0), None)
+
+
+def score_tokens_w4(lib, stream, x, gamma, beta, y, q, scale, zero, group, logits, targets, logprob,
+                    entropy, top_ids, top_logprobs, temperature: float = 1.0,
+                    eps: float = 1e-5) -> int:
+    """What a served language model answers with: the head's logits (layer_norm_project_w4),
+    the log probabilities of given tokens, the entropy and the alternatives.
+
+    logits: [M, vocab]; targets: int64 [M]; logprob, entropy: [M]; top_ids (int64) and
+    top_logprobs: [M, n]."""
+    rc = layer_norm_project_w4(lib, stream, x, gamma, beta, y, q, scale, zero, group, None, 0,
+                               logits, eps)
+    if rc != 0:
+        return rc
+    return lib.nplk_token_logprobs(stream, logits.shape[0], logits.shape[1], _dtype(logits),
+                                   _p(logits), logits.stride(0), 1.0 / temperature, _p(targets),
+                                   _p(logprob), _p(entropy), None, top_ids.shape[1], _p(top_ids),
+                                   _p(top_logprobs))
+
+
+def token_loss(lib, stream, logits, targets, logprob, entropy, stats, d_logprob, d_entropy,
+               dlogits, temperature: float = 1.0) -> int:
+    """A training step's end: log probabilities and entropy of [rows, vocab] logits, and the
+    gradient of sum(d_logprob logprob + d_entropy entropy) into dlogits (which may be logits
+    itself). For the mean cross entropy d_logprob is -1 / rows. targets: int64 [rows];
+    stats: [rows, 2]; the others [rows], d_entropy or None."""
+    rows, vocab = logits.shape
+    code, ld = _dtype(logits), logits.stride(0)
+    rc = lib.nplk_token_logprobs(stream, rows, vocab, code, _p(logits), ld, 1.0 / temperature,
+                                 _p(targets), _p(logprob), _p(entropy), _p(stats), 0, None, None)
+    if rc != 0:
+        return rc
+    return lib.nplk_token_logprobs_backward(stream, rows, vocab, code, _p(logits), ld,
+                                            1.0 / temperature, _p(targets), _p(stats), _p(entropy),
+                                            _p(d_logprob),
+                                            _p(d_entropy) if d_entropy is not None else None,
+                                            _p(dlogits), dlogits.stride(0))
