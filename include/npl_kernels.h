@@ -432,8 +432,8 @@ NPL_API int nplk_gemm_i8(void *stream, int64_t M, int64_t N, int64_t K, const in
  * `scale`, by which the quotients (fp32, rounded to nearest, ties to even) are taken.
  * Nibbles and zeros are clamped to 0..15. The half byte behind an odd K is 0; bytes
  * from (K + 1) / 2 to ldq are left as they are. A group that holds a NaN gets scale
- * NaN, one whose s is infinite in scale_dtype infinity, both with equal nibbles
- * and zeros. w and the results must not overlap. N, K <= 2^30. */
+ * NaN, one whose s is infinite in scale_dtype, or whose high - low is in fp32,
+ * infinity, both with equal nibbles and zeros. w and the results must not overlap. N, K <= 2^30. */
 NPL_API int nplk_quantize_w4(void *stream, int64_t N, int64_t K, int64_t group, int dtype,
                              const void *w, int64_t ldw, uint8_t *q, int64_t ldq,
                              int scale_dtype, void *scale, int64_t lds, uint8_t *zero,
@@ -454,7 +454,7 @@ NPL_API int nplk_gemm_w4(void *stream, int64_t M, int64_t N, int64_t K, int64_t 
 
 /* ---- log probabilities of given tokens --------------------------------------------- */
 /* For each row r of logits (rows x vocab of type dtype, pitch ld), with z = scale * l
- * (scale > 0: the reciprocal of the temperature), p = softmax(z) and t = targets[r]:
+ * (0 < scale <= 2^126: the reciprocal of the temperature), p = softmax(z) and t = targets[r]:
  *   logprob[r]  = log p[t]; 0 where t is not in 0..vocab - 1 (no token asked for)
  *   entropy[r]  = -sum p log p (a p of 0 counts 0)
  *   stats[2r], stats[2r + 1] = m = max l and log sum exp(z - scale * m), for the

@@ -18,6 +18,7 @@ namespace nplk {
 namespace {
 
 constexpr float kInf = __builtin_huge_valf(), kLowest = -3.402823466e38f;
+constexpr float kMostScale = 0x1p126f;  // times log2 e still finite
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kMostTop = 32;      // alternatives: one a lane
@@ -657,7 +658,7 @@ int run_gradient(cudaStream_t s, int64_t rows, const LogprobGradArgs &p, const T
 int check(int64_t rows, int64_t vocab, int dtype, const void *logits, int64_t ld, float scale) {
   const int size = dtype_bytes(dtype);
   if (rows < 1 || vocab < 1 || !size || !logits || ld < vocab || !(scale > 0.0f) ||
-      !(scale < kInf) || reinterpret_cast<uintptr_t>(logits) % size)
+      !(scale <= kMostScale) || reinterpret_cast<uintptr_t>(logits) % size)
     return kErrInvalidArg;
   if (vocab >= (int64_t(1) << 31) - 65536 || rows > (int64_t(1) << 40)) return kErrUnsupported;
   return kOk;

@@ -210,3 +210,23 @@ def test_masks_and_nan_in_every_form(rows, vocab, dtype):
     dx = backward(lib, x, vocab, t, st, ent, g, h)
     assert (dx[nothing] == 0).all() and dx[nan].isnan().all() and dx[inf].isnan().all()
     check_backward(x[rest], vocab, t[rest], st[rest], ent[rest], g[rest], h[rest], 1.0, dx[rest])
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 126, 1e30, 1e-30, 1e-44])
+def test_the_largest_and_smallest_scales(scale):
+    # all on the largest logit, and all alike: the limits of softmax
+    lib, rows, vocab = S.gpu_lib(), 3, 1000
+    x = torch.randint(-50, 50, (rows, vocab), device="cuda", generator=gen(6)).float()
+    x[:, 7] = 60.0
+    t = torch.tensor([7, 8, 7], device="cuda")
+    lp, ent, st, ids, tlp = forward(lib, x, vocab, t, 2, scale)
+    if scale > 1:
+        d = torch.full_like(lp, -scale) * (60.0 - x[:, 8])
+        assert torch.equal(lp, torch.where(t == 7, torch.zeros_like(lp), d))
+        assert (ent == 0).all() and (st[:, 1] == 0).all() and (tlp[:, 0] == 0).all()
+    else:
+        # a thousand equal terms: log 1000 within the sums' roundings
+        uniform = torch.full((), vocab, dtype=torch.float64).log().item()
+        assert ((ent.double() - uniform).abs() <= 2.0 ** -18).all()
+        assert ((lp.double() + uniform).abs() <= 2.0 ** -18).all()
+    assert (ids[:, 0] == 7).all()

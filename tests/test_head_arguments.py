@@ -98,3 +98,8 @@ def test_too_many_alternatives_or_tokens(lib):
     assert forward(lib, top=33) == UNSUP
     assert forward(lib, vocab=1 << 31, ld=1 << 31) == UNSUP
     assert backward(lib, vocab=1 << 31, ld=1 << 31, ldd=1 << 31) == UNSUP
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 126 * 1.001, 3.4e38])
+def test_scales_whose_exponents_would_not_be_numbers(lib, scale):
+    assert forward(lib, scale=scale) == BAD and backward(lib, scale=scale) == BAD
