@@ -118,23 +118,16 @@ struct Slot {
   }
 };
 
-// kCols consecutive TMEM columns of this thread's lane, awaited.
+// kCols consecutive TMEM columns of this thread's lane, and the wait for them.
 template <int kCols>
 __device__ __forceinline__ void tmem_ld(uint32_t from, uint32_t (&v)[kCols]) {
-  if constexpr (kCols == 16) {
-    tmem_ld16(from, v);
-    tmem_wait_ld16(v);
-  } else if constexpr (kCols == 32) {
-    tmem_ld32(from, v);
-    tmem_wait_ld(v);
-  } else {
-    static_assert(kCols == 64, "columns");
-    uint32_t(&a)[32] = *reinterpret_cast<uint32_t(*)[32]>(v);
-    uint32_t(&b)[32] = *reinterpret_cast<uint32_t(*)[32]>(v + 32);
-    tmem_ld32(from, a);
-    tmem_ld32(from + 32, b);
-    tmem_wait_ld2(a, b);
-  }
+  if constexpr (kCols == 16) tmem_ld16(from, v);
+  else tmem_ld32(from, v);
+}
+template <int kCols>
+__device__ __forceinline__ void tmem_landed(uint32_t (&v)[kCols]) {
+  if constexpr (kCols == 16) tmem_wait_ld16(v);
+  else tmem_wait_ld(v);
 }
 
 template <typename X, int NTOK, int kGroup, bool kTma>
@@ -325,31 +318,53 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
     };
     uint32_t s_next = scale_at(group_of(0)), s_after = scale_at(group_of(1));
     have = true;
-    bool ready = false;
     // A group's chain -- the wait, the read, the sums -- is what bounds short groups: the next
-    // group's barrier is asked for and the scale brought along under this one's sums.
+    // group's barrier is asked for and the scale brought along under this one's sums. 64
+    // columns are read half by half, under each other's sums.
+    constexpr int kRead = kCols < 32 ? kCols : 32;
+    const auto add = [&](const uint32_t(&v)[kRead], int at, float s) {
+#pragma unroll
+      for (int c = 0; c < kRead / 2; ++c)
+        sum[at / 2 + c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
+                               both(s), sum[at / 2 + c]);
+    };
+    uint32_t va[kRead], vb[kRead];
+    bool ready = false;  // the next group; where columns are 64, read as far as va
     for (int j = 0; group_of(j) < g_end; ++j) {
-      const AccSlot<Tr::kAcc> acc = slot_of(j);
+      const AccSlot<Tr::kAcc> acc = slot_of(j), next = slot_of(j + 1);
+      const uint32_t from = row + static_cast<uint32_t>(acc.at * NTOK);
       if (!all(ready)) {
         have = all(mbar_wait(&acc_full[acc.at], acc.phase, abort_flag, p.status,
                              kStatusTimeoutEpilogue));
         if (!have) break;
       }
-      tc_fence_after_sync();
-      uint32_t v[kCols];
-      tmem_ld<kCols>(row + static_cast<uint32_t>(acc.at * NTOK), v);
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[acc.at]);  // all read: it is free again
-      const AccSlot<Tr::kAcc> next = slot_of(j + 1);
-      ready = mbar_test(&acc_full[next.at], next.phase);
+      if (kCols <= 32 || !ready) {
+        tc_fence_after_sync();
+        tmem_ld<kRead>(from, va);
+      }
       const float s = scale_value(s_next, p.scale_type);
       s_next = s_after;
       s_after = scale_at(group_of(j + 2));
-#pragma unroll
-      for (int c = 0; c < kCols / 2; ++c)
-        sum[c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
-                      both(s), sum[c]);
+      tmem_landed<kRead>(va);
+      if constexpr (kCols == 64) {
+        tmem_ld<kRead>(from + kRead, vb);
+        add(va, 0, s);
+        tmem_landed<kRead>(vb);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc.at]);  // all read: it is free again
+      ready = mbar_test(&acc_full[next.at], next.phase);
+      if constexpr (kCols == 64) {
+        ready = group_of(j + 1) < g_end && all(ready);
+        if (ready) {
+          tc_fence_after_sync();
+          tmem_ld<kRead>(row + static_cast<uint32_t>(next.at * NTOK), va);
+        }
+        add(vb, kRead, s);
+      } else {
+        add(va, 0, s);
+      }
     }
     // [team][token][channel], over the rings. Another team's groups may still be at work on
     // them: all their MMAs have read the rings once the whole epilogue is here.
