@@ -330,8 +330,9 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
     };
     uint32_t va[kRead], vb[kRead];
     bool ready = false;  // the next group; where columns are 64, read as far as va
+    AccSlot<Tr::kAcc> acc = slot_of(0);
     for (int j = 0; group_of(j) < g_end; ++j) {
-      const AccSlot<Tr::kAcc> acc = slot_of(j), next = slot_of(j + 1);
+      const AccSlot<Tr::kAcc> next = slot_of(j + 1);
       const uint32_t from = row + static_cast<uint32_t>(acc.at * NTOK);
       if (!all(ready)) {
         have = all(mbar_wait(&acc_full[acc.at], acc.phase, abort_flag, p.status,
@@ -365,6 +366,7 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
       } else {
         add(va, 0, s);
       }
+      acc = next;
     }
     // [team][token][channel], over the rings. Another team's groups may still be at work on
     // them: all their MMAs have read the rings once the whole epilogue is here.
