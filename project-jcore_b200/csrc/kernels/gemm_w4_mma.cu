@@ -12,12 +12,12 @@
 // x comes by TMA where it can (16-bit, 16-byte aligned rows); otherwise, and for fp32, whose
 // three bf16 parts each take a product of their own, eight more warps bring it.
 //
-// Measured (group 128, cold weights): 512 x 4096 x 4096 bf16 23.6 us, 512 x 16384 x 4096 93,
-// 48 x 16384 x 4096 with zeros 21, 256 x 4096 x 4096 fp32 47. What bounds it is instructions:
-// 66% of issue slots over the whole of a call of 512 tokens, three to a pair of weights (128
-// channels widened anew for each tile of tokens) and 70 to an epilogue warp's group, against
-// 38% of the tensor cores. Groups of 64 and 32 have two and four times the sums to add: 512 x
-// 4096 x 4096 43 and 73 us.
+// Measured (group 128, cold weights): 512 x 4096 x 4096 bf16 22.6 us, 512 x 16384 x 4096 90,
+// 48 x 16384 x 4096 with zeros 20, 256 x 4096 x 4096 fp32 47. What bounds it is instructions:
+// 59% of issue slots over the whole of a call of 512 tokens, its start and end included, three
+// to a pair of weights (128 channels widened anew for each tile of tokens) and some 70 to an
+// epilogue warp's group, against 40% of the tensor cores. Groups of 64 and 32 have two and four
+// times the sums to add: 512 x 4096 x 4096 41 and 69 us.
 #include <algorithm>
 
 #include "gemm_w4.cuh"
@@ -36,7 +36,8 @@ constexpr int kACols = kBK / 2;            // TMEM columns of a stage's widened 
 //
 // Epilogue: sixteen warps where groups' sums are many, 128 tokens or short groups (512 x 4096 x
 // 4096 23.6 us, 25.3 with eight; 48 x 16384 x 4096 with groups of 32 37 and 42); eight otherwise
-// (48 x 16384 x 4096 21.1 us, 22.0 with sixteen; 17 x 4096 x 4096 9.3 and 10.1).
+// (48 x 16384 x 4096 21.1 us, 22.0 with sixteen; 17 x 4096 x 4096 9.3 and 10.1; all before
+// halves were read under sums, which took another 4%).
 //
 // Warps, threads, and registers a thread: at launch, and as the warpgroups share them.
 template <int NTOK, int kGroup, bool kTma>

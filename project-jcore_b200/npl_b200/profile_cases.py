@@ -294,6 +294,47 @@ def case_gemm_i8(reps: int = 3, m: int = 4096, n: int = 4096, k: int = 4096):
     assert lib.nplk_read_status(s) == 0
 
 
+def case_gemm_w4(reps: int = 3, m: int = 4, n: int = 128000, k: int = 4096, group: int = 64,
+                 dtype: str = "float16"):
+    from . import NPLK_DTYPE_FP32, workloads
+    torch, lib, s = _setup()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    w, x = (torch.randn(r, k, device="cuda", generator=gen).to(getattr(torch, dtype))
+            for r in (n, m))
+    code, groups = workloads._dtype(x), -(-k // group)
+    q = torch.empty(n, k // 2, device="cuda", dtype=torch.uint8)
+    scale = torch.empty(n, groups, device="cuda", dtype=x.dtype)
+    c = torch.empty(m, n, device="cuda")
+    for _ in range(reps):
+        assert lib.nplk_quantize_w4(s, n, k, group, code, _p(w), k, _p(q), k // 2, code, _p(scale),
+                                    groups, None, 0) == 0
+        assert lib.nplk_gemm_w4(s, m, n, k, group, code, _p(x), k, _p(q), k // 2, code, _p(scale),
+                                groups, None, 0, None, 0, 0.0, NPLK_DTYPE_FP32, _p(c), n,
+                                None) == 0
+    torch.cuda.synchronize()
+    assert lib.nplk_read_status(s) == 0
+
+
+def case_token_logprobs(reps: int = 3, rows: int = 2048, vocab: int = 50021, top: int = 5,
+                        dtype: str = "float16"):
+    from . import workloads
+    torch, lib, s = _setup()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(rows, vocab, device="cuda", generator=gen).to(getattr(torch, dtype))
+    dx, code = torch.empty_like(x), workloads._dtype(x)
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+    lp, ent, g = torch.ones(3, rows, device="cuda")
+    stats, tlp = torch.empty(rows, 2, device="cuda"), torch.empty(rows, top, device="cuda")
+    ids = torch.empty(rows, top, device="cuda", dtype=torch.int64)
+    for _ in range(reps):
+        assert lib.nplk_token_logprobs(s, rows, vocab, code, _p(x), vocab, 1.0, _p(t), _p(lp),
+                                       _p(ent), _p(stats), top, _p(ids), _p(tlp)) == 0
+        assert lib.nplk_token_logprobs_backward(s, rows, vocab, code, _p(x), vocab, 1.0, _p(t),
+                                                _p(stats), _p(ent), _p(g), None, _p(dx),
+                                                vocab) == 0
+    torch.cuda.synchronize()
+
+
 CASES = {"conv": case_conv, "chain_fused": case_chain_fused,
          "conv_direct": lambda: case_conv(algo=1),
          "conv_window_tma": lambda: case_conv(algo=3),
@@ -308,7 +349,10 @@ CASES = {"conv": case_conv, "chain_fused": case_chain_fused,
          "conv_n256": lambda: case_conv(n=256),
          "stem_fused": case_stem_fused, "norm": case_norm,
          "norm_wide": lambda: case_norm(n=1, hw=262144, c=128, dtype="float32"),
-         "dropout": case_dropout, "quantize": case_quantize, "gemm_i8": case_gemm_i8}
+         "dropout": case_dropout, "quantize": case_quantize, "gemm_i8": case_gemm_i8,
+         "gemm_w4": case_gemm_w4,
+         "gemm_w4_512": lambda: case_gemm_w4(m=512, n=4096, group=128, dtype="bfloat16"),
+         "token_logprobs": case_token_logprobs}
 
 if __name__ == "__main__":
     name = sys.argv[1] if len(sys.argv) > 1 else "conv"
