@@ -13,7 +13,7 @@
 // three bf16 parts each take a product of their own, eight more warps bring it.
 //
 // Measured (group 128, cold weights): 512 x 4096 x 4096 bf16 22.6 us, 512 x 16384 x 4096 90,
-// 48 x 16384 x 4096 with zeros 20, 256 x 4096 x 4096 fp32 47. What bounds it is instructions:
+// 48 x 16384 x 4096 with zeros 19.6, 256 x 4096 x 4096 fp32 47. What bounds it is instructions:
 // 59% of issue slots over the whole of a call of 512 tokens, its start and end included, three
 // to a pair of weights (128 channels widened anew for each tile of tokens) and some 70 to an
 // epilogue warp's group, against 40% of the tensor cores. Groups of 64 and 32 have two and four
@@ -66,6 +66,7 @@ struct MmaTraits {
   static constexpr int kTeams = NTOK <= 64 && kTma ? 2 : 1;
   static constexpr int kParts = MmaThreads<NTOK, kGroup, kTma>::kEpiWarps / 4 / kTeams;
   static constexpr int kCols = NTOK / kParts;
+  static constexpr int kAccCols = NTOK == 48 ? 64 : NTOK;  // from one accumulator to the next
   static constexpr int kXAtom = NTOK * 128;  // NTOK rows x 64 values
   static constexpr int kXBytes = 2 * kXAtom * P;
   // Rings: widened weights in TMEM, x (its loads take some 2000 cycles, of which a stage of 64
@@ -80,7 +81,7 @@ struct MmaTraits {
   // at least what keeps other clusters' TMEM off this SM
   static constexpr int kNeeded = 1024 + kRings + 8 * kBarriers + 64;
   static constexpr int kSmem = kNeeded > 200 * 1024 ? kNeeded : 200 * 1024;
-  static_assert(kAcc * NTOK + kA * kACols <= kTmemCols, "TMEM columns");
+  static_assert(kAcc * kAccCols + kA * kACols <= kTmemCols, "TMEM columns");
   static_assert(kRaw >= 2 && kRaw % 2 == 0 && kA % 2 == 0 && kX % 2 == 0 && kAcc % 2 == 0,
                 "a slot belongs to one of two teams");
   static_assert(kTeams * NTOK * kChannels * 4 <= kRings, "partial sums over the rings");
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot, tmem_a = tmem_base + Tr::kAcc * NTOK;
+  const uint32_t tmem_base = *tmem_slot, tmem_a = tmem_base + Tr::kAcc * Tr::kAccCols;
   griddep_wait();
   griddep_launch_dependents();
 
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
                                kStatusTimeoutAccFree));
           if (!go) break;
           tc_fence_after_sync();
-          const uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * NTOK);
+          const uint32_t d = tmem_base + static_cast<uint32_t>(acc.at * Tr::kAccCols);
           if (elect_lane()) {
 #pragma unroll
             for (int kk = 0; kk < kGroup / 16; ++kk) {
@@ -320,21 +321,21 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
     uint32_t s_next = scale_at(group_of(0)), s_after = scale_at(group_of(1));
     have = true;
     // A group's chain -- the wait, the read, the sums -- is what bounds short groups: the next
-    // group's barrier is asked for and the scale brought along under this one's sums. 64
-    // columns are read half by half, under each other's sums.
-    constexpr int kRead = kCols < 32 ? kCols : 32;
-    const auto add = [&](const uint32_t(&v)[kRead], int at, float s) {
+    // group's barrier is asked for and the scale brought along under this one's sums. More
+    // than 32 columns are read in two parts, under each other's sums.
+    constexpr int kRead = kCols < 32 ? kCols : 32, kRest = kCols > 32 ? kCols - 32 : 16;
+    const auto add = [&](const auto &v, int at, float s) {
 #pragma unroll
-      for (int c = 0; c < kRead / 2; ++c)
+      for (int c = 0; c < static_cast<int>(sizeof(v) / 8); ++c)
         sum[at / 2 + c] = fma2(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
                                both(s), sum[at / 2 + c]);
     };
-    uint32_t va[kRead], vb[kRead];
-    bool ready = false;  // the next group; where columns are 64, read as far as va
+    uint32_t va[kRead], vb[kRest];
+    bool ready = false;  // the next group; where columns are more than 32, read as far as va
     AccSlot<Tr::kAcc> acc = slot_of(0);
     for (int j = 0; group_of(j) < g_end; ++j) {
       const AccSlot<Tr::kAcc> next = slot_of(j + 1);
-      const uint32_t from = row + static_cast<uint32_t>(acc.at * NTOK);
+      const uint32_t from = row + static_cast<uint32_t>(acc.at * Tr::kAccCols);
       if (!all(ready)) {
         have = all(mbar_wait(&acc_full[acc.at], acc.phase, abort_flag, p.status,
                              kStatusTimeoutEpilogue));
@@ -348,20 +349,20 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
       s_next = s_after;
       s_after = scale_at(group_of(j + 2));
       tmem_landed<kRead>(va);
-      if constexpr (kCols == 64) {
-        tmem_ld<kRead>(from + kRead, vb);
+      if constexpr (kCols > 32) {
+        tmem_ld<kRest>(from + kRead, vb);
         add(va, 0, s);
-        tmem_landed<kRead>(vb);
+        tmem_landed<kRest>(vb);
       }
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[acc.at]);  // all read: it is free again
       ready = mbar_test(&acc_full[next.at], next.phase);
-      if constexpr (kCols == 64) {
+      if constexpr (kCols > 32) {
         ready = group_of(j + 1) < g_end && all(ready);
         if (ready) {
           tc_fence_after_sync();
-          tmem_ld<kRead>(row + static_cast<uint32_t>(next.at * NTOK), va);
+          tmem_ld<kRead>(row + static_cast<uint32_t>(next.at * Tr::kAccCols), va);
         }
         add(vb, kRead, s);
       } else {
@@ -590,6 +591,7 @@ int by_group(cudaStream_t s, const W4Args &p, const MmaPlan &plan) {
 template <typename X>
 int by_tokens(cudaStream_t s, const W4Args &p, const MmaPlan &plan, int tokens, bool tma) {
   if (!tma) return by_group<X, 64, false>(s, p, plan);
+  if (tokens == 48) return launch<X, 48, 128, true>(s, p, plan);
   return tokens == 32   ? by_group<X, 32, true>(s, p, plan)
          : tokens == 64 ? by_group<X, 64, true>(s, p, plan)
                         : by_group<X, 128, true>(s, p, plan);
@@ -607,7 +609,13 @@ int gemm_w4_mma(cudaStream_t s, const W4Args &args) {
   const bool tma = p.x_type != NPLK_DTYPE_FP32 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 &&
                    (p.ldx % 8 == 0 || p.M == 1);
   if (p.M == 1) p.ldx = static_cast<int64_t>(align_up(p.K, 8));
-  const int tokens = !tma ? 64 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  // tiles of 48 tokens where there are eight epilogue warps (48 x 16384 x 4096 with zeros 19.6 us,
+  // as 64 columns 20.4)
+  const int tokens = !tma                               ? 64
+                     : p.M <= 32                        ? 32
+                     : p.M <= 48 && p.group == kBK ? 48
+                     : p.M <= 64                        ? 64
+                                                        : 128;
   const int64_t sms = sm_count(), blocks = ceil_div(p.K, kBK);
   const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, tokens);
   MmaPlan plan{1, 0, 0};
