@@ -69,8 +69,8 @@ struct MmaTraits {
   static constexpr int kAccCols = NTOK == 48 ? 64 : NTOK;  // from one accumulator to the next
   static constexpr int kXAtom = NTOK * 128;  // NTOK rows x 64 values
   static constexpr int kXBytes = 2 * kXAtom * P;
-  // Rings: widened weights in TMEM, x (its loads take some 2000 cycles, of which a stage of 64
-  // tokens has 400) and packed weights in shared memory.
+  // Rings: widened weights in TMEM, x (its loads take some 2000 cycles, a stage about
+  // 600) and packed weights in shared memory.
   static constexpr int kA = 4, kX = kXBytes <= 16 * 1024 ? 8 : 4;
   static constexpr int kRaw =
       208 * 1024 - kX * kXBytes > 8 * kRawBytes ? 8 : (208 * 1024 - kX * kXBytes) / kRawBytes;
