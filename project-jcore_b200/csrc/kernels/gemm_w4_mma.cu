@@ -13,11 +13,11 @@
 // three bf16 parts each take a product of their own, eight more warps bring it.
 //
 // Measured (group 128, cold weights): 512 x 4096 x 4096 bf16 22.6 us, 512 x 16384 x 4096 90,
-// 48 x 16384 x 4096 with zeros 19.6, 256 x 4096 x 4096 fp32 47. What bounds it is instructions:
-// 59% of issue slots over the whole of a call of 512 tokens, its start and end included, three
-// to a pair of weights (128 channels widened anew for each tile of tokens) and some 70 to an
-// epilogue warp's group, against 40% of the tensor cores. Groups of 64 and 32 have two and four
-// times the sums to add: 512 x 4096 x 4096 41 and 69 us.
+// 48 x 16384 x 4096 with zeros 19.6, 256 x 4096 x 4096 fp32 47. What bounds it are the roles'
+// waits for one another: without loads, widening, products and sums they alone take 15 us of
+// the 48 tokens' time and 20 of the 512's (issue is at 59%, three instructions to a pair of
+// weights and some 70 to an epilogue warp's group; the tensor cores are at 40%). Groups of 64
+// and 32 have two and four times the sums to add: 512 x 4096 x 4096 41 and 69 us.
 #include <algorithm>
 
 #include "gemm_w4.cuh"
