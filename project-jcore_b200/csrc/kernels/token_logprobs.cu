@@ -254,9 +254,11 @@ __device__ __noinline__ void collect(const T *xp, int from, int end, int lead, f
   __syncthreads();
 }
 
-// kTop: with alternatives. The launch's CTAs are whole clusters of `cluster`.
+// kTop: with alternatives. The launch's CTAs are whole clusters of `cluster`. A row's end is a
+// third of a CTA's time then, under which others load: 28 warps an SM (2048 x 50021 fp16 with
+// five 50.8 us; 24 warps 55.4, 32, which spill, 58.9; 1024 x 128000 bf16 with 20 60, 73, 68).
 template <typename T, bool kTop, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 24 : 32) / kWarps)
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 32) / kWarps)
     token_logprobs_kernel(LogprobArgs p, const T *logits, int cluster) {
   using B = Batch<T>;
   constexpr int E = B::E, U = B::U, kThreads = kWarps * 32;
@@ -588,9 +590,8 @@ auto pick_forward(bool top, int warps) {
 
 // One warp for rows of up to four packs a lane, else four, or 16 where rows do not fill the SMs;
 // then clusters too, while each CTA has two packs a thread. Eight warps a row instead of
-// four are slower (2048 x 50021 fp16 48 us against 43, with five alternatives 65 against 57; 4096 x
-// 32000 bf16 88 against 65) but for long rows with alternatives (1024 x 128000 bf16, 20 of them:
-// 73 against 76).
+// four are slower (2048 x 50021 fp16 48 us against 43, with five alternatives 65 against 51; 4096 x
+// 32000 bf16 88 against 65; 1024 x 128000 bf16 with 20 73 against 61).
 template <typename T>
 int run_forward(cudaStream_t s, const LogprobArgs &p, const T *logits) {
   constexpr int E = 16 / sizeof(T);
