@@ -33,9 +33,12 @@ constexpr int kStagePitch = kStageK / 2;  // bytes
 constexpr int kStageBytes = kRows * kStagePitch;
 constexpr int kDepth = 2;                 // stages in flight and at work
 constexpr int kMostWarps = 16;
-constexpr int kMostX = 64 * 1024;         // bytes of x in shared memory
+// Bytes of x in shared memory, for up to eight tokens and for more; the first leave room for
+// twelve warps.
+constexpr int kMostX = 100 * 1024, kMostX16 = 64 * 1024;
 constexpr int kRedBytes = kRows * 8 * 4;  // sums of a warp and eight tokens
-static_assert(kMostX + kMostWarps * (kDepth * kStageBytes + 2 * kRedBytes) <= 232448,
+constexpr int kWarpBytes = kDepth * kStageBytes + 2 * kRedBytes, kSmem = 232448;
+static_assert(kMostX + 12 * kWarpBytes <= kSmem && kMostX16 + kMostWarps * kWarpBytes <= kSmem,
               "shared memory");
 
 struct RowsPlan {
@@ -411,10 +414,13 @@ auto pick(const W4Args &p) {
 
 // Up to 16 tokens, as far as x fits, this way is the faster or even, against the tensor cores'
 // tiles of 32 tokens: 1 and 8 x 4096 x 4096 bf16 6.7 and 8.2 us (9.1, 9.2), 1 x 16384 x 4096
-// 12 (17), 16 x 128000 x 2048 52 (77), 16 x 4096 x 2048 7.9 (7.6).
+// 12 (17), 16 x 128000 x 2048 52 (77), 16 x 4096 x 2048 7.9 (7.6). With more of x than leaves
+// room for sixteen warps: 4 x 4096 x 11008 12.3 (14.6), 3 x 4096 x 16384 15.7 (18.5), 4 x 4096 x
+// 4096 fp32 10.3 (16.1), 12 x 16384 x 4096 17.7 (17.3), 8 x 4096 x 8192, where ten are left,
+// 13.4 (12.1).
 bool gemm_w4_rows_fits(const W4Args &p) {
-  return p.M <= 16 && x_units(p) * 16 <= kMostX && reinterpret_cast<uintptr_t>(p.q) % 16 == 0 &&
-         (p.ldq % 16 == 0 || p.N == 1);
+  return p.M <= 16 && x_units(p) * 16 <= (p.M <= 8 ? kMostX : kMostX16) &&
+         reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && (p.ldq % 16 == 0 || p.N == 1);
 }
 
 // Slices and teams of least estimated time: rounds of (stages of K, 1.5 us each for 16
@@ -424,10 +430,12 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
   RowsPlan plan{};
   const int64_t sms = sm_count(), stages = ceil_div(p.K, kStageK);
   plan.tiles = static_cast<int>(ceil_div(p.N, kRows));
+  plan.x_bytes = static_cast<int>(align_up(static_cast<size_t>(x_units(p)) * 16, 128));
+  const int64_t most = std::min(kMostWarps, (kSmem - plan.x_bytes) / kWarpBytes);
   double least = 1e30;
-  for (int64_t want = 1; want <= std::min<int64_t>(stages, kMostWarps); ++want) {
+  for (int64_t want = 1; want <= std::min(stages, most); ++want) {
     const int64_t steps = ceil_div(stages, want), slices = ceil_div(stages, steps);
-    const int64_t teams = std::min<int64_t>(kMostWarps / slices, std::max<int64_t>(1, ceil_div(plan.tiles, sms)));
+    const int64_t teams = std::min<int64_t>(most / slices, std::max<int64_t>(1, ceil_div(plan.tiles, sms)));
     const int64_t rounds = ceil_div(plan.tiles, teams * sms);
     const double warps = static_cast<double>(slices * teams);
     const double us =
@@ -443,13 +451,12 @@ int gemm_w4_rows(cudaStream_t s, const W4Args &p) {
     }
   }
   plan.words = make_fastdiv(static_cast<uint32_t>(ceil_div(p.K, p.group) * (p.group / 8)));
-  plan.x_bytes = static_cast<int>(align_up(static_cast<size_t>(x_units(p)) * 16, 128));
   // pieces of 2 (256 / group) bytes
   const int64_t piece = kStageK / p.group;
   plan.packed = p.scale_type != NPLK_DTYPE_FP32 && p.lds % piece == 0 &&
                 reinterpret_cast<uintptr_t>(p.scale) % (2 * piece) == 0;
   const int warps = plan.slices * plan.teams, nt = p.M <= 8 ? 1 : 2;
-  const int smem = plan.x_bytes + warps * (kDepth * kStageBytes + 2 * kRedBytes);
+  const int smem = plan.x_bytes + warps * kWarpBytes;
   auto *fn = p.x_type == NPLK_DTYPE_FP32   ? (nt == 1 ? pick<float, 1>(p) : pick<float, 2>(p))
              : p.x_type == NPLK_DTYPE_FP16 ? (nt == 1 ? pick<__half, 1>(p) : pick<__half, 2>(p))
                                            : (nt == 1 ? pick<__nv_bfloat16, 1>(p)

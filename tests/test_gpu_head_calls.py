@@ -230,3 +230,14 @@ def test_the_largest_and_smallest_scales(scale):
         assert ((ent.double() - uniform).abs() <= 2.0 ** -18).all()
         assert ((lp.double() + uniform).abs() <= 2.0 ** -18).all()
     assert (ids[:, 0] == 7).all()
+
+
+# as much of x as a CTA holds for a few tokens, just under and just over
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("m,n,k,group,dtype", [
+    (4, 100, 11008, 128, "bf16"), (8, 70, 6200, 32, "fp16"), (8, 40, 2100, 64, "fp32"),
+    (3, 1000, 16000, 64, "bf16"), (1, 33, 51200, 128, "bf16"), (1, 33, 51201, 32, "fp16"),
+    (8, 100, 6400, 128, "bf16"), (8, 100, 6432, 32, "bf16"), (16, 100, 2048, 128, "fp16"),
+    (16, 100, 2080, 32, "fp16"), (9, 50, 3640, 32, "bf16")])
+def test_long_rows_of_few_tokens(m, n, k, group, dtype, zeros):
+    check_whole(S.gpu_lib(), m, n, k, group, dtype, TYPES[dtype][0], zeros)
