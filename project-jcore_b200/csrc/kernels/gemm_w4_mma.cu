@@ -12,8 +12,8 @@
 // x comes by TMA where it can (16-bit, 16-byte aligned rows); otherwise, and for fp32, whose
 // three bf16 parts each take a product of their own, eight more warps bring it.
 //
-// Measured (group 128, cold weights): 512 x 4096 x 4096 bf16 22.6 us, 512 x 16384 x 4096 90,
-// 48 x 16384 x 4096 with zeros 19.6, 256 x 4096 x 4096 fp32 47. What bounds it are the roles'
+// Measured (group 128, cold weights): 512 x 4096 x 4096 bf16 22.3 us, 512 x 16384 x 4096 89,
+// 48 x 16384 x 4096 with zeros 18.5, 256 x 4096 x 4096 fp32 47. What bounds it are the roles'
 // waits for one another: without loads, widening, products and sums they alone take 15 us of
 // the 48 tokens' time and 20 of the 512's (issue is at 59%, three instructions to a pair of
 // weights and some 70 to an epilogue warp's group; the tensor cores are at 40%). Groups of 64
@@ -409,9 +409,12 @@ __global__ void __launch_bounds__(MmaThreads<NTOK, kGroup, kTma>::kThreads, 1)
         off[i] = w4_adjacent_offset<F>(static_cast<int>(z_next[i] & 15u));
         z_next[i] = zero_at(kb + 2, i);
       }
-      if (!all(mbar_wait(&raw_full[r.at], r.phase, abort_flag, p.status, kStatusTimeoutStage)))
-        break;
-      if (!all(mbar_wait(&a_empty[st.at], st.phase ^ 1u, abort_flag, p.status, kStatusTimeoutStage)))
+      const bool raw_ready = mbar_test(&raw_full[r.at], r.phase),
+                 a_free = mbar_test(&a_empty[st.at], st.phase ^ 1u);
+      if (!all(raw_ready && a_free) &&
+          !all(mbar_wait(&raw_full[r.at], r.phase, abort_flag, p.status, kStatusTimeoutStage) &&
+               mbar_wait(&a_empty[st.at], st.phase ^ 1u, abort_flag, p.status,
+                         kStatusTimeoutStage)))
         break;
       tc_fence_after_sync();
       const uint8_t *from = ring_raw + r.at * kRawBytes + row * 64;
