@@ -468,7 +468,8 @@ NPL_API int nplk_gemm_w4(void *stream, int64_t M, int64_t N, int64_t K, int64_t 
  * masked: it has p = 0 and is no alternative; where there are fewer alternatives than
  * n_top, the rest have id -1 and -infinity. A row of masked logits alone has logprob
  * -infinity, entropy 0 and stats -infinity. A row that holds a NaN or +infinity has NaN
- * for each result (ids -1). One pass over the logits; sums are fp32 in a fixed order, which
+ * for each result (ids -1), both its stats among them; but logprob is 0 without a token,
+ * whatever the row holds. One pass over the logits; sums are fp32 in a fixed order, which
  * goes by rows, vocab, n_top and the row's alignment to 16 bytes. Results must not overlap
  * the logits. vocab < 2^31 - 65536. The reference's softmax
  * (npl_activation_norm.cpp:88-112) is the nearest it has. */

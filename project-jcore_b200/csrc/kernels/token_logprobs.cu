@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
       const bool bad = total.s != total.s;  // a NaN or +infinity in the row
       if (lane == 0) {
         if (p.stats) {
-          p.stats[2 * row] = total.m;
+          p.stats[2 * row] = bad ? log_sum : total.m;  // (the maximum has left out NaNs)
           p.stats[2 * row + 1] = log_sum;
         }
         if (p.entropy)
