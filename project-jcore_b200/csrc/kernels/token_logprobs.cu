@@ -57,22 +57,40 @@ struct Part {
   float m, s, w;
 };
 
-// The part relative to `m`, not below its own maximum. c = scale * log2 e.
-__device__ __forceinline__ Part rebase(const Part &a, float m, float c) {
-  // nothing but -infinity so far: d is -infinity then, kept finite
-  const float u = at_least(a.m - (m == -kInf ? 0.0f : m), kLowest);
-  const float d = at_least(u * c, kLowest), e = exp2_approx(d);
+// Exponents are scale log2 e (l - m), as c (f l - f m): f is 1/2 for scales below 1, under which a
+// distance beyond fp32 may count (above, its exponential is 0 and its logarithm -infinity). f is a
+// power of two, so nothing else changes.
+struct Factors {
+  float f, scale, c;  // f; scale / f, and that times log2 e
+  __device__ __forceinline__ explicit Factors(float of)
+      : f(of < 1.0f ? 0.5f : 1.0f), scale(of < 1.0f ? 2.0f * of : of), c(scale * kLog2e) {}
+  // -f m; 0 where there is nothing but -infinity
+  __device__ __forceinline__ float origin(float m) const { return m == -kInf ? 0.0f : -f * m; }
+  // Kept finite: 0 times a masked logit's would be NaN. Not before the product with c, which may
+  // bring any finite number back to 0.
+  __device__ __forceinline__ float exponent(float l, float origin) const {
+    return at_least(fmaf(l, f, origin) * c, kLowest);
+  }
+  // scale (l - m) - log_sum
+  __device__ __forceinline__ float log_p(float l, float m, float log_sum) const {
+    return fmaf(fmaf(l, f, -f * m), scale, -log_sum);
+  }
+};
+
+// The part relative to `m`, not below its own maximum.
+__device__ __forceinline__ Part rebase(const Part &a, float m, const Factors &k) {
+  const float d = k.exponent(a.m, k.origin(m)), e = exp2_approx(d);
   // d e first: d s may leave fp32 where e is 0
   return {m, a.s * e, a.w * e + d * e * a.s};
 }
 
 // The parts of the 2 * `half` lanes of a group joined, in all of them.
 template <int half>
-__device__ __forceinline__ Part join_lanes(Part a, float c) {
+__device__ __forceinline__ Part join_lanes(Part a, const Factors &k) {
   float m = a.m;
 #pragma unroll
   for (int o = half; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-  a = rebase(a, m, c);
+  a = rebase(a, m, k);
 #pragma unroll
   for (int o = half; o; o >>= 1) {
     a.s += __shfl_xor_sync(kAll, a.s, o);
@@ -276,7 +294,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
 
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(blockIdx.x) % cluster;
-  const float c = p.scale * kLog2e;
+  const Factors k(p.scale);
   if (cluster > 1) {  // the first CTA has started before anything is stored into it
     cluster_arrive_relaxed();
     cluster_wait();
@@ -315,8 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
     const float lone_value = lone ? to_float(x[lone_index]) : -kInf;
     if (lone) {
       mine.m = fmaxf(lone_value, -kInf);  // the maximum of a NaN and nothing
-      const float u = at_least(lone_value - (mine.m == -kInf ? 0.0f : mine.m), kLowest);
-      const float d = at_least(u * c, kLowest);
+      const float d = k.exponent(lone_value, k.origin(mine.m));
       mine.s = exp2_approx(d);
       mine.w = mine.s * d;
     }
@@ -332,14 +349,13 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (whole || u < here) most = fmaxf(most, most_of(now.p[u]));
-      if (most > mine.m) mine = rebase(mine, most, c);
-      const float base = mine.m == -kInf ? 0.0f : mine.m;
+      if (most > mine.m) mine = rebase(mine, most, k);
+      const float origin = k.origin(mine.m);
       float ss[2] = {}, ww[2] = {};
       const auto add = [&](const Pack<T, E> &p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          // (a masked logit's t kept finite: 0 times it is 0)
-          const float t = at_least((to_float(p.e[e]) - base) * c, kLowest);
+          const float t = k.exponent(to_float(p.e[e]), origin);
           const float r = exp2_approx(t);
           ss[e & 1] += r;
           ww[e & 1] = fmaf(r, t, ww[e & 1]);
@@ -366,7 +382,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
     }
 
     // the warp's, then the CTA's, then the cluster's sums
-    mine = join_lanes<16>(mine, c);
+    mine = join_lanes<16>(mine, k);
     if (lane == 0) warp_part[warp] = mine;
     __syncthreads();
     if constexpr (kTop)
@@ -374,7 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
     Part total{-kInf, 0.0f, 0.0f};
     if (warp == 0) {
       if (lane < kWarps) total = warp_part[lane];
-      total = join_lanes<kWarps / 2>(total, c);
+      total = join_lanes<kWarps / 2>(total, k);
     }
     if (cluster > 1) {
       if (tid == 0) {
@@ -390,7 +406,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
       if (rank != 0) continue;
       if (warp == 0) {
         total = lane < cluster ? cta_part[parity][lane] : Part{-kInf, 0.0f, 0.0f};
-        total = join_lanes<kMostCluster / 2>(total, c);
+        total = join_lanes<kMostCluster / 2>(total, k);
       }
       if constexpr (kTop) {
         uint64_t most = 0;  // n keys reach any CTA's n-th
@@ -420,7 +436,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
           p.logprob[row] = target < 0              ? 0.0f
                            : bad                   ? log_sum
                            : target_logit == -kInf ? -kInf
-                                                   : fmaf(target_logit - total.m, p.scale, -log_sum);
+                                                   : k.log_p(target_logit, total.m, log_sum);
         }
       }
       if (kTop && lane < p.top) {
@@ -428,7 +444,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
         const int64_t to = row * p.top + lane;
         p.top_ids[to] = key && !bad ? key_index(key) : -1;
         p.top_logprobs[to] = bad ? log_sum
-                             : key ? fmaf(value_of(key_order(key)) - total.m, p.scale, -log_sum)
+                             : key ? k.log_p(value_of(key_order(key)), total.m, log_sum)
                                    : -kInf;
       }
     }
@@ -468,6 +484,7 @@ __global__ void __launch_bounds__(kThreads, 3 * 256 / kThreads)
   griddep_wait();
   griddep_launch_dependents();
   const int tid = static_cast<int>(threadIdx.x);
+  const Factors k(p.scale);
   const auto row_of = [&](uint32_t run) {
     GradRow r{};
     if (run >= runs) return r;
@@ -523,14 +540,14 @@ __global__ void __launch_bounds__(kThreads, 3 * 256 / kThreads)
     const float g = hit_row ? now.g : 0.0f, h = now.h;
     const float a = -p.scale * (h != 0.0f ? fmaf(h, now.entropy, g) : g);
     const float2 aa = both(a), bb = both(-p.scale * h * kLn2);
-    const float2 c = both(p.scale * kLog2e), base = both(-now.m), ll = both(-now.log_sum * kLog2e);
+    const float2 f = both(k.f), c = both(k.c), base = both(-k.f * now.m),
+                 ll = both(-now.log_sum * kLog2e);
     const float hot = p.scale * g;
     const int lead = lead_of(x), packs = (p.vocab - lead) / E, tail = lead + packs * E;
     const int hit = hit_row ? static_cast<int>(now.target) : -1;
     const auto pairs = [&](float2 v) {
-      const float2 u = at_least(add2(v, base), kLowest);
-      // (2^-1000 is 0, and 0 times a finite number too)
-      const float2 t = at_least(fma2(u, c, ll), -1000.0f);
+      // (2^-1000 is 0, and 0 times a finite number too; a masked logit's t is -infinity up to here)
+      const float2 t = at_least(fma2(fma2(v, f, base), c, ll), -1000.0f);
       const float2 e = make_float2(exp2_approx(t.x), exp2_approx(t.y));
       return mul2(e, fma2(t, bb, aa));
     };

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import support as S
-from test_gpu_token_logprobs import INF, NAN, TYPES, backward, forward, logits
+from test_gpu_token_logprobs import (INF, NAN, TYPES, U, backward, check_backward, check_forward,
+                                     forward, logits)
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,63 @@ def test_both_stats_of_a_row_with_a_nan_or_infinity(rows, vocab, dtype):
     assert (dx[1:4] == 0).all() and dx[4:6].isnan().all()
     dx = backward(lib, x, vocab, t, st, ent, g, g)
     assert dx[bad].isnan().all() and torch.isfinite(dx[0]).all() and torch.isfinite(dx[6:]).all()
+
+
+# 2.5e-37: the lowest finite number times such a scale is an exponent of some -100
+SMALL = [1e-30, 2.5e-37, 3e-39, 1e-44]
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("scale", SMALL)
+def test_masks_under_the_smallest_scales(rows, vocab, dtype, scale):
+    # all of a row's logits that are left are alike: log n, wherever in the row they lie
+    lib, x = S.gpu_lib(), logits(rows, vocab, dtype)
+    x[0] = -INF
+    x[1, ::2] = -INF
+    x[2, 1::2] = -INF
+    x[3, :-1] = -INF  # one left
+    x[4, 1:] = -INF
+    x[5, :vocab // 2] = -INF
+    x[6] = x[6].abs().neg()  # none above 0
+    x[6, -1] = -INF
+    t = torch.full((rows,), vocab - 1, device="cuda")
+    left = x != -INF
+    n = left.sum(1).double()
+    lp, ent, st, ids, tlp = forward(lib, x, vocab, t, 3, scale)
+    assert lp[0] == -INF and ent[0] == 0 and (st[0] == -INF).all()
+    assert (ids[0] == -1).all() and (tlp[0] == -INF).all()
+    log_n = n[1:].log()
+    # scale |d| is below 1e-28; the sum of n terms is off by (n / 512 + 64) 2^-24 at most, relative
+    tol = (vocab / 512 + 66) * U * (1 + log_n)
+    has = left[1:, -1]
+    assert ((lp[1:].double() + log_n).abs() <= tol)[has].all() and (lp[1:][~has] == -INF).all()
+    assert ((ent[1:].double() - log_n).abs() <= tol).all()
+    assert ((st[1:, 1].double() - log_n).abs() <= tol).all()
+    assert torch.equal(st[1:, 0].double(), x[1:].double().amax(1))
+    g = torch.full((rows,), 2.0 ** 90, device="cuda")
+    dx = backward(lib, x, vocab, t, st, ent, g, g, scale)
+    assert torch.isfinite(dx).all()
+    hit = torch.zeros_like(left)
+    hit[:, -1] = True
+    assert (dx[0] == 0).all() and (dx[~left & ~hit] == 0).all()
+    check_backward(x[1:], vocab, t[1:], st[1:], ent[1:], g[1:], g[1:], scale, dx[1:])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("scale", [1.0, 0.3] + SMALL)
+def test_distances_beyond_fp32(rows, vocab, dtype, scale):
+    # l - m down to -6e38, in every place of a row; scale (l - m) may be small all the same
+    lib, x = S.gpu_lib(), logits(rows, vocab, dtype)
+    far = torch.arange(vocab, device="cuda") % 3 == 1
+    far[0] = far[-1] = True
+    x[:, far] = -3e38
+    x[:, vocab // 3] = 3e38
+    t = torch.full((rows,), vocab - 1, device="cuda")
+    t[::2] = vocab // 2
+    got = forward(lib, x, vocab, t, 2, scale)
+    check_forward(x, vocab, t, scale, got, 2)
+    g = torch.ones(rows, device="cuda")
+    dx = backward(lib, x, vocab, t, got[2], got[1], g, g, scale)
+    check_backward(x, vocab, t, got[2], got[1], g, g, scale, dx)
