@@ -481,7 +481,8 @@ NPL_API int nplk_token_logprobs(void *stream, int64_t rows, int64_t vocab, int d
 /* Gradient into the logits for d_logprob[r] = g and d_entropy[r] = h (each may be NULL,
  * not both), from the stats, and where d_entropy is given the entropy, of the forward call:
  *   dlogits[r,v] = scale * (g ([v = t] - p[v]) - h p[v] (log p[v] + entropy[r])).
- * A row without a target counts g = 0. Rows with g = h = 0, and rows of masked logits
+ * |g| and |h| are up to 2^85 (larger ones may give NaN where p is 0). A row without a target
+ * counts g = 0. Rows with g = h = 0, and rows of masked logits
  * alone, get zeros, whatever else they hold. dlogits (type dtype, pitch ldd) may be
  * logits itself (with the same pitch), overwritten. Other arguments as the forward call. */
 NPL_API int nplk_token_logprobs_backward(void *stream, int64_t rows, int64_t vocab, int dtype,

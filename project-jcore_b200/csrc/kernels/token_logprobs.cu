@@ -454,7 +454,9 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 16 ? 1 : (kTop ? 28 : 3
 
 // ---------------------------------------------------------------------------
 // Gradient: dl = p (A + B t) + [v = target] scale g with t = (d - L) log2 e, p = 2^t,
-// A = -scale (g + h H), B = -scale h ln 2. CTAs go round runs of packs of a row; a run's
+// A = -scale (g + h H), B = -scale h ln 2. Under scales above kMostInner (kLast) the scale comes
+// last instead: where p is 0, or A p and scale g cancel, they must be finite (for every scale it
+// would cost 2% at 4096 x 32000 bf16, 8% at 8192 x 500). CTAs go round runs of packs of a row; a run's
 // logits load under the one before, and its row's numbers, which say whether they are
 // needed at all, one run earlier still. Bound by memory: 4096 x 32000 bf16 takes 92 us, of 80
 // for its bytes (121 us with a CTA a run, which waited for one and then for the other).
@@ -469,6 +471,7 @@ struct LogprobGradArgs {
 };
 
 constexpr int kGradPacks = 4;
+constexpr float kMostInner = 0x1p32f;  // A + B t and scale g are finite for g and h up to 2^85
 
 // What a run needs to know of its row.
 struct GradRow {
@@ -477,7 +480,7 @@ struct GradRow {
   int first;  // pack
 };
 
-template <typename T, int E, int kThreads>
+template <typename T, int E, int kThreads, bool kLast>
 __global__ void __launch_bounds__(kThreads, 3 * 256 / kThreads)
     token_logprobs_grad_kernel(LogprobGradArgs p, const T *logits, T *dlogits, uint32_t runs,
                                FastDiv per_row) {
@@ -538,11 +541,12 @@ __global__ void __launch_bounds__(kThreads, 3 * 256 / kThreads)
     T *dx = dlogits + now.row * p.ldd;
     const bool none = zeros(now), hit_row = asked(now);
     const float g = hit_row ? now.g : 0.0f, h = now.h;
-    const float a = -p.scale * (h != 0.0f ? fmaf(h, now.entropy, g) : g);
-    const float2 aa = both(a), bb = both(-p.scale * h * kLn2);
+    const float inner = kLast ? 1.0f : p.scale;
+    const float a = -inner * (h != 0.0f ? fmaf(h, now.entropy, g) : g);
+    const float2 aa = both(a), bb = both(-inner * h * kLn2);
     const float2 f = both(k.f), c = both(k.c), base = both(-k.f * now.m),
                  ll = both(-now.log_sum * kLog2e);
-    const float hot = p.scale * g;
+    const float hot = inner * g;
     const int lead = lead_of(x), packs = (p.vocab - lead) / E, tail = lead + packs * E;
     const int hit = hit_row ? static_cast<int>(now.target) : -1;
     const auto pairs = [&](float2 v) {
@@ -574,6 +578,10 @@ __global__ void __launch_bounds__(kThreads, 3 * 256 / kThreads)
           for (int e = 0; e < E; ++e)
             if (hit == index + e) v[e] += hot;
         }
+        if constexpr (kLast) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] *= p.scale;
+        }
       }
       store_pack(dx + index, pack<T, E>(v));
     }
@@ -584,6 +592,7 @@ __global__ void __launch_bounds__(kThreads, 3 * 256 / kThreads)
       if (!none) {
         v = pairs(both(to_float(x[index]))).x;
         if (index == hit) v += hot;
+        if (kLast) v *= p.scale;
       }
       dx[index] = from_float<T>(v);
     }
@@ -637,6 +646,12 @@ int run_forward(cudaStream_t s, const LogprobArgs &p, const T *logits) {
   return map_cuda_error(cudaLaunchKernelEx(&cfg, fn, p, logits, cluster));
 }
 
+template <typename T, int E, bool kLast>
+auto pick_gradient(int threads) {
+  return threads == 32 ? token_logprobs_grad_kernel<T, E, 32, kLast>
+                       : token_logprobs_grad_kernel<T, E, 256, kLast>;
+}
+
 template <typename T>
 int run_gradient(cudaStream_t s, int64_t rows, const LogprobGradArgs &p, const T *logits,
                  T *dlogits) {
@@ -648,10 +663,9 @@ int run_gradient(cudaStream_t s, int64_t rows, const LogprobGradArgs &p, const T
                      (rows == 1 || (p.ld - p.ldd) % E == 0);
   const int packs = p.vocab / (alike ? E : 1), threads = packs <= 32 * kGradPacks ? 32 : 256;
   const int64_t per_row = std::max<int64_t>(1, ceil_div(packs, threads * kGradPacks));
-  auto *fn = threads == 32 ? (alike ? token_logprobs_grad_kernel<T, E, 32>
-                                    : token_logprobs_grad_kernel<T, 1, 32>)
-                           : (alike ? token_logprobs_grad_kernel<T, E, 256>
-                                    : token_logprobs_grad_kernel<T, 1, 256>);
+  auto *fn = p.scale > kMostInner
+                 ? (alike ? pick_gradient<T, E, true>(threads) : pick_gradient<T, 1, true>(threads))
+                 : (alike ? pick_gradient<T, E, false>(threads) : pick_gradient<T, 1, false>(threads));
   // rows of a launch: their runs are counted in 31 bits
   const int64_t most = std::max<int64_t>(1, (int64_t(1) << 30) / per_row);
   for (int64_t r = 0; r < rows; r += most) {

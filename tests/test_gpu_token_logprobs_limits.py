@@ -5,7 +5,7 @@ import torch
 
 import support as S
 from test_gpu_token_logprobs import (INF, NAN, TYPES, U, backward, check_backward, check_forward,
-                                     forward, logits)
+                                     forward, gen, logits)
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,31 @@ def test_distances_beyond_fp32(rows, vocab, dtype, scale):
     g = torch.ones(rows, device="cuda")
     dx = backward(lib, x, vocab, t, got[2], got[1], g, g, scale)
     check_backward(x, vocab, t, got[2], got[1], g, g, scale, dx)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("scale", [1e30, 1e36, 2.0 ** 126])
+def test_gradient_under_the_largest_scales(rows, vocab, dtype, scale):
+    # p is 0 but for the largest logits: a gradient of 0 there, however large g and h times the
+    # scale and the exponent
+    lib = S.gpu_lib()
+    x = torch.randint(-50, 50, (rows, vocab), device="cuda", generator=gen(6)).to(TYPES[dtype][0])
+    x[:, 2] = 60.0
+    x[::3, vocab - 1] = 60.0       # two of them
+    x[1] = 1.0                     # all
+    x[:, 4] = -INF
+    x[5, 5:] = -INF
+    t = torch.full((rows,), 2, device="cuda")
+    t[::2] = 3
+    g = torch.rand(rows, device="cuda", generator=gen(1)) * 6 - 3
+    h = torch.rand(rows, device="cuda", generator=gen(2)) * 6 - 3
+    _, ent, st, _, _ = forward(lib, x, vocab, t, 0, scale)
+    for gg, hh in ((g, None), (None, h), (g, h)):
+        dx = backward(lib, x, vocab, t, st, ent if hh is not None else None, gg, hh, scale)
+        assert torch.isfinite(dx).all()
+        check_backward(x, vocab, t, st, ent, gg, hh, scale, dx)
+    # all of p on the token: nothing left to change, also where scale g leaves fp32
+    sure = torch.arange(rows, device="cuda") % 6 == 5
+    dx = backward(lib, x, vocab, t, st, None, torch.full_like(g, 1e4), None, scale)
+    assert (dx[sure] == 0).all()
