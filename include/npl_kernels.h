@@ -441,9 +441,12 @@ NPL_API int nplk_quantize_w4(void *stream, int64_t N, int64_t K, int64_t group, 
 
 /* C[m,n] = act(sum_k x[m,k] * weight[n,k] + bias[n]): x is [M][K] (tokens) of type
  * x_dtype, pitch ldx; C row-major of type c_dtype, pitch ldc; bias [N] fp32 or NULL;
- * act is 0..10 as in nplk_group_norm_act. Products are exact, sums fp32 in a fixed
- * order (the same call gives the same bits; the order goes by M, N, K, group, x_dtype and
- * alignment), C is rounded once.
+ * act is 0..10 as in nplk_group_norm_act. A group's sum of x * (nibble - zero) comes first,
+ * then its scale: these products are exact (but for bits of fp32 tokens below 2^-133), sums
+ * are fp32 in a fixed order (the same call gives the same bits; the order goes by M, N, K,
+ * group, x_dtype and alignment), in which the tensor cores may cut where an fp32 sum rounds:
+ * 2^-23 a step instead of 2^-24. A group's sum beyond fp32 is infinite whatever its scale.
+ * C is rounded once.
  * Any pitch and alignment is taken; q 16-byte aligned with ldq a multiple of 16
  * is needed for the fast kernels. M, N, K <= 2^30. No workspace. C must not overlap the
  * inputs. status as in nplk_gemm_i8. */

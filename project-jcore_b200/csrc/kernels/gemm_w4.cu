@@ -15,18 +15,21 @@ namespace nplk {
 namespace {
 
 // ---------------------------------------------------------------------------
-// tiles: 64 x 64 results a CTA, 32 of K at a time as fp32 in shared memory. 256 threads,
-// 4 x 4 results each.
+// tiles: 64 x 64 results a CTA, 32 of K at a time as fp32 in shared memory, all of one group.
+// 256 threads, 4 x 4 results each: the group's sums, which its scales multiply at its end, and
+// the results'; four CTAs an SM (three, which the registers of both would leave, took 1388 us at 512 x
+// 4096 x 4096 bf16, now 1030; single bytes and values are loaded, 1 x 4096 x 4096 takes 390).
 // ---------------------------------------------------------------------------
 constexpr int kTile = 64, kTileK = 32, kTilePitch = kTileK + 1;
 
 template <typename X, typename T>
-__global__ void __launch_bounds__(256) gemm_w4_tiles_kernel(W4Args p, const X *x, T *C) {
-  __shared__ float sx[kTile * kTilePitch], sw[kTile * kTilePitch];
+__global__ void __launch_bounds__(256, 4) gemm_w4_tiles_kernel(W4Args p, const X *x, T *C) {
+  __shared__ float sx[kTile * kTilePitch], sw[kTile * kTilePitch], scales[kTile];
   const int64_t m_tiles = (static_cast<int64_t>(p.M) + kTile - 1) / kTile;
   const int64_t m0 = blockIdx.x % m_tiles * kTile, n0 = blockIdx.x / m_tiles * kTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
+  const int group_bits = __ffs(p.group) - 1;
+  float acc[4][4] = {}, part[4][4] = {};
   griddep_wait();
   griddep_launch_dependents();
   for (int k0 = 0; k0 < p.K; k0 += kTileK) {
@@ -36,13 +39,16 @@ __global__ void __launch_bounds__(256) gemm_w4_tiles_kernel(W4Args p, const X *x
       if (k < p.K && m0 + r < p.M) v = to_float(x[(m0 + r) * p.ldx + k]);
       if (k < p.K && n0 + r < p.N) {
         const int64_t n = n0 + r;
-        const int g = k / p.group;
         const int nibble = p.q[n * p.ldq + k / 2] >> (k % 2 * 4) & 15;
-        const int zero = p.zero ? p.zero[n * p.ldz + g] & 15 : 8;
-        w = load_scale(p.scale, p.scale_type, n * p.lds + g) * static_cast<float>(nibble - zero);
+        const int zero = p.zero ? p.zero[n * p.ldz + (k0 >> group_bits)] & 15 : 8;
+        w = static_cast<float>(nibble - zero);
       }
       sx[r * kTilePitch + i % kTileK] = v;
       sw[r * kTilePitch + i % kTileK] = w;
+    }
+    if ((k0 & (p.group - 1)) == 0 && threadIdx.x < kTile) {
+      const int64_t n = min(n0 + threadIdx.x, static_cast<int64_t>(p.N) - 1);
+      scales[threadIdx.x] = load_scale(p.scale, p.scale_type, n * p.lds + (k0 >> group_bits));
     }
     __syncthreads();
 #pragma unroll 8
@@ -56,7 +62,18 @@ __global__ void __launch_bounds__(256) gemm_w4_tiles_kernel(W4Args p, const X *x
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(a[i], b[j], part[i][j]);
+    }
+    if (((k0 + kTileK) & (p.group - 1)) == 0 || k0 + kTileK >= p.K) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s = scales[tx + 16 * j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[i][j] = fmaf(s, part[i][j], acc[i][j]);
+          part[i][j] = 0.0f;
+        }
+      }
     }
     __syncthreads();
   }
