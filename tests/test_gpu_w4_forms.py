@@ -4,7 +4,9 @@ import pytest
 import torch
 
 import support as S
-from test_gpu_w4 import U, gen
+from test_gpu_group_norm import act64
+from test_gpu_head_calls import PRODUCTS
+from test_gpu_w4 import U, check_whole, gen, random_operands
 from w4 import TYPES, pack, product, weights64
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +51,31 @@ def test_weights_at_odd_addresses_with_scales_of_24_bits(m, n, k, group, dtype):
     # a value is in at most `group` sums within its group, and in one with each group's scale
     size = x.double().abs() @ w.abs().t()
     assert ((c - x.double() @ w.t()).abs() <= (group + groups + 1) * U * size).all()
+
+
+# tiles of 32, 48 (groups of 128), 64 and 128 tokens with x by TMA; one stage of K, an odd count
+# of them, a share of every CTA of a cluster, and no cluster
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m", [17, 24, 32, 33, 48, 49, 57, 64, 65, 128])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_tiles_by_tma(m, group, dtype, zeros):
+    lib = S.gpu_lib()
+    for n, k in ((130, 96), (300, 640), (70, 1024), (200, 4096), (20001, 384)):
+        check_whole(lib, m, n, k, group, dtype, TYPES[dtype][0], zeros)
+
+
+@pytest.mark.parametrize("case", PRODUCTS)
+def test_against_64_bits(case):
+    # the calls of test_gpu_head_calls.PRODUCTS, which are compared with their own repetition there
+    m, n, k, group, dtype = case
+    lib = S.gpu_lib()
+    x, q, sc, z, b = random_operands(*case, zeros=True)
+    for zero in (None, z):
+        c = product(lib, x, q, sc, zero, group, n, k, b, act=6).double()
+        w = weights64(q, sc, zero, group, k)
+        v = x.double() @ w.t() + b.double()
+        want = act64(v, 6)
+        # steps of a sum as in test_gpu_w4; the slope of swish is up to 1.1, 2e-5 for its formula
+        err = 1.1 * (3 * k / 16 + 24 + k / 32) * 2 * U * (x.double().abs() @ w.abs().t() + b.abs())
+        assert ((c - want).abs() <= err + 2e-5 * (1 + want.abs())).all()
