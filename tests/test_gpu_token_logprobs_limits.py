@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import support as S
-from test_gpu_token_logprobs import (INF, NAN, TYPES, U, backward, check_backward, check_forward,
+from test_gpu_token_logprobs import (INF, NAN, TYPES, U, backward, check_backward, check_forward, f32,
                                      forward, gen, logits)
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +129,32 @@ def test_gradient_under_the_largest_scales(rows, vocab, dtype, scale):
     sure = torch.arange(rows, device="cuda") % 6 == 5
     dx = backward(lib, x, vocab, t, st, None, torch.full_like(g, 1e4), None, scale)
     assert (dx[sure] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("scale", [1.0, 1 / 0.7, 2.0])
+def test_the_gradient_of_a_masked_logit_is_zero(rows, vocab, dtype, scale):
+    lib, x = S.gpu_lib(), logits(rows, vocab, dtype)
+    x[0, ::2] = -INF
+    x[1, 1::2] = -INF
+    x[2, 3:] = -INF
+    x[3, :-2] = -INF
+    x[4, vocab // 3:vocab // 2] = -INF
+    x[5, 1:] = -INF
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=gen(5))
+    t[0], t[1], t[5] = 0, 0, vocab - 1  # a masked token, one that is left, a masked one
+    _, ent, st, _, _ = forward(lib, x, vocab, t, 0, scale)
+    g = torch.randn(rows, device="cuda", generator=gen(1))
+    h = torch.randn(rows, device="cuda", generator=gen(2))
+    masked = x == -INF
+    at = torch.arange(rows, device="cuda")
+    masked[at, t] = False
+    assert masked[:6].any(1).all()
+    for gg, hh in ((g, None), (None, h), (g, h)):
+        dx = backward(lib, x, vocab, t, st, ent if hh is not None else None, gg, hh, scale)
+        assert (dx[masked] == 0).all()
+        # the masked tokens' own: scale g, rounded in fp32 and to the type
+        for r in (0, 5):
+            want = f32(scale) * gg[r].double() if gg is not None else torch.zeros((), device="cuda")
+            assert abs(dx[r, t[r]] - want) <= (U + torch.finfo(x.dtype).eps) * abs(want)
