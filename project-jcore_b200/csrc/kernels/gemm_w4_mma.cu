@@ -622,7 +622,11 @@ int gemm_w4_mma(cudaStream_t s, const W4Args &args) {
   const int64_t sms = sm_count(), blocks = ceil_div(p.K, kBK);
   const int64_t tiles = ceil_div(p.N, kChannels) * ceil_div(p.M, tokens);
   MmaPlan plan{1, 0, 0};
-  // waves of (start and end, stages of a slice), and the slices' meeting, as measured
+  // waves of (start and end, stages of a slice), and the slices' meeting, as measured for groups of 128
+  // in 16 bits. Shorter groups' and fp32 tokens' stages take two to four times as long, which moves
+  // the choice little; it is the best of the four for them too (us for 1, 2, 4, 8 slices: 64 x 4096 x 4096 18.7,
+  // 13.3, 11.7, 30.2; with groups of 32 34.1, 20.9, 15.9, 39.2; 256 tokens with groups of 32 69, 38.6, 46,
+  // 78; 512 69, 77, 91, 141; 40 x 4096 x 4096 fp32 52, 29.8, 17.5, 36; 64 x 1000 x 16384 bf16 58, 33, 20, 15.1).
   double least = 1e30;
   for (int slices : {1, 2, 4, 8}) {
     if (slices > blocks) break;

@@ -614,10 +614,17 @@ auto pick_forward(bool top, int warps) {
   }
 }
 
-// One warp for rows of up to four packs a lane, else four, or 16 where rows do not fill the SMs;
-// then clusters too, while each CTA has two packs a thread. Eight warps a row instead of
-// four are slower (2048 x 50021 fp16 48 us against 43, with five alternatives 65 against 51; 4096 x
-// 32000 bf16 88 against 65; 1024 x 128000 bf16 with 20 73 against 61).
+// One warp for rows of up to four packs a lane (8192 x 1000 bf16 11.3 us, by four 25.9; 500 x 500 3.2,
+// 3.4), else four, or 16 where rows do not fill the SMs (256 x 128000 bf16 22.0 us, by four 25.8;
+// 297, where the rule takes four, 27.7, by 16 29.5, with five alternatives 30.7, 38.3); then clusters too,
+// while each CTA has two packs a thread and the cluster's double takes up to 3/4 of the SMs (us at
+// 128000 bf16 for clusters of 1, 2, 4, 8: one row 8.9, 6.4, 4.6, 4.0; 8 rows 9.2, 6.5, 4.8, 4.2; 16 10.6,
+// 7.3, 5.4, 8.2; 37 11.1, 7.8, 10.1, 12.5; 55 11.2, 8.2, 10.7, 16.4; 111 11.7, 15.3, 19.7, 31.2). A cluster
+// too many costs more than one too few, but short of these borders the next larger form would win: 28
+// rows in fours 5.8 (in twos 7.6), 64 in twos 8.3 (11.3); so would fewer warps for shorter rows, 256 x
+// 9000 with five by four 8.2 (13.7), 8192 x 1100 by one 12.3 (28.3). Eight warps a row instead of
+// four were slower (measured with a slower loop: 2048 x 50021 fp16 48 us against 43, with five
+// alternatives 65 against 51; 4096 x 32000 bf16 88 against 65; 1024 x 128000 bf16 with 20 73 against 61).
 template <typename T>
 int run_forward(cudaStream_t s, const LogprobArgs &p, const T *logits) {
   constexpr int E = 16 / sizeof(T);
