@@ -445,8 +445,8 @@ NPL_API int nplk_quantize_w4(void *stream, int64_t N, int64_t K, int64_t group, 
  * then its scale: these products are exact (but for bits of fp32 tokens below 2^-133), sums
  * are fp32 in a fixed order (the same call gives the same bits; the order goes by M, N, K,
  * group, x_dtype and alignment), in which the tensor cores may cut where an fp32 sum rounds:
- * 2^-23 a step instead of 2^-24. A group's sum beyond fp32 is infinite whatever its scale.
- * C is rounded once.
+ * 2^-23 a step instead of 2^-24. A group's sum that leaves fp32 is infinite or NaN, however
+ * small its scale. C is rounded once.
  * Any pitch and alignment is taken; q 16-byte aligned with ldq a multiple of 16
  * is needed for the fast kernels. M, N, K <= 2^30. No workspace. C must not overlap the
  * inputs. status as in nplk_gemm_i8. */
@@ -485,9 +485,9 @@ NPL_API int nplk_token_logprobs(void *stream, int64_t rows, int64_t vocab, int d
  * not both), from the stats, and where d_entropy is given the entropy, of the forward call:
  *   dlogits[r,v] = scale * (g ([v = t] - p[v]) - h p[v] (log p[v] + entropy[r])).
  * |g| and |h| are up to 2^85 (larger ones may give NaN where p is 0). A row without a target
- * counts g = 0. Rows with g = h = 0, and rows of masked logits
- * alone, get zeros, whatever else they hold. dlogits (type dtype, pitch ldd) may be
- * logits itself (with the same pitch), overwritten. Other arguments as the forward call. */
+ * counts g = 0. Rows with g = h = 0, and rows of masked logits alone, get zeros, whatever else
+ * they hold. dlogits (type dtype, pitch ldd) may be logits itself (with the same pitch),
+ * overwritten. Other arguments as the forward call. */
 NPL_API int nplk_token_logprobs_backward(void *stream, int64_t rows, int64_t vocab, int dtype,
                                          const void *logits, int64_t ld, float scale,
                                          const int64_t *targets, const float *stats,
